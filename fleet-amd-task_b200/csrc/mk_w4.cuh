@@ -1,0 +1,122 @@
+// mk_w4.cuh -- the 4-bit weight format and the warp-level pieces of its products (mk_w4.cu).
+//
+// A weight W [N, K] is 4-bit codes with one scale, and optionally one zero point, per row and group
+// of 32, 64 or 128 values along K: W[n, k] = s[n, k / G] (q[n, k] - z[n, k / G]), z = 8 without zero
+// points. Products sum exactly that: q - z is an integer of at most 5 bits (exact in BF16 and FP16),
+// its product with a 16-bit activation is exact in FP32, a group is summed by the tensor cores in
+// FP32 and the group's sum is multiplied by its scale in FP32. Nothing is rounded to 16 bits before
+// the result.
+//
+// The laid-out form (fleet/w4.py lay_out) is the order in which the lanes of a warp want the codes
+// for mma.sync m16n8k16 with the weights as the 16-row operand and the tokens as its 8 columns:
+//   codes  [experts][tiles][chunks][32 lanes][4 words]: a tile is 16 rows, a chunk 64 values of K.
+//          lane 4 g + t, word 2 h + j (h, j in 0..1) holds rows g and g + 8 at the four values
+//          k = 64 chunk + 32 h + 8 t + 4 j + (0..3): bits 4i..4i+3 (k even) and 16+4i.. (k odd) are,
+//          for i = 0..3, (row g, k 0/1), (row g + 8, k 0/1), (row g, k 2/3), (row g + 8, k 2/3):
+//          the four A registers of one MMA, two codes each, one AND and OR apart from a 16-bit float
+//   scales [experts][tiles][groups][8][2]: rows g and g + 8 side by side (one 32-bit load a lane)
+//   zeros  [experts][tiles][groups][8][2] bytes, or none
+// The MMA's k slots are a permutation of the 64 values (lane t of a quad has 8 consecutive ones of
+// each 32), the same one for the activations: a sum does not ask for their order, and a lane's share
+// of the activations is then one 16-byte load per 32 values. Rows and K are padded to whole tiles
+// and chunks with scale 0 and activations 0.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace w4 {
+
+constexpr int TILE_ROWS = 16, CHUNK_K = 64, CHUNK_BYTES = 512;
+
+struct Bf16 {
+  static constexpr uint32_t MAGIC = 0x43004300u;   // 128 + code in the low mantissa bits
+  static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 d = __hsub2(reinterpret_cast<const __nv_bfloat162&>(a), reinterpret_cast<const __nv_bfloat162&>(b));
+    return reinterpret_cast<const uint32_t&>(d);
+  }
+  static __device__ __forceinline__ float2 to_f32(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ float one_to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+  static __device__ __forceinline__ uint16_t round(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+struct Fp16 {
+  static constexpr uint32_t MAGIC = 0x64006400u;   // 1024 + code
+  static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+    const __half2 d = __hsub2(reinterpret_cast<const __half2&>(a), reinterpret_cast<const __half2&>(b));
+    return reinterpret_cast<const uint32_t&>(d);
+  }
+  static __device__ __forceinline__ float2 to_f32(uint32_t v) {
+    return __half22float2(reinterpret_cast<const __half2&>(v));
+  }
+  static __device__ __forceinline__ float one_to_f32(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+  static __device__ __forceinline__ uint16_t round(float v) { return __half_as_ushort(__float2half_rn(v)); }
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// one word's four A registers: codes to 16-bit floats, their zero points taken off (exact)
+template <class D>
+__device__ __forceinline__ void decode(uint32_t w, uint32_t z0, uint32_t z1, uint32_t (&a)[4]) {
+  constexpr uint32_t M = 0x000F000Fu;
+  a[0] = D::sub2((w & M) | D::MAGIC, z0);
+  a[1] = D::sub2(((w >> 4) & M) | D::MAGIC, z1);
+  a[2] = D::sub2(((w >> 8) & M) | D::MAGIC, z0);
+  a[3] = D::sub2(((w >> 12) & M) | D::MAGIC, z1);
+}
+
+// 32 values of K: two words against each column tile's 16 bytes of activations
+template <class D, int NT>
+__device__ __forceinline__ void half_chunk(uint32_t w0, uint32_t w1, uint32_t z0, uint32_t z1, const uint4 (&xb)[NT],
+                                           float (&acc)[NT][4]) {
+  uint32_t a[4];
+  decode<D>(w0, z0, z1, a);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].x, xb[n].y);
+  decode<D>(w1, z0, z1, a);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].z, xb[n].w);
+}
+
+// tot += scale (rows g, g + 8) * acc; acc = 0
+template <class D, int NT>
+__device__ __forceinline__ void fold(uint32_t scale, float (&acc)[NT][4], float (&tot)[NT][4]) {
+  const float2 s = D::to_f32(scale);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    tot[n][0] = fmaf(s.x, acc[n][0], tot[n][0]);
+    tot[n][1] = fmaf(s.x, acc[n][1], tot[n][1]);
+    tot[n][2] = fmaf(s.y, acc[n][2], tot[n][2]);
+    tot[n][3] = fmaf(s.y, acc[n][3], tot[n][3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+  }
+}
+
+}  // namespace w4

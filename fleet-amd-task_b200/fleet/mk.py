@@ -81,11 +81,25 @@ class MkTraceRecord(ctypes.Structure):
                 ("t_body", ctypes.c_uint64), ("t_stages", ctypes.c_uint64), ("wait_ns", ctypes.c_uint64)]
 
 
+class MkRoute(ctypes.Structure):
+    _fields_ = [("experts", ctypes.c_int32), ("topk", ctypes.c_int32), ("n_forced", ctypes.c_int32),
+                ("n_group", ctypes.c_int32), ("topk_group", ctypes.c_int32), ("group_top2", ctypes.c_int32),
+                ("score", ctypes.c_int32), ("renormalize", ctypes.c_int32), ("logits_dtype", ctypes.c_int32),
+                ("scaling", ctypes.c_float)]
+
+
+class MkW4(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p),
+                ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("group", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("experts", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 EXPORTS = ["mk_version", "mk_last_error", "mk_create", "mk_add_op", "mk_finalize", "mk_launch", "mk_decode_token",
            "mk_status",
            "mk_reset", "mk_trace", "mk_op_tasks", "mk_destroy", "mk_debug_block_op", "mk_selftest_math",
            "mk_mla_decode_noalloc", "mk_set_op_deps", "mk_ep_alloc", "mk_ep_free", "mk_ep_ipc_handle",
-           "mk_ep_ipc_open", "mk_ep_ipc_close"]
+           "mk_ep_ipc_open", "mk_ep_ipc_close", "mk_route", "mk_w4_linear", "mk_w4_experts_workspace",
+           "mk_w4_experts"]
 
 _lib = None
 
@@ -128,6 +142,10 @@ def lib():
         L.mk_selftest_math.argtypes = [i32, vp, vp, i64, vp]
         L.mk_mla_decode_noalloc.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32,
                                             ctypes.c_float, vp]
+        L.mk_route.argtypes = [vp, vp, i64, i32, vp, vp, vp, vp]
+        L.mk_w4_linear.argtypes = [vp, vp, i64, i32, vp, i64, vp, i64, i32, vp]
+        L.mk_w4_experts_workspace.argtypes = [vp, vp, i32, i32, ctypes.POINTER(i64)]
+        L.mk_w4_experts.argtypes = [vp, vp, vp, i64, vp, vp, i32, i32, vp, i64, vp, i64, vp, i64, vp]
         for name in EXPORTS:
             getattr(L, name).restype = ctypes.c_int if name != "mk_last_error" else ctypes.c_char_p
         _lib = L
@@ -145,6 +163,41 @@ def _ptr(t):
     if isinstance(t, int):
         return t
     return t.data_ptr()
+
+
+def stream_of(t):
+    """The handle of the current stream of tensor t's device: where torch's own operators on t run."""
+    import torch
+    if not t.is_cuda:
+        raise MkError(MK_EINVAL, f"tensors are on a CUDA device, not {t.device}")
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def on_stream(t, stream):
+    """A context with `stream` (a torch stream, or a raw handle on tensor t's device) current, so that
+    what a call allocates belongs to the stream that uses it."""
+    import torch
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=t.device)
+    return torch.cuda.stream(stream)
+
+
+class on_device_of:
+    """With t's device current (the library launches on the current device)."""
+
+    def __init__(self, t):
+        self.index = t.device.index
+
+    def __enter__(self):
+        import torch
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        import torch
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
 
 
 def make_op(type_, flags=0, ptrs=None, ips=None, fps=None, ntasks=0):

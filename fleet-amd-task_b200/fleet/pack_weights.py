@@ -250,6 +250,37 @@ def fp8_experts(W13, W2):
     return W13q, s13, regroup_w2(W2q), s2.reshape(-1).contiguous()
 
 
+def quantize_w4(w, group=128, zero_point=False, dtype=None):
+    """Weight-only 4 bits (fleet.w4 has the form): w [..., N, K] -> (codes [..., N, ceil(K / 2)] uint8,
+    scales [..., N, ceil(K / group)] of `dtype` (default: w's), zeros uint8 or None), round to nearest
+    (ties to even) with one scale per row and group. Symmetric: scale amax / 7, codes 1..15 around 8.
+    zero_point: scale (max - min) / 15 over the group's range widened to hold 0, zeros
+    round(-min / scale). The scale is rounded to its type before the codes are taken; a group of
+    zeros has scale 0 and decodes to 0."""
+    dtype = dtype or w.dtype
+    K = w.shape[-1]
+    g = -(-K // group)
+    v = torch.nn.functional.pad(w.float(), (0, g * group - K)).unflatten(-1, (g, group))
+    if zero_point:
+        lo, hi = v.amin(-1).clamp(max=0), v.amax(-1).clamp(min=0)
+        scale = ((hi - lo) / 15).to(dtype)
+    else:
+        lo, scale = None, (v.abs().amax(-1) / 7).to(dtype)
+    step = torch.where(scale > 0, scale, torch.ones_like(scale)).float()
+    zero = (-lo / step).round().clamp(0, 15) if zero_point else torch.full_like(step, 8)
+    q = (v / step[..., None]).round_().add_(zero[..., None]).clamp_(0, 15).to(torch.uint8).flatten(-2)[..., :K]
+    q = torch.nn.functional.pad(q, (0, K % 2))
+    codes = (q[..., 0::2] | (q[..., 1::2] << 4)).contiguous()
+    return codes, scale.contiguous(), zero.to(torch.uint8).contiguous() if zero_point else None
+
+
+def dequantize_w4(codes, scales, zeros, k, group=128):
+    """The FP32 weight [..., N, k] that the codes stand for."""
+    q = torch.stack([codes & 15, codes >> 4], -1).flatten(-2)[..., :k].float()
+    spread = lambda v: v.float().repeat_interleave(group, -1)[..., :k]  # noqa: E731
+    return (q - (8 if zeros is None else spread(zeros))) * spread(scales)
+
+
 def pack_attention(d: Dims, get):
     """The attention and norm tensors of one layer; get(suffix) -> the layer's tensor."""
     w_uk, w_uv = split_uk_uv(d, get("self_attn.kv_b_proj.weight"))

@@ -1,0 +1,210 @@
+"""4-bit weights for a batch of sequences: W4Linear (one weight) and W4Experts (a layer's routed
+experts), over mk_w4_linear / mk_w4_experts (csrc/mk_w4.cu).
+
+A 4-bit weight W [..., N, K] is
+
+* ``codes`` [..., N, ceil(K / 2)] uint8, the even k in the low nibble,
+* ``scales`` [..., N, ceil(K / group)] of the activations' type (bfloat16 or float16),
+* ``zeros`` [..., N, ceil(K / group)] uint8 in 0..15, or None (8 everywhere),
+
+with W[n, k] = scales[n, k // group] * (code[n, k] - zeros[n, k // group]) and group 32, 64 or 128
+(pack_weights.quantize_w4 makes one from a BF16 weight). The constructors lay the codes out once in
+the order the kernels stream them (csrc/mk_w4.cuh) and keep only that form.
+"""
+import ctypes
+
+import torch
+
+from fleet import mk
+
+DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+GROUPS = (32, 64, 128)
+
+
+def lay_out(codes, scales, zeros, k, group, gate_up=False):
+    """(codes, scales, zeros) of weights [E, N, K] in the kernels' order: codes [E, tiles, chunks, 512]
+    uint8, scales and zeros [E, tiles, groups, 16]. gate_up: rows 2i / 2i + 1 are gate / up row i
+    (pack_weights.interleave_gate_up) and a tile takes 8 gate rows, then their 8 up rows."""
+    E, N = codes.shape[:2]
+    tiles, chunks = -(-N // 16), -(-k // 64)
+    groups = -(-64 * chunks // group)
+
+    def rows(v, fill):
+        """[E, N, m] -> [E, tiles, 2 (row g, row g + 8), 8 (g), m]"""
+        v = torch.nn.functional.pad(v, (0, 0, 0, tiles * 16 - N), value=fill)
+        if gate_up:
+            return v.view(E, tiles, 8, 2, -1).transpose(2, 3)
+        return v.view(E, tiles, 2, 8, -1)
+
+    q = torch.full((E, N, chunks * 64), 8, dtype=torch.uint8, device=codes.device)
+    q[..., 0:k:2] = codes[..., :(k + 1) // 2] & 15
+    q[..., 1:k:2] = codes[..., :k // 2] >> 4
+    # k = 64 chunk + 32 h + 8 t + 4 j + 2 p + low/high half; bytes of a word: (half, p), nibbles: the two rows
+    q = rows(q, 8).view(E, tiles, 2, 8, chunks, 2, 4, 2, 2, 2)          # e, tile, r, g, chunk, h, t, j, p, half
+    q = q[:, :, 0] | (q[:, :, 1] << 4)
+    q = q.permute(0, 1, 3, 2, 5, 4, 6, 8, 7).contiguous().view(E, tiles, chunks, 512)   # ... chunk, g, t, h, j, half, p
+
+    def grouped(v, fill):
+        v = torch.nn.functional.pad(v, (0, groups - v.shape[-1]), value=fill)
+        return rows(v, fill).permute(0, 1, 4, 3, 2).contiguous().view(E, tiles, groups, 16)
+
+    return q, grouped(scales, 0), None if zeros is None else grouped(zeros, 8)
+
+
+class W4Weight:
+    """A laid-out weight [E, N, K] (or [N, K]) and the struct the library reads."""
+
+    def __init__(self, codes, scales, zeros=None, k=None, group=128, gate_up=False):
+        if codes.dim() == 2:
+            codes, scales, zeros = codes[None], scales[None], None if zeros is None else zeros[None]
+        k = 2 * codes.shape[-1] if k is None else k
+        if group not in GROUPS:
+            raise ValueError(f"group {group} is one of {GROUPS}")
+        E, N = codes.shape[0], codes.shape[1] if codes.dim() == 3 else 0
+        want = (E, N, -(-k // group))
+        if codes.dim() != 3 or codes.dtype != torch.uint8 or k < 1 or codes.shape[2] != (k + 1) // 2 or N < 1 or E < 1:
+            raise ValueError(f"codes [N, {(k + 1) // 2}] uint8 expected for k = {k}, got {codes.dtype} {tuple(codes.shape)}")
+        if scales.dtype not in DTYPES or tuple(scales.shape) != want:
+            raise ValueError(f"scales {want} bfloat16 or float16 expected, got {scales.dtype} {tuple(scales.shape)}")
+        if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != want):
+            raise ValueError(f"zeros {want} uint8 expected, got {zeros.dtype} {tuple(zeros.shape)}")
+        if gate_up and N % 2:
+            raise ValueError(f"gate and up rows come in pairs, got {N} rows")
+        if any(v is not None and v.device != codes.device for v in (scales, zeros)):
+            raise ValueError("codes, scales and zeros are on one device")
+        self.n, self.k, self.group, self.experts, self.dtype, self.device = N, k, group, E, scales.dtype, codes.device
+        self.codes, self.scales, self.zeros = lay_out(codes, scales, zeros, k, group, gate_up)
+        self.c = mk.MkW4(self.codes.data_ptr(), self.scales.data_ptr(), mk._ptr(self.zeros), N, k, group,
+                         DTYPES[scales.dtype], E, 0)
+        self.ptr = ctypes.addressof(self.c)
+
+
+def _rows(t, shape, dtypes, device, name):
+    """The row stride of a 2-D tensor of unit column stride."""
+    if tuple(t.shape) != shape or t.dtype not in dtypes or t.device != device or (shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: {' or '.join(map(str, dtypes))} {shape} with unit stride along its rows on {device} "
+                         f"expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()} on {t.device}")
+    return t.stride(0)
+
+
+def _span(t):
+    """[first byte, past the last byte) of a 2-D tensor of unit column stride."""
+    n = ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size() if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + n
+
+
+def _out(out, shape, dtypes, device, x, residual):
+    """The row stride of a caller's output: rows apart from one another and from x, and the residual's
+    own rows or none of them."""
+    ld = _rows(out, shape, dtypes, device, "out")
+    if shape[0] > 1 and ld < shape[1]:
+        raise ValueError(f"out: rows overlap (stride {ld}, {shape[1]} values)")
+    lo, hi = _span(out)
+    apart = lambda t: _span(t)[1] <= lo or hi <= _span(t)[0]  # noqa: E731
+    if not apart(x):
+        raise ValueError("out overlaps x")
+    if residual is not None and not apart(residual) and not (
+            residual.data_ptr() == lo and residual.stride(0) == ld and residual.dtype == out.dtype):
+        raise ValueError("out is the residual itself or apart from it")
+    return ld
+
+
+class W4Linear:
+    """out [T, N] = x [T, K] W^T (+ residual [T, N]) with a 4-bit W, for the tokens of a decode or
+    verification step. x in the scales' type with any row stride; products and sums are FP32 and rounded
+    once, to the type of x or not at all (out_dtype / out float32). Runs on `stream` (default: the
+    current stream of the weight's device)."""
+
+    def __init__(self, codes, scales, zeros=None, k=None, group=128):
+        if codes.dim() != 2:
+            raise ValueError(f"codes [N, ceil(K / 2)] expected, got {tuple(codes.shape)}")
+        self.w = W4Weight(codes, scales, zeros, k, group)
+
+    def __call__(self, x, out=None, residual=None, out_dtype=None, stream=None):
+        if stream is not None:
+            with mk.on_stream(x, stream):
+                return self(x, out, residual, out_dtype)
+        w = self.w
+        T = x.shape[0] if x.dim() == 2 else -1
+        shape = (T, w.n)
+        ldx = _rows(x, (T, w.k), (w.dtype,), w.device, "x")
+        ldr = 0 if residual is None else _rows(residual, shape, (w.dtype,), w.device, "residual")
+        if out is None:
+            if out_dtype is not None and out_dtype != w.dtype and out_dtype != torch.float32:
+                raise ValueError(f"out_dtype is {w.dtype} or float32, not {out_dtype}")
+            out = torch.empty(shape, dtype=out_dtype or w.dtype, device=w.device)
+            ldo = w.n
+        else:
+            if out_dtype is not None and out_dtype != out.dtype:
+                raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+            ldo = _out(out, shape, (w.dtype, torch.float32), w.device, x, residual)
+        s = mk.stream_of(x)
+        with mk.on_device_of(x):
+            rc = mk.lib().mk_w4_linear(w.ptr, x.data_ptr(), ldx, T, mk._ptr(residual), ldr, out.data_ptr(), ldo,
+                                       int(out.dtype == torch.float32), s)
+        mk._check(rc, "mk_w4_linear")
+        return out
+
+
+class W4Experts:
+    """The routed experts of a layer with 4-bit weights: out [T, H] = (residual [T, H] +) the sum over a
+    token's slots of weights[t, s] W2[e] (silu(g) u), (g, u) = W13[e] x[t], e = ids[t, s].
+
+    w13, w2: (codes, scales, zeros or None) of W13 [E, 2 I, H] (gate/up rows interleaved as
+    pack_weights packs them) and W2 [E, H, I] (`inter` = I). ids [T, S] int32 and weights [T, S] float32 as
+    route_experts returns them; a slot whose id is outside [0, E) is empty. The activation silu(g) u
+    is rounded to the type of x (the down projection's tensor-core operand), all sums are FP32. Runs on
+    `stream` (default: the current stream); the workspace comes from torch's allocator for each call,
+    so calls on several streams do not share one."""
+
+    def __init__(self, w13, w2, group=128, inter=None):
+        hidden = w2[0].shape[1] if w2[0].dim() == 3 else -1
+        if w13[0].dim() != 3 or w2[0].dim() != 3 or w13[0].shape[0] != w2[0].shape[0]:
+            raise ValueError(f"w13 [E, 2 I, H / 2] and w2 [E, H, I / 2] codes expected, got {tuple(w13[0].shape)} and {tuple(w2[0].shape)}")
+        inter = w13[0].shape[1] // 2 if inter is None else inter
+        self.w13 = W4Weight(*w13, k=hidden, group=group, gate_up=True)
+        self.w2 = W4Weight(*w2, k=inter, group=group)
+        if self.w13.n != 2 * inter or self.w13.dtype != self.w2.dtype or self.w13.device != self.w2.device:
+            raise ValueError(f"w13 has {self.w13.n} rows, {self.w13.dtype}, {self.w13.device}; w2 has rows of {inter}, {self.w2.dtype}, {self.w2.device}")
+        self.hidden = hidden
+        self._need = {}            # (T, S) -> workspace bytes
+
+    def workspace_bytes(self, T, S):
+        got = self._need.get((T, S))
+        if got is None:
+            n = ctypes.c_int64()
+            mk._check(mk.lib().mk_w4_experts_workspace(self.w13.ptr, self.w2.ptr, T, S, ctypes.byref(n)),
+                      "mk_w4_experts_workspace")
+            if len(self._need) > 4096:
+                self._need.clear()
+            got = self._need[(T, S)] = n.value
+        return got
+
+    def __call__(self, x, ids, weights, residual=None, out=None, stream=None):
+        if stream is not None:
+            with mk.on_stream(x, stream):
+                return self(x, ids, weights, residual, out)
+        w = self.w13
+        T = x.shape[0] if x.dim() == 2 else -1
+        shape = (T, self.hidden)
+        ldx = _rows(x, shape, (w.dtype,), w.device, "x")
+        ldr = 0 if residual is None else _rows(residual, shape, (w.dtype,), w.device, "residual")
+        if ids.dim() != 2 or ids.shape[0] != T or ids.dtype != torch.int32 or not ids.is_contiguous() or ids.device != w.device:
+            raise ValueError(f"ids: contiguous int32 [{T}, S] on {w.device} expected, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
+        if weights.shape != ids.shape or weights.dtype != torch.float32 or not weights.is_contiguous() or weights.device != w.device:
+            raise ValueError(f"weights: contiguous float32 {tuple(ids.shape)} on {w.device} expected, got {weights.dtype} "
+                             f"{tuple(weights.shape)} on {weights.device}")
+        if out is None:
+            out = torch.empty(shape, dtype=w.dtype, device=w.device)
+            ldo = self.hidden
+        else:
+            ldo = _out(out, shape, (w.dtype,), w.device, x, residual)
+        s = mk.stream_of(x)
+        S = ids.shape[1]
+        nbytes = self.workspace_bytes(T, S)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
+        with mk.on_device_of(x):
+            rc = mk.lib().mk_w4_experts(self.w13.ptr, self.w2.ptr, x.data_ptr(), ldx, ids.data_ptr(), weights.data_ptr(), T, S,
+                                        mk._ptr(residual), ldr, out.data_ptr(), ldo, ws.data_ptr(), nbytes, s)
+        mk._check(rc, "mk_w4_experts")
+        return out

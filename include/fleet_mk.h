@@ -329,6 +329,59 @@ int mk_mla_decode_noalloc(const void* ql_nope, const void* q_pe, const void* c_k
                           const void* w_uv, void* attn_out, int32_t nh, int32_t d_c, int32_t d_r, int32_t d_v,
                           int32_t pos, int32_t split, float softmax_scale, void* stream);
 
+/* ---- Serving a batch of sequences with 4-bit weights (no counterpart in the reference, whose path
+   decodes one sequence in BF16). Each call launches its kernels on `stream` and returns; nothing is
+   allocated, so the calls may be captured in a CUDA graph. Tensors are on the current device.
+   ---- */
+
+/* Routing of t tokens to experts (csrc/mk_route.cu has the formulas and the rules for ties, -inf and
+   NaN). logits [t, experts] with row stride ld (elements; 0: one row for every token). bias [experts]
+   FP32 or NULL is added to the scores for the selection only. ids [t, topk + n_forced] int32 and
+   weights [t, topk + n_forced] FP32, contiguous: the topk experts in descending order, then the
+   always-selected experts `experts`, `experts` + 1, ... with weight 1 (shared experts folded in).
+   Limits: experts <= 512, topk <= 32, n_group <= 32, n_forced <= 32. */
+#define MK_ROUTE_SOFTMAX 0
+#define MK_ROUTE_SIGMOID 1
+#define MK_ROUTE_FP32 0
+#define MK_ROUTE_BF16 1
+typedef struct MkRoute {
+  int32_t experts, topk, n_forced;
+  int32_t n_group, topk_group;   /* 1, 1: no groups */
+  int32_t group_top2;            /* a group's score: 0 its largest, 1 the sum of its two largest */
+  int32_t score;                 /* MK_ROUTE_SOFTMAX or MK_ROUTE_SIGMOID */
+  int32_t renormalize;           /* divide the topk weights by their sum */
+  int32_t logits_dtype;          /* MK_ROUTE_FP32 or MK_ROUTE_BF16 */
+  float scaling;                 /* the topk weights' factor */
+} MkRoute;
+int mk_route(const MkRoute* r, const void* logits, int64_t ld, int32_t t, const float* bias, int32_t* ids,
+             float* weights, void* stream);
+
+/* A laid-out 4-bit weight [experts, n, k] (csrc/mk_w4.cuh has the format and the order; fleet/w4.py
+   lay_out makes it). scales have the activations' type. */
+#define MK_W4_BF16 0
+#define MK_W4_FP16 1
+typedef struct MkW4 {
+  const void* codes;     /* 16-byte aligned */
+  const void* scales;
+  const void* zeros;     /* or NULL: 8 */
+  int32_t n, k, group, dtype, experts;
+  int32_t reserved;
+} MkW4;
+/* out [t, n] = x [t, k] W^T (+ residual [t, n]), each with its row stride in elements; x, residual in
+   w->dtype, out in w->dtype or (out_f32) FP32. out may be residual; it may not overlap x. */
+int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t, const void* residual, int64_t ldr, void* out,
+                 int64_t ldo, int32_t out_f32, void* stream);
+/* The routed experts of a layer: out [t, H] = (residual [t, H] +) sum over the slots s of a token of
+   weights[t, s] W2[e] (silu(g) u), (g, u) = W13[e] x [t, H], e = ids[t, s]. w13 [E, 2 I, H] with each
+   of its tiles holding 8 gate rows, then their 8 up rows (lay_out(..., gate_up=True)); w2 [E, H, I].
+   ids [t, slots] int32 and weights [t, slots] FP32, contiguous; a slot whose id is outside [0, E) is
+   empty. The workspace (mk_w4_experts_workspace bytes, 256-byte aligned) holds nothing between
+   calls; calls that overlap on the GPU need one each. */
+int mk_w4_experts_workspace(const MkW4* w13, const MkW4* w2, int32_t t, int32_t slots, int64_t* bytes);
+int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int64_t ldx, const int32_t* ids, const float* weights,
+                  int32_t t, int32_t slots, const void* residual, int64_t ldr, void* out, int64_t ldo, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
