@@ -15,8 +15,8 @@
 // One kernel, three modes. The work is a list of items (a block of at most 8 NT columns that share a
 // weight: the linear's token blocks; an expert and up to 8 NT of the slots routed to it) times the
 // weight's tiles; each CTA (one per SM, 16 warps) takes an equal contiguous range of that product. A
-// team of kw warps owns a tile and splits its chunks; each warp streams its chunks through its own
-// cp.async ring (DEPTH - 1 chunks in flight, across tile and item boundaries), so no barrier stands
+// team of kw warps owns a tile and splits its units; each warp streams its units through its own
+// cp.async ring (DEPTH - 1 units of 128 values in flight, across tile and item boundaries), so no barrier stands
 // between the copies and the MMAs. The item's activations are staged in shared memory in the MMA's
 // order. A tile's partial sums meet in shared memory and are added in warp order: the result does
 // not depend on timing.
@@ -35,17 +35,19 @@ using namespace w4;
 namespace {
 
 constexpr int WARPS = 16, THREADS = WARPS * 32;
-constexpr int STAGE_BYTES = CHUNK_BYTES + 64 + 32;   // codes, up to two groups' scales, their zero points
 constexpr int RED_STRIDE = 20;                       // floats per column of a tile's partial sums (16 + 4: no conflicts)
 constexpr int SMEM_LIMIT = 227 * 1024;
 constexpr int MAX_EXPERTS = 1024;
 enum Mode { LINEAR = 0, GATEUP = 1, DOWN = 2 };
 
-template <int NT>
+// shared memory: the warps' rings, the partial sums, the activations
+template <int NT, int G, bool ZP>
 struct Shape {
-  static constexpr int DEPTH = NT <= 2 ? 8 : 4;
-  static constexpr int RING = WARPS * DEPTH * STAGE_BYTES;
-  static constexpr int RED = WARPS * NT * 8 * RED_STRIDE * 4;
+  static constexpr int GROUPS = UNIT_K / G;          // per unit
+  static constexpr int STAGE = UNIT_BYTES + GROUPS * (ZP ? 48 : 32);
+  static constexpr int DEPTH = NT <= 2 ? 6 : 4;      // stages a warp
+  static constexpr int RING = WARPS * DEPTH * STAGE;
+  static constexpr int RED = WARPS * 8 * RED_STRIDE * 4;
   static constexpr int FIXED = RING + RED;
 };
 
@@ -53,13 +55,15 @@ struct Args {
   const uint8_t* codes;
   const uint8_t* scales;
   const uint8_t* zeros;     // or null: 8
-  int tiles, chunks, groups, gshift, rows, k;
+  int tiles, units, rows, k;
+  int mode;
   int n_items;              // LINEAR: known on the host; else *items_n
   const int* items_n;
   const int4* items;        // {expert, first column, columns, 0}
   const int* col_token;     // GATEUP: the token of a column
   int t, tb;                // LINEAR: tokens, tokens per item
   int kw;                   // warps per team
+  int ks;                   // CTAs (of one cluster) that split K
   const uint16_t* x;
   int64_t ldx;
   int x_vec;                // x rows may be read 16 bytes at a time
@@ -75,92 +79,109 @@ __device__ __forceinline__ void team_sync(int team, int kw) {
   if (kw == 1) __syncwarp();
   else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(kw * 32) : "memory");
 }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the float at the same shared-memory place in the cluster's CTA `rank`
+__device__ __forceinline__ float peer_float(const float* p, int rank) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(p);
+  uint32_t there;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+  return v;
+}
 
-// the item's activations in the MMA's order: [K / 32][columns][4] 16-byte vectors
-template <int MODE>
-__device__ __forceinline__ void stage_x(const Args& a, uint4* xs, int start, int count) {
-  const int nv = a.chunks * 8;
+// the item's activations [8 v0, 8 v1) in the MMA's order: [(v - v0) / 4][columns][4] 16-byte vectors
+__device__ __forceinline__ void stage_x(const Args& a, uint4* xs, int start, int count, int v0, int v1) {
+  const int nv = v1 - v0;
+  const uint32_t xs_s = (uint32_t)__cvta_generic_to_shared(xs);
   for (int i = threadIdx.x; i < count * nv; i += THREADS) {
-    const int col = i / nv, v = i - col * nv;
-    const int row = MODE == GATEUP ? a.col_token[start + col] : start + col;
+    const int col = i / nv, r = i - col * nv, v = v0 + r;
+    const int row = a.mode == GATEUP ? a.col_token[start + col] : start + col;
     const uint16_t* src = a.x + (int64_t)row * a.ldx + 8 * v;
-    uint4 d;
+    const int at = ((r >> 2) * count + col) * 4 + (r & 3);
     if (a.x_vec && 8 * v + 8 <= a.k) {
-      d = *reinterpret_cast<const uint4*>(src);
+      cp16(xs_s + at * 16, src);
     } else {
       uint32_t h[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) h[j] = 8 * v + j < a.k ? (uint32_t)src[j] : 0u;
-      d = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+      xs[at] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
     }
-    xs[((v >> 2) * count + col) * 4 + (v & 3)] = d;
   }
 }
 
-template <class D, int NT, bool HALF, int MODE>
+template <class D, int NT, int G, bool ZP>
 __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const Args a) {
-  constexpr int DEPTH = Shape<NT>::DEPTH;
+  using S = Shape<NT, G, ZP>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * (DEPTH * STAGE_BYTES);
-  float* red = reinterpret_cast<float*>(smem + Shape<NT>::RING);
-  uint4* xs = reinterpret_cast<uint4*>(smem + Shape<NT>::FIXED);
+  uint8_t* ring = smem + warp * (S::DEPTH * S::STAGE);
+  float* red = reinterpret_cast<float*>(smem + S::RING);
+  uint4* xs = reinterpret_cast<uint4*>(smem + S::FIXED);
   const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
 
-  const int n_items = MODE == LINEAR ? a.n_items : *a.items_n;
-  const int64_t total = (int64_t)n_items * a.tiles;
-  const int64_t lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
+  const int n_items = a.mode == LINEAR ? a.n_items : *a.items_n;
+  const int64_t total = (int64_t)n_items * a.tiles;   // below 2^31
+  const int ks = a.ks, rank = blockIdx.x % ks, group = blockIdx.x / ks, n_groups = gridDim.x / ks;
+  const int lo = (int)(total * group / n_groups), hi = (int)(total * (group + 1) / n_groups);
   const int kw = a.kw, teams = WARPS / kw, team = warp / kw, part = warp - team * kw;
+  const int u0 = a.units * rank / ks, u1 = a.units * (rank + 1) / ks;
+  const int n_units = max(0, (u1 - u0 - part + kw - 1) / kw);   // this warp's units of a tile
 
   // the copy cursor: the team's tiles of each segment (the part of the range within one item)
-  int64_t c_f, c_end;
-  int c_chunk = part;
-  const uint8_t *c_codes = nullptr, *c_scales = nullptr, *c_zeros = nullptr;
-  auto at_segment = [&](int64_t from) {
-    const int item = (int)(from / a.tiles);
-    c_end = min(hi, (int64_t)(item + 1) * a.tiles);
-    c_f = from + team;
-    const int64_t e = MODE == LINEAR ? 0 : a.items[item].x;
-    // base so that tile f - item * tiles is at f
-    const int64_t tile0 = (e - item) * a.tiles;
-    c_codes = a.codes + tile0 * a.chunks * CHUNK_BYTES;
-    c_scales = a.scales + tile0 * a.groups * 32;
-    c_zeros = a.zeros ? a.zeros + tile0 * a.groups * 16 : nullptr;
+  int c_f = 0, c_end = 0, c_left = 0;
+  int c_tile0 = 0;                         // from a flat tile number to the tile of the item's weight
+  const uint8_t *c_code = nullptr, *c_meta = nullptr;
+  // lanes 0.. carry the scales' 16-byte pieces, lanes 16.. the zero points'
+  const bool scale_lane = lane < 2 * S::GROUPS, zero_lane = ZP && lane >= 16 && lane < 16 + S::GROUPS;
+  const int meta_unit = scale_lane ? S::GROUPS * 32 : S::GROUPS * 16;
+  const uint32_t meta_at = UNIT_BYTES + (scale_lane ? lane * 16 : S::GROUPS * 32 + (lane - 16) * 16);
+  auto at_tile = [&]() {
+    const int64_t first = (int64_t)(c_f + c_tile0) * a.units + u0 + part;
+    c_code = a.codes + first * UNIT_BYTES + lane * 16;
+    if (scale_lane) c_meta = a.scales + first * (S::GROUPS * 32) + lane * 16;
+    else if (zero_lane) c_meta = a.zeros + first * (S::GROUPS * 16) + (lane - 16) * 16;
+    c_left = n_units;
   };
-  bool more = lo < hi && part < a.chunks;
-  if (more) {
-    at_segment(lo);
+  auto at_segment = [&](int from) {
+    const int item = from / a.tiles;
+    c_end = min(hi, (item + 1) * a.tiles);
+    c_f = from + team;
+    c_tile0 = ((a.mode == LINEAR ? 0 : a.items[item].x) - item) * a.tiles;
+  };
+  auto skip_empty = [&]() {
     while (c_f >= c_end && c_end < hi) at_segment(c_end);
-    more = c_f < c_end;
+    if (c_f < c_end) at_tile();
+  };
+  if (lo < hi && n_units > 0) {
+    at_segment(lo);
+    skip_empty();
   }
-  auto issue = [&](int slot) {
-    if (more) {
-      const uint32_t dst = ring_s + slot * STAGE_BYTES;
-      cp16(dst + lane * 16, c_codes + (c_f * a.chunks + c_chunk) * CHUNK_BYTES + lane * 16);
-      const int64_t grp = c_f * a.groups + ((c_chunk * CHUNK_K) >> a.gshift);
-      if (lane < (HALF ? 16 : 8))
-        cp4(dst + CHUNK_BYTES + lane * 4, c_scales + grp * 32 + lane * 4);
-      else if (a.zeros && lane >= 16 && lane < (HALF ? 24 : 20))
-        cp4(dst + CHUNK_BYTES + 64 + (lane - 16) * 4, c_zeros + grp * 16 + (lane - 16) * 4);
-      c_chunk += kw;
-      if (c_chunk >= a.chunks) {
-        c_chunk = part;
+  auto issue = [&](uint32_t dst) {
+    if (c_left > 0) {
+      cp16(dst + lane * 16, c_code);
+      cp16(dst + 512 + lane * 16, c_code + 512);
+      if (scale_lane || zero_lane) cp16(dst + meta_at, c_meta);
+      c_code += kw * UNIT_BYTES;
+      c_meta += kw * meta_unit;
+      if (--c_left == 0) {
         c_f += teams;
-        while (c_f >= c_end && c_end < hi) at_segment(c_end);
-        more = c_f < c_end;
+        skip_empty();
       }
     }
     cp_commit();
   };
 #pragma unroll
-  for (int s = 0; s < DEPTH - 1; ++s) issue(s);
+  for (int s = 0; s < S::DEPTH - 1; ++s) issue(ring_s + s * S::STAGE);
 
-  int slot = 0;
-  for (int64_t seg = lo; seg < hi;) {
-    const int item = (int)(seg / a.tiles);
-    const int64_t seg_end = min(hi, (int64_t)(item + 1) * a.tiles);
+  uint32_t slot = 0, freed = (S::DEPTH - 1) * S::STAGE;   // the stage to read, the stage read before it
+  for (int seg = lo; seg < hi;) {
+    const int item = seg / a.tiles;
+    const int seg_end = min(hi, (item + 1) * a.tiles);
     int start, count;
-    if (MODE == LINEAR) {
+    if (a.mode == LINEAR) {
       start = item * a.tb;
       count = min(a.tb, a.t - start);
     } else {
@@ -169,74 +190,113 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const Args a) {
       count = it.z;
     }
     __syncthreads();   // every warp is done with the last item's activations
-    stage_x<MODE>(a, xs, start, count);
+    stage_x(a, xs, start, count, u0 * 16, u1 * 16);
+    cp_commit();
+    cp_wait<0>();
     __syncthreads();
-    for (int64_t f = seg + team; f < seg_end; f += teams) {
-      float tot[NT][4], acc[NT][4];
+    // a lane past the columns reads the last one's activations: its sums are not used
+    const uint4* xl[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) xl[n] = xs + (part * 4 * count + min(n * 8 + g, count - 1)) * 4 + t;
+    for (int first = seg; first < seg_end; first += teams) {
+      const int f = first + team;
+      const bool live = f < seg_end;
+      if (!live && ks == 1) break;
+      float tot[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tot[n][i] = acc[n][i] = 0.0f;
-      for (int c = part; c < a.chunks; c += kw) {
-        cp_wait<DEPTH - 2>();
+        for (int i = 0; i < 4; ++i) tot[n][i] = 0.0f;
+      int x_at = 0;
+      for (int u = live ? n_units : 0; u > 0; --u) {
+        cp_wait<S::DEPTH - 2>();
         __syncwarp();
-        const uint8_t* st = ring + slot * STAGE_BYTES;
-        const uint4 w = *reinterpret_cast<const uint4*>(st + lane * 16);
-        uint32_t sc[HALF ? 2 : 1], z0[HALF ? 2 : 1], z1[HALF ? 2 : 1];
+        const uint8_t* st = ring + slot;
+        const uint4 w0 = *reinterpret_cast<const uint4*>(st + lane * 16);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(st + 512 + lane * 16);
+        uint32_t sc[S::GROUPS], z0[S::GROUPS], z1[S::GROUPS];
 #pragma unroll
-        for (int h = 0; h < (HALF ? 2 : 1); ++h) {
-          sc[h] = *reinterpret_cast<const uint32_t*>(st + CHUNK_BYTES + h * 32 + g * 4);
-          const uint32_t z = a.zeros ? *reinterpret_cast<const uint16_t*>(st + CHUNK_BYTES + 64 + h * 16 + g * 2) : 0x0808u;
-          z0[h] = (z & 0xFFu) * 0x00010001u | D::MAGIC;
-          z1[h] = (z >> 8) * 0x00010001u | D::MAGIC;
+        for (int i = 0; i < S::GROUPS; ++i) {
+          sc[i] = *reinterpret_cast<const uint32_t*>(st + UNIT_BYTES + i * 32 + g * 4);
+          if (ZP) {
+            const uint32_t z = *reinterpret_cast<const uint16_t*>(st + UNIT_BYTES + S::GROUPS * 32 + i * 16 + g * 2);
+            z0[i] = (z & 0xFFu) * 0x00010001u | D::MAGIC;
+            z1[i] = (z >> 8) * 0x00010001u | D::MAGIC;
+          } else {
+            z0[i] = z1[i] = D::MAGIC + 0x00080008u;
+          }
         }
-        issue(slot == 0 ? DEPTH - 1 : slot - 1);
-        slot = slot == DEPTH - 1 ? 0 : slot + 1;
+        issue(ring_s + freed);
+        freed = slot;
+        slot = slot == (S::DEPTH - 1) * S::STAGE ? 0 : slot + S::STAGE;
+        float acc[NT][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 4; ++h) {
           uint4 xb[NT];
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-            xb[n] = n * 8 + g < count ? xs[((2 * c + h) * count + n * 8 + g) * 4 + t] : make_uint4(0, 0, 0, 0);
-          half_chunk<D, NT>(h ? w.z : w.x, h ? w.w : w.y, z0[HALF ? h : 0], z1[HALF ? h : 0], xb, acc);
-          if (HALF || h == 1) fold<D, NT>(sc[HALF ? h : 0], acc, tot);
+          for (int n = 0; n < NT; ++n) xb[n] = xl[n][x_at + h * count * 4];
+          const uint4& w = h < 2 ? w0 : w1;
+          const int i = h * 32 / G;
+          if (h * 32 % G == 0) half_chunk<D, NT, true>(h & 1 ? w.z : w.x, h & 1 ? w.w : w.y, z0[i], z1[i], xb, acc);
+          else half_chunk<D, NT, false>(h & 1 ? w.z : w.x, h & 1 ? w.w : w.y, z0[i], z1[i], xb, acc);
+          if ((h + 1) * 32 % G == 0) fold<D, NT>(sc[i], acc, tot);
         }
+        x_at += kw * count * 16;
       }
-      // the team's partial sums, [column][row], added in warp order
-      float* mine = red + warp * (NT * 8 * RED_STRIDE);
+      // the team's partial sums, [column][row], eight columns at a time, added in warp order
+      constexpr int RED_WARP = 8 * RED_STRIDE;
+      float* mine = red + warp * RED_WARP;
+      float* theirs = red + team * kw * RED_WARP;
+      const int row0 = (f - item * a.tiles) * TILE_ROWS, me = part * 32 + lane;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        const int cols = min(count - n * 8, 8);
+        if (cols <= 0) break;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine[(n * 8 + 2 * t + (i & 1)) * RED_STRIDE + g + (i >> 1) * 8] = tot[n][i];
-      team_sync(team, kw);
-      const float* theirs = red + team * kw * (NT * 8 * RED_STRIDE);
-      const int row0 = (int)(f - (int64_t)item * a.tiles) * TILE_ROWS, me = part * 32 + lane;
-      if (MODE == GATEUP) {   // tile rows 0..7 are gate rows, 8..15 their up rows
-        for (int i = me; i < count * 8; i += kw * 32) {
-          const int col = i >> 3, r = i & 7, j = row0 / 2 + r;
-          float gt = 0.0f, up = 0.0f;
-          for (int w = 0; w < kw; ++w) {
-            gt += theirs[w * (NT * 8 * RED_STRIDE) + col * RED_STRIDE + r];
-            up += theirs[w * (NT * 8 * RED_STRIDE) + col * RED_STRIDE + r + 8];
+        for (int i = 0; i < 4; ++i) mine[(2 * t + (i & 1)) * RED_STRIDE + g + (i >> 1) * 8] = tot[n][i];
+        team_sync(team, kw);
+        if (a.mode == GATEUP) {   // tile rows 0..7 are gate rows, 8..15 their up rows
+          for (int i = me; i < cols * 8; i += kw * 32) {
+            const int col = i >> 3, r = i & 7, j = row0 / 2 + r;
+            float gt = 0.0f, up = 0.0f;
+            for (int w = 0; w < kw; ++w) {
+              gt += theirs[w * RED_WARP + col * RED_STRIDE + r];
+              up += theirs[w * RED_WARP + col * RED_STRIDE + r + 8];
+            }
+            // rounded to the activations' type: the down projection's tensor-core operand
+            if (j < a.rows / 2)
+              static_cast<uint16_t*>(a.out)[(int64_t)(start + n * 8 + col) * a.ldo + j] =
+                  D::round(__fdiv_rn(gt, 1.0f + expf(-gt)) * up);
           }
-          // rounded to the activations' type: the down projection's tensor-core operand
-          if (j < a.rows / 2)
-            static_cast<uint16_t*>(a.out)[(int64_t)(start + col) * a.ldo + j] =
-                D::round(__fdiv_rn(gt, 1.0f + expf(-gt)) * up);
+        } else {
+          auto store = [&](int col, int r, float v) {
+            const int64_t row = start + n * 8 + col, o = row * a.ldo + row0 + r;
+            if (row0 + r >= a.rows) return;
+            if (a.residual) v += D::one_to_f32(a.residual[row * a.ldr + row0 + r]);
+            if (a.out_f32) static_cast<float*>(a.out)[o] = v;
+            else static_cast<uint16_t*>(a.out)[o] = D::round(v);
+          };
+          for (int i = me; i < cols * 16; i += kw * 32) {
+            const int col = i >> 4, r = i & 15;
+            float v = 0.0f;
+            for (int w = 0; w < kw; ++w) v += theirs[w * RED_WARP + col * RED_STRIDE + r];
+            if (ks > 1) theirs[col * RED_STRIDE + r] = v;   // this thread's own place: the CTA's sum for the cluster
+            else store(col, r, v);
+          }
+          if (ks > 1) {   // K is split over the cluster: each CTA adds and stores the columns col % ks == rank
+            cluster_sync();
+            for (int i = me; i < cols * 16; i += kw * 32) {
+              const int col = i >> 4, r = i & 15;
+              if (col % ks != rank || !live) continue;
+              float v = 0.0f;
+              for (int c = 0; c < ks; ++c) v += peer_float(theirs + col * RED_STRIDE + r, c);
+              store(col, r, v);
+            }
+            cluster_sync();
+          }
         }
-      } else {
-        for (int i = me; i < count * 16; i += kw * 32) {
-          const int col = i >> 4, r = i & 15, n = row0 + r;
-          if (n >= a.rows) continue;
-          float v = 0.0f;
-          for (int w = 0; w < kw; ++w) v += theirs[w * (NT * 8 * RED_STRIDE) + col * RED_STRIDE + r];
-          const int64_t o = (int64_t)(start + col) * a.ldo + n;
-          if (MODE == LINEAR && a.residual) v += D::one_to_f32(a.residual[(int64_t)(start + col) * a.ldr + n]);
-          if (MODE == DOWN || a.out_f32) static_cast<float*>(a.out)[o] = v;
-          else static_cast<uint16_t*>(a.out)[o] = D::round(v);
-        }
+        team_sync(team, kw);   // the sums are read before the next ones are written
       }
-      team_sync(team, kw);   // the sums are read before the next tile's are written
     }
     seg = seg_end;
   }
@@ -305,15 +365,13 @@ __global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ 
 
 int fail(int code, const char* msg) { return mk::set_last_error(code, msg); }
 
-int gshift_of(int group) { return group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : -1; }
-
 const char* bad_weight(const MkW4* w) {
   if (!w || !w->codes || !w->scales) return "null 4-bit weight";
   if (w->n < 1 || w->k < 1 || w->experts < 1) return "a 4-bit weight has at least one row, value and expert";
-  if (gshift_of(w->group) < 0) return "the group size is 32, 64 or 128";
+  if (w->group != 32 && w->group != 64 && w->group != 128) return "the group size is 32, 64 or 128";
   if (w->dtype != MK_W4_BF16 && w->dtype != MK_W4_FP16) return "the activations are BF16 or FP16";
-  if (((uintptr_t)w->codes & 15) || ((uintptr_t)w->scales & 3) || ((uintptr_t)w->zeros & 3))
-    return "laid-out codes start at a 16-byte boundary, scales and zeros at a 4-byte one";
+  if (((uintptr_t)w->codes & 15) || ((uintptr_t)w->scales & 15) || ((uintptr_t)w->zeros & 15))
+    return "laid-out codes, scales and zeros start at 16-byte boundaries";
   return nullptr;
 }
 
@@ -322,19 +380,22 @@ void fill(Args& a, const MkW4* w) {
   a.scales = static_cast<const uint8_t*>(w->scales);
   a.zeros = static_cast<const uint8_t*>(w->zeros);
   a.tiles = (w->n + TILE_ROWS - 1) / TILE_ROWS;
-  a.chunks = (w->k + CHUNK_K - 1) / CHUNK_K;
-  a.gshift = gshift_of(w->group);
-  a.groups = (a.chunks * CHUNK_K + w->group - 1) >> a.gshift;
+  a.units = (w->k + UNIT_K - 1) / UNIT_K;
+  a.ks = 1;
   a.rows = w->n;
   a.k = w->k;
 }
 
-// columns of K values that fit beside the ring (at most 32): 128 bytes per column and chunk
-int columns_that_fit(int chunks, int want) {
-  const int per = chunks * CHUNK_K * 2;
+// shared memory beside the activations, for the group size and zero points that take most
+int fixed_bytes(int nt) {
+  return nt == 1 ? Shape<1, 32, true>::FIXED : nt == 2 ? Shape<2, 32, true>::FIXED : Shape<4, 32, true>::FIXED;
+}
+
+// columns (at most `want`, at most 32) whose activations of `units` units fit
+int columns_that_fit(int units, int want) {
+  const int per = units * UNIT_K * 2;
   for (int nt = want <= 8 ? 1 : want <= 16 ? 2 : 4;; nt /= 2) {
-    const int fixed = nt == 1 ? Shape<1>::FIXED : nt == 2 ? Shape<2>::FIXED : Shape<4>::FIXED;
-    const int fit = std::min({(SMEM_LIMIT - fixed) / per, nt * 8, want});
+    const int fit = std::min({(SMEM_LIMIT - fixed_bytes(nt)) / per, nt * 8, want});
     if (fit > nt * 4 || nt == 1) return fit;
   }
 }
@@ -360,39 +421,43 @@ int device_sms(int* sms) {
   return MK_OK;
 }
 
-template <class D, int NT, bool HALF, int MODE>
+template <class D, int NT, int G, bool ZP>
 int launch(const Args& a, int grid, cudaStream_t s) {
-  const int smem = Shape<NT>::FIXED + a.tb * a.chunks * CHUNK_K * 2;
-  cudaError_t e = cudaFuncSetAttribute(w4_kernel<D, NT, HALF, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
-  if (e == cudaSuccess) {
-    w4_kernel<D, NT, HALF, MODE><<<grid, THREADS, smem, s>>>(a);
-    e = cudaGetLastError();
-  }
+  cudaLaunchConfig_t c{};
+  cudaLaunchAttribute cluster[1];
+  c.gridDim = dim3((unsigned)grid);
+  c.blockDim = dim3(THREADS);
+  c.dynamicSmemBytes = Shape<NT, G, ZP>::FIXED + (size_t)a.tb * ((a.units + a.ks - 1) / a.ks) * UNIT_K * 2;
+  c.stream = s;
+  cluster[0].id = cudaLaunchAttributeClusterDimension;
+  cluster[0].val.clusterDim = {(unsigned)a.ks, 1, 1};
+  c.attrs = cluster;
+  c.numAttrs = 1;
+  cudaError_t e = cudaFuncSetAttribute(w4_kernel<D, NT, G, ZP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&c, w4_kernel<D, NT, G, ZP>, a);
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
 }
 
-template <int MODE>
-int launch_mode(const Args& a, int dtype, int grid, cudaStream_t s) {
+template <class D, int NT>
+int launch_group(const Args& a, int group, int grid, cudaStream_t s) {
+  if (group == 32) return a.zeros ? launch<D, NT, 32, true>(a, grid, s) : launch<D, NT, 32, false>(a, grid, s);
+  if (group == 64) return a.zeros ? launch<D, NT, 64, true>(a, grid, s) : launch<D, NT, 64, false>(a, grid, s);
+  return a.zeros ? launch<D, NT, 128, true>(a, grid, s) : launch<D, NT, 128, false>(a, grid, s);
+}
+
+int launch_weight(const Args& a, const MkW4* w, int grid, cudaStream_t s) {
   const int nt = a.tb <= 8 ? 1 : a.tb <= 16 ? 2 : 4;
-  const bool half = a.gshift == 5;
-#define W4_CASE(D, NT, HALF) return launch<D, NT, HALF, MODE>(a, grid, s)
-#define W4_NT(D, HALF)                     \
-  if (nt == 1) W4_CASE(D, 1, HALF);        \
-  else if (nt == 2) W4_CASE(D, 2, HALF);   \
-  else W4_CASE(D, 4, HALF)
-  if (dtype == MK_W4_BF16) {
-    if (half) { W4_NT(Bf16, true); } else { W4_NT(Bf16, false); }
-  } else {
-    if (half) { W4_NT(Fp16, true); } else { W4_NT(Fp16, false); }
-  }
-#undef W4_NT
-#undef W4_CASE
+  if (w->dtype == MK_W4_BF16)
+    return nt == 1 ? launch_group<Bf16, 1>(a, w->group, grid, s) : nt == 2 ? launch_group<Bf16, 2>(a, w->group, grid, s)
+                                                                          : launch_group<Bf16, 4>(a, w->group, grid, s);
+  return nt == 1 ? launch_group<Fp16, 1>(a, w->group, grid, s) : nt == 2 ? launch_group<Fp16, 2>(a, w->group, grid, s)
+                                                                        : launch_group<Fp16, 4>(a, w->group, grid, s);
 }
 
 // warps per tile: few tiles are split over many warps, many are left to few
-int team_warps(int64_t tiles, int chunks, int grid) {
+int team_warps(int64_t tiles, int units, int grid) {
   int kw = 16;
-  while (kw > 1 && (kw > chunks || tiles > (int64_t)grid * (WARPS / kw) * 4)) kw /= 2;
+  while (kw > 1 && (kw > units || tiles > (int64_t)grid * (WARPS / kw) * 8)) kw /= 2;
   return kw;
 }
 
@@ -409,14 +474,17 @@ const char* plan_experts(const MkW4* w13, const MkW4* w2, int64_t t, int64_t s, 
   if (w13->dtype != w2->dtype || w13->experts != w2->experts || w13->n % 2 || w13->n / 2 != w2->k || w13->k != w2->n)
     return "W13 [E, 2 I, H] and W2 [E, H, I] do not belong together";
   if (w13->experts > MAX_EXPERTS) return "at most 1024 experts";
+  const int64_t tiles = std::max((w13->n + TILE_ROWS - 1) / TILE_ROWS, (w2->n + TILE_ROWS - 1) / TILE_ROWS);
+  if (w13->experts * tiles > INT32_MAX / 2) return "too many experts times rows";
   if (t < 0 || s < 0 || t * s >= (1 << 24)) return "slots (tokens x slots per token) are from 0 to 2^24 - 1";
   const int want = t >= 32 ? 32 : (int)std::max<int64_t>(t, 1);
-  p->tb1 = columns_that_fit((w13->k + CHUNK_K - 1) / CHUNK_K, want);
-  p->tb2 = columns_that_fit((w2->k + CHUNK_K - 1) / CHUNK_K, want);
+  p->tb1 = columns_that_fit((w13->k + UNIT_K - 1) / UNIT_K, want);
+  p->tb2 = columns_that_fit((w2->k + UNIT_K - 1) / UNIT_K, want);
   if (p->tb1 < 1 || p->tb2 < 1) return "rows are too long for the shared memory";
   p->tb1 = p->tb2 = std::min(p->tb1, p->tb2);
   p->ldact = (w2->k + 7) / 8 * 8;
   const int64_t n = std::max<int64_t>(t * s, 1);
+  if ((w13->experts + n / p->tb1 + 1) * tiles > INT32_MAX - 4096) return "too many slots times rows";
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t r = at; at += (bytes + 255) / 256 * 256; return r; };
   p->items_n = take(4);
@@ -445,7 +513,10 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   Args a{};
   fill(a, w);
   a.t = t;
-  a.tb = columns_that_fit(a.chunks, std::min(t, 32));
+  // split K over a cluster while the tokens' activations do not fit one CTA's shared memory
+  const int want = std::min(t, 32);
+  for (a.ks = 1; a.ks < 8 && columns_that_fit((a.units + a.ks - 1) / a.ks, want) < want; a.ks *= 2) {}
+  a.tb = columns_that_fit((a.units + a.ks - 1) / a.ks, want);
   if (a.tb < 1) return fail(MK_EINVAL, "rows are too long for the shared memory");
   a.n_items = (t + a.tb - 1) / a.tb;
   a.x = static_cast<const uint16_t*>(x);
@@ -457,9 +528,10 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   a.ldo = ldo;
   a.out_f32 = out_f32;
   const int64_t total = (int64_t)a.n_items * a.tiles;
-  const int grid = (int)std::min<int64_t>(sms, total);
-  a.kw = team_warps(total, a.chunks, grid);
-  return launch_mode<LINEAR>(a, w->dtype, grid, static_cast<cudaStream_t>(stream));
+  if (total > INT32_MAX - 4096) return fail(MK_EINVAL, "too many tokens times rows");
+  const int groups = (int)std::min<int64_t>(sms / a.ks, total);
+  a.kw = team_warps(total, a.units / a.ks, groups);
+  return launch_weight(a, w, groups * a.ks, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mk_w4_experts_workspace(const MkW4* w13, const MkW4* w2, int32_t t, int32_t slots, int64_t* bytes) {
@@ -502,8 +574,9 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   a.x_vec = aligned16(x, ldx);
   a.out = ws + p.act;
   a.ldo = p.ldact;
-  a.kw = team_warps(items_about * a.tiles, a.chunks, sms);
-  if (int rc = launch_mode<GATEUP>(a, w13->dtype, sms, st)) return rc;
+  a.kw = team_warps(items_about * a.tiles, a.units, sms);
+  a.mode = GATEUP;
+  if (int rc = launch_weight(a, w13, sms, st)) return rc;
   Args b{};
   fill(b, w2);
   b.items = items;
@@ -514,8 +587,10 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   b.x_vec = 1;
   b.out = ws + p.y;
   b.ldo = w2->n;
-  b.kw = team_warps(items_about * b.tiles, b.chunks, sms);
-  if (int rc = launch_mode<DOWN>(b, w2->dtype, sms, st)) return rc;
+  b.out_f32 = 1;
+  b.mode = DOWN;
+  b.kw = team_warps(items_about * b.tiles, b.units, sms);
+  if (int rc = launch_weight(b, w2, sms, st)) return rc;
   const dim3 grid((unsigned)((w2->n + 255) / 256), (unsigned)t);
   const float* y = reinterpret_cast<const float*>(ws + p.y);
   if (w2->dtype == MK_W4_BF16)

@@ -9,17 +9,18 @@
 //
 // The laid-out form (fleet/w4.py lay_out) is the order in which the lanes of a warp want the codes
 // for mma.sync m16n8k16 with the weights as the 16-row operand and the tokens as its 8 columns:
-//   codes  [experts][tiles][chunks][32 lanes][4 words]: a tile is 16 rows, a chunk 64 values of K.
-//          lane 4 g + t, word 2 h + j (h, j in 0..1) holds rows g and g + 8 at the four values
-//          k = 64 chunk + 32 h + 8 t + 4 j + (0..3): bits 4i..4i+3 (k even) and 16+4i.. (k odd) are,
-//          for i = 0..3, (row g, k 0/1), (row g + 8, k 0/1), (row g, k 2/3), (row g + 8, k 2/3):
-//          the four A registers of one MMA, two codes each, one AND and OR apart from a 16-bit float
-//   scales [experts][tiles][groups][8][2]: rows g and g + 8 side by side (one 32-bit load a lane)
+//   codes  [experts][tiles][units][2 chunks][32 lanes][4 words]: a tile is 16 rows, a unit 128 values
+//          of K in two chunks of 64. Lane 4 g + t, word 2 h + j (h, j in 0..1) holds rows g and g + 8
+//          at the four values k = 64 chunk + 32 h + 8 t + 4 j + (0..3): bits 4i..4i+3 (k even) and
+//          16+4i.. (k odd) are, for i = 0..3, (row g, k 0/1), (row g + 8, k 0/1), (row g, k 2/3),
+//          (row g + 8, k 2/3): the four A registers of one MMA, two codes each, a shift and one
+//          AND-OR from a 16-bit float
+//   scales [experts][tiles][128 units / G groups][8][2]: rows g and g + 8 side by side (one 32-bit load)
 //   zeros  [experts][tiles][groups][8][2] bytes, or none
-// The MMA's k slots are a permutation of the 64 values (lane t of a quad has 8 consecutive ones of
-// each 32), the same one for the activations: a sum does not ask for their order, and a lane's share
-// of the activations is then one 16-byte load per 32 values. Rows and K are padded to whole tiles
-// and chunks with scale 0 and activations 0.
+// The MMA's k slots are a permutation of the values (lane t of a quad has 8 consecutive ones of each
+// 32), the same one for the activations: a sum does not ask for their order, and a lane's share of
+// the activations is then one 16-byte load per 32 values. Rows and K are padded to whole tiles and
+// units with scale 0 and activations 0.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -29,7 +30,7 @@
 
 namespace w4 {
 
-constexpr int TILE_ROWS = 16, CHUNK_K = 64, CHUNK_BYTES = 512;
+constexpr int TILE_ROWS = 16, UNIT_K = 128, UNIT_BYTES = 1024;
 
 struct Bf16 {
   static constexpr uint32_t MAGIC = 0x43004300u;   // 128 + code in the low mantissa bits
@@ -47,6 +48,13 @@ struct Bf16 {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  // d = a b
+  static __device__ __forceinline__ void mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
   }
 };
 
@@ -67,13 +75,17 @@ struct Fp16 {
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
+  // d = a b
+  static __device__ __forceinline__ void mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+  }
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -91,22 +103,26 @@ __device__ __forceinline__ void decode(uint32_t w, uint32_t z0, uint32_t z1, uin
   a[3] = D::sub2(((w >> 12) & M) | D::MAGIC, z1);
 }
 
-// 32 values of K: two words against each column tile's 16 bytes of activations
-template <class D, int NT>
+// 32 values of K: two words against each column tile's 16 bytes of activations; FIRST: acc = instead
+// of acc +=
+template <class D, int NT, bool FIRST>
 __device__ __forceinline__ void half_chunk(uint32_t w0, uint32_t w1, uint32_t z0, uint32_t z1, const uint4 (&xb)[NT],
                                            float (&acc)[NT][4]) {
   uint32_t a[4];
   decode<D>(w0, z0, z1, a);
 #pragma unroll
-  for (int n = 0; n < NT; ++n) D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].x, xb[n].y);
+  for (int n = 0; n < NT; ++n) {
+    if (FIRST) D::mma0(acc[n], a[0], a[1], a[2], a[3], xb[n].x, xb[n].y);
+    else D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].x, xb[n].y);
+  }
   decode<D>(w1, z0, z1, a);
 #pragma unroll
   for (int n = 0; n < NT; ++n) D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].z, xb[n].w);
 }
 
-// tot += scale (rows g, g + 8) * acc; acc = 0
+// tot += scale (rows g, g + 8) * acc
 template <class D, int NT>
-__device__ __forceinline__ void fold(uint32_t scale, float (&acc)[NT][4], float (&tot)[NT][4]) {
+__device__ __forceinline__ void fold(uint32_t scale, const float (&acc)[NT][4], float (&tot)[NT][4]) {
   const float2 s = D::to_f32(scale);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -114,8 +130,6 @@ __device__ __forceinline__ void fold(uint32_t scale, float (&acc)[NT][4], float 
     tot[n][1] = fmaf(s.x, acc[n][1], tot[n][1]);
     tot[n][2] = fmaf(s.y, acc[n][2], tot[n][2]);
     tot[n][3] = fmaf(s.y, acc[n][3], tot[n][3]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
   }
 }
 

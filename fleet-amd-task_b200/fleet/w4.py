@@ -26,8 +26,8 @@ def lay_out(codes, scales, zeros, k, group, gate_up=False):
     uint8, scales and zeros [E, tiles, groups, 16]. gate_up: rows 2i / 2i + 1 are gate / up row i
     (pack_weights.interleave_gate_up) and a tile takes 8 gate rows, then their 8 up rows."""
     E, N = codes.shape[:2]
-    tiles, chunks = -(-N // 16), -(-k // 64)
-    groups = -(-64 * chunks // group)
+    tiles, chunks = -(-N // 16), 2 * -(-k // 128)
+    groups = 64 * chunks // group
 
     def rows(v, fill):
         """[E, N, m] -> [E, tiles, 2 (row g, row g + 8), 8 (g), m]"""
