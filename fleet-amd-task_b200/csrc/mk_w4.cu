@@ -35,27 +35,27 @@ using namespace w4;
 namespace {
 
 constexpr int WARPS = 16, THREADS = WARPS * 32;
-constexpr int RED_STRIDE = 20;                       // floats per column of a tile's partial sums (16 + 4: no conflicts)
 constexpr int SMEM_LIMIT = 227 * 1024;
 constexpr int MAX_EXPERTS = 1024;
 enum Mode { LINEAR = 0, GATEUP = 1, DOWN = 2 };
 
-// shared memory: the warps' rings, the partial sums, the activations
-template <int NT, int G, bool ZP>
+// a warp's step: a unit of RT tiles
+template <int RT, int G, bool ZP>
 struct Shape {
   static constexpr int GROUPS = UNIT_K / G;          // per unit
-  static constexpr int STAGE = UNIT_BYTES + GROUPS * (ZP ? 48 : 32);
-  static constexpr int DEPTH = NT <= 2 ? 6 : 4;      // stages a warp
-  static constexpr int RING = WARPS * DEPTH * STAGE;
+  static constexpr int SCALES = RT * GROUPS * 32, ZEROS = ZP ? RT * GROUPS * 16 : 0;
+  static constexpr int STAGE = RT * TILE_UNIT_BYTES + SCALES + ZEROS;
+  static constexpr int RED_STRIDE = RT * 16 + 4;     // floats per column of the partial sums (4: no bank conflicts)
   static constexpr int RED = WARPS * 8 * RED_STRIDE * 4;
-  static constexpr int FIXED = RING + RED;
 };
 
 struct Args {
   const uint8_t* codes;
   const uint8_t* scales;
   const uint8_t* zeros;     // or null: 8
-  int tiles, units, rows, k;
+  int tiles;                // steps of RT tiles down the rows
+  int units, rows, k;
+  int depth;                // stages of a warp's ring: 2, 4 or 8
   int mode;
   int n_items;              // LINEAR: known on the host; else *items_n
   const int* items_n;
@@ -112,156 +112,163 @@ __device__ __forceinline__ void stage_x(const Args& a, uint4* xs, int start, int
   }
 }
 
-template <class D, int NT, int G, bool ZP>
-__global__ void __launch_bounds__(THREADS, 1) w4_kernel(const Args a) {
-  using S = Shape<NT, G, ZP>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * (S::DEPTH * S::STAGE);
-  float* red = reinterpret_cast<float*>(smem + S::RING);
-  uint4* xs = reinterpret_cast<uint4*>(smem + S::FIXED);
-  const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+// One warp's copies: its units of its team's tiles, in order, across the items of the CTA's range.
+template <int RT, int G, bool ZP>
+struct Copies {
+  using S = Shape<RT, G, ZP>;
+  int f = 0, end = 0, left = 0;            // the flat tile, the segment's end, the tile's units to come
+  int tile0 = 0;                           // from a flat tile to the tile of the item's weight
+  const uint8_t *code = nullptr, *meta = nullptr;
+  bool scale_lane, zero_lane;              // lanes 0.. carry the scales' 16-byte pieces, then the zero points'
+  uint32_t meta_at;
+  int meta_step;
 
-  const int n_items = a.mode == LINEAR ? a.n_items : *a.items_n;
-  const int64_t total = (int64_t)n_items * a.tiles;   // below 2^31
-  const int ks = a.ks, rank = blockIdx.x % ks, group = blockIdx.x / ks, n_groups = gridDim.x / ks;
-  const int lo = (int)(total * group / n_groups), hi = (int)(total * (group + 1) / n_groups);
-  const int kw = a.kw, teams = WARPS / kw, team = warp / kw, part = warp - team * kw;
-  const int u0 = a.units * rank / ks, u1 = a.units * (rank + 1) / ks;
-  const int n_units = max(0, (u1 - u0 - part + kw - 1) / kw);   // this warp's units of a tile
-
-  // the copy cursor: the team's tiles of each segment (the part of the range within one item)
-  int c_f = 0, c_end = 0, c_left = 0;
-  int c_tile0 = 0;                         // from a flat tile number to the tile of the item's weight
-  const uint8_t *c_code = nullptr, *c_meta = nullptr;
-  // lanes 0.. carry the scales' 16-byte pieces, lanes 16.. the zero points'
-  const bool scale_lane = lane < 2 * S::GROUPS, zero_lane = ZP && lane >= 16 && lane < 16 + S::GROUPS;
-  const int meta_unit = scale_lane ? S::GROUPS * 32 : S::GROUPS * 16;
-  const uint32_t meta_at = UNIT_BYTES + (scale_lane ? lane * 16 : S::GROUPS * 32 + (lane - 16) * 16);
-  auto at_tile = [&]() {
-    const int64_t first = (int64_t)(c_f + c_tile0) * a.units + u0 + part;
-    c_code = a.codes + first * UNIT_BYTES + lane * 16;
-    if (scale_lane) c_meta = a.scales + first * (S::GROUPS * 32) + lane * 16;
-    else if (zero_lane) c_meta = a.zeros + first * (S::GROUPS * 16) + (lane - 16) * 16;
-    c_left = n_units;
-  };
-  auto at_segment = [&](int from) {
-    const int item = from / a.tiles;
-    c_end = min(hi, (item + 1) * a.tiles);
-    c_f = from + team;
-    c_tile0 = ((a.mode == LINEAR ? 0 : a.items[item].x) - item) * a.tiles;
-  };
-  auto skip_empty = [&]() {
-    while (c_f >= c_end && c_end < hi) at_segment(c_end);
-    if (c_f < c_end) at_tile();
-  };
-  if (lo < hi && n_units > 0) {
-    at_segment(lo);
-    skip_empty();
+  __device__ __forceinline__ void init(int lane) {
+    constexpr int NS = S::SCALES / 16, NZ = S::ZEROS / 16;
+    static_assert(NS + NZ <= 32, "one copy a lane");
+    scale_lane = lane < NS;
+    zero_lane = ZP && lane >= NS && lane < NS + NZ;
+    meta_at = RT * TILE_UNIT_BYTES + lane * 16;
   }
-  auto issue = [&](uint32_t dst) {
-    if (c_left > 0) {
-      cp16(dst + lane * 16, c_code);
-      cp16(dst + 512 + lane * 16, c_code + 512);
-      if (scale_lane || zero_lane) cp16(dst + meta_at, c_meta);
-      c_code += kw * UNIT_BYTES;
-      c_meta += kw * meta_unit;
-      if (--c_left == 0) {
-        c_f += teams;
-        skip_empty();
-      }
-    }
-    cp_commit();
-  };
-#pragma unroll
-  for (int s = 0; s < S::DEPTH - 1; ++s) issue(ring_s + s * S::STAGE);
+  // tile f in units of RT tiles: with RT 1 the two tiles of a strip lie side by side in each unit
+  __device__ __forceinline__ void at_tile(const Args& a, int first_unit, int n_units, int lane) {
+    const int64_t w = f + tile0;
+    const int64_t strip = RT == 2 ? w : w >> 1;
+    const int half = RT == 2 ? 0 : (int)(w & 1);
+    const int64_t u = (strip * a.units + first_unit) * 2 + half;         // in tiles' units
+    code = a.codes + u * TILE_UNIT_BYTES + lane * 16;
+    if (scale_lane) meta = a.scales + u * (S::GROUPS * 32) + lane * 16;
+    else if (zero_lane) meta = a.zeros + u * (S::GROUPS * 16) + (lane - S::SCALES / 16) * 16;
+    left = n_units;
+  }
+  __device__ __forceinline__ void at_segment(const Args& a, int from, int hi, int team) {
+    const int item = from / a.tiles;
+    end = min(hi, (item + 1) * a.tiles);
+    f = from + team;
+    tile0 = ((a.mode == LINEAR ? 0 : a.items[item].x) - item) * a.tiles;
+  }
+  __device__ __forceinline__ void skip_empty(const Args& a, int hi, int team, int first_unit, int n_units, int lane) {
+    while (f >= end && end < hi) at_segment(a, end, hi, team);
+    if (f < end) at_tile(a, first_unit, n_units, lane);
+  }
+};
 
-  uint32_t slot = 0, freed = (S::DEPTH - 1) * S::STAGE;   // the stage to read, the stage read before it
-  for (int seg = lo; seg < hi;) {
-    const int item = seg / a.tiles;
-    const int seg_end = min(hi, (item + 1) * a.tiles);
-    int start, count;
-    if (a.mode == LINEAR) {
-      start = item * a.tb;
-      count = min(a.tb, a.t - start);
-    } else {
-      const int4 it = a.items[item];
-      start = it.y;
-      count = it.z;
-    }
-    __syncthreads();   // every warp is done with the last item's activations
-    stage_x(a, xs, start, count, u0 * 16, u1 * 16);
+template <class D, int RT, int G, bool ZP>
+struct Kernel {
+  using S = Shape<RT, G, ZP>;
+  const Args& a;
+  Masks m;
+  int warp, lane, g, t;
+  int kw, teams, team, part;
+  int ks, rank, u0, n_units, hi;
+  uint8_t* ring;
+  uint32_t ring_s;
+  float* red;
+  uint4* xs;
+  Copies<RT, G, ZP> c;
+  uint32_t slot = 0;
+
+  __device__ __forceinline__ Kernel(const Args& args) : a(args) {}
+
+  __device__ __forceinline__ void issue(uint32_t dst) {
+    const bool on = c.left > 0;
+#pragma unroll
+    for (int i = 0; i < RT * 2; ++i) cp16_if(on, dst + i * 512 + lane * 16, c.code + i * 512);
+    cp16_if(on && (c.scale_lane || c.zero_lane), dst + c.meta_at, c.meta);
     cp_commit();
-    cp_wait<0>();
-    __syncthreads();
+    c.code += kw * (2 * TILE_UNIT_BYTES);
+    c.meta += c.meta_step;
+    if (--c.left == 0) {
+      c.f += teams;
+      c.skip_empty(a, hi, team, u0 + part, n_units, lane);
+    }
+  }
+
+  // the tiles [seg, seg_end) of one item's columns [start, start + count), count <= 8 NT
+  template <int NT>
+  __device__ __forceinline__ void segment(int seg, int seg_end, int item, int start, int count) {
     // a lane past the columns reads the last one's activations: its sums are not used
     const uint4* xl[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) xl[n] = xs + (part * 4 * count + min(n * 8 + g, count - 1)) * 4 + t;
+    const int x_h = count * 4, x_u = kw * count * 16;
     for (int first = seg; first < seg_end; first += teams) {
       const int f = first + team;
       const bool live = f < seg_end;
       if (!live && ks == 1) break;
-      float tot[NT][4];
+      float tot[RT][NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tot[n][i] = 0.0f;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tot[r][n][i] = 0.0f;
       int x_at = 0;
       for (int u = live ? n_units : 0; u > 0; --u) {
-        cp_wait<S::DEPTH - 2>();
+        if (a.depth == 2) cp_wait<1>();
+        else if (a.depth == 4) cp_wait<3>();
+        else cp_wait<7>();
         __syncwarp();
         const uint8_t* st = ring + slot;
-        const uint4 w0 = *reinterpret_cast<const uint4*>(st + lane * 16);
-        const uint4 w1 = *reinterpret_cast<const uint4*>(st + 512 + lane * 16);
-        uint32_t sc[S::GROUPS], z0[S::GROUPS], z1[S::GROUPS];
+        uint4 w[RT][2];
+        uint32_t sc[RT][S::GROUPS], z0[RT][S::GROUPS], z1[RT][S::GROUPS];
 #pragma unroll
-        for (int i = 0; i < S::GROUPS; ++i) {
-          sc[i] = *reinterpret_cast<const uint32_t*>(st + UNIT_BYTES + i * 32 + g * 4);
-          if (ZP) {
-            const uint32_t z = *reinterpret_cast<const uint16_t*>(st + UNIT_BYTES + S::GROUPS * 32 + i * 16 + g * 2);
-            z0[i] = (z & 0xFFu) * 0x00010001u | D::MAGIC;
-            z1[i] = (z >> 8) * 0x00010001u | D::MAGIC;
-          } else {
-            z0[i] = z1[i] = D::MAGIC + 0x00080008u;
+        for (int r = 0; r < RT; ++r) {
+          w[r][0] = *reinterpret_cast<const uint4*>(st + r * TILE_UNIT_BYTES + lane * 16);
+          w[r][1] = *reinterpret_cast<const uint4*>(st + r * TILE_UNIT_BYTES + 512 + lane * 16);
+#pragma unroll
+          for (int i = 0; i < S::GROUPS; ++i) {
+            sc[r][i] = *reinterpret_cast<const uint32_t*>(st + RT * TILE_UNIT_BYTES + (r * S::GROUPS + i) * 32 + g * 4);
+            if (ZP) {
+              const uint32_t z =
+                  *reinterpret_cast<const uint16_t*>(st + RT * TILE_UNIT_BYTES + S::SCALES + (r * S::GROUPS + i) * 16 + g * 2);
+              z0[r][i] = (z & 0xFFu) * 0x00010001u | D::MAGIC;
+              z1[r][i] = (z >> 8) * 0x00010001u | D::MAGIC;
+            } else {
+              z0[r][i] = z1[r][i] = D::MAGIC + 0x00080008u;
+            }
           }
         }
-        issue(ring_s + freed);
-        freed = slot;
-        slot = slot == (S::DEPTH - 1) * S::STAGE ? 0 : slot + S::STAGE;
-        float acc[NT][4];
+        __syncwarp();            // every lane has read the stage
+        issue(ring_s + slot);
+        slot = slot == (a.depth - 1) * S::STAGE ? 0 : slot + S::STAGE;
+        float acc[RT][NT][4];
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
           uint4 xb[NT];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) xb[n] = xl[n][x_at + h * count * 4];
-          const uint4& w = h < 2 ? w0 : w1;
+          for (int n = 0; n < NT; ++n) xb[n] = xl[n][x_at + h * x_h];
           const int i = h * 32 / G;
-          if (h * 32 % G == 0) half_chunk<D, NT, true>(h & 1 ? w.z : w.x, h & 1 ? w.w : w.y, z0[i], z1[i], xb, acc);
-          else half_chunk<D, NT, false>(h & 1 ? w.z : w.x, h & 1 ? w.w : w.y, z0[i], z1[i], xb, acc);
-          if ((h + 1) * 32 % G == 0) fold<D, NT>(sc[i], acc, tot);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const uint4& v = w[r][h >> 1];
+            if (h * 32 % G == 0) half_chunk<D, NT, true>(m, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0[r][i], z1[r][i], xb, acc[r]);
+            else half_chunk<D, NT, false>(m, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0[r][i], z1[r][i], xb, acc[r]);
+            if ((h + 1) * 32 % G == 0) fold<D, NT>(sc[r][i], acc[r], tot[r]);
+          }
         }
-        x_at += kw * count * 16;
+        x_at += x_u;
       }
       // the team's partial sums, [column][row], eight columns at a time, added in warp order
-      constexpr int RED_WARP = 8 * RED_STRIDE;
+      constexpr int RED_WARP = 8 * S::RED_STRIDE, ROWS = RT * 16;
       float* mine = red + warp * RED_WARP;
       float* theirs = red + team * kw * RED_WARP;
-      const int row0 = (f - item * a.tiles) * TILE_ROWS, me = part * 32 + lane;
+      const int row0 = (f - item * a.tiles) * ROWS, me = part * 32 + lane;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int cols = min(count - n * 8, 8);
-        if (cols <= 0) break;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine[(2 * t + (i & 1)) * RED_STRIDE + g + (i >> 1) * 8] = tot[n][i];
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mine[(2 * t + (i & 1)) * S::RED_STRIDE + r * 16 + g + (i >> 1) * 8] = tot[r][n][i];
         team_sync(team, kw);
-        if (a.mode == GATEUP) {   // tile rows 0..7 are gate rows, 8..15 their up rows
-          for (int i = me; i < cols * 8; i += kw * 32) {
-            const int col = i >> 3, r = i & 7, j = row0 / 2 + r;
+        if (a.mode == GATEUP) {   // a tile's rows 0..7 are gate rows, 8..15 their up rows
+          for (int i = me; i < cols * (ROWS / 2); i += kw * 32) {
+            const int col = i / (ROWS / 2), q = i % (ROWS / 2), r = (q >> 3) * 16 + (q & 7), j = row0 / 2 + q;
             float gt = 0.0f, up = 0.0f;
-            for (int w = 0; w < kw; ++w) {
-              gt += theirs[w * RED_WARP + col * RED_STRIDE + r];
-              up += theirs[w * RED_WARP + col * RED_STRIDE + r + 8];
+            for (int v = 0; v < kw; ++v) {
+              gt += theirs[v * RED_WARP + col * S::RED_STRIDE + r];
+              up += theirs[v * RED_WARP + col * S::RED_STRIDE + r + 8];
             }
             // rounded to the activations' type: the down projection's tensor-core operand
             if (j < a.rows / 2)
@@ -276,31 +283,87 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const Args a) {
             if (a.out_f32) static_cast<float*>(a.out)[o] = v;
             else static_cast<uint16_t*>(a.out)[o] = D::round(v);
           };
-          for (int i = me; i < cols * 16; i += kw * 32) {
-            const int col = i >> 4, r = i & 15;
+          for (int i = me; i < cols * ROWS; i += kw * 32) {
+            const int col = i / ROWS, r = i % ROWS;
             float v = 0.0f;
-            for (int w = 0; w < kw; ++w) v += theirs[w * RED_WARP + col * RED_STRIDE + r];
-            if (ks > 1) theirs[col * RED_STRIDE + r] = v;   // this thread's own place: the CTA's sum for the cluster
+            for (int w = 0; w < kw; ++w) v += theirs[w * RED_WARP + col * S::RED_STRIDE + r];
+            if (ks > 1) theirs[col * S::RED_STRIDE + r] = v;   // this thread's own place: the CTA's sum for the cluster
             else store(col, r, v);
           }
           if (ks > 1) {   // K is split over the cluster: each CTA adds and stores the columns col % ks == rank
             cluster_sync();
-            for (int i = me; i < cols * 16; i += kw * 32) {
-              const int col = i >> 4, r = i & 15;
+            for (int i = me; i < cols * ROWS; i += kw * 32) {
+              const int col = i / ROWS, r = i % ROWS;
               if (col % ks != rank || !live) continue;
               float v = 0.0f;
-              for (int c = 0; c < ks; ++c) v += peer_float(theirs + col * RED_STRIDE + r, c);
+              for (int p = 0; p < ks; ++p) v += peer_float(theirs + col * S::RED_STRIDE + r, p);
               store(col, r, v);
             }
             cluster_sync();
           }
         }
         team_sync(team, kw);   // the sums are read before the next ones are written
+        if (cols < 8) break;
       }
     }
-    seg = seg_end;
   }
-  cp_wait<0>();
+
+  __device__ __forceinline__ void run(uint8_t* smem) {
+    warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    m = masks<D>();
+    ring = smem + warp * (a.depth * S::STAGE);
+    ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+    red = reinterpret_cast<float*>(smem + WARPS * a.depth * S::STAGE);
+    xs = reinterpret_cast<uint4*>(smem + WARPS * a.depth * S::STAGE + S::RED);
+    const int n_items = a.mode == LINEAR ? a.n_items : *a.items_n;
+    const int64_t total = (int64_t)n_items * a.tiles;   // below 2^31
+    ks = a.ks;
+    rank = blockIdx.x % ks;
+    const int group = blockIdx.x / ks, n_groups = gridDim.x / ks;
+    const int lo = (int)(total * group / n_groups);
+    hi = (int)(total * (group + 1) / n_groups);
+    kw = a.kw, teams = WARPS / kw, team = warp / kw, part = warp - team * kw;
+    u0 = a.units * rank / ks;
+    const int u1 = a.units * (rank + 1) / ks;
+    n_units = max(0, (u1 - u0 - part + kw - 1) / kw);   // this warp's units of a tile
+    c.init(lane);
+    c.meta_step = kw * 2 * S::GROUPS * (c.scale_lane ? 32 : 16);
+    if (lo < hi && n_units > 0) {
+      c.at_segment(a, lo, hi, team);
+      c.skip_empty(a, hi, team, u0 + part, n_units, lane);
+    }
+    for (int s = 0; s < a.depth; ++s) issue(ring_s + s * S::STAGE);
+    for (int seg = lo; seg < hi;) {
+      const int item = seg / a.tiles;
+      const int seg_end = min(hi, (item + 1) * a.tiles);
+      int start, count;
+      if (a.mode == LINEAR) {
+        start = item * a.tb;
+        count = min(a.tb, a.t - start);
+      } else {
+        const int4 it = a.items[item];
+        start = it.y;
+        count = it.z;
+      }
+      __syncthreads();   // every warp is done with the last item's activations
+      stage_x(a, xs, start, count, u0 * 16, u1 * 16);
+      cp_commit();
+      cp_wait<0>();
+      __syncthreads();
+      if (count <= 8) segment<1>(seg, seg_end, item, start, count);
+      else if (count <= 16) segment<2>(seg, seg_end, item, start, count);
+      else segment<4>(seg, seg_end, item, start, count);
+      seg = seg_end;
+    }
+    cp_wait<0>();
+  }
+};
+
+template <class D, int RT, int G, bool ZP>
+__global__ void __launch_bounds__(THREADS, 1) w4_kernel(const Args a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  Kernel<D, RT, G, ZP> k(a);
+  k.run(smem);
 }
 
 // The slots grouped by expert: columns (slots in expert order), col_token, slot_col (a slot's
@@ -379,26 +442,18 @@ void fill(Args& a, const MkW4* w) {
   a.codes = static_cast<const uint8_t*>(w->codes);
   a.scales = static_cast<const uint8_t*>(w->scales);
   a.zeros = static_cast<const uint8_t*>(w->zeros);
-  a.tiles = (w->n + TILE_ROWS - 1) / TILE_ROWS;
   a.units = (w->k + UNIT_K - 1) / UNIT_K;
   a.ks = 1;
   a.rows = w->n;
   a.k = w->k;
 }
 
-// shared memory beside the activations, for the group size and zero points that take most
-int fixed_bytes(int nt) {
-  return nt == 1 ? Shape<1, 32, true>::FIXED : nt == 2 ? Shape<2, 32, true>::FIXED : Shape<4, 32, true>::FIXED;
-}
+// shared memory beside the activations for the group size and zero points that take most, at a depth
+// that keeps 4 KB a warp in flight (twice what the HBM's rate times its latency asks for)
+constexpr int FIXED = WARPS * 2 * Shape<2, 32, true>::STAGE + Shape<2, 32, true>::RED;
 
 // columns (at most `want`, at most 32) whose activations of `units` units fit
-int columns_that_fit(int units, int want) {
-  const int per = units * UNIT_K * 2;
-  for (int nt = want <= 8 ? 1 : want <= 16 ? 2 : 4;; nt /= 2) {
-    const int fit = std::min({(SMEM_LIMIT - fixed_bytes(nt)) / per, nt * 8, want});
-    if (fit > nt * 4 || nt == 1) return fit;
-  }
-}
+int columns_that_fit(int units, int want) { return std::min({(SMEM_LIMIT - FIXED) / (units * UNIT_K * 2), 32, want}); }
 
 struct Device {
   int sms = 0;
@@ -421,37 +476,32 @@ int device_sms(int* sms) {
   return MK_OK;
 }
 
-template <class D, int NT, int G, bool ZP>
-int launch(const Args& a, int grid, cudaStream_t s) {
+template <class D, int RT, int G, bool ZP>
+int launch(Args a, int grid, cudaStream_t s) {
+  using S = Shape<RT, G, ZP>;
+  const int xbytes = a.tb * ((a.units + a.ks - 1) / a.ks) * UNIT_K * 2;
+  a.depth = RT == 2 ? 2 : 4;
+  if (WARPS * a.depth * 2 * S::STAGE + S::RED + xbytes <= SMEM_LIMIT) a.depth *= 2;
   cudaLaunchConfig_t c{};
   cudaLaunchAttribute cluster[1];
   c.gridDim = dim3((unsigned)grid);
   c.blockDim = dim3(THREADS);
-  c.dynamicSmemBytes = Shape<NT, G, ZP>::FIXED + (size_t)a.tb * ((a.units + a.ks - 1) / a.ks) * UNIT_K * 2;
+  c.dynamicSmemBytes = (size_t)WARPS * a.depth * S::STAGE + S::RED + xbytes;
   c.stream = s;
   cluster[0].id = cudaLaunchAttributeClusterDimension;
   cluster[0].val.clusterDim = {(unsigned)a.ks, 1, 1};
   c.attrs = cluster;
-  c.numAttrs = 1;
-  cudaError_t e = cudaFuncSetAttribute(w4_kernel<D, NT, G, ZP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&c, w4_kernel<D, NT, G, ZP>, a);
+  c.numAttrs = a.ks > 1 ? 1 : 0;
+  cudaError_t e = cudaFuncSetAttribute(w4_kernel<D, RT, G, ZP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&c, w4_kernel<D, RT, G, ZP>, a);
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
 }
 
-template <class D, int NT>
+template <class D, int RT>
 int launch_group(const Args& a, int group, int grid, cudaStream_t s) {
-  if (group == 32) return a.zeros ? launch<D, NT, 32, true>(a, grid, s) : launch<D, NT, 32, false>(a, grid, s);
-  if (group == 64) return a.zeros ? launch<D, NT, 64, true>(a, grid, s) : launch<D, NT, 64, false>(a, grid, s);
-  return a.zeros ? launch<D, NT, 128, true>(a, grid, s) : launch<D, NT, 128, false>(a, grid, s);
-}
-
-int launch_weight(const Args& a, const MkW4* w, int grid, cudaStream_t s) {
-  const int nt = a.tb <= 8 ? 1 : a.tb <= 16 ? 2 : 4;
-  if (w->dtype == MK_W4_BF16)
-    return nt == 1 ? launch_group<Bf16, 1>(a, w->group, grid, s) : nt == 2 ? launch_group<Bf16, 2>(a, w->group, grid, s)
-                                                                          : launch_group<Bf16, 4>(a, w->group, grid, s);
-  return nt == 1 ? launch_group<Fp16, 1>(a, w->group, grid, s) : nt == 2 ? launch_group<Fp16, 2>(a, w->group, grid, s)
-                                                                        : launch_group<Fp16, 4>(a, w->group, grid, s);
+  if (group == 32) return a.zeros ? launch<D, RT, 32, true>(a, grid, s) : launch<D, RT, 32, false>(a, grid, s);
+  if (group == 64) return a.zeros ? launch<D, RT, 64, true>(a, grid, s) : launch<D, RT, 64, false>(a, grid, s);
+  return a.zeros ? launch<D, RT, 128, true>(a, grid, s) : launch<D, RT, 128, false>(a, grid, s);
 }
 
 // warps per tile: few tiles are split over many warps, many are left to few
@@ -459,6 +509,20 @@ int team_warps(int64_t tiles, int units, int grid) {
   int kw = 16;
   while (kw > 1 && (kw > units || tiles > (int64_t)grid * (WARPS / kw) * 8)) kw /= 2;
   return kw;
+}
+
+// `items` (about) items over the CTAs, in groups of ks; a.tiles and a.kw are set here
+int launch_weight(Args& a, const MkW4* w, int64_t items, int ctas, cudaStream_t s) {
+  const int strips = (w->n + STRIP_ROWS - 1) / STRIP_ROWS;
+  const int64_t max_groups = ctas / a.ks;
+  const bool two = items * strips >= max_groups * 2;   // enough strips for every CTA: two tiles a warp share the activations
+  a.tiles = two ? strips : 2 * strips;
+  const int groups = (int)(a.mode == LINEAR ? std::min<int64_t>(max_groups, items * a.tiles) : max_groups);
+  a.kw = team_warps(items * a.tiles, a.units / a.ks, groups);
+  const int grid = groups * a.ks;
+  if (w->dtype == MK_W4_BF16)
+    return two ? launch_group<Bf16, 2>(a, w->group, grid, s) : launch_group<Bf16, 1>(a, w->group, grid, s);
+  return two ? launch_group<Fp16, 2>(a, w->group, grid, s) : launch_group<Fp16, 1>(a, w->group, grid, s);
 }
 
 bool aligned16(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
@@ -474,7 +538,7 @@ const char* plan_experts(const MkW4* w13, const MkW4* w2, int64_t t, int64_t s, 
   if (w13->dtype != w2->dtype || w13->experts != w2->experts || w13->n % 2 || w13->n / 2 != w2->k || w13->k != w2->n)
     return "W13 [E, 2 I, H] and W2 [E, H, I] do not belong together";
   if (w13->experts > MAX_EXPERTS) return "at most 1024 experts";
-  const int64_t tiles = std::max((w13->n + TILE_ROWS - 1) / TILE_ROWS, (w2->n + TILE_ROWS - 1) / TILE_ROWS);
+  const int64_t tiles = std::max(w13->n, w2->n) / 16 + 2;
   if (w13->experts * tiles > INT32_MAX / 2) return "too many experts times rows";
   if (t < 0 || s < 0 || t * s >= (1 << 24)) return "slots (tokens x slots per token) are from 0 to 2^24 - 1";
   const int want = t >= 32 ? 32 : (int)std::max<int64_t>(t, 1);
@@ -527,11 +591,8 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   a.out = out;
   a.ldo = ldo;
   a.out_f32 = out_f32;
-  const int64_t total = (int64_t)a.n_items * a.tiles;
-  if (total > INT32_MAX - 4096) return fail(MK_EINVAL, "too many tokens times rows");
-  const int groups = (int)std::min<int64_t>(sms / a.ks, total);
-  a.kw = team_warps(total, a.units / a.ks, groups);
-  return launch_weight(a, w, groups * a.ks, static_cast<cudaStream_t>(stream));
+  if ((int64_t)a.n_items * (w->n / 16 + 2) > INT32_MAX - 4096) return fail(MK_EINVAL, "too many tokens times rows");
+  return launch_weight(a, w, a.n_items, sms, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mk_w4_experts_workspace(const MkW4* w13, const MkW4* w2, int32_t t, int32_t slots, int64_t* bytes) {
@@ -574,9 +635,8 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   a.x_vec = aligned16(x, ldx);
   a.out = ws + p.act;
   a.ldo = p.ldact;
-  a.kw = team_warps(items_about * a.tiles, a.units, sms);
   a.mode = GATEUP;
-  if (int rc = launch_weight(a, w13, sms, st)) return rc;
+  if (int rc = launch_weight(a, w13, items_about, sms, st)) return rc;
   Args b{};
   fill(b, w2);
   b.items = items;
@@ -589,8 +649,7 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   b.ldo = w2->n;
   b.out_f32 = 1;
   b.mode = DOWN;
-  b.kw = team_warps(items_about * b.tiles, b.units, sms);
-  if (int rc = launch_weight(b, w2, sms, st)) return rc;
+  if (int rc = launch_weight(b, w2, items_about, sms, st)) return rc;
   const dim3 grid((unsigned)((w2->n + 255) / 256), (unsigned)t);
   const float* y = reinterpret_cast<const float*>(ws + p.y);
   if (w2->dtype == MK_W4_BF16)

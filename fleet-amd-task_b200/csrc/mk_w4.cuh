@@ -8,18 +8,18 @@
 // the result.
 //
 // The laid-out form (fleet/w4.py lay_out) is the order in which the lanes of a warp want the codes
-// for mma.sync m16n8k16 with the weights as the 16-row operand and the tokens as its 8 columns:
-//   codes  [experts][tiles][units][2 chunks][32 lanes][4 words]: a tile is 16 rows, a unit 128 values
-//          of K in two chunks of 64. Lane 4 g + t, word 2 h + j (h, j in 0..1) holds rows g and g + 8
-//          at the four values k = 64 chunk + 32 h + 8 t + 4 j + (0..3): bits 4i..4i+3 (k even) and
-//          16+4i.. (k odd) are, for i = 0..3, (row g, k 0/1), (row g + 8, k 0/1), (row g, k 2/3),
-//          (row g + 8, k 2/3): the four A registers of one MMA, two codes each, a shift and one
-//          AND-OR from a 16-bit float
-//   scales [experts][tiles][128 units / G groups][8][2]: rows g and g + 8 side by side (one 32-bit load)
-//   zeros  [experts][tiles][groups][8][2] bytes, or none
+// for mma.sync m16n8k16 with the weights as the 16-row operand and the tokens as its 8 columns. A
+// strip is 32 rows (two tiles of 16), a unit 128 values of K:
+//   codes  [experts][strips][units][2 tiles][2 chunks of 64][32 lanes][4 words]: lane 4 g + t, word
+//          2 h + j (h, j in 0..1) holds the tile's rows g and g + 8 at the four values
+//          k = 64 chunk + 32 h + 8 t + 4 j + (0..3): bits 4i..4i+3 (k even) and 16+4i.. (k odd) are,
+//          for i = 0..3, (row g, k 0/1), (row g + 8, k 0/1), (row g, k 2/3), (row g + 8, k 2/3): the
+//          four A registers of one MMA, two codes each, a shift and one AND-OR from a 16-bit float
+//   scales [experts][strips][units][2 tiles][128 / G groups][8][2]: rows g and g + 8 side by side
+//   zeros  the same, bytes, or none
 // The MMA's k slots are a permutation of the values (lane t of a quad has 8 consecutive ones of each
 // 32), the same one for the activations: a sum does not ask for their order, and a lane's share of
-// the activations is then one 16-byte load per 32 values. Rows and K are padded to whole tiles and
+// the activations is then one 16-byte load per 32 values. Rows and K are padded to whole strips and
 // units with scale 0 and activations 0.
 #pragma once
 #include <cuda_bf16.h>
@@ -30,7 +30,7 @@
 
 namespace w4 {
 
-constexpr int TILE_ROWS = 16, UNIT_K = 128, UNIT_BYTES = 1024;
+constexpr int STRIP_ROWS = 32, UNIT_K = 128, TILE_UNIT_BYTES = 1024;   // a tile's codes of a unit
 
 struct Bf16 {
   static constexpr uint32_t MAGIC = 0x43004300u;   // 128 + code in the low mantissa bits
@@ -87,35 +87,60 @@ struct Fp16 {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// the same if p (no branch)
+__device__ __forceinline__ void cp16_if(bool p, uint32_t dst, const void* src) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t"
+      "@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst), "l"(src), "r"((uint32_t)p)
+      : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// (w & mask) | magic in one instruction: both constants in registers (an instruction takes one
+// immediate, and the compiler would otherwise spend two)
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(mask), "r"(magic));
+  return d;
+}
+
+struct Masks {
+  uint32_t low, magic;
+};
+template <class D>
+__device__ __forceinline__ Masks masks() {
+  Masks m;
+  asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(m.low));
+  asm volatile("mov.b32 %0, %1;" : "=r"(m.magic) : "n"(D::MAGIC));
+  return m;
+}
+
 // one word's four A registers: codes to 16-bit floats, their zero points taken off (exact)
 template <class D>
-__device__ __forceinline__ void decode(uint32_t w, uint32_t z0, uint32_t z1, uint32_t (&a)[4]) {
-  constexpr uint32_t M = 0x000F000Fu;
-  a[0] = D::sub2((w & M) | D::MAGIC, z0);
-  a[1] = D::sub2(((w >> 4) & M) | D::MAGIC, z1);
-  a[2] = D::sub2(((w >> 8) & M) | D::MAGIC, z0);
-  a[3] = D::sub2(((w >> 12) & M) | D::MAGIC, z1);
+__device__ __forceinline__ void decode(const Masks& m, uint32_t w, uint32_t z0, uint32_t z1, uint32_t (&a)[4]) {
+  a[0] = D::sub2(and_or(w, m.low, m.magic), z0);
+  a[1] = D::sub2(and_or(w >> 4, m.low, m.magic), z1);
+  a[2] = D::sub2(and_or(w >> 8, m.low, m.magic), z0);
+  a[3] = D::sub2(and_or(w >> 12, m.low, m.magic), z1);
 }
 
 // 32 values of K: two words against each column tile's 16 bytes of activations; FIRST: acc = instead
 // of acc +=
 template <class D, int NT, bool FIRST>
-__device__ __forceinline__ void half_chunk(uint32_t w0, uint32_t w1, uint32_t z0, uint32_t z1, const uint4 (&xb)[NT],
+__device__ __forceinline__ void half_chunk(const Masks& m, uint32_t w0, uint32_t w1, uint32_t z0, uint32_t z1, const uint4 (&xb)[NT],
                                            float (&acc)[NT][4]) {
   uint32_t a[4];
-  decode<D>(w0, z0, z1, a);
+  decode<D>(m, w0, z0, z1, a);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     if (FIRST) D::mma0(acc[n], a[0], a[1], a[2], a[3], xb[n].x, xb[n].y);
     else D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].x, xb[n].y);
   }
-  decode<D>(w1, z0, z1, a);
+  decode<D>(m, w1, z0, z1, a);
 #pragma unroll
   for (int n = 0; n < NT; ++n) D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].z, xb[n].w);
 }

@@ -22,31 +22,33 @@ GROUPS = (32, 64, 128)
 
 
 def lay_out(codes, scales, zeros, k, group, gate_up=False):
-    """(codes, scales, zeros) of weights [E, N, K] in the kernels' order: codes [E, tiles, chunks, 512]
-    uint8, scales and zeros [E, tiles, groups, 16]. gate_up: rows 2i / 2i + 1 are gate / up row i
-    (pack_weights.interleave_gate_up) and a tile takes 8 gate rows, then their 8 up rows."""
+    """(codes, scales, zeros) of weights [E, N, K] in the kernels' order (csrc/mk_w4.cuh): codes
+    [E, strips, units, 2048] uint8, scales and zeros [E, strips, units, 2, 128 / group, 16]. gate_up:
+    rows 2i / 2i + 1 are gate / up row i (pack_weights.interleave_gate_up) and a tile takes 8 gate
+    rows, then their 8 up rows."""
     E, N = codes.shape[:2]
-    tiles, chunks = -(-N // 16), 2 * -(-k // 128)
-    groups = 64 * chunks // group
+    strips, units = -(-N // 32), -(-k // 128)
 
     def rows(v, fill):
-        """[E, N, m] -> [E, tiles, 2 (row g, row g + 8), 8 (g), m]"""
-        v = torch.nn.functional.pad(v, (0, 0, 0, tiles * 16 - N), value=fill)
+        """[E, N, m] -> [E, strips, 2 (tile), 2 (row g, row g + 8), 8 (g), m]"""
+        v = torch.nn.functional.pad(v, (0, 0, 0, strips * 32 - N), value=fill)
         if gate_up:
-            return v.view(E, tiles, 8, 2, -1).transpose(2, 3)
-        return v.view(E, tiles, 2, 8, -1)
+            return v.view(E, strips, 2, 8, 2, -1).transpose(3, 4)
+        return v.view(E, strips, 2, 2, 8, -1)
 
-    q = torch.full((E, N, chunks * 64), 8, dtype=torch.uint8, device=codes.device)
+    q = torch.full((E, N, units * 128), 8, dtype=torch.uint8, device=codes.device)
     q[..., 0:k:2] = codes[..., :(k + 1) // 2] & 15
     q[..., 1:k:2] = codes[..., :k // 2] >> 4
-    # k = 64 chunk + 32 h + 8 t + 4 j + 2 p + low/high half; bytes of a word: (half, p), nibbles: the two rows
-    q = rows(q, 8).view(E, tiles, 2, 8, chunks, 2, 4, 2, 2, 2)          # e, tile, r, g, chunk, h, t, j, p, half
-    q = q[:, :, 0] | (q[:, :, 1] << 4)
-    q = q.permute(0, 1, 3, 2, 5, 4, 6, 8, 7).contiguous().view(E, tiles, chunks, 512)   # ... chunk, g, t, h, j, half, p
+    # k = 128 unit + 64 chunk + 32 h + 8 t + 4 j + 2 p + half; a word's bytes: (half, p), its nibbles: the two rows
+    q = rows(q, 8)
+    q = (q[:, :, :, 0] | (q[:, :, :, 1] << 4)).view(E, strips, 2, 8, units, 2, 2, 4, 2, 2, 2)
+    # e, strip, tile, g, unit, chunk, h, t, j, p, half -> e, strip, unit, tile, chunk, g, t, h, j, half, p
+    q = q.permute(0, 1, 4, 2, 5, 3, 7, 6, 8, 10, 9).contiguous().view(E, strips, units, 2048)
 
     def grouped(v, fill):
-        v = torch.nn.functional.pad(v, (0, groups - v.shape[-1]), value=fill)
-        return rows(v, fill).permute(0, 1, 4, 3, 2).contiguous().view(E, tiles, groups, 16)
+        v = torch.nn.functional.pad(v, (0, units * 128 // group - v.shape[-1]), value=fill)
+        v = rows(v, fill).view(E, strips, 2, 2, 8, units, 128 // group)
+        return v.permute(0, 1, 5, 2, 6, 4, 3).contiguous().view(E, strips, units, 2, 128 // group, 16)
 
     return q, grouped(scales, 0), None if zeros is None else grouped(zeros, 8)
 

@@ -37,24 +37,16 @@ def decode_layout(q, s, z, N, k, group, gate_up):
     """W [E, N, k] from the laid-out tensors, word by word as csrc/mk_w4.cuh states the order."""
     q, s = q.numpy(), s.float().numpy()
     z = np.full_like(s, 8) if z is None else z.numpy().astype(np.float32)
-    E, tiles, chunks, _ = q.shape
-    words = q.reshape(E, tiles, chunks, 32, 16).view(np.uint32)              # [.., lane, word]
-    w = np.zeros((E, tiles * 16, chunks * 64), np.float32)
-    for lane in range(32):
+    E, strips, units, _ = q.shape
+    words = q.reshape(E, strips, units, 2, 2, 32, 16).view(np.uint32)        # [.., tile, chunk, lane, word]
+    w = np.zeros((E, strips * 32, units * 128), np.float32)
+    for tile, chunk, lane, h, j, i, half in np.ndindex(2, 2, 32, 2, 2, 4, 2):
         g, t = lane >> 2, lane & 3
-        for h in range(2):
-            for j in range(2):
-                word = words[:, :, :, lane, 2 * h + j]
-                for i in range(4):
-                    for half in range(2):
-                        code = (word >> (4 * i + 16 * half)) & 15
-                        r = g + 8 * (i & 1)
-                        kk = 32 * h + 8 * t + 4 * j + 2 * (i >> 1) + half
-                        for c in range(chunks):
-                            grp = (64 * c + kk) // group
-                            sc, ze = s[:, :, grp, 2 * g + (i & 1)], z[:, :, grp, 2 * g + (i & 1)]
-                            rows = (np.arange(tiles) * 16 + r) if not gate_up else np.arange(tiles) * 16 + 2 * g + (i & 1)
-                            w[:, rows, 64 * c + kk] = sc * (code[:, :, c].astype(np.float32) - ze)
+        code = (words[:, :, :, tile, chunk, lane, 2 * h + j] >> (4 * i + 16 * half)) & 15
+        kk = 64 * chunk + 32 * h + 8 * t + 4 * j + 2 * (i >> 1) + half
+        sc, ze = (v[:, :, :, tile, kk // group, 2 * g + (i & 1)] for v in (s, z))
+        row = 16 * tile + (2 * g + (i & 1) if gate_up else g + 8 * (i & 1))
+        w[:, row::32, kk::128] = sc * (code.astype(np.float32) - ze)
     return w[:, :N, :k], w
 
 
