@@ -94,6 +94,10 @@ __device__ __forceinline__ void cp16_if(bool p, uint32_t dst, const void* src) {
       "@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst), "l"(src), "r"((uint32_t)p)
       : "memory");
 }
+// the first `bytes` (0..16) of 16, then zeros
+__device__ __forceinline__ void cp16_part(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
@@ -145,16 +149,16 @@ __device__ __forceinline__ void half_chunk(const Masks& m, uint32_t w0, uint32_t
   for (int n = 0; n < NT; ++n) D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].z, xb[n].w);
 }
 
-// tot += scale (rows g, g + 8) * acc
-template <class D, int NT>
-__device__ __forceinline__ void fold(uint32_t scale, const float (&acc)[NT][4], float (&tot)[NT][4]) {
+// tot += scale (rows g, g + 8) * acc (* cw, the columns' weights)
+template <class D, int NT, bool CW>
+__device__ __forceinline__ void fold(uint32_t scale, const float2 (&cw)[NT], const float (&acc)[NT][4], float (&tot)[NT][4]) {
   const float2 s = D::to_f32(scale);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    tot[n][0] = fmaf(s.x, acc[n][0], tot[n][0]);
-    tot[n][1] = fmaf(s.x, acc[n][1], tot[n][1]);
-    tot[n][2] = fmaf(s.y, acc[n][2], tot[n][2]);
-    tot[n][3] = fmaf(s.y, acc[n][3], tot[n][3]);
+    tot[n][0] = fmaf(CW ? s.x * cw[n].x : s.x, acc[n][0], tot[n][0]);
+    tot[n][1] = fmaf(CW ? s.x * cw[n].y : s.x, acc[n][1], tot[n][1]);
+    tot[n][2] = fmaf(CW ? s.y * cw[n].x : s.y, acc[n][2], tot[n][2]);
+    tot[n][3] = fmaf(CW ? s.y * cw[n].y : s.y, acc[n][3], tot[n][3]);
   }
 }
 
