@@ -9,9 +9,13 @@
 // E, E + 1, ... with weight 1 follow each token's topk. A logit of -inf scores 0; a NaN counts as
 // -inf, +inf logits of a softmax share its probability.
 //
-// One warp per token: lane l holds experts l V .. l V + V - 1 (V = ceil(E / 32) rounded to a built
-// width) in registers, so one pass reads the logits and everything else is shuffles: topk rounds of
-// one redux over order-preserving integer keys and one ballot for the lowest lane that has it.
+// One warp per token: lane l holds experts l V .. l V + V - 1 in registers, V the smallest built width
+// with 32 V >= E, so one pass reads the logits (16 bytes a lane at a time where they are aligned)
+// and the rest is registers and shuffles. The selection ranks few candidates instead of sorting: no
+// expert below the topk-th best of the 32 lanes' best ones can be among the topk, so the experts at
+// or above that (about 1.5 topk for scores spread over the lanes) go to shared memory, one to a lane,
+// and a lane counts how many are better than its own. More than 32 of them (long ties, more topk than
+// lanes with experts) are taken one by one instead.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -36,6 +40,8 @@ struct Args {
   float* weights;
   int t, e, topk, n_group, topk_group, gsize, forced;
   uint32_t gmul;        // ceil(2^20 / gsize): e / gsize = e * gmul >> 20 for e < 512
+  int lanes;            // log2 of the lanes that hold a group, or -1 (a lane's experts are of several)
+  int vec;              // rows may be read a lane's share at a time
   float scaling;
   int sigmoid, top2, renorm;
 };
@@ -44,121 +50,204 @@ __device__ __forceinline__ float ninf() { return -__int_as_float(0x7F800000); }
 // unsigned order of the key = order of the float; every float's key is above 0
 __device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t u = __float_as_uint(v);
-  return (u >> 31) ? ~u : u | 0x80000000u;
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float logistic(float x) { return __frcp_rn(__fadd_rn(1.0f, expf(-x))); }
 
-template <typename L>
-__device__ __forceinline__ float load(const L* p);
-template <>
-__device__ __forceinline__ float load<float>(const float* p) { return *p; }
-template <>
-__device__ __forceinline__ float load<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+// V values from p, aligned to the largest power of two (at most 16 bytes) that divides their size
+template <typename L, int V>
+__device__ __forceinline__ void load_lane(const L* p, float (&s)[V]) {
+  constexpr int BYTES = V * sizeof(L), STEP = BYTES % 16 == 0 ? 16 : BYTES % 8 == 0 ? 8 : BYTES % 4 == 0 ? 4 : 2;
+  L v[V];
+#pragma unroll
+  for (int i = 0; i < BYTES / STEP; ++i) {
+    const char* src = reinterpret_cast<const char*>(p) + i * STEP;
+    char* dst = reinterpret_cast<char*>(v) + i * STEP;
+    if (STEP == 16) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+    else if (STEP == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
+    else if (STEP == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+    else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) s[i] = to_f32(v[i]);
+}
 
 template <typename L, int V>
 __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
-  __shared__ float cs[WARPS][V * 32];
+  __shared__ __align__(16) uint64_t shared[WARPS][V * 32 > 64 ? V * 16 : 32];   // scores of the groups, or candidates
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t tok = (int64_t)blockIdx.x * WARPS + warp;
   if (tok >= a.t) return;
   const L* row = static_cast<const L*>(a.logits) + tok * a.ld;
-  float s[V], c[V];
+  float c[V];           // logits, then the selection's values
+  if (a.vec) {
+    if (lane * V < a.e) {
+      load_lane<L, V>(row + lane * V, c);
+    } else {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = lane * V + i;
-    s[i] = e < a.e ? load<L>(row + e) : ninf();
-    if (isnan(s[i])) s[i] = ninf();
+      for (int i = 0; i < V; ++i) c[i] = ninf();
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) c[i] = lane * V + i < a.e ? to_f32(row[lane * V + i]) : ninf();
   }
-  float sum = 1.0f;   // what a score is divided by
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (isnan(c[i])) c[i] = ninf();
+  float sum = 1.0f, m = 0.0f;   // of a softmax
   if (a.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-s[i])));
+    for (int i = 0; i < V; ++i) c[i] = logistic(c[i]);
   } else {
-    float m = ninf();
+    m = ninf();
 #pragma unroll
-    for (int i = 0; i < V; ++i) m = fmaxf(m, s[i]);
+    for (int i = 0; i < V; ++i) m = fmaxf(m, c[i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
     sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      s[i] = m == ninf() ? 0.0f : s[i] == m ? 1.0f : expf(s[i] - m);
-      sum += s[i];
+      c[i] = m == ninf() ? 0.0f : c[i] == m ? 1.0f : expf(c[i] - m);
+      sum += c[i];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
     if (sum == 0.0f) sum = 1.0f;
   }
+  if (a.bias) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = lane * V + i;
-    c[i] = s[i];
-    if (a.bias && e < a.e) c[i] = __fadd_rn(a.sigmoid ? s[i] : __fdiv_rn(s[i], sum), a.bias[e]);
-    if (isnan(c[i])) c[i] = ninf();
-  }
-  uint32_t kept = FULL;
-  if (a.n_group > 1) {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (lane * V + i < a.e) cs[warp][lane * V + i] = c[i];
-    __syncwarp();
-    float score = ninf();
-    if (lane < a.n_group) {
-      float m1 = ninf(), m2 = ninf();
-      for (int i = 0; i < a.gsize; ++i) {
-        const float v = cs[warp][lane * a.gsize + i];
-        m2 = fmaxf(m2, fminf(m1, v));
-        m1 = fmaxf(m1, v);
-      }
-      score = a.top2 && a.gsize > 1 ? __fadd_rn(m1, m2) : m1;
-      if (isnan(score)) score = ninf();
+    for (int i = 0; i < V; ++i) {
+      const int e = lane * V + i;
+      if (e < a.e) c[i] = __fadd_rn(a.sigmoid ? c[i] : __fdiv_rn(c[i], sum), a.bias[e]);
+      if (isnan(c[i])) c[i] = ninf();
     }
-    int better = 0;
-    for (int j = 0; j < a.n_group; ++j) {
-      const float o = __shfl_sync(FULL, score, j);
-      better += o > score || (o == score && j < lane);
-    }
-    kept = __ballot_sync(FULL, lane < a.n_group && better < a.topk_group);
   }
   uint32_t key[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const uint32_t e = lane * V + i, grp = e * a.gmul >> 20;
-    key[i] = e < (uint32_t)a.e && (kept >> (grp & 31) & 1) ? key_of(c[i]) : 0u;
-  }
-  int my_id = 0;
-  float my_s = 0.0f;
-  for (int k = 0; k < a.topk; ++k) {
-    uint32_t best = 0;
+  for (int i = 0; i < V; ++i) key[i] = lane * V + i < a.e ? key_of(c[i]) : 0u;
+  if (a.n_group > 1) {
+    const bool top2 = a.top2 && a.gsize > 1;
+    float score = ninf();
+    int mine, stride;     // this lane's group; the lane of group j is j * stride
+    if (a.lanes >= 0) {
+      float m1 = ninf(), m2 = ninf();
 #pragma unroll
-    for (int i = 0; i < V; ++i) best = max(best, key[i]);
-    const uint32_t top = __reduce_max_sync(FULL, best);
-    const int who = __ffs(__ballot_sync(FULL, best == top)) - 1;
-    int at = 0;
-    float sc = 0.0f;
-    bool done = false;
+      for (int i = 0; i < V; ++i) {
+        m2 = fmaxf(m2, fminf(m1, c[i]));
+        m1 = fmaxf(m1, c[i]);
+      }
+      for (int o = 1; o < 1 << a.lanes; o <<= 1) {
+        const float o1 = __shfl_xor_sync(FULL, m1, o), o2 = __shfl_xor_sync(FULL, m2, o);
+        m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
+        m1 = fmaxf(m1, o1);
+      }
+      score = top2 ? __fadd_rn(m1, m2) : m1;
+      mine = lane >> a.lanes;
+      stride = 1 << a.lanes;
+    } else {
+      float* cs = reinterpret_cast<float*>(shared[warp]);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (lane * V + i < a.e) cs[lane * V + i] = c[i];
+      __syncwarp();
+      if (lane < a.n_group) {
+        float m1 = ninf(), m2 = ninf();
+        for (int i = 0; i < a.gsize; ++i) {
+          const float v = cs[lane * a.gsize + i];
+          m2 = fmaxf(m2, fminf(m1, v));
+          m1 = fmaxf(m1, v);
+        }
+        score = top2 ? __fadd_rn(m1, m2) : m1;
+      }
+      __syncwarp();
+      mine = lane;
+      stride = 1;
+    }
+    if (isnan(score)) score = ninf();
+    int better = 0;
+    for (int j = 0; j < a.n_group; ++j) {
+      const float o = __shfl_sync(FULL, score, j * stride);
+      better += o > score || (o == score && j < mine);
+    }
+    const bool keep = mine < a.n_group && better < a.topk_group;
+    const uint32_t kept = __ballot_sync(FULL, keep);   // by lane, or by group
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (!done && key[i] == top) {
-        at = i;
-        sc = s[i];
-        done = true;
-        if (lane == who) key[i] = 0;
-      }
-    const int id = __shfl_sync(FULL, lane * V + at, who);
-    const float w = __shfl_sync(FULL, sc, who);
-    if (lane == k) { my_id = id; my_s = w; }
+      if (a.lanes >= 0 ? !keep : !(kept >> (((lane * V + i) * a.gmul >> 20) & 31) & 1)) key[i] = 0;
+  }
+  // the topk-th best of the lanes' best (equal ones leave together: fewer than topk may stay above it)
+  uint32_t best = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) best = max(best, key[i]);
+  uint32_t least = 1;
+  for (int k = 0; k < a.topk; ++k) {
+    const uint32_t top = __reduce_max_sync(FULL, best);
+    least = max(top, 1u);
+    if (best == top) best = 0;
+  }
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) count += key[i] >= least;
+  int upto = count;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(FULL, upto, o);
+    if (lane >= o) upto += v;
+  }
+  const int total = __shfl_sync(FULL, upto, 31);
+  int id = 0;
+  if (total <= 32) {
+    uint64_t* cand = shared[warp];    // (key, the higher the lower the expert)
+    int at = upto - count;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (key[i] >= least) cand[at++] = (uint64_t)key[i] << 32 | (uint32_t)~(lane * V + i);
+    __syncwarp();
+    const uint64_t mine = lane < total ? cand[lane] : 0;
+    int rank = 0;
+    for (int j = 0; j < total; ++j) rank += cand[j] > mine;
+    __syncwarp();
+    int* ranked = reinterpret_cast<int*>(cand);
+    if (lane < total && rank < a.topk) ranked[rank] = ~(uint32_t)mine;
+    __syncwarp();
+    if (lane < a.topk) id = ranked[lane];
+  } else {
+    for (int k = 0; k < a.topk; ++k) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) most = max(most, key[i]);
+      const uint32_t top = __reduce_max_sync(FULL, most);
+      const int who = __ffs(__ballot_sync(FULL, most == top)) - 1;
+      int at = 0;
+#pragma unroll
+      for (int i = V - 1; i >= 0; --i)
+        if (key[i] == top) at = i;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (lane == who && i == at) key[i] = 0;
+      const int winner = __shfl_sync(FULL, lane * V + at, who);
+      if (lane == k) id = winner;
+    }
   }
   const bool mine = lane < a.topk;
-  float w = mine && !a.sigmoid ? __fdiv_rn(my_s, sum) : my_s;
+  float w = 0.0f;
+  if (mine) {           // the score again, from its logit
+    float x = to_f32(row[id]);
+    if (isnan(x)) x = ninf();
+    if (a.sigmoid) w = logistic(x);
+    else w = __fdiv_rn(m == ninf() ? 0.0f : x == m ? 1.0f : expf(x - m), sum);
+  }
   if (a.renorm) {
-    float all = mine ? w : 0.0f;
+    float all = w;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(FULL, all, o);
     w = all == 0.0f ? 0.0f : __fdiv_rn(w, all);
   }
   const int64_t o = tok * (a.topk + a.forced);
   if (mine) {
-    a.ids[o + lane] = my_id;
+    a.ids[o + lane] = id;
     a.weights[o + lane] = w * a.scaling;
   }
   if (lane < a.forced) {
@@ -169,17 +258,26 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
 
 int fail(int code, const char* msg) { return mk::set_last_error(code, msg); }
 
+template <typename L, int V>
+cudaError_t launch_width(Args a, cudaStream_t s) {
+  // a lane's share as vectors: its size's largest power of two up to 16 divides the rows' starts, and no
+  // lane's share crosses the row's end
+  constexpr int BYTES = V * sizeof(L), STEP = BYTES % 16 == 0 ? 16 : BYTES % 8 == 0 ? 8 : BYTES % 4 == 0 ? 4 : 2;
+  a.vec = a.e % V == 0 && (uintptr_t)a.logits % STEP == 0 && a.ld * (int64_t)sizeof(L) % STEP == 0;
+  a.lanes = -1;
+  if (a.gsize % V == 0)
+    for (int l = 0; l <= 5; ++l)
+      if (a.gsize / V == 1 << l) a.lanes = l;
+  route_kernel<L, V><<<(unsigned)((a.t + WARPS - 1) / WARPS), WARPS * 32, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
 template <typename L>
 cudaError_t launch(const Args& a, cudaStream_t s) {
-  const unsigned grid = (unsigned)((a.t + WARPS - 1) / WARPS);
   const int v = (a.e + 31) / 32;
-  if (v <= 1) route_kernel<L, 1><<<grid, WARPS * 32, 0, s>>>(a);
-  else if (v <= 2) route_kernel<L, 2><<<grid, WARPS * 32, 0, s>>>(a);
-  else if (v <= 4) route_kernel<L, 4><<<grid, WARPS * 32, 0, s>>>(a);
-  else if (v <= 5) route_kernel<L, 5><<<grid, WARPS * 32, 0, s>>>(a);
-  else if (v <= 8) route_kernel<L, 8><<<grid, WARPS * 32, 0, s>>>(a);
-  else route_kernel<L, 16><<<grid, WARPS * 32, 0, s>>>(a);
-  return cudaGetLastError();
+  return v <= 1 ? launch_width<L, 1>(a, s) : v <= 2 ? launch_width<L, 2>(a, s) : v <= 3 ? launch_width<L, 3>(a, s)
+       : v <= 4 ? launch_width<L, 4>(a, s) : v <= 5 ? launch_width<L, 5>(a, s) : v <= 6 ? launch_width<L, 6>(a, s)
+       : v <= 8 ? launch_width<L, 8>(a, s) : v <= 12 ? launch_width<L, 12>(a, s) : launch_width<L, 16>(a, s);
 }
 
 }  // namespace

@@ -165,14 +165,6 @@ def _ptr(t):
     return t.data_ptr()
 
 
-def stream_of(t):
-    """The handle of the current stream of tensor t's device: where torch's own operators on t run."""
-    import torch
-    if not t.is_cuda:
-        raise MkError(MK_EINVAL, f"tensors are on a CUDA device, not {t.device}")
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
-
-
 def on_stream(t, stream):
     """A context with `stream` (a torch stream, or a raw handle on tensor t's device) current, so that
     what a call allocates belongs to the stream that uses it."""
@@ -182,22 +174,26 @@ def on_stream(t, stream):
     return torch.cuda.stream(stream)
 
 
-class on_device_of:
-    """With t's device current (the library launches on the current device)."""
+_entries = {}
 
-    def __init__(self, t):
-        self.index = t.device.index
 
-    def __enter__(self):
+def entry(name):
+    """(the library's function `name`, the current device, the current stream's handle on a device,
+    the context that makes a device current): what a call on torch tensors needs, looked up once."""
+    e = _entries.get(name)
+    if e is None:
         import torch
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
+        e = _entries[name] = (getattr(lib(), name), torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream,
+                              torch.cuda.device)
+    return e
 
-    def __exit__(self, *exc):
-        import torch
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
+
+def off_device(name, index, context, again):
+    """again() with CUDA device `index` current; raises for tensors that are on none."""
+    if index < 0:
+        raise MkError(MK_EINVAL, f"{name}: tensors are on a CUDA device")
+    with context(index):
+        return again()
 
 
 def make_op(type_, flags=0, ptrs=None, ips=None, fps=None, ntasks=0):

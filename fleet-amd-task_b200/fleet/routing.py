@@ -27,12 +27,9 @@ def _params(experts, topk, n_forced, n_group, topk_group, group_score, score, re
     return p, ctypes.addressof(p)
 
 
-def _out(t, shape, dtype, like, name):
-    if t is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != like.device:
-        raise ValueError(f"{name}: contiguous {dtype} {shape} on {like.device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t
+def _given(t, shape, dtype, device, name):
+    if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name}: contiguous {dtype} {shape} on {device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def route_experts(logits, topk, *, score="softmax", bias=None, n_group=1, topk_group=1, group_score="max",
@@ -58,16 +55,29 @@ def route_experts(logits, topk, *, score="softmax", bias=None, n_group=1, topk_g
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError(f"logits [T, E] with unit stride along E expected, got {tuple(logits.shape)}, strides {logits.stride()}")
     T, E = logits.shape
-    _, params = _params(E, topk, n_forced, n_group, topk_group, group_score, score, renormalize, logits.dtype, scaling)
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,) or not bias.is_contiguous() or
-                             bias.device != logits.device):
-        raise ValueError(f"bias: contiguous float32 [{E}] on {logits.device} expected, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
-    s = mk.stream_of(logits)
-    shape = (T, topk + n_forced)
-    ids = _out(ids, shape, torch.int32, logits, "ids")
-    weights = _out(weights, shape, torch.float32, logits, "weights")
-    with mk.on_device_of(logits):
-        rc = mk.lib().mk_route(params, logits.data_ptr(), logits.stride(0), T, None if bias is None else bias.data_ptr(),
-                               ids.data_ptr(), weights.data_ptr(), s)
-    mk._check(rc, "mk_route")
+    params = _params(E, topk, n_forced, n_group, topk_group, group_score, score, renormalize, logits.dtype, scaling)[1]
+    call, device, current_stream, context = mk.entry("mk_route")
+    index = logits.get_device()
+    if index < 0 or device() != index:
+        return mk.off_device("mk_route", index, context, lambda: route_experts(
+            logits, topk, score=score, bias=bias, n_group=n_group, topk_group=topk_group, group_score=group_score,
+            renormalize=renormalize, scaling=scaling, n_forced=n_forced, ids=ids, weights=weights))
+    b = 0
+    if bias is not None:
+        if (bias.dtype is not torch.float32 or bias.shape != (E,) or not bias.is_contiguous() or bias.get_device() != index):
+            raise ValueError(f"bias: contiguous float32 [{E}] on {logits.device} expected, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+        b = bias.data_ptr()
+    k = topk + n_forced
+    shape = (T, k)
+    if ids is None:
+        ids = torch.empty_strided(shape, (k, 1), dtype=torch.int32, device=logits.device)
+    else:
+        _given(ids, shape, torch.int32, logits.device, "ids")
+    if weights is None:
+        weights = torch.empty_strided(shape, (k, 1), dtype=torch.float32, device=logits.device)
+    else:
+        _given(weights, shape, torch.float32, logits.device, "weights")
+    rc = call(params, logits.data_ptr(), logits.stride(0), T, b, ids.data_ptr(), weights.data_ptr(), current_stream(index))
+    if rc:
+        mk._check(rc, "mk_route")
     return ids, weights

@@ -75,18 +75,25 @@ class W4Weight:
         if any(v is not None and v.device != codes.device for v in (scales, zeros)):
             raise ValueError("codes, scales and zeros are on one device")
         self.n, self.k, self.group, self.experts, self.dtype, self.device = N, k, group, E, scales.dtype, codes.device
+        self.index = -1 if codes.device.index is None else codes.device.index
         self.codes, self.scales, self.zeros = lay_out(codes, scales, zeros, k, group, gate_up)
         self.c = mk.MkW4(self.codes.data_ptr(), self.scales.data_ptr(), mk._ptr(self.zeros), N, k, group,
                          DTYPES[scales.dtype], E, 0)
         self.ptr = ctypes.addressof(self.c)
 
 
-def _rows(t, shape, dtypes, device, name):
-    """The row stride of a 2-D tensor of unit column stride."""
-    if tuple(t.shape) != shape or t.dtype not in dtypes or t.device != device or (shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name}: {' or '.join(map(str, dtypes))} {shape} with unit stride along its rows on {device} "
-                         f"expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()} on {t.device}")
-    return t.stride(0)
+def _fits(t, shape, dtype, index):
+    """The row stride of t if it is `shape` of dtype on CUDA device `index` (-1: the CPU) with unit column
+    stride, or None."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != index:
+        return None
+    rows, cols = t.stride()
+    return rows if cols == 1 or shape[1] == 1 else None
+
+
+def _refuse(t, shape, dtypes, device, name):
+    raise ValueError(f"{name}: {' or '.join(map(str, dtypes))} {shape} with unit stride along its rows on {device} "
+                     f"expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()} on {t.device}")
 
 
 def _span(t):
@@ -98,7 +105,9 @@ def _span(t):
 def _out(out, shape, dtypes, device, x, residual):
     """The row stride of a caller's output: rows apart from one another and from x, and the residual's
     own rows or none of them."""
-    ld = _rows(out, shape, dtypes, device, "out")
+    ld = _fits(out, shape, out.dtype, -1 if device.index is None else device.index)
+    if ld is None or out.dtype not in dtypes:
+        _refuse(out, shape, dtypes, device, "out")
     if shape[0] > 1 and ld < shape[1]:
         raise ValueError(f"out: rows overlap (stride {ld}, {shape[1]} values)")
     lo, hi = _span(out)
@@ -127,24 +136,34 @@ class W4Linear:
             with mk.on_stream(x, stream):
                 return self(x, out, residual, out_dtype)
         w = self.w
+        call, device, current_stream, context = mk.entry("mk_w4_linear")
+        n, index, dtype = w.n, w.index, w.dtype
+        if index < 0 or device() != index:
+            return mk.off_device("mk_w4_linear", index, context, lambda: self(x, out, residual, out_dtype))
         T = x.shape[0] if x.dim() == 2 else -1
-        shape = (T, w.n)
-        ldx = _rows(x, (T, w.k), (w.dtype,), w.device, "x")
-        ldr = 0 if residual is None else _rows(residual, shape, (w.dtype,), w.device, "residual")
+        ldx = _fits(x, (T, w.k), dtype, index)
+        if ldx is None:
+            _refuse(x, ("T", w.k), (dtype,), w.device, "x")
+        shape = (T, n)
+        res = ldr = 0
+        if residual is not None:
+            ldr = _fits(residual, shape, dtype, index)
+            if ldr is None:
+                _refuse(residual, shape, (dtype,), w.device, "residual")
+            res = residual.data_ptr()
         if out is None:
-            if out_dtype is not None and out_dtype != w.dtype and out_dtype != torch.float32:
-                raise ValueError(f"out_dtype is {w.dtype} or float32, not {out_dtype}")
-            out = torch.empty(shape, dtype=out_dtype or w.dtype, device=w.device)
-            ldo = w.n
+            if out_dtype is None:
+                out_dtype = dtype
+            elif out_dtype is not dtype and out_dtype is not torch.float32:
+                raise ValueError(f"out_dtype is {dtype} or float32, not {out_dtype}")
+            out, ldo = torch.empty_strided(shape, (n, 1), dtype=out_dtype, device=w.device), n
         else:
             if out_dtype is not None and out_dtype != out.dtype:
                 raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
-            ldo = _out(out, shape, (w.dtype, torch.float32), w.device, x, residual)
-        s = mk.stream_of(x)
-        with mk.on_device_of(x):
-            rc = mk.lib().mk_w4_linear(w.ptr, x.data_ptr(), ldx, T, mk._ptr(residual), ldr, out.data_ptr(), ldo,
-                                       int(out.dtype == torch.float32), s)
-        mk._check(rc, "mk_w4_linear")
+            ldo, out_dtype = _out(out, shape, (dtype, torch.float32), w.device, x, residual), out.dtype
+        rc = call(w.ptr, x.data_ptr(), ldx, T, res, ldr, out.data_ptr(), ldo, out_dtype is torch.float32, current_stream(index))
+        if rc:
+            mk._check(rc, "mk_w4_linear")
         return out
 
 
@@ -187,26 +206,35 @@ class W4Experts:
             with mk.on_stream(x, stream):
                 return self(x, ids, weights, residual, out)
         w = self.w13
+        call, device, current_stream, context = mk.entry("mk_w4_experts")
+        H, index, dtype = self.hidden, w.index, w.dtype
+        if index < 0 or device() != index:
+            return mk.off_device("mk_w4_experts", index, context, lambda: self(x, ids, weights, residual, out))
         T = x.shape[0] if x.dim() == 2 else -1
-        shape = (T, self.hidden)
-        ldx = _rows(x, shape, (w.dtype,), w.device, "x")
-        ldr = 0 if residual is None else _rows(residual, shape, (w.dtype,), w.device, "residual")
-        if ids.dim() != 2 or ids.shape[0] != T or ids.dtype != torch.int32 or not ids.is_contiguous() or ids.device != w.device:
+        shape = (T, H)
+        ldx = _fits(x, shape, dtype, index)
+        if ldx is None:
+            _refuse(x, ("T", H), (dtype,), w.device, "x")
+        slots = (T, ids.shape[1] if ids.dim() == 2 else -1)
+        if _fits(ids, slots, torch.int32, index) is None or not ids.is_contiguous():
             raise ValueError(f"ids: contiguous int32 [{T}, S] on {w.device} expected, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
-        if weights.shape != ids.shape or weights.dtype != torch.float32 or not weights.is_contiguous() or weights.device != w.device:
-            raise ValueError(f"weights: contiguous float32 {tuple(ids.shape)} on {w.device} expected, got {weights.dtype} "
+        if _fits(weights, slots, torch.float32, index) is None or not weights.is_contiguous():
+            raise ValueError(f"weights: contiguous float32 {slots} on {w.device} expected, got {weights.dtype} "
                              f"{tuple(weights.shape)} on {weights.device}")
+        res = ldr = 0
+        if residual is not None:
+            ldr = _fits(residual, shape, dtype, index)
+            if ldr is None:
+                _refuse(residual, shape, (dtype,), w.device, "residual")
+            res = residual.data_ptr()
         if out is None:
-            out = torch.empty(shape, dtype=w.dtype, device=w.device)
-            ldo = self.hidden
+            out, ldo = torch.empty_strided(shape, (H, 1), dtype=dtype, device=w.device), H
         else:
-            ldo = _out(out, shape, (w.dtype,), w.device, x, residual)
-        s = mk.stream_of(x)
-        S = ids.shape[1]
-        nbytes = self.workspace_bytes(T, S)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
-        with mk.on_device_of(x):
-            rc = mk.lib().mk_w4_experts(self.w13.ptr, self.w2.ptr, x.data_ptr(), ldx, ids.data_ptr(), weights.data_ptr(), T, S,
-                                        mk._ptr(residual), ldr, out.data_ptr(), ldo, ws.data_ptr(), nbytes, s)
-        mk._check(rc, "mk_w4_experts")
+            ldo = _out(out, shape, (dtype,), w.device, x, residual)
+        nbytes = self._need.get(slots) or self.workspace_bytes(*slots)
+        ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=w.device)
+        rc = call(w.ptr, self.w2.ptr, x.data_ptr(), ldx, ids.data_ptr(), weights.data_ptr(), T, slots[1], res, ldr,
+                  out.data_ptr(), ldo, ws.data_ptr(), nbytes, current_stream(index))
+        if rc:
+            mk._check(rc, "mk_w4_experts")
         return out
