@@ -41,7 +41,7 @@ struct Args {
   int t, e, topk, n_group, topk_group, gsize, forced;
   uint32_t gmul;        // ceil(2^20 / gsize): e / gsize = e * gmul >> 20 for e < 512
   int lanes;            // log2 of the lanes that hold a group, or -1 (a lane's experts are of several)
-  int vec;              // rows may be read a lane's share at a time
+  int vec, bias_vec;    // rows, the bias may be read a lane's share at a time
   float scaling;
   int sigmoid, top2, renorm;
 };
@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
   const int64_t tok = (int64_t)blockIdx.x * WARPS + warp;
   if (tok >= a.t) return;
   const L* row = static_cast<const L*>(a.logits) + tok * a.ld;
+  const int past = lane * V + V - a.e;     // above 0: this lane's last `past` places hold no expert
   float c[V];           // logits, then the selection's values
   if (a.vec) {
     if (lane * V < a.e) {
@@ -94,8 +95,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
     for (int i = 0; i < V; ++i) c[i] = lane * V + i < a.e ? to_f32(row[lane * V + i]) : ninf();
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    if (isnan(c[i])) c[i] = ninf();
+  for (int i = 0; i < V; ++i) c[i] = fmaxf(c[i], ninf());   // a NaN is the other argument's loss
   float sum = 1.0f, m = 0.0f;   // of a softmax
   if (a.sigmoid) {
 #pragma unroll
@@ -117,16 +117,27 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
     if (sum == 0.0f) sum = 1.0f;
   }
   if (a.bias) {
+    float b[V];
+    if (a.bias_vec && past <= 0) {
+      load_lane<float, V>(a.bias + lane * V, b);
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = lane * V + i;
-      if (e < a.e) c[i] = __fadd_rn(a.sigmoid ? c[i] : __fdiv_rn(c[i], sum), a.bias[e]);
-      if (isnan(c[i])) c[i] = ninf();
+      for (int i = 0; i < V; ++i) b[i] = lane * V + i < a.e ? a.bias[lane * V + i] : 0.0f;
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i) c[i] = fmaxf(__fadd_rn(a.sigmoid ? c[i] : __fdiv_rn(c[i], sum), b[i]), ninf());
   }
   uint32_t key[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) key[i] = lane * V + i < a.e ? key_of(c[i]) : 0u;
+  for (int i = 0; i < V; ++i) key[i] = key_of(c[i]);
+  if (past > 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i >= V - past) {
+        key[i] = 0;
+        c[i] = ninf();
+      }
+  }
   if (a.n_group > 1) {
     const bool top2 = a.top2 && a.gsize > 1;
     float score = ninf();
@@ -181,12 +192,13 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
   uint32_t best = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) best = max(best, key[i]);
-  uint32_t least = 1;
+  uint32_t least = 0;
+#pragma unroll 2
   for (int k = 0; k < a.topk; ++k) {
-    const uint32_t top = __reduce_max_sync(FULL, best);
-    least = max(top, 1u);
-    if (best == top) best = 0;
+    least = __reduce_max_sync(FULL, best);
+    best = best == least ? 0 : best;
   }
+  least = max(least, 1u);
   int count = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) count += key[i] >= least;
@@ -201,13 +213,18 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
   if (total <= 32) {
     uint64_t* cand = shared[warp];    // (key, the higher the lower the expert)
     int at = upto - count;
+    cand[lane] = 0;                   // below every candidate
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (key[i] >= least) cand[at++] = (uint64_t)key[i] << 32 | (uint32_t)~(lane * V + i);
     __syncwarp();
     const uint64_t mine = lane < total ? cand[lane] : 0;
     int rank = 0;
-    for (int j = 0; j < total; ++j) rank += cand[j] > mine;
+    for (int j = 0; j < total; j += 4) {
+      const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(cand + j), v = *reinterpret_cast<const ulonglong2*>(cand + j + 2);
+      rank += (u.x > mine) + (u.y > mine) + (v.x > mine) + (v.y > mine);
+    }
     __syncwarp();
     int* ranked = reinterpret_cast<int*>(cand);
     if (lane < total && rank < a.topk) ranked[rank] = ~(uint32_t)mine;
@@ -234,8 +251,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const Args a) {
   const bool mine = lane < a.topk;
   float w = 0.0f;
   if (mine) {           // the score again, from its logit
-    float x = to_f32(row[id]);
-    if (isnan(x)) x = ninf();
+    const float x = fmaxf(to_f32(row[id]), ninf());
     if (a.sigmoid) w = logistic(x);
     else w = __fdiv_rn(m == ninf() ? 0.0f : x == m ? 1.0f : expf(x - m), sum);
   }
@@ -264,6 +280,8 @@ cudaError_t launch_width(Args a, cudaStream_t s) {
   // lane's share crosses the row's end
   constexpr int BYTES = V * sizeof(L), STEP = BYTES % 16 == 0 ? 16 : BYTES % 8 == 0 ? 8 : BYTES % 4 == 0 ? 4 : 2;
   a.vec = a.e % V == 0 && (uintptr_t)a.logits % STEP == 0 && a.ld * (int64_t)sizeof(L) % STEP == 0;
+  constexpr int BSTEP = V % 4 == 0 ? 16 : V % 2 == 0 ? 8 : 4;
+  a.bias_vec = (uintptr_t)a.bias % BSTEP == 0;
   a.lanes = -1;
   if (a.gsize % V == 0)
     for (int l = 0; l <= 5; ++l)
