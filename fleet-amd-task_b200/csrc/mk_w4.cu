@@ -137,14 +137,14 @@ int device_sms(int* device, int* sms) {
 }
 
 // about `items` items over the SMs; known: exactly that many
-int launch_weight(Args& a, const MkW4* w, int64_t items, bool known, bool through_ring, int sms, cudaStream_t s) {
+int launch_weight(Args& a, const MkW4* w, int64_t items, bool known, bool xr, int sms, cudaStream_t s) {
   const int strips = (w->n + STRIP_ROWS - 1) / STRIP_ROWS;
   // enough strips for every CTA: two tiles a warp share the activations
-  const bool two = items * strips >= 2 * sms && !(through_ring && !two_tiles_fit_ring(a.cols));
+  const bool two = items * strips >= 2 * sms && !(xr && a.cols > 8);
   a.strips = div_by(two ? strips : 2 * strips);
   const int grid = (int)(known ? std::min<int64_t>(sms, items * a.strips.d) : sms);
-  return w->dtype == MK_W4_BF16 ? launch_bf16(a, w->group, two, through_ring, grid, s)
-                                : launch_fp16(a, w->group, two, through_ring, grid, s);
+  return w->dtype == MK_W4_BF16 ? launch_bf16(a, w->group, two, xr, grid, s)
+                                : launch_fp16(a, w->group, two, xr, grid, s);
 }
 
 bool aligned16(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
@@ -211,10 +211,10 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   // even blocks of at most 16 tokens
   const int blocks = (t + MAX_COLS - 1) / MAX_COLS;
   a.tb = (t + blocks - 1) / blocks;
-  const bool through_ring = a.x_vec && !fits(a.units.d, a.tb);
-  if (!through_ring)
+  const bool xr = a.x_vec && w->k % 8 == 0 && !fits(a.units.d, a.tb);
+  if (!xr)
     while (a.tb > 1 && !fits(a.units.d, a.tb)) --a.tb;
-  if (!through_ring && !fits(a.units.d, a.tb)) return fail(MK_EINVAL, "rows that are not 16-byte aligned are too long for the shared memory");
+  if (!xr && !fits(a.units.d, a.tb)) return fail(MK_EINVAL, "rows that are not 16-byte aligned are too long for the shared memory");
   a.n_items = (t + a.tb - 1) / a.tb;
   a.cols = a.tb;
   a.residual = static_cast<const uint16_t*>(residual);
@@ -223,7 +223,7 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   a.ldo = ldo;
   a.out_f32 = out_f32;
   if ((int64_t)a.n_items * (w->n / 16 + 2) * a.units.d > INT32_MAX / 2) return fail(MK_EINVAL, "too many tokens times weights");
-  return launch_weight(a, w, a.n_items, true, through_ring, sms, static_cast<cudaStream_t>(stream));
+  return launch_weight(a, w, a.n_items, true, xr, sms, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mk_w4_experts_workspace(const MkW4* w13, const MkW4* w2, int32_t t, int32_t slots, int64_t* bytes) {

@@ -15,7 +15,8 @@
 //          k = 64 chunk + 32 h + 8 t + 4 j + (0..3): bits 4i..4i+3 (k even) and 16+4i.. (k odd) are,
 //          for i = 0..3, (row g, k 0/1), (row g + 8, k 0/1), (row g, k 2/3), (row g + 8, k 2/3): the
 //          four A registers of one MMA, two codes each, a shift and one AND-OR from a 16-bit float
-//   scales [experts][strips][units][2 tiles][128 / G groups][8][2]: rows g and g + 8 side by side
+//   scales [experts][strips][units][2 tiles][8][128 / G groups][2]: for g the groups' scales of rows g
+//          and g + 8, one load a lane
 //   zeros  the same, bytes, or none
 // The MMA's k slots are a permutation of the values (lane t of a quad has 8 consecutive ones of each
 // 32), the same one for the activations: a sum does not ask for their order, and a lane's share of
@@ -84,82 +85,82 @@ struct Fp16 {
   }
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// weights are read once: past L1
+__device__ __forceinline__ uint4 ldg128(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
-// the same if p (no branch)
-__device__ __forceinline__ void cp16_if(bool p, uint32_t dst, const void* src) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t"
-      "@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst), "l"(src), "r"((uint32_t)p)
-      : "memory");
+// N (1, 2 or 4) words
+template <int N>
+__device__ __forceinline__ void ldg_words(const void* p, uint32_t (&v)[N]) {
+  if (N == 4) {
+    const uint4 q = ldg128(p);
+    v[0] = q.x, v[N > 1 ? 1 : 0] = q.y, v[N > 2 ? 2 : 0] = q.z, v[N > 3 ? 3 : 0] = q.w;
+  } else if (N == 2) {
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[N > 1 ? 1 : 0]) : "l"(p));
+  } else {
+    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v[0]) : "l"(p));
+  }
 }
-// the first `bytes` (0..16) of 16, then zeros
-__device__ __forceinline__ void cp16_part(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ uint32_t ldg16(const void* p) {
+  uint16_t v;
+  asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(v) : "l"(p));
+  return v;
+}
+// activations that other CTAs of the launch's predecessor wrote
+__device__ __forceinline__ uint4 ldg128_x(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t at) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
   return v;
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t at) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
-  return v;
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint32_t lds16(uint32_t at) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// (w & mask) | magic in one instruction: both constants in registers (an instruction takes one
+// (w & 0x000F000F) | magic in one instruction: the magic in a register (an instruction takes one
 // immediate, and the compiler would otherwise spend two)
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t magic) {
   uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(mask), "r"(magic));
+  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(d) : "r"(w), "r"(magic));
   return d;
 }
 
-struct Masks {
-  uint32_t low, magic;
-};
 template <class D>
-__device__ __forceinline__ Masks masks() {
-  Masks m;
-  asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(m.low));
-  asm volatile("mov.b32 %0, %1;" : "=r"(m.magic) : "n"(D::MAGIC));
+__device__ __forceinline__ uint32_t magic_register() {
+  uint32_t m;
+  asm volatile("mov.b32 %0, %1;" : "=r"(m) : "n"(D::MAGIC));
   return m;
 }
 
 // one word's four A registers: codes to 16-bit floats, their zero points taken off (exact)
 template <class D>
-__device__ __forceinline__ void decode(const Masks& m, uint32_t w, uint32_t z0, uint32_t z1, uint32_t (&a)[4]) {
-  a[0] = D::sub2(and_or(w, m.low, m.magic), z0);
-  a[1] = D::sub2(and_or(w >> 4, m.low, m.magic), z1);
-  a[2] = D::sub2(and_or(w >> 8, m.low, m.magic), z0);
-  a[3] = D::sub2(and_or(w >> 12, m.low, m.magic), z1);
+__device__ __forceinline__ void decode(uint32_t magic, uint32_t w, uint32_t z0, uint32_t z1, uint32_t (&a)[4]) {
+  a[0] = D::sub2(and_or(w, magic), z0);
+  a[1] = D::sub2(and_or(w >> 4, magic), z1);
+  a[2] = D::sub2(and_or(w >> 8, magic), z0);
+  a[3] = D::sub2(and_or(w >> 12, magic), z1);
 }
 
 // 32 values of K: two words against each column tile's 16 bytes of activations; FIRST: acc = instead
 // of acc +=
 template <class D, int NT, bool FIRST>
-__device__ __forceinline__ void half_chunk(const Masks& m, uint32_t w0, uint32_t w1, uint32_t z0, uint32_t z1, const uint4 (&xb)[NT],
+__device__ __forceinline__ void half_chunk(uint32_t magic, uint32_t w0, uint32_t w1, uint32_t z0, uint32_t z1, const uint4 (&xb)[NT],
                                            float (&acc)[NT][4]) {
   uint32_t a[4];
-  decode<D>(m, w0, z0, z1, a);
+  decode<D>(magic, w0, z0, z1, a);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     if (FIRST) D::mma0(acc[n], a[0], a[1], a[2], a[3], xb[n].x, xb[n].y);
     else D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].x, xb[n].y);
   }
-  decode<D>(m, w1, z0, z1, a);
+  decode<D>(magic, w1, z0, z1, a);
 #pragma unroll
   for (int n = 0; n < NT; ++n) D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].z, xb[n].w);
 }

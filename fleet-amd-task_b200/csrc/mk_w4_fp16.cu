@@ -1,6 +1,6 @@
 // mk_w4_fp16.cu -- the products with 4-bit weights for FP16 activations.
 #include "mk_w4_kernel.cuh"
 
-int w4::launch_fp16(const Args& a, int group, bool two, bool through_ring, int grid, cudaStream_t s) {
-  return two ? launch_group<Fp16, 2>(a, group, through_ring, grid, s) : launch_group<Fp16, 1>(a, group, through_ring, grid, s);
+int w4::launch_fp16(const Args& a, int group, bool two, bool xr, int grid, cudaStream_t s) {
+  return two ? launch_group<Fp16, 2>(a, group, xr, grid, s) : launch_group<Fp16, 1>(a, group, xr, grid, s);
 }

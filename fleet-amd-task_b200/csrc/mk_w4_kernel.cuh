@@ -30,14 +30,6 @@ enum Mode {
   DOWN_SMALL = 4     // one item; a strip's units run over all selected experts; x: act as above
 };
 
-// a warp's step: a unit of RT tiles
-template <int RT, int G, bool ZP>
-struct Shape {
-  static constexpr int GROUPS = UNIT_K / G;          // per unit
-  static constexpr int SCALES = RT * GROUPS * 32, ZEROS = ZP ? RT * GROUPS * 16 : 0;
-  static constexpr int STAGE = RT * TILE_UNIT_BYTES + SCALES + ZEROS;   // without activations
-};
-
 // n / d for 0 <= n < 2^31 by one multiplication: with k = 31 + ceil(log2 d), m = ceil(2^k / d) is off by
 // less than d / 2^k of itself, so n m / 2^k is off by less than 1 / d
 struct Div {
@@ -60,7 +52,7 @@ struct Args {
   Div strips;               // of RT tiles, per weight
   Div units, nv;            // units of K; 16-byte pieces of a staged row (16 units)
   int rows, k, experts;
-  int mode, depth;          // depth: stages of a warp's ring, 2, 4 or 8
+  int mode;
   int device;
   int n_items;              // LINEAR
   const int* items_n;       // GATEUP, DOWN: the plan
@@ -159,41 +151,35 @@ __device__ __forceinline__ void stage_x(const Args& a, uint4* xs, int start, int
   }
 }
 
-// at most n copies of this thread's newest stay in flight
-__device__ __forceinline__ void wait_older(int n) {
-  if (n <= 2) {
-    if (n == 2) cp_wait<2>();
-    else cp_wait<1>();
-  } else if (n <= 4) {
-    if (n == 4) cp_wait<4>();
-    else cp_wait<3>();
-  } else {
-    if (n == 8) cp_wait<8>();
-    else cp_wait<7>();
-  }
-}
-
-// XR: the activations travel through the ring; SMALL2: DOWN_SMALL
+// XR: the activations are loaded with each unit instead of staged; SMALL2: DOWN_SMALL
 template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2>
 struct Kernel {
-  using S = Shape<RT, G, ZP>;
+  static constexpr int GROUPS = UNIT_K / G, ZWORDS = GROUPS / 2 > 0 ? GROUPS / 2 : 1;
+  // units a warp has in flight while it computes another: what its registers hold
+  static constexpr int AHEAD = RT == 2 || (XR && NT == 2) ? 2 : 3;
+
+  // a unit of RT tiles in registers
+  struct Unit {
+    uint4 w[RT][2];
+    uint32_t sc[RT][GROUPS];
+    uint32_t z[RT][ZP ? ZWORDS : 1];
+    uint4 x[XR ? 4 : 1][XR ? NT : 1];
+  };
+
   const Args& a;
-  Masks m;
+  uint32_t magic;
   int warp, lane, g, t;
-  uint32_t ring_s;
-  int stage;                     // bytes of a stage
   uint4* xs;
   float* slots;                  // [WARPS][RT NT 4][32]: the parts of strips that an earlier warp began
   float* cw;                     // SMALL2: [experts][16] the tokens' weights
   const SmallPlan* plan;
   int U;                         // units of a strip's sums (SMALL2: over all selected experts)
-  // the copy cursor: the next unit to copy, the last one's end, the run of consecutive bytes it is in
+  // the load cursor: the next unit to load, the last one's end, the run of consecutive bytes it is in
   int cp, cp_end, run;
-  const uint8_t *code = nullptr, *meta = nullptr, *xsrc = nullptr;
-  int x_k;                       // XR LINEAR: the unit's first value
-  bool scale_lane, zero_lane;
+  const uint8_t *code, *scale, *zero;
+  const uint16_t* x_at[XR ? NT : 1];
+  int x_k;                       // XR LINEAR: the lane's first value of the unit
   int item_start, item_count;    // the columns (XR: of every item)
-  uint32_t slot;
 
   __device__ __forceinline__ Kernel(const Args& args) : a(args) {}
 
@@ -218,43 +204,49 @@ struct Kernel {
     const int pairs = RT == 2 ? a.strips.d : a.strips.d >> 1;
     const int64_t first = (int64_t)((expert * pairs + pair) * a.units.d + u) * 2 + half;      // in tiles' units
     code = a.codes + first * TILE_UNIT_BYTES + lane * 16;
-    if (scale_lane) meta = a.scales + first * (S::GROUPS * 32) + lane * 16;
-    else if (zero_lane) meta = a.zeros + first * (S::GROUPS * 16) + (lane - S::SCALES / 16) * 16;
+    scale = a.scales + first * (GROUPS * 32) + g * (GROUPS * 4);
+    if (ZP) zero = a.zeros + first * (GROUPS * 16) + g * (GROUPS * 2);
     if (XR) {
-      if (SMALL2) xsrc = reinterpret_cast<const uint8_t*>(a.x) + ((int64_t)(item * a.units.d + u) * item_count * 16 + lane) * 16;
-      else xsrc = reinterpret_cast<const uint8_t*>(a.x + (int64_t)(item_start + (lane >> 4)) * a.ldx + u * UNIT_K + (lane & 15) * 8);
-      x_k = u * UNIT_K + (lane & 15) * 8;
-    }
-  }
-  __device__ __forceinline__ void copy_x(uint32_t dst, bool on) {
-    if (SMALL2) {   // already in the MMA's order
-      for (int i = lane; i < item_count * 16; i += 32) cp16_if(on, dst + i * 16, xsrc + (i - lane) * 16);
-    } else {        // lane: a 16-byte piece of a column's 256 bytes; two columns a step
-      const int left = min(max(2 * (a.k - x_k), 0), 16), piece = lane & 15;
-      for (int col = lane >> 4; col < item_count; col += 2) {
-        const uint32_t to = dst + (((piece >> 2) * item_count + col) * 4 + (piece & 3)) * 16;
-        if (on) cp16_part(to, left > 0 ? xsrc + (int64_t)(col - (lane >> 4)) * a.ldx * 2 : reinterpret_cast<const uint8_t*>(a.x), left);
+      x_k = u * UNIT_K + t * 8;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {   // a lane past the columns takes the last one's: its sums are not used
+        const int col = min(i * 8 + g, item_count - 1);
+        x_at[i] = SMALL2 ? a.x + (((int64_t)(item * a.units.d + u) * 4 * item_count + col) * 4 + t) * 8
+                         : a.x + (int64_t)(item_start + col) * a.ldx + x_k;
       }
     }
   }
-  template <bool WITH_X>
-  __device__ __forceinline__ void issue(uint32_t dst) {
-    const bool on = cp < cp_end;
+  __device__ __forceinline__ void load(Unit& n) {
+    if (cp >= cp_end) return;
 #pragma unroll
-    for (int i = 0; i < RT * 2; ++i) cp16_if(on, dst + i * 512 + lane * 16, code + i * 512);
-    cp16_if(on && (scale_lane || zero_lane), dst + RT * TILE_UNIT_BYTES + lane * 16, meta);
-    if (XR && WITH_X) copy_x(dst + S::STAGE, on);
-    cp_commit();
-    ++cp;
-    code += 2 * TILE_UNIT_BYTES;
-    meta += 2 * S::GROUPS * (scale_lane ? 32 : 16);
+    for (int r = 0; r < RT; ++r) {
+      n.w[r][0] = ldg128(code + r * TILE_UNIT_BYTES);
+      n.w[r][1] = ldg128(code + r * TILE_UNIT_BYTES + 512);
+      ldg_words<GROUPS>(scale + r * (GROUPS * 32), n.sc[r]);
+      if (ZP) {
+        if (GROUPS == 1) n.z[r][0] = ldg16(zero + r * 16);
+        else ldg_words<ZP ? ZWORDS : 1>(zero + r * (GROUPS * 16), n.z[r]);
+      }
+    }
     if (XR) {
-      xsrc += SMALL2 ? item_count * 256 : UNIT_K * 2;
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          if (SMALL2) n.x[h][i] = ldg128_x(x_at[i] + h * item_count * 32);
+          else if (x_k + 32 * h < a.k) n.x[h][i] = ldg128_x(x_at[i] + 32 * h);
+          else n.x[h][i] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) x_at[i] += SMALL2 ? item_count * 128 : UNIT_K;
       x_k += UNIT_K;
     }
+    code += 2 * TILE_UNIT_BYTES;
+    scale += 2 * GROUPS * 32;
+    if (ZP) zero += 2 * GROUPS * 16;
+    ++cp;
     if (--run == 0 && cp < cp_end) locate();
   }
-
   // where warp w's units of a phase begin
   static __device__ __forceinline__ int part_of(int p0, int n, int w) {
     return p0 + (n / WARPS) * w + n % WARPS * w / WARPS;
@@ -312,85 +304,78 @@ struct Kernel {
       }
   }
 
-  // the units [p, p_end) of the phase that begins at unit p0 and has n units; at most 8 NT columns
-  __device__ __forceinline__ void units(int p, const int p_end, const int p0, const int n) {
+  // tot += the unit's products; staged activations at shared address xl + x_off
+  __device__ __forceinline__ void multiply(const Unit& n, const uint32_t (&xl)[NT], uint32_t x_off, uint32_t x_h,
+                                           const float2 (&w2)[NT], float (&tot)[RT][NT][4]) {
+    float acc[RT][NT][4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      uint4 xb[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) xb[i] = XR ? n.x[XR ? h : 0][XR ? i : 0] : lds128(xl[i] + x_off + h * x_h);
+      const int i = h * 32 / G;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        uint32_t z0 = D::MAGIC + 0x00080008u, z1 = z0;
+        if (ZP) {   // rows g and g + 8 of group i: two bytes
+          const uint32_t z = n.z[r][i / 2] >> (i % 2 * 16);
+          z0 = (z & 0xFFu) * 0x00010001u | D::MAGIC;
+          z1 = (z >> 8 & 0xFFu) * 0x00010001u | D::MAGIC;
+        }
+        const uint4& v = n.w[r][h >> 1];
+        if (h * 32 % G == 0) half_chunk<D, NT, true>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
+        else half_chunk<D, NT, false>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
+        if ((h + 1) * 32 % G == 0) fold<D, NT, SMALL2>(n.sc[r][i], w2, acc[r], tot[r]);
+      }
+    }
+  }
+
+  // the units [p, p_end) of the phase that begins at unit p0 and has n units; at most 8 NT columns.
+  // un holds the first AHEAD of them.
+  __device__ __forceinline__ void units(Unit (&un)[AHEAD], int p, const int p_end, const int p0, const int n) {
     constexpr int WORDS = RT * NT * 4;
     float tot[RT][NT][4];
     // a lane past the columns reads the last one's activations: its sums are not used
     uint32_t xl[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
-      xl[i] = (XR ? ring_s + S::STAGE : (uint32_t)__cvta_generic_to_shared(xs)) + (min(i * 8 + g, item_count - 1) * 4 + t) * 16;
-    const uint32_t x_h = item_count * 64, x_u = item_count * 256;
+      xl[i] = XR ? 0 : (uint32_t)__cvta_generic_to_shared(xs) + (min(i * 8 + g, item_count - 1) * 4 + t) * 16;
+    const uint32_t x_h = item_count * 64;
     bool met = false;                     // this warp has been at the barrier
-    int strip_flat = 0;
+    int next = 0;                         // the place in un of the next unit
     while (p < p_end) {
-      strip_flat = by_u(p);
+      const int strip_flat = by_u(p);
       const int q0 = p - strip_flat * U, q1 = min(U, q0 + p_end - p);
 #pragma unroll
       for (int i = 0; i < WORDS; ++i) (&tot[0][0][0])[i] = 0.0f;
-      uint32_t x_at = XR ? 0 : q0 * x_u;
+      uint32_t x_off = q0 * x_h * 4;
       float2 w2[NT];
-      int to_expert = 0, expert = 0;        // SMALL2: units to the next expert, its place in the plan
+      int to_expert = 0, expert = 0;      // SMALL2: units to the next expert, its place in the plan
+      auto weigh = [&]() {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) w2[i] = *reinterpret_cast<const float2*>(cw + expert * MAX_COLS + i * 8 + 2 * t);
+      };
       if (SMALL2) {
         expert = q0 / a.units;
         to_expert = (expert + 1) * a.units.d - q0;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) w2[i] = *reinterpret_cast<const float2*>(cw + expert * MAX_COLS + i * 8 + 2 * t);
+        weigh();
       }
-      for (int q = q0; q < q1; ++q) {
-        wait_older(a.depth - 1);
-        __syncwarp();
-        const uint32_t st = ring_s + slot;
-        uint4 w[RT][2], xr[XR ? 4 : 1][NT];
-        uint32_t sc[RT][S::GROUPS], z0[RT][S::GROUPS], z1[RT][S::GROUPS];
+      int left = q1 - q0;
+      while (left > 0) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          w[r][0] = lds128(st + lane * 16 + r * TILE_UNIT_BYTES);
-          w[r][1] = lds128(st + lane * 16 + r * TILE_UNIT_BYTES + 512);
-#pragma unroll
-          for (int i = 0; i < S::GROUPS; ++i) {
-            sc[r][i] = lds32(st + g * 4 + RT * TILE_UNIT_BYTES + (r * S::GROUPS + i) * 32);
-            if (ZP) {
-              const uint32_t z = lds16(st + g * 2 + RT * TILE_UNIT_BYTES + S::SCALES + (r * S::GROUPS + i) * 16);
-              z0[r][i] = (z & 0xFFu) * 0x00010001u | D::MAGIC;
-              z1[r][i] = (z >> 8) * 0x00010001u | D::MAGIC;
-            } else {
-              z0[r][i] = z1[r][i] = D::MAGIC + 0x00080008u;
+        for (int i = 0; i < AHEAD; ++i) {
+          if (next == i && left > 0) {
+            multiply(un[i], xl, x_off, x_h, w2, tot);
+            load(un[i]);
+            next = i + 1 == AHEAD ? 0 : i + 1;
+            --left;
+            x_off += x_h * 4;
+            if (SMALL2 && --to_expert == 0 && left > 0) {
+              to_expert = a.units.d;
+              ++expert;
+              weigh();
             }
           }
-        }
-        if (XR) {
-#pragma unroll
-          for (int h = 0; h < 4; ++h)
-#pragma unroll
-            for (int i = 0; i < NT; ++i) xr[h][i] = lds128(xl[i] + slot + h * x_h);
-        }
-        __syncwarp();            // every lane has read the stage
-        issue<true>(ring_s + slot);
-        slot += stage;
-        if (slot == (uint32_t)(a.depth * stage)) slot = 0;
-        float acc[RT][NT][4];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          uint4 xb[NT];
-#pragma unroll
-          for (int i = 0; i < NT; ++i) xb[i] = XR ? xr[XR ? h : 0][i] : lds128(xl[i] + x_at + h * x_h);
-          const int i = h * 32 / G;
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const uint4& v = w[r][h >> 1];
-            if (h * 32 % G == 0) half_chunk<D, NT, true>(m, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0[r][i], z1[r][i], xb, acc[r]);
-            else half_chunk<D, NT, false>(m, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0[r][i], z1[r][i], xb, acc[r]);
-            if ((h + 1) * 32 % G == 0) fold<D, NT, SMALL2>(sc[r][i], w2, acc[r], tot[r]);
-          }
-        }
-        if (!XR) x_at += x_u;
-        if (SMALL2 && --to_expert == 0 && q + 1 < q1) {
-          to_expert = a.units.d;
-          ++expert;
-#pragma unroll
-          for (int i = 0; i < NT; ++i) w2[i] = *reinterpret_cast<const float2*>(cw + expert * MAX_COLS + i * 8 + 2 * t);
         }
       }
       p += q1 - q0;
@@ -418,14 +403,8 @@ struct Kernel {
 
   __device__ __forceinline__ void run_all(uint8_t* smem, SmallPlan& sp) {
     warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    m = masks<D>();
-    constexpr int NS = S::SCALES / 16, NZ = S::ZEROS / 16;
-    static_assert(NS + NZ <= 32, "one copy a lane");
-    scale_lane = lane < NS;
-    zero_lane = ZP && lane >= NS && lane < NS + NZ;
-    stage = S::STAGE + (XR ? a.cols * UNIT_K * 2 : 0);
-    ring_s = (uint32_t)__cvta_generic_to_shared(smem + warp * (a.depth * stage));
-    uint8_t* after = smem + WARPS * (a.depth * stage);
+    magic = magic_register<D>();
+    uint8_t* after = smem;
     slots = reinterpret_cast<float*>(after);
     after += WARPS * RT * NT * 4 * 32 * 4;
     xs = reinterpret_cast<uint4*>(after);
@@ -485,23 +464,20 @@ struct Kernel {
       cp = p;
       cp_end = p_end;
       run = 0;
-      slot = 0;
       if (p < p_end) locate();
       if (staged) __syncthreads();   // every warp is done with the last phase's activations and parts
+      if (!XR) stage_x(a, xs, item_start, item_count);
+      Unit un[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) load(un[i]);
       if (!XR) {
-        stage_x(a, xs, item_start, item_count);
-        cp_commit();
-      }
-      for (int s = 0; s < a.depth; ++s) issue<true>(ring_s + s * stage);
-      if (!XR) {
-        wait_older(a.depth);
+        cp_wait_all();
         __syncthreads();
       }
       staged = true;
-      units(p, p_end, p0, n);
+      units(un, p, p_end, p0, n);
       from = to;
     }
-    cp_wait<0>();
   }
 };
 
@@ -513,30 +489,19 @@ __global__ void __launch_bounds__(THREADS, 1) w4_kernel(const Args a) {
   k.run_all(smem, plan);
 }
 
-// bytes beside rings and activations: the parts and the small plan (static)
+// shared memory: the parts of strips, a small batch's weights, the plan (static), the activations
 constexpr int parts_bytes(int rt, int cols) { return WARPS * rt * (cols <= 8 ? 1 : 2) * 4 * 32 * 4; }
-constexpr int STATIC_BYTES = (sizeof(SmallPlan) + 1023) / 1024 * 1024;
-// a ring of two stages of two tiles, for the group size and zero points that take most
-constexpr int LEAST_RING = WARPS * 2 * Shape<2, 32, true>::STAGE;
-
-// whether the activations of `cols` columns can be staged beside the least ring
-inline bool fits(int units, int cols) {
-  return LEAST_RING + parts_bytes(2, cols) + STATIC_BYTES + (int64_t)cols * units * UNIT_K * 2 <= SMEM_LIMIT;
-}
-
-// beside a ring that carries the activations: the weights of a small batch's slots
 constexpr int CW_BYTES = SMALL_SLOTS * MAX_COLS * 4;
-inline bool two_tiles_fit_ring(int cols) {
-  return WARPS * 2 * (Shape<2, 32, true>::STAGE + cols * UNIT_K * 2) + parts_bytes(2, cols) + CW_BYTES + STATIC_BYTES <= SMEM_LIMIT;
+constexpr int STATIC_BYTES = (sizeof(SmallPlan) + 1023) / 1024 * 1024;
+
+// whether the activations of `cols` columns can be staged
+inline bool fits(int units, int cols) {
+  return parts_bytes(2, cols) + STATIC_BYTES + (int64_t)cols * units * UNIT_K * 2 <= SMEM_LIMIT;
 }
 
 template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2>
-static int launch(Args a, int grid, cudaStream_t s) {
-  using S = Shape<RT, G, ZP>;
-  const int stage = S::STAGE + (XR ? a.cols * UNIT_K * 2 : 0);
-  const int64_t rest = parts_bytes(RT, a.cols) + (SMALL2 ? CW_BYTES : XR ? 0 : (int64_t)a.cols * a.units.d * UNIT_K * 2);
-  a.depth = 8;
-  while (a.depth > 2 && (int64_t)WARPS * a.depth * stage + rest + STATIC_BYTES > SMEM_LIMIT) a.depth /= 2;
+static int launch(const Args& a, int grid, cudaStream_t s) {
+  const int smem = parts_bytes(RT, a.cols) + (SMALL2 ? CW_BYTES : XR ? 0 : a.cols * a.units.d * UNIT_K * 2);
   const auto kernel = w4_kernel<D, RT, NT, G, ZP, XR, SMALL2>;
   static std::atomic<bool> ready[MAX_DEVICES];   // the kernel may use that much shared memory on the device
   cudaError_t e = cudaSuccess;
@@ -545,16 +510,19 @@ static int launch(Args a, int grid, cudaStream_t s) {
     if (e == cudaSuccess) ready[a.device].store(true, std::memory_order_release);
   }
   if (e == cudaSuccess) {
-    kernel<<<grid, THREADS, (size_t)(WARPS * a.depth * stage + rest), s>>>(a);
+    kernel<<<grid, THREADS, smem, s>>>(a);
     e = cudaGetLastError();
   }
   return e == cudaSuccess ? MK_OK : mk::set_last_error(MK_ECUDA, cudaGetErrorString(e));
 }
 
 template <class D, int RT, int NT, int G, bool ZP>
-static int launch_nt(const Args& a, bool through_ring, int grid, cudaStream_t s) {
-  if (a.mode == DOWN_SMALL) return launch<D, RT, NT, G, ZP, true, true>(a, grid, s);
-  return through_ring ? launch<D, RT, NT, G, ZP, true, false>(a, grid, s) : launch<D, RT, NT, G, ZP, false, false>(a, grid, s);
+static int launch_nt(const Args& a, bool xr, int grid, cudaStream_t s) {
+  if constexpr (RT == 1 || NT == 1) {   // two tiles and two column tiles leave no registers for activations in flight
+    if (a.mode == DOWN_SMALL) return launch<D, RT, NT, G, ZP, true, true>(a, grid, s);
+    if (xr) return launch<D, RT, NT, G, ZP, true, false>(a, grid, s);
+  }
+  return launch<D, RT, NT, G, ZP, false, false>(a, grid, s);
 }
 
 template <class D, int RT, int G, bool ZP>
@@ -569,8 +537,9 @@ static int launch_group(const Args& a, int group, bool xr, int grid, cudaStream_
   return a.zeros ? launch_x<D, RT, 128, true>(a, xr, grid, s) : launch_x<D, RT, 128, false>(a, xr, grid, s);
 }
 
-// mk_w4_bf16.cu, mk_w4_fp16.cu: `two` tiles a warp or one, the activations through the ring or staged
-int launch_bf16(const Args& a, int group, bool two, bool through_ring, int grid, cudaStream_t s);
-int launch_fp16(const Args& a, int group, bool two, bool through_ring, int grid, cudaStream_t s);
+// mk_w4_bf16.cu, mk_w4_fp16.cu: `two` tiles a warp or one (one if more than 8 columns' activations
+// are not staged), the activations loaded with the units (xr) or staged
+int launch_bf16(const Args& a, int group, bool two, bool xr, int grid, cudaStream_t s);
+int launch_fp16(const Args& a, int group, bool two, bool xr, int grid, cudaStream_t s);
 
 }  // namespace w4

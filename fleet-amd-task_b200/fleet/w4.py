@@ -23,7 +23,7 @@ GROUPS = (32, 64, 128)
 
 def lay_out(codes, scales, zeros, k, group, gate_up=False):
     """(codes, scales, zeros) of weights [E, N, K] in the kernels' order (csrc/mk_w4.cuh): codes
-    [E, strips, units, 2048] uint8, scales and zeros [E, strips, units, 2, 128 / group, 16]. gate_up:
+    [E, strips, units, 2048] uint8, scales and zeros [E, strips, units, 2, 8, 128 / group, 2]. gate_up:
     rows 2i / 2i + 1 are gate / up row i (pack_weights.interleave_gate_up) and a tile takes 8 gate
     rows, then their 8 up rows."""
     E, N = codes.shape[:2]
@@ -48,7 +48,8 @@ def lay_out(codes, scales, zeros, k, group, gate_up=False):
     def grouped(v, fill):
         v = torch.nn.functional.pad(v, (0, units * 128 // group - v.shape[-1]), value=fill)
         v = rows(v, fill).view(E, strips, 2, 2, 8, units, 128 // group)
-        return v.permute(0, 1, 5, 2, 6, 4, 3).contiguous().view(E, strips, units, 2, 128 // group, 16)
+        # e, strip, tile, row half, g, unit, group -> e, strip, unit, tile, g, group, row half
+        return v.permute(0, 1, 5, 2, 4, 6, 3).contiguous().view(E, strips, units, 2, 8, 128 // group, 2)
 
     return q, grouped(scales, 0), None if zeros is None else grouped(zeros, 8)
 

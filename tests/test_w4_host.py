@@ -44,7 +44,7 @@ def decode_layout(q, s, z, N, k, group, gate_up):
         g, t = lane >> 2, lane & 3
         code = (words[:, :, :, tile, chunk, lane, 2 * h + j] >> (4 * i + 16 * half)) & 15
         kk = 64 * chunk + 32 * h + 8 * t + 4 * j + 2 * (i >> 1) + half
-        sc, ze = (v[:, :, :, tile, kk // group, 2 * g + (i & 1)] for v in (s, z))
+        sc, ze = (v[:, :, :, tile, g, kk // group, i & 1] for v in (s, z))
         row = 16 * tile + (2 * g + (i & 1) if gate_up else g + 8 * (i & 1))
         w[:, row::32, kk::128] = sc * (code.astype(np.float32) - ze)
     return w[:, :N, :k], w
