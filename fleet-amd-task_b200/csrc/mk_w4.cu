@@ -42,6 +42,7 @@ namespace {
 __global__ void __launch_bounds__(1024) plan_kernel(const int* __restrict__ ids, int t, int s, int experts, int tb,
                                                     int4* items, int* items_n, int* col_token, int* slot_col) {
   __shared__ int cnt[MAX_EXPERTS], first[MAX_EXPERTS];
+  start_dependents();
   const int n = t * s;
   for (int e = threadIdx.x; e < MAX_EXPERTS; e += blockDim.x) cnt[e] = 0;
   __syncthreads();
@@ -86,6 +87,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ 
                                                       const float* __restrict__ weights, int s, int h,
                                                       const uint16_t* residual, int64_t ldr, uint16_t* out, int64_t ldo) {
   const int tok = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
+  wait_predecessor();
   if (j >= h) return;
   float v = residual ? D::one_to_f32(residual[(int64_t)tok * ldr + j]) : 0.0f;
   for (int k = 0; k < s; ++k) {
@@ -140,7 +142,7 @@ int device_sms(int* device, int* sms) {
 int launch_weight(Args& a, const MkW4* w, int64_t items, bool known, bool xr, int sms, cudaStream_t s) {
   const int strips = (w->n + STRIP_ROWS - 1) / STRIP_ROWS;
   // enough strips for every CTA: two tiles a warp share the activations
-  const bool two = items * strips >= 2 * sms && !(xr && a.cols > 8);
+  const bool two = items * strips >= 2 * sms && !(xr && a.cols > 8) && a.cols <= MAX_COLS;
   a.strips = div_by(two ? strips : 2 * strips);
   const int grid = (int)(known ? std::min<int64_t>(sms, items * a.strips.d) : sms);
   return w->dtype == MK_W4_BF16 ? launch_bf16(a, w->group, two, xr, grid, s)
@@ -208,8 +210,9 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   a.x = static_cast<const uint16_t*>(x);
   a.ldx = ldx;
   a.x_vec = aligned16(x, ldx);
-  // even blocks of at most 16 tokens
-  const int blocks = (t + MAX_COLS - 1) / MAX_COLS;
+  // even blocks of at most 16 tokens, or 32 if their activations fit
+  const int most = t > MAX_COLS && fits(a.units.d, 2 * MAX_COLS) ? 2 * MAX_COLS : MAX_COLS;
+  const int blocks = (t + most - 1) / most;
   a.tb = (t + blocks - 1) / blocks;
   const bool xr = a.x_vec && w->k % 8 == 0 && !fits(a.units.d, a.tb);
   if (!xr)
@@ -271,6 +274,7 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
     if (slots)
       if (int rc = launch_weight(a, w13, items_about, false, false, sms, st)) return rc;
     b.mode = DOWN_SMALL;
+    b.follows = slots > 0;
     b.weights = weights;
     b.residual = static_cast<const uint16_t*>(residual);
     b.ldr = ldr;
@@ -284,6 +288,7 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   int* slot_col = reinterpret_cast<int*>(ws + p.slot_col);
   plan_kernel<<<1, 1024, 0, st>>>(ids, t, slots, w13->experts, p.cols, items, items_n, col_token, slot_col);
   a.mode = GATEUP;
+  a.follows = b.follows = 1;
   a.items = b.items = items;
   a.items_n = b.items_n = items_n;
   a.col_token = col_token;
@@ -296,12 +301,8 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   if (int rc = launch_weight(b, w2, items_about, false, false, sms, st)) return rc;
   const dim3 grid((unsigned)((w2->n + 255) / 256), (unsigned)t);
   const float* y = reinterpret_cast<const float*>(ws + p.y);
-  if (w2->dtype == MK_W4_BF16)
-    combine_kernel<Bf16><<<grid, 256, 0, st>>>(y, slot_col, weights, slots, w2->n, static_cast<const uint16_t*>(residual), ldr,
-                                               static_cast<uint16_t*>(out), ldo);
-  else
-    combine_kernel<Fp16><<<grid, 256, 0, st>>>(y, slot_col, weights, slots, w2->n, static_cast<const uint16_t*>(residual), ldr,
-                                               static_cast<uint16_t*>(out), ldo);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_behind(
+      w2->dtype == MK_W4_BF16 ? combine_kernel<Bf16> : combine_kernel<Fp16>, grid, 256, 0, st, true, y, (const int*)slot_col, weights, (int)slots,
+      (int)w2->n, static_cast<const uint16_t*>(residual), ldr, static_cast<uint16_t*>(out), ldo);
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
 }

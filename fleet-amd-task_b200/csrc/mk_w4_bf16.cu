@@ -2,5 +2,5 @@
 #include "mk_w4_kernel.cuh"
 
 int w4::launch_bf16(const Args& a, int group, bool two, bool xr, int grid, cudaStream_t s) {
-  return two ? launch_group<Bf16, 2>(a, group, xr, grid, s) : launch_group<Bf16, 1>(a, group, xr, grid, s);
+  return launch_type<Bf16>(a, group, two, xr, grid, s);
 }

@@ -13,11 +13,11 @@ int set_last_error(int code, const char* msg);   // mk_runtime.cu: the message m
 
 namespace w4 {
 
-constexpr int WARPS = 16, THREADS = WARPS * 32;
+constexpr int MAX_WARPS = 24;
 constexpr int SMEM_LIMIT = 227 * 1024;
 constexpr int MAX_EXPERTS = 1024;
 constexpr int MAX_DEVICES = 64;
-constexpr int MAX_COLS = 16;           // columns of an item
+constexpr int MAX_COLS = 16;           // columns of an item (of a LINEAR: 32)
 constexpr int SMALL_T = MAX_COLS;      // tokens and slots of the two-launch experts
 constexpr int SMALL_SLOTS = 256;
 
@@ -54,6 +54,7 @@ struct Args {
   int rows, k, experts;
   int mode;
   int device;
+  int follows;              // launched behind another launch of the same call
   int n_items;              // LINEAR
   const int* items_n;       // GATEUP, DOWN: the plan
   const int4* items;        // {expert, first column, columns, 0}
@@ -73,6 +74,11 @@ struct Args {
   int out_f32;
 };
 
+// The launches of one call overlap: each lets the next one start while it runs (the next's blocks take
+// SMs as this one's leave them) and waits for its predecessor's results before it reads them.
+__device__ __forceinline__ void wait_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void start_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // the selected experts of a small batch, in the order of their first slots
 struct SmallPlan {
   int first[MAX_EXPERTS];               // an expert's first slot, then its place in the list
@@ -80,7 +86,7 @@ struct SmallPlan {
   float weight[SMALL_SLOTS];
   int expert[SMALL_SLOTS];
   uint32_t tokens[SMALL_SLOTS];         // the tokens that selected it, one bit each
-  int warp_n[WARPS];
+  int warp_n[MAX_WARPS];
   int n;
 };
 
@@ -108,7 +114,7 @@ __device__ __forceinline__ void plan_small(const Args& a, SmallPlan& p) {
       }
       if (lane == 0) p.n = __popc(ballot);
     } else {
-      for (int k = i; k < a.experts; k += THREADS) p.first[k] = SMALL_SLOTS;
+      for (int k = i; k < a.experts; k += blockDim.x) p.first[k] = SMALL_SLOTS;
       if (i < SMALL_SLOTS) p.tokens[i] = 0;
       __syncthreads();
       if (valid) atomicMin(&p.first[e], i);
@@ -123,7 +129,7 @@ __device__ __forceinline__ void plan_small(const Args& a, SmallPlan& p) {
         p.expert[at] = e;
         p.first[e] = at;
       }
-      if (i == THREADS - 1) p.n = at + leads;
+      if (i == (int)blockDim.x - 1) p.n = at + leads;
       __syncthreads();
       if (valid) atomicOr(&p.tokens[p.first[e]], 1u << (i / a.s_div));
     }
@@ -135,7 +141,7 @@ __device__ __forceinline__ void plan_small(const Args& a, SmallPlan& p) {
 __device__ __forceinline__ void stage_x(const Args& a, uint4* xs, int start, int count) {
   const int nv = a.nv.d;
   const uint32_t xs_s = (uint32_t)__cvta_generic_to_shared(xs);
-  for (int i = threadIdx.x; i < count * nv; i += THREADS) {
+  for (int i = threadIdx.x; i < count * nv; i += blockDim.x) {
     const int col = i / a.nv, v = i - col * nv;
     const int row = a.mode == GATEUP ? a.col_token[start + col] : start + col;
     const uint16_t* src = a.x + (int64_t)row * a.ldx + 8 * v;
@@ -151,13 +157,16 @@ __device__ __forceinline__ void stage_x(const Args& a, uint4* xs, int start, int
   }
 }
 
-// XR: the activations are loaded with each unit instead of staged; SMALL2: DOWN_SMALL
-template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2>
+// RT, NT: tiles of 16 rows and 8 columns a warp computes at a time. XR: the activations are loaded with
+// each unit instead of staged. SMALL2: DOWN_SMALL. MIXED: items of up to 8 columns among the wider ones.
+template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2, bool MIXED>
 struct Kernel {
+  // Warps and the units each has in flight. 8 columns: 24 warps of 80 registers, one unit each, its halves
+  // reloaded as they are used; more columns (or too few rows for two tiles a warp): 16 warps of 128
+  static constexpr bool NARROW = NT == 1 && (RT == 2 || XR);
+  static constexpr int WARPS = NARROW ? 24 : 16, THREADS = WARPS * 32;
+  static constexpr int AHEAD = NARROW ? 1 : RT == 2 || NT > 1 ? 2 : 3;
   static constexpr int GROUPS = UNIT_K / G, ZWORDS = GROUPS / 2 > 0 ? GROUPS / 2 : 1;
-  // units a warp has in flight while it computes another: what its registers hold
-  static constexpr int AHEAD = RT == 2 || (XR && NT == 2) ? 2 : 3;
-
   // a unit of RT tiles in registers
   struct Unit {
     uint4 w[RT][2];
@@ -216,11 +225,18 @@ struct Kernel {
       }
     }
   }
-  __device__ __forceinline__ void load(Unit& n) {
+  // the first half of the next unit's codes
+  __device__ __forceinline__ void load_half(Unit& n) {
+    if (cp >= cp_end) return;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) n.w[r][0] = ldg128(code + r * TILE_UNIT_BYTES);
+  }
+  // the next unit; rest: without that half
+  __device__ __forceinline__ void load(Unit& n, bool rest) {
     if (cp >= cp_end) return;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      n.w[r][0] = ldg128(code + r * TILE_UNIT_BYTES);
+      if (!rest) n.w[r][0] = ldg128(code + r * TILE_UNIT_BYTES);
       n.w[r][1] = ldg128(code + r * TILE_UNIT_BYTES + 512);
       ldg_words<GROUPS>(scale + r * (GROUPS * 32), n.sc[r]);
       if (ZP) {
@@ -261,14 +277,15 @@ struct Kernel {
   __device__ __forceinline__ void all_warps() { asm volatile("barrier.sync 1, %0;" ::"n"(THREADS) : "memory"); }
 
   // one finished strip
-  __device__ __forceinline__ void finish(int strip_flat, const float (&tot)[RT][NT][4]) {
+  template <int NB>
+  __device__ __forceinline__ void finish(int strip_flat, const float (&tot)[RT][NB][4]) {
     const int item = SMALL2 ? 0 : strip_flat / a.strips, strip = strip_flat - item * a.strips.d;
     if (!SMALL2 && a.mode == GATEUP_SMALL && strip == a.strips.d - 1) {   // act's padding to whole units is zero
       const int j0 = a.rows / 2, pad = (int)a.ldo * UNIT_K - j0;
       for (int i = lane; i < pad * item_count; i += 32) act_at(item, i / pad, j0 + i % pad) = 0;
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int ci = 0; ci < 2; ++ci) {
         const int col = n * 8 + 2 * t + ci;
@@ -305,14 +322,15 @@ struct Kernel {
   }
 
   // tot += the unit's products; staged activations at shared address xl + x_off
-  __device__ __forceinline__ void multiply(const Unit& n, const uint32_t (&xl)[NT], uint32_t x_off, uint32_t x_h,
-                                           const float2 (&w2)[NT], float (&tot)[RT][NT][4]) {
-    float acc[RT][NT][4];
+  template <int NB>
+  __device__ __forceinline__ void multiply(Unit& n, const uint32_t (&xl)[NB], uint32_t x_off, uint32_t x_h,
+                                           const float2 (&w2)[NB], float (&tot)[RT][NB][4]) {
+    float acc[RT][NB][4];
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      uint4 xb[NT];
+      uint4 xb[NB];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) xb[i] = XR ? n.x[XR ? h : 0][XR ? i : 0] : lds128(xl[i] + x_off + h * x_h);
+      for (int i = 0; i < NB; ++i) xb[i] = XR ? n.x[XR ? h : 0][XR ? i : 0] : lds128(xl[i] + x_off + h * x_h);
       const int i = h * 32 / G;
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
@@ -323,22 +341,24 @@ struct Kernel {
           z1 = (z >> 8 & 0xFFu) * 0x00010001u | D::MAGIC;
         }
         const uint4& v = n.w[r][h >> 1];
-        if (h * 32 % G == 0) half_chunk<D, NT, true>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
-        else half_chunk<D, NT, false>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
-        if ((h + 1) * 32 % G == 0) fold<D, NT, SMALL2>(n.sc[r][i], w2, acc[r], tot[r]);
+        if (h * 32 % G == 0) half_chunk<D, NB, true>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
+        else half_chunk<D, NB, false>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
+        if ((h + 1) * 32 % G == 0) fold<D, NB, SMALL2>(n.sc[r][i], w2, acc[r], tot[r]);
       }
+      if (AHEAD == 1 && h == 1) load_half(n);
     }
   }
 
-  // the units [p, p_end) of the phase that begins at unit p0 and has n units; at most 8 NT columns.
+  // the units [p, p_end) of the phase that begins at unit p0 and has n units; at most 8 NB columns.
   // un holds the first AHEAD of them.
+  template <int NB>
   __device__ __forceinline__ void units(Unit (&un)[AHEAD], int p, const int p_end, const int p0, const int n) {
-    constexpr int WORDS = RT * NT * 4;
-    float tot[RT][NT][4];
+    constexpr int WORDS = RT * NB * 4;
+    float tot[RT][NB][4];
     // a lane past the columns reads the last one's activations: its sums are not used
-    uint32_t xl[NT];
+    uint32_t xl[NB];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < NB; ++i)
       xl[i] = XR ? 0 : (uint32_t)__cvta_generic_to_shared(xs) + (min(i * 8 + g, item_count - 1) * 4 + t) * 16;
     const uint32_t x_h = item_count * 64;
     bool met = false;                     // this warp has been at the barrier
@@ -349,11 +369,11 @@ struct Kernel {
 #pragma unroll
       for (int i = 0; i < WORDS; ++i) (&tot[0][0][0])[i] = 0.0f;
       uint32_t x_off = q0 * x_h * 4;
-      float2 w2[NT];
+      float2 w2[NB];
       int to_expert = 0, expert = 0;      // SMALL2: units to the next expert, its place in the plan
       auto weigh = [&]() {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) w2[i] = *reinterpret_cast<const float2*>(cw + expert * MAX_COLS + i * 8 + 2 * t);
+        for (int i = 0; i < NB; ++i) w2[i] = *reinterpret_cast<const float2*>(cw + expert * MAX_COLS + i * 8 + 2 * t);
       };
       if (SMALL2) {
         expert = q0 / a.units;
@@ -365,8 +385,8 @@ struct Kernel {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
           if (next == i && left > 0) {
-            multiply(un[i], xl, x_off, x_h, w2, tot);
-            load(un[i]);
+            multiply<NB>(un[i], xl, x_off, x_h, w2, tot);
+            load(un[i], AHEAD == 1);
             next = i + 1 == AHEAD ? 0 : i + 1;
             --left;
             x_off += x_h * 4;
@@ -396,7 +416,7 @@ struct Kernel {
           }
         }
       }
-      finish(strip_flat, tot);
+      finish<NB>(strip_flat, tot);
     }
     if (!met) all_warps();
   }
@@ -432,15 +452,18 @@ struct Kernel {
         __syncthreads();
       }
     } else {
+      if (a.follows) wait_predecessor();
       n_items = a.mode == LINEAR ? a.n_items : *a.items_n;
     }
     // the CTA's strips: the first total % grid CTAs have one more
     const int total = n_items * a.strips.d, each = total / (int)gridDim.x, more = total - each * (int)gridDim.x;
     const int lo = each * (int)blockIdx.x + min((int)blockIdx.x, more), hi = lo + each + ((int)blockIdx.x < more);
+    if (SMALL2 && a.follows) wait_predecessor();   // its activations; the plan came from the call's inputs
+    start_dependents();
     if (SMALL2 && U == 0) {   // no slot selects an expert
       for (int strip = lo + warp; strip < hi; strip += WARPS) {
-        float zero[RT][NT][4] = {};
-        finish(strip, zero);
+        const float zero[RT][NT][4] = {};
+        finish<NT>(strip, zero);
       }
       return;
     }
@@ -469,76 +492,94 @@ struct Kernel {
       if (!XR) stage_x(a, xs, item_start, item_count);
       Unit un[AHEAD];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) load(un[i]);
+      for (int i = 0; i < AHEAD; ++i) load(un[i], false);
       if (!XR) {
         cp_wait_all();
         __syncthreads();
       }
       staged = true;
-      units(un, p, p_end, p0, n);
+      if (MIXED && item_count <= 8) units<1>(un, p, p_end, p0, n);
+      else units<NT>(un, p, p_end, p0, n);
       from = to;
     }
   }
 };
 
-template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2>
-__global__ void __launch_bounds__(THREADS, 1) w4_kernel(const Args a) {
+template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2, bool MIXED>
+__global__ void __launch_bounds__(Kernel<D, RT, NT, G, ZP, XR, SMALL2, MIXED>::THREADS, 1) w4_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ SmallPlan plan;
-  Kernel<D, RT, NT, G, ZP, XR, SMALL2> k(a);
+  Kernel<D, RT, NT, G, ZP, XR, SMALL2, MIXED> k(a);
   k.run_all(smem, plan);
 }
 
 // shared memory: the parts of strips, a small batch's weights, the plan (static), the activations
-constexpr int parts_bytes(int rt, int cols) { return WARPS * rt * (cols <= 8 ? 1 : 2) * 4 * 32 * 4; }
+constexpr int PARTS_BYTES = 32 * 1024;     // at most: 16 warps x 4 x 4 (or 24 x 2 x 4) words of 128 bytes
 constexpr int CW_BYTES = SMALL_SLOTS * MAX_COLS * 4;
 constexpr int STATIC_BYTES = (sizeof(SmallPlan) + 1023) / 1024 * 1024;
 
 // whether the activations of `cols` columns can be staged
 inline bool fits(int units, int cols) {
-  return parts_bytes(2, cols) + STATIC_BYTES + (int64_t)cols * units * UNIT_K * 2 <= SMEM_LIMIT;
+  return PARTS_BYTES + STATIC_BYTES + (int64_t)cols * units * UNIT_K * 2 <= SMEM_LIMIT;
 }
 
-template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2>
+template <typename... P>
+cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, bool follows, P... args) {
+  cudaLaunchConfig_t c{};
+  cudaLaunchAttribute overlap[1];
+  c.gridDim = grid;
+  c.blockDim = dim3((unsigned)threads);
+  c.dynamicSmemBytes = (size_t)smem;
+  c.stream = s;
+  overlap[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = overlap;
+  c.numAttrs = follows ? 1 : 0;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
+template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2, bool MIXED>
 static int launch(const Args& a, int grid, cudaStream_t s) {
-  const int smem = parts_bytes(RT, a.cols) + (SMALL2 ? CW_BYTES : XR ? 0 : a.cols * a.units.d * UNIT_K * 2);
-  const auto kernel = w4_kernel<D, RT, NT, G, ZP, XR, SMALL2>;
+  using K = Kernel<D, RT, NT, G, ZP, XR, SMALL2, MIXED>;
+  constexpr int parts = K::WARPS * RT * NT * 4 * 32 * 4;
+  static_assert(parts <= PARTS_BYTES, "the parts of strips");
+  const int smem = parts + (SMALL2 ? CW_BYTES : XR ? 0 : a.cols * a.units.d * UNIT_K * 2);
+  const auto kernel = w4_kernel<D, RT, NT, G, ZP, XR, SMALL2, MIXED>;
   static std::atomic<bool> ready[MAX_DEVICES];   // the kernel may use that much shared memory on the device
   cudaError_t e = cudaSuccess;
   if (!ready[a.device].load(std::memory_order_acquire)) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT - STATIC_BYTES);
     if (e == cudaSuccess) ready[a.device].store(true, std::memory_order_release);
   }
-  if (e == cudaSuccess) {
-    kernel<<<grid, THREADS, smem, s>>>(a);
-    e = cudaGetLastError();
-  }
+  if (e == cudaSuccess) e = launch_behind(kernel, dim3((unsigned)grid), K::THREADS, smem, s, a.follows, a);
   return e == cudaSuccess ? MK_OK : mk::set_last_error(MK_ECUDA, cudaGetErrorString(e));
 }
 
-template <class D, int RT, int NT, int G, bool ZP>
-static int launch_nt(const Args& a, bool xr, int grid, cudaStream_t s) {
-  if constexpr (RT == 1 || NT == 1) {   // two tiles and two column tiles leave no registers for activations in flight
-    if (a.mode == DOWN_SMALL) return launch<D, RT, NT, G, ZP, true, true>(a, grid, s);
-    if (xr) return launch<D, RT, NT, G, ZP, true, false>(a, grid, s);
+// two: two tiles a warp; xr: the activations come with the units (one tile a warp if over 8 columns)
+template <class D, int G, bool ZP>
+static int launch_form(const Args& a, bool two, bool xr, int grid, cudaStream_t s) {
+  const bool small2 = a.mode == DOWN_SMALL;
+  if (a.cols <= 8) {
+    if (small2) return two ? launch<D, 2, 1, G, ZP, true, true, false>(a, grid, s) : launch<D, 1, 1, G, ZP, true, true, false>(a, grid, s);
+    if (xr) return two ? launch<D, 2, 1, G, ZP, true, false, false>(a, grid, s) : launch<D, 1, 1, G, ZP, true, false, false>(a, grid, s);
+    return two ? launch<D, 2, 1, G, ZP, false, false, false>(a, grid, s) : launch<D, 1, 1, G, ZP, false, false, false>(a, grid, s);
   }
-  return launch<D, RT, NT, G, ZP, false, false>(a, grid, s);
+  if (small2) return launch<D, 1, 2, G, ZP, true, true, false>(a, grid, s);
+  if (xr) return launch<D, 1, 2, G, ZP, true, false, false>(a, grid, s);
+  if (a.cols > MAX_COLS) return launch<D, 1, 4, G, ZP, false, false, false>(a, grid, s);
+  if (a.mode == GATEUP || a.mode == DOWN)
+    return two ? launch<D, 2, 2, G, ZP, false, false, true>(a, grid, s) : launch<D, 1, 2, G, ZP, false, false, true>(a, grid, s);
+  return two ? launch<D, 2, 2, G, ZP, false, false, false>(a, grid, s) : launch<D, 1, 2, G, ZP, false, false, false>(a, grid, s);
 }
 
-template <class D, int RT, int G, bool ZP>
-static int launch_x(const Args& a, bool xr, int grid, cudaStream_t s) {
-  return a.cols <= 8 ? launch_nt<D, RT, 1, G, ZP>(a, xr, grid, s) : launch_nt<D, RT, 2, G, ZP>(a, xr, grid, s);
+template <class D>
+static int launch_type(const Args& a, int group, bool two, bool xr, int grid, cudaStream_t s) {
+  if (group == 32) return a.zeros ? launch_form<D, 32, true>(a, two, xr, grid, s) : launch_form<D, 32, false>(a, two, xr, grid, s);
+  if (group == 64) return a.zeros ? launch_form<D, 64, true>(a, two, xr, grid, s) : launch_form<D, 64, false>(a, two, xr, grid, s);
+  return a.zeros ? launch_form<D, 128, true>(a, two, xr, grid, s) : launch_form<D, 128, false>(a, two, xr, grid, s);
 }
 
-template <class D, int RT>
-static int launch_group(const Args& a, int group, bool xr, int grid, cudaStream_t s) {
-  if (group == 32) return a.zeros ? launch_x<D, RT, 32, true>(a, xr, grid, s) : launch_x<D, RT, 32, false>(a, xr, grid, s);
-  if (group == 64) return a.zeros ? launch_x<D, RT, 64, true>(a, xr, grid, s) : launch_x<D, RT, 64, false>(a, xr, grid, s);
-  return a.zeros ? launch_x<D, RT, 128, true>(a, xr, grid, s) : launch_x<D, RT, 128, false>(a, xr, grid, s);
-}
-
-// mk_w4_bf16.cu, mk_w4_fp16.cu: `two` tiles a warp or one (one if more than 8 columns' activations
-// are not staged), the activations loaded with the units (xr) or staged
+// mk_w4_bf16.cu, mk_w4_fp16.cu
 int launch_bf16(const Args& a, int group, bool two, bool xr, int grid, cudaStream_t s);
 int launch_fp16(const Args& a, int group, bool two, bool xr, int grid, cudaStream_t s);
 
