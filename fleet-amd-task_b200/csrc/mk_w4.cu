@@ -149,6 +149,8 @@ int launch_weight(Args& a, const MkW4* w, int64_t items, bool known, bool xr, in
                                 : launch_fp16(a, w->group, two, xr, grid, s);
 }
 
+// 16-bit rows that start at 4-byte boundaries
+bool aligned4(const void* p, int64_t ld) { return ((uintptr_t)p & 3) == 0 && ld % 2 == 0; }
 bool aligned16(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
 
 struct Plan {   // the workspace of mk_w4_experts, in bytes from its start
@@ -167,7 +169,7 @@ const char* plan_experts(const MkW4* w13, const MkW4* w2, int64_t t, int64_t s, 
     if ((int64_t)w->experts * (w->n / STRIP_ROWS + 1) * units_of(w) > INT32_MAX / 2) return "the experts have too many weights";
   if (t < 0 || s < 0 || t * s >= (1 << 24)) return "slots (tokens x slots per token) are from 0 to 2^24 - 1";
   p->small = t <= SMALL_T && t * s <= SMALL_SLOTS && fits(units_of(w13), (int)std::max<int64_t>(t, 1));
-  p->cols = (int)std::min<int64_t>(std::max<int64_t>(t, 1), MAX_COLS);
+  p->cols = (int)std::min<int64_t>(std::max<int64_t>(t, 1), p->small ? MAX_COLS : GROUPED_COLS);
   while (p->cols > 1 && !(fits(units_of(w13), p->cols) && (p->small || fits(units_of(w2), p->cols)))) --p->cols;
   if (!fits(units_of(w13), p->cols) || (!p->small && !fits(units_of(w2), p->cols))) return "rows are too long for the shared memory";
   const int64_t n = std::max<int64_t>(t * s, 1), items = w13->experts + n / p->cols + 1;
@@ -225,6 +227,7 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   a.out = out;
   a.ldo = ldo;
   a.out_f32 = out_f32;
+  a.pairs = !out_f32 && aligned4(out, ldo) && (!residual || aligned4(residual, ldr));
   if ((int64_t)a.n_items * (w->n / 16 + 2) * a.units.d > INT32_MAX / 2) return fail(MK_EINVAL, "too many tokens times weights");
   return launch_weight(a, w, a.n_items, true, xr, sms, static_cast<cudaStream_t>(stream));
 }
@@ -280,6 +283,7 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
     b.ldr = ldr;
     b.out = out;
     b.ldo = ldo;
+    b.pairs = aligned4(out, ldo) && (!residual || aligned4(residual, ldr));
     return launch_weight(b, w2, 1, true, true, sms, st);
   }
   int4* items = reinterpret_cast<int4*>(ws + p.items);

@@ -44,6 +44,7 @@ struct Bf16 {
   }
   static __device__ __forceinline__ float one_to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
   static __device__ __forceinline__ uint16_t round(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+  static __device__ __forceinline__ uint32_t round2(float lo, float hi) { return (uint32_t)round(lo) | (uint32_t)round(hi) << 16; }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -70,6 +71,7 @@ struct Fp16 {
   }
   static __device__ __forceinline__ float one_to_f32(uint16_t v) { return __half2float(__ushort_as_half(v)); }
   static __device__ __forceinline__ uint16_t round(float v) { return __half_as_ushort(__float2half_rn(v)); }
+  static __device__ __forceinline__ uint32_t round2(float lo, float hi) { return (uint32_t)round(lo) | (uint32_t)round(hi) << 16; }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -123,6 +125,13 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// an 8 x 8 matrix of 16-bit values, lane 4 g + t holding columns 2 t, 2 t + 1 of row g, transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
 
 // (w & 0x000F000F) | magic in one instruction: the magic in a register (an instruction takes one
 // immediate, and the compiler would otherwise spend two)

@@ -18,6 +18,7 @@ constexpr int SMEM_LIMIT = 227 * 1024;
 constexpr int MAX_EXPERTS = 1024;
 constexpr int MAX_DEVICES = 64;
 constexpr int MAX_COLS = 16;           // columns of an item (of a LINEAR: 32)
+constexpr int GROUPED_COLS = 8;        // of an expert's item: about what a routed expert gets
 constexpr int SMALL_T = MAX_COLS;      // tokens and slots of the two-launch experts
 constexpr int SMALL_SLOTS = 256;
 
@@ -72,6 +73,7 @@ struct Args {
   void* out;
   int64_t ldo;
   int out_f32;
+  int pairs;                // 16-bit out and residual rows start at 4-byte boundaries
 };
 
 // The launches of one call overlap: each lets the next one start while it runs (the next's blocks take
@@ -158,8 +160,8 @@ __device__ __forceinline__ void stage_x(const Args& a, uint4* xs, int start, int
 }
 
 // RT, NT: tiles of 16 rows and 8 columns a warp computes at a time. XR: the activations are loaded with
-// each unit instead of staged. SMALL2: DOWN_SMALL. MIXED: items of up to 8 columns among the wider ones.
-template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2, bool MIXED>
+// each unit instead of staged. SMALL2: DOWN_SMALL.
+template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2>
 struct Kernel {
   // Warps and the units each has in flight. 8 columns: 24 warps of 80 registers, one unit each, its halves
   // reloaded as they are used; more columns (or too few rows for two tiles a warp): 16 warps of 128
@@ -276,61 +278,103 @@ struct Kernel {
   // a barrier that warps meet at from two places
   __device__ __forceinline__ void all_warps() { asm volatile("barrier.sync 1, %0;" ::"n"(THREADS) : "memory"); }
 
-  // one finished strip
-  template <int NB>
-  __device__ __forceinline__ void finish(int strip_flat, const float (&tot)[RT][NB][4]) {
+  // A finished strip. 16-bit outputs go through a transposition, so that a lane holds two rows (which are
+  // neighbours in memory) of one column: lane 4 g + t rows 2 t, 2 t + 1 of column 8 n + g.
+  __device__ __forceinline__ void finish(int strip_flat, const float (&tot)[RT][NT][4]) {
     const int item = SMALL2 ? 0 : strip_flat / a.strips, strip = strip_flat - item * a.strips.d;
-    if (!SMALL2 && a.mode == GATEUP_SMALL && strip == a.strips.d - 1) {   // act's padding to whole units is zero
-      const int j0 = a.rows / 2, pad = (int)a.ldo * UNIT_K - j0;
-      for (int i = lane; i < pad * item_count; i += 32) act_at(item, i / pad, j0 + i % pad) = 0;
+    if (!SMALL2 && (a.mode == GATEUP || a.mode == GATEUP_SMALL)) finish_act(item, strip, tot);
+    else if (a.pairs) finish_pairs(strip, tot);
+    else finish_single(strip, tot);
+  }
+  // gate and up rows: a tile's rows g and g + 8
+  __device__ __forceinline__ void finish_act(int item, int strip, const float (&tot)[RT][NT][4]) {
+    const int I = a.rows / 2;
+    if (a.mode == GATEUP_SMALL && strip == a.strips.d - 1) {   // act's padding to whole units is zero
+      const int pad = (int)a.ldo * UNIT_K - I;
+      for (int i = lane; i < pad * item_count; i += 32) act_at(item, i / pad, I + i % pad) = 0;
     }
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        float v[2];
+#pragma unroll
+        for (int ci = 0; ci < 2; ++ci) {
+          const float gt = tot[r][n][ci], up = tot[r][n][2 + ci];
+          v[ci] = __fdiv_rn(gt, 1.0f + expf(-gt)) * up;
+        }
+        // rounded to the activations' type: the down projection's tensor-core operand
+        const uint32_t two = transpose8(D::round2(v[0], v[1]));
+        const int col = n * 8 + g, j = (strip * RT + r) * 8 + 2 * t;
+        if (col >= item_count || j >= I) continue;
+        if (a.mode == GATEUP) {      // (the place after an odd last j is padding)
+          *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (int64_t)(item_start + col) * a.ldo + j) = two;
+        } else {
+          const uint32_t w = plan->tokens[item] >> col & 1 ? two : 0u;
+          if (j + 1 < I) *reinterpret_cast<uint32_t*>(&act_at(item, col, j)) = w;
+          else act_at(item, col, j) = (uint16_t)w;
+        }
+      }
+  }
+  __device__ __forceinline__ void finish_pairs(int strip, const float (&tot)[RT][NT][4]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (n * 8 >= item_count) break;
+      const int64_t col = item_start + n * 8 + g;
+      const bool live = n * 8 + g < item_count;
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = (strip * RT + r) * 16 + 8 * h + 2 * t;
+          float lo = tot[r][n][2 * h], hi = tot[r][n][2 * h + 1];
+          if (a.residual) {
+            const uint16_t* p = a.residual + col * a.ldr + row;
+            uint32_t two = 0;
+            if (live && row + 1 < a.rows) two = *reinterpret_cast<const uint32_t*>(p);
+            else if (live && row < a.rows) two = *p;
+            const float2 f = D::to_f32(transpose8(two));
+            lo += f.x;
+            hi += f.y;
+          }
+          const uint32_t two = transpose8(D::round2(lo, hi));
+          uint16_t* o = static_cast<uint16_t*>(a.out) + col * a.ldo + row;
+          if (live && row + 1 < a.rows) *reinterpret_cast<uint32_t*>(o) = two;
+          else if (live && row < a.rows) *o = (uint16_t)two;
+        }
+    }
+  }
+  // FP32 outputs and rows that do not start at 4-byte boundaries
+  __device__ __forceinline__ void finish_single(int strip, const float (&tot)[RT][NT][4]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int ci = 0; ci < 2; ++ci) {
-        const int col = n * 8 + 2 * t + ci;
-        if (col >= item_count) continue;
+        if (n * 8 + 2 * t + ci >= item_count) continue;
+        const int64_t col = item_start + n * 8 + 2 * t + ci;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const float lo = tot[r][n][ci], hi = tot[r][n][2 + ci];     // rows g, g + 8 of the tile
-          const int tile = strip * RT + r;
-          if (!SMALL2 && (a.mode == GATEUP || a.mode == GATEUP_SMALL)) {   // a gate row and its up row
-            const int j = tile * 8 + g;
-            if (j >= a.rows / 2) continue;
-            // rounded to the activations' type: the down projection's tensor-core operand
-            uint16_t v = D::round(__fdiv_rn(lo, 1.0f + expf(-lo)) * hi);
-            if (a.mode == GATEUP) {
-              static_cast<uint16_t*>(a.out)[(int64_t)(item_start + col) * a.ldo + j] = v;
-            } else {
-              if (!(plan->tokens[item] >> col & 1)) v = 0;
-              act_at(item, col, j) = v;
-            }
-          } else {
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int row = tile * 16 + g + 8 * h;
-              if (row >= a.rows) continue;
-              float v = h ? hi : lo;
-              const int64_t at = item_start + col;
-              if (a.residual) v += D::one_to_f32(a.residual[at * a.ldr + row]);
-              if (a.out_f32) static_cast<float*>(a.out)[at * a.ldo + row] = v;
-              else static_cast<uint16_t*>(a.out)[at * a.ldo + row] = D::round(v);
-            }
+          for (int h = 0; h < 2; ++h) {
+            const int row = (strip * RT + r) * 16 + g + 8 * h;
+            if (row >= a.rows) continue;
+            float v = tot[r][n][2 * h + ci];
+            if (a.residual) v += D::one_to_f32(a.residual[col * a.ldr + row]);
+            if (a.out_f32) static_cast<float*>(a.out)[col * a.ldo + row] = v;
+            else static_cast<uint16_t*>(a.out)[col * a.ldo + row] = D::round(v);
           }
-        }
       }
   }
 
   // tot += the unit's products; staged activations at shared address xl + x_off
-  template <int NB>
-  __device__ __forceinline__ void multiply(Unit& n, const uint32_t (&xl)[NB], uint32_t x_off, uint32_t x_h,
-                                           const float2 (&w2)[NB], float (&tot)[RT][NB][4]) {
-    float acc[RT][NB][4];
+  __device__ __forceinline__ void multiply(Unit& n, const uint32_t (&xl)[NT], uint32_t x_off, uint32_t x_h,
+                                           const float2 (&w2)[NT], float (&tot)[RT][NT][4]) {
+    float acc[RT][NT][4];
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      uint4 xb[NB];
+      uint4 xb[NT];
 #pragma unroll
-      for (int i = 0; i < NB; ++i) xb[i] = XR ? n.x[XR ? h : 0][XR ? i : 0] : lds128(xl[i] + x_off + h * x_h);
+      for (int i = 0; i < NT; ++i) xb[i] = XR ? n.x[XR ? h : 0][XR ? i : 0] : lds128(xl[i] + x_off + h * x_h);
       const int i = h * 32 / G;
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
@@ -341,24 +385,23 @@ struct Kernel {
           z1 = (z >> 8 & 0xFFu) * 0x00010001u | D::MAGIC;
         }
         const uint4& v = n.w[r][h >> 1];
-        if (h * 32 % G == 0) half_chunk<D, NB, true>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
-        else half_chunk<D, NB, false>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
-        if ((h + 1) * 32 % G == 0) fold<D, NB, SMALL2>(n.sc[r][i], w2, acc[r], tot[r]);
+        if (h * 32 % G == 0) half_chunk<D, NT, true>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
+        else half_chunk<D, NT, false>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
+        if ((h + 1) * 32 % G == 0) fold<D, NT, SMALL2>(n.sc[r][i], w2, acc[r], tot[r]);
       }
       if (AHEAD == 1 && h == 1) load_half(n);
     }
   }
 
-  // the units [p, p_end) of the phase that begins at unit p0 and has n units; at most 8 NB columns.
+  // the units [p, p_end) of the phase that begins at unit p0 and has n units; at most 8 NT columns.
   // un holds the first AHEAD of them.
-  template <int NB>
   __device__ __forceinline__ void units(Unit (&un)[AHEAD], int p, const int p_end, const int p0, const int n) {
-    constexpr int WORDS = RT * NB * 4;
-    float tot[RT][NB][4];
+    constexpr int WORDS = RT * NT * 4;
+    float tot[RT][NT][4];
     // a lane past the columns reads the last one's activations: its sums are not used
-    uint32_t xl[NB];
+    uint32_t xl[NT];
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < NT; ++i)
       xl[i] = XR ? 0 : (uint32_t)__cvta_generic_to_shared(xs) + (min(i * 8 + g, item_count - 1) * 4 + t) * 16;
     const uint32_t x_h = item_count * 64;
     bool met = false;                     // this warp has been at the barrier
@@ -369,11 +412,11 @@ struct Kernel {
 #pragma unroll
       for (int i = 0; i < WORDS; ++i) (&tot[0][0][0])[i] = 0.0f;
       uint32_t x_off = q0 * x_h * 4;
-      float2 w2[NB];
+      float2 w2[NT];
       int to_expert = 0, expert = 0;      // SMALL2: units to the next expert, its place in the plan
       auto weigh = [&]() {
 #pragma unroll
-        for (int i = 0; i < NB; ++i) w2[i] = *reinterpret_cast<const float2*>(cw + expert * MAX_COLS + i * 8 + 2 * t);
+        for (int i = 0; i < NT; ++i) w2[i] = *reinterpret_cast<const float2*>(cw + expert * MAX_COLS + i * 8 + 2 * t);
       };
       if (SMALL2) {
         expert = q0 / a.units;
@@ -385,7 +428,7 @@ struct Kernel {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
           if (next == i && left > 0) {
-            multiply<NB>(un[i], xl, x_off, x_h, w2, tot);
+            multiply(un[i], xl, x_off, x_h, w2, tot);
             load(un[i], AHEAD == 1);
             next = i + 1 == AHEAD ? 0 : i + 1;
             --left;
@@ -416,7 +459,7 @@ struct Kernel {
           }
         }
       }
-      finish<NB>(strip_flat, tot);
+      finish(strip_flat, tot);
     }
     if (!met) all_warps();
   }
@@ -463,7 +506,7 @@ struct Kernel {
     if (SMALL2 && U == 0) {   // no slot selects an expert
       for (int strip = lo + warp; strip < hi; strip += WARPS) {
         const float zero[RT][NT][4] = {};
-        finish<NT>(strip, zero);
+        finish(strip, zero);
       }
       return;
     }
@@ -498,18 +541,17 @@ struct Kernel {
         __syncthreads();
       }
       staged = true;
-      if (MIXED && item_count <= 8) units<1>(un, p, p_end, p0, n);
-      else units<NT>(un, p, p_end, p0, n);
+      units(un, p, p_end, p0, n);
       from = to;
     }
   }
 };
 
-template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2, bool MIXED>
-__global__ void __launch_bounds__(Kernel<D, RT, NT, G, ZP, XR, SMALL2, MIXED>::THREADS, 1) w4_kernel(const Args a) {
+template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2>
+__global__ void __launch_bounds__(Kernel<D, RT, NT, G, ZP, XR, SMALL2>::THREADS, 1) w4_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ SmallPlan plan;
-  Kernel<D, RT, NT, G, ZP, XR, SMALL2, MIXED> k(a);
+  Kernel<D, RT, NT, G, ZP, XR, SMALL2> k(a);
   k.run_all(smem, plan);
 }
 
@@ -538,13 +580,13 @@ cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, int threads, int smem
   return cudaLaunchKernelEx(&c, kernel, args...);
 }
 
-template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2, bool MIXED>
+template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2>
 static int launch(const Args& a, int grid, cudaStream_t s) {
-  using K = Kernel<D, RT, NT, G, ZP, XR, SMALL2, MIXED>;
+  using K = Kernel<D, RT, NT, G, ZP, XR, SMALL2>;
   constexpr int parts = K::WARPS * RT * NT * 4 * 32 * 4;
   static_assert(parts <= PARTS_BYTES, "the parts of strips");
   const int smem = parts + (SMALL2 ? CW_BYTES : XR ? 0 : a.cols * a.units.d * UNIT_K * 2);
-  const auto kernel = w4_kernel<D, RT, NT, G, ZP, XR, SMALL2, MIXED>;
+  const auto kernel = w4_kernel<D, RT, NT, G, ZP, XR, SMALL2>;
   static std::atomic<bool> ready[MAX_DEVICES];   // the kernel may use that much shared memory on the device
   cudaError_t e = cudaSuccess;
   if (!ready[a.device].load(std::memory_order_acquire)) {
@@ -560,16 +602,14 @@ template <class D, int G, bool ZP>
 static int launch_form(const Args& a, bool two, bool xr, int grid, cudaStream_t s) {
   const bool small2 = a.mode == DOWN_SMALL;
   if (a.cols <= 8) {
-    if (small2) return two ? launch<D, 2, 1, G, ZP, true, true, false>(a, grid, s) : launch<D, 1, 1, G, ZP, true, true, false>(a, grid, s);
-    if (xr) return two ? launch<D, 2, 1, G, ZP, true, false, false>(a, grid, s) : launch<D, 1, 1, G, ZP, true, false, false>(a, grid, s);
-    return two ? launch<D, 2, 1, G, ZP, false, false, false>(a, grid, s) : launch<D, 1, 1, G, ZP, false, false, false>(a, grid, s);
+    if (small2) return two ? launch<D, 2, 1, G, ZP, true, true>(a, grid, s) : launch<D, 1, 1, G, ZP, true, true>(a, grid, s);
+    if (xr) return two ? launch<D, 2, 1, G, ZP, true, false>(a, grid, s) : launch<D, 1, 1, G, ZP, true, false>(a, grid, s);
+    return two ? launch<D, 2, 1, G, ZP, false, false>(a, grid, s) : launch<D, 1, 1, G, ZP, false, false>(a, grid, s);
   }
-  if (small2) return launch<D, 1, 2, G, ZP, true, true, false>(a, grid, s);
-  if (xr) return launch<D, 1, 2, G, ZP, true, false, false>(a, grid, s);
-  if (a.cols > MAX_COLS) return launch<D, 1, 4, G, ZP, false, false, false>(a, grid, s);
-  if (a.mode == GATEUP || a.mode == DOWN)
-    return two ? launch<D, 2, 2, G, ZP, false, false, true>(a, grid, s) : launch<D, 1, 2, G, ZP, false, false, true>(a, grid, s);
-  return two ? launch<D, 2, 2, G, ZP, false, false, false>(a, grid, s) : launch<D, 1, 2, G, ZP, false, false, false>(a, grid, s);
+  if (small2) return launch<D, 1, 2, G, ZP, true, true>(a, grid, s);
+  if (xr) return launch<D, 1, 2, G, ZP, true, false>(a, grid, s);
+  if (a.cols > MAX_COLS) return launch<D, 1, 4, G, ZP, false, false>(a, grid, s);
+  return two ? launch<D, 2, 2, G, ZP, false, false>(a, grid, s) : launch<D, 1, 2, G, ZP, false, false>(a, grid, s);
 }
 
 template <class D>
