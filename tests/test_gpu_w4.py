@@ -44,6 +44,9 @@ SHAPES = [  # T, N, K, group, zeros
     (16, 64, 2048, 64, False), (17, 33, 130, 64, True), (31, 40, 1350, 32, True), (32, 80, 512, 128, False),
     (33, 20, 200, 32, False), (70, 24, 129, 128, True), (4, 5000, 192, 64, False), (12, 16, 10944, 64, False),
     (1, 32, 20000, 32, True), (1, 2400, 64, 32, False),
+    # rows for two tiles a warp, and with rows too long for staged activations
+    (1, 9601, 160, 128, False), (7, 9500, 300, 32, True), (16, 9477, 129, 64, False), (32, 9472, 64, 32, True),
+    (8, 9500, 12000, 64, False), (8, 40, 24008, 128, True),
 ]
 
 
@@ -95,6 +98,16 @@ def test_linear_strides_and_alignment():
     want = (big[:T, :K].double() @ W.T + res.double()).to(torch.bfloat16)
     lin(big[:T, :K], out=res, residual=res)                      # in place
     assert torch.equal(res, want)
+
+
+def test_linear_long_rows_without_alignment():
+    """Rows too long to be staged for all tokens and not 16-byte aligned: fewer tokens at a time."""
+    g = gen(8)
+    w = codes_of(g, (24,), 10949, 64, True, torch.bfloat16, "exact")
+    big = torch.randint(-3, 4, (13, 10952), generator=g, device=DEV).to(torch.bfloat16)
+    x = big[:, 1:10950]
+    want = x.double() @ dequantize_w4(*w, 10949, 64).double().T
+    assert torch.equal(W4Linear(*w, k=10949, group=64)(x, out_dtype=torch.float32).double(), want)
 
 
 def test_linear_no_tokens_and_refusals():
@@ -159,6 +172,7 @@ EXPERTS = [  # T, H, I, E, S, group, zeros, residual
     (7, 130, 50, 9, 4, 64, True, True), (8, 256, 96, 66, 8, 64, True, True), (16, 200, 174, 20, 5, 32, True, False),
     (17, 96, 33, 5, 1, 128, False, True), (40, 500, 174, 6, 3, 32, True, False), (33, 128, 72, 2, 2, 64, False, True),
     (64, 64, 200, 80, 8, 32, False, True), (150, 48, 16, 7, 4, 32, True, True),
+    (5, 9500, 40, 3, 2, 64, False, True), (12, 9500, 33, 2, 2, 32, True, False), (20, 4800, 24, 6, 2, 128, False, True),
 ]
 
 
