@@ -22,7 +22,7 @@
 // (many strips per CTA use them) or travel with the codes through the rings (few strips per CTA, or
 // rows too long for shared memory).
 //
-// The experts of a small batch (at most 16 tokens) take two launches: gate/up with the tokens as the
+// The experts of a small batch (at most 8 tokens) take two launches: gate/up with the tokens as the
 // columns of every expert, then the down projection as one long dot product over the selected
 // experts' activations, each expert's part scaled by the tokens' weights for it. A larger batch is
 // grouped by expert first (plan_kernel), each expert's slots being its columns, and the slots' outputs
@@ -169,7 +169,7 @@ const char* plan_experts(const MkW4* w13, const MkW4* w2, int64_t t, int64_t s, 
     if ((int64_t)w->experts * (w->n / STRIP_ROWS + 1) * units_of(w) > INT32_MAX / 2) return "the experts have too many weights";
   if (t < 0 || s < 0 || t * s >= (1 << 24)) return "slots (tokens x slots per token) are from 0 to 2^24 - 1";
   p->small = t <= SMALL_T && t * s <= SMALL_SLOTS && fits(units_of(w13), (int)std::max<int64_t>(t, 1));
-  p->cols = (int)std::min<int64_t>(std::max<int64_t>(t, 1), p->small ? MAX_COLS : GROUPED_COLS);
+  p->cols = (int)std::min<int64_t>(std::max<int64_t>(t, 1), GROUPED_COLS);
   while (p->cols > 1 && !(fits(units_of(w13), p->cols) && (p->small || fits(units_of(w2), p->cols)))) --p->cols;
   if (!fits(units_of(w13), p->cols) || (!p->small && !fits(units_of(w2), p->cols))) return "rows are too long for the shared memory";
   const int64_t n = std::max<int64_t>(t * s, 1), items = w13->experts + n / p->cols + 1;

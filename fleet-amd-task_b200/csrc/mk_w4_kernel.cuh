@@ -19,7 +19,7 @@ constexpr int MAX_EXPERTS = 1024;
 constexpr int MAX_DEVICES = 64;
 constexpr int MAX_COLS = 16;           // columns of an item (of a LINEAR: 32)
 constexpr int GROUPED_COLS = 8;        // of an expert's item: about what a routed expert gets
-constexpr int SMALL_T = MAX_COLS;      // tokens and slots of the two-launch experts
+constexpr int SMALL_T = 8;             // tokens and slots of the two-launch experts (12 tokens: 80 us against 70 grouped)
 constexpr int SMALL_SLOTS = 256;
 
 // what a launch computes and where its columns and outputs are
@@ -182,7 +182,7 @@ struct Kernel {
   int warp, lane, g, t;
   uint4* xs;
   float* slots;                  // [WARPS][RT NT 4][32]: the parts of strips that an earlier warp began
-  float* cw;                     // SMALL2: [experts][16] the tokens' weights
+  float* cw;                     // SMALL2: [experts][SMALL_T] the tokens' weights
   const SmallPlan* plan;
   int U;                         // units of a strip's sums (SMALL2: over all selected experts)
   // the load cursor: the next unit to load, the last one's end, the run of consecutive bytes it is in
@@ -416,7 +416,7 @@ struct Kernel {
       int to_expert = 0, expert = 0;      // SMALL2: units to the next expert, its place in the plan
       auto weigh = [&]() {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) w2[i] = *reinterpret_cast<const float2*>(cw + expert * MAX_COLS + i * 8 + 2 * t);
+        for (int i = 0; i < NT; ++i) w2[i] = *reinterpret_cast<const float2*>(cw + expert * SMALL_T + i * 8 + 2 * t);
       };
       if (SMALL2) {
         expert = q0 / a.units;
@@ -484,8 +484,8 @@ struct Kernel {
       if (SMALL2) {
         U = sp.n * a.units.d;
         n_items = 1;
-        for (int i = threadIdx.x; i < sp.n * MAX_COLS; i += THREADS) {
-          const int e = sp.expert[i / MAX_COLS], tok = i % MAX_COLS;
+        for (int i = threadIdx.x; i < sp.n * SMALL_T; i += THREADS) {
+          const int e = sp.expert[i / SMALL_T], tok = i % SMALL_T;
           float w = 0.0f;
           if (tok < a.t)
             for (int k = 0; k < a.s; ++k)
@@ -557,7 +557,7 @@ __global__ void __launch_bounds__(Kernel<D, RT, NT, G, ZP, XR, SMALL2>::THREADS,
 
 // shared memory: the parts of strips, a small batch's weights, the plan (static), the activations
 constexpr int PARTS_BYTES = 32 * 1024;     // at most: 16 warps x 4 x 4 (or 24 x 2 x 4) words of 128 bytes
-constexpr int CW_BYTES = SMALL_SLOTS * MAX_COLS * 4;
+constexpr int CW_BYTES = SMALL_SLOTS * SMALL_T * 4;
 constexpr int STATIC_BYTES = (sizeof(SmallPlan) + 1023) / 1024 * 1024;
 
 // whether the activations of `cols` columns can be staged
@@ -600,13 +600,11 @@ static int launch(const Args& a, int grid, cudaStream_t s) {
 // two: two tiles a warp; xr: the activations come with the units (one tile a warp if over 8 columns)
 template <class D, int G, bool ZP>
 static int launch_form(const Args& a, bool two, bool xr, int grid, cudaStream_t s) {
-  const bool small2 = a.mode == DOWN_SMALL;
   if (a.cols <= 8) {
-    if (small2) return two ? launch<D, 2, 1, G, ZP, true, true>(a, grid, s) : launch<D, 1, 1, G, ZP, true, true>(a, grid, s);
+    if (a.mode == DOWN_SMALL) return two ? launch<D, 2, 1, G, ZP, true, true>(a, grid, s) : launch<D, 1, 1, G, ZP, true, true>(a, grid, s);
     if (xr) return two ? launch<D, 2, 1, G, ZP, true, false>(a, grid, s) : launch<D, 1, 1, G, ZP, true, false>(a, grid, s);
     return two ? launch<D, 2, 1, G, ZP, false, false>(a, grid, s) : launch<D, 1, 1, G, ZP, false, false>(a, grid, s);
   }
-  if (small2) return launch<D, 1, 2, G, ZP, true, true>(a, grid, s);
   if (xr) return launch<D, 1, 2, G, ZP, true, false>(a, grid, s);
   if (a.cols > MAX_COLS) return launch<D, 1, 4, G, ZP, false, false>(a, grid, s);
   return two ? launch<D, 2, 2, G, ZP, false, false>(a, grid, s) : launch<D, 1, 2, G, ZP, false, false>(a, grid, s);
