@@ -16,6 +16,11 @@
 // or above that (about 1.5 topk for scores spread over the lanes) go to shared memory, one to a lane,
 // and a lane counts how many are better than its own. More than 32 of them (long ties, more topk than
 // lanes with experts) are taken one by one instead.
+//
+// 16384 tokens of 256 experts (sigmoid, bias, 8 groups by their two best, topk 8, renormalised) read 17 MB,
+// 2.6 us at the copy rate, and take 15.9 us: bound by issue (82 % of the issue slots, 830 instructions a
+// token, about 160 of them the exact exponentials and reciprocals). topk rounds over all experts
+// took 38 us. Two tokens a warp (16 lanes of 16 experts) took 18.2. One token: 2.3 us, a launch.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

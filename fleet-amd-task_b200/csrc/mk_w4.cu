@@ -7,26 +7,37 @@
 // slot whose id is outside [0, experts) is empty.
 //
 // What bounds them. A token costs 2 operations per weight and a weight half a byte, so a batch of T
-// tokens does 4 T operations a byte: the stream of codes is the bound for a decode batch, then the
-// instructions that turn codes into tensor-core operands (11 per 8 codes), not the tensor cores
-// (2 cycles an m16n8k16 per SM against 5.5 cycles for its 128 bytes at 6.5 TB/s). mma.sync takes a
-// tile of 16 rows by 8 tokens without padding the batch to a tcgen05 tile's 64 or 128 rows.
+// tokens does 4 T operations a byte: by the numbers the stream of codes bounds a decode batch of up to
+// some forty tokens. What it comes to on B200 (a 16 x 128 block of weights a step, per SM): 133
+// instructions at 8 columns, 88 of them to make tensor-core operands of the codes (11 per 8 codes:
+// three shifts, four AND-ORs, four subtractions), and 8 MMAs; 157 and 16 at 16 columns. Timed with
+// parts left out, a step takes instructions / 4 + 2 cycles an MMA (49 cycles modelled, 52 measured at
+// 8 columns; 71 and 74 at 16): an SM partition issues nothing beside an mma.sync. The codes of a step
+// take 44 cycles at 6.5 TB/s, so a head of 102400 x 2048 reads at 5.3 TB/s within its 25.6 us (107 MB;
+// about 5 us are the launch, the first instructions and loads, and the end), 16 tokens take 37 us and
+// 32 tokens 59, bound by issue. tcgen05 was built beside it (codes decoded into tensor memory, 128 rows a
+// tile, 16 or 32 columns): 48 to 62 us for 9 to 32 tokens, bound by the chain of a tile (decode, store,
+// barrier, MMA, commit, read back), and not kept.
 //
-// The work is a row of sums (a strip: RT tiles of 16 rows, for up to 16 columns) times its units of
-// 128 values of K. Each CTA (one per SM, 16 warps) takes an equal range of strips, and each warp an
-// equal, contiguous range of the CTA's units, wherever strips begin and end in it: the warps finish
-// together whatever the sizes, and nothing is synchronised between them until the end of the range,
-// where the warp that began a strip adds the parts of the warps after it, in warp order (the result
-// does not depend on timing). A warp streams its units, which lie one after the other in memory,
-// through its own ring of cp.async stages. The activations are either staged once in shared memory
-// (many strips per CTA use them) or travel with the codes through the rings (few strips per CTA, or
-// rows too long for shared memory).
+// The work is a row of sums (a strip: RT tiles of 16 rows, for up to 8 NT columns) times its units of
+// 128 values of K. Each CTA (one per SM) takes an equal range of strips, and each warp an equal,
+// contiguous range of the CTA's units, wherever strips begin and end in it: the warps finish together
+// whatever the sizes, and nothing is synchronised between them until the end of the range, where the
+// warp that began a strip adds the parts of the warps after it, in warp order (the result does not
+// depend on timing). (Teams of warps on a strip with a barrier each: 31 us for that head.) A warp loads
+// its units, which lie one after the other in memory, straight into registers, one or more ahead; a
+// cp.async ring in shared memory took as long and more instructions. The activations are either staged
+// once in shared memory in the MMA's order, or, where they do not fit, loaded with each unit (xr): 16
+// tokens of K 10944 in 13 us, against 27 in blocks of the 6 tokens whose activations fit (an earlier form).
 //
 // The experts of a small batch (at most 8 tokens) take two launches: gate/up with the tokens as the
 // columns of every expert, then the down projection as one long dot product over the selected
 // experts' activations, each expert's part scaled by the tokens' weights for it. A larger batch is
 // grouped by expert first (plan_kernel), each expert's slots being its columns, and the slots' outputs
-// are added afterwards in slot order (combine_kernel).
+// are added afterwards in slot order (combine_kernel). The launches of one call overlap
+// (programmatic dependent launches): 24 us instead of 30 for a small layer's four.
+// Measured, a layer of 66 experts of 2048 x 1408, 8 slots a token: 1 token 20.6 us (36 MB, 5.4 us at the
+// copy rate), 8 tokens 50 (165 MB of distinct experts, 25 us), 64 tokens 97 (295 MB, 45 us).
 #include <algorithm>
 
 #include "mk_w4_kernel.cuh"
@@ -141,7 +152,8 @@ int device_sms(int* device, int* sms) {
 // about `items` items over the SMs; known: exactly that many
 int launch_weight(Args& a, const MkW4* w, int64_t items, bool known, bool xr, int sms, cudaStream_t s) {
   const int strips = (w->n + STRIP_ROWS - 1) / STRIP_ROWS;
-  // enough strips for every CTA: two tiles a warp share the activations
+  // Two tiles a warp share its activations and its loop, one tile spreads few strips over more CTAs (K 2048,
+  // one / two tiles: 2048 rows 6.2 / 8.3 us, 8192 rows 8.3 / 9.3, 20000 rows of 8 tokens 14.1 / 13.0)
   const bool two = items * strips >= 2 * sms && !(xr && a.cols > 8) && a.cols <= MAX_COLS;
   a.strips = div_by(two ? strips : 2 * strips);
   const int grid = (int)(known ? std::min<int64_t>(sms, items * a.strips.d) : sms);
@@ -212,7 +224,8 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   a.x = static_cast<const uint16_t*>(x);
   a.ldx = ldx;
   a.x_vec = aligned16(x, ldx);
-  // even blocks of at most 16 tokens, or 32 if their activations fit
+  // even blocks of at most 16 tokens, or 32 if their activations fit (102400 x 2048, 32 tokens: 59 us, two
+  // blocks of 16 63)
   const int most = t > MAX_COLS && fits(a.units.d, 2 * MAX_COLS) ? 2 * MAX_COLS : MAX_COLS;
   const int blocks = (t + most - 1) / most;
   a.tb = (t + blocks - 1) / blocks;
