@@ -255,8 +255,8 @@ def quantize_w4(w, group=128, zero_point=False, dtype=None):
     scales [..., N, ceil(K / group)] of `dtype` (default: w's), zeros uint8 or None), round to nearest
     (ties to even) with one scale per row and group. Symmetric: scale amax / 7, codes 1..15 around 8.
     zero_point: scale (max - min) / 15 over the group's range widened to hold 0, zeros
-    round(-min / scale). The scale is rounded to its type before the codes are taken; a group of
-    zeros has scale 0 and decodes to 0."""
+    round(-min / scale). The scale is rounded to its type (saturating) before the codes are taken; a group
+    of zeros has scale 0 and decodes to 0."""
     dtype = dtype or w.dtype
     K = w.shape[-1]
     g = -(-K // group)
@@ -266,6 +266,7 @@ def quantize_w4(w, group=128, zero_point=False, dtype=None):
         scale = ((hi - lo) / 15).to(dtype)
     else:
         lo, scale = None, (v.abs().amax(-1) / 7).to(dtype)
+    scale = scale.clamp(max=torch.finfo(dtype).max)          # (an FP16 scale of weights past its range)
     step = torch.where(scale > 0, scale, torch.ones_like(scale)).float()
     zero = (-lo / step).round().clamp(0, 15) if zero_point else torch.full_like(step, 8)
     q = (v / step[..., None]).round_().add_(zero[..., None]).clamp_(0, 15).to(torch.uint8).flatten(-2)[..., :K]

@@ -110,6 +110,26 @@ def test_linear_long_rows_without_alignment():
     assert torch.equal(W4Linear(*w, k=10949, group=64)(x, out_dtype=torch.float32).double(), want)
 
 
+def test_linear_weight_past_4_gib():
+    """Codes of 4.6 GiB: the last rows, whose bytes lie past 32 bits."""
+    g, N, K = gen(3), 300032, 32768
+    w = codes_of(g, (N,), K, 128, False, torch.bfloat16, "exact")
+    x = torch.randint(-3, 4, (2, K), generator=g, device=DEV).to(torch.bfloat16)
+    got = W4Linear(*w, k=K, group=128)(x, out_dtype=torch.float32)
+    assert w[0].numel() > 2 ** 32
+    for rows in (slice(0, 40), slice(N - 100, N)):
+        want = x.double() @ dequantize_w4(w[0][rows], w[1][rows], None, K, 128).double().T
+        assert torch.equal(got[:, rows].double(), want)
+
+
+def test_linear_many_tokens():
+    g = gen(4)
+    w = codes_of(g, (50,), 100, 32, True, torch.float16, "exact")
+    x = torch.randint(-3, 4, (3001, 100), generator=g, device=DEV).half()
+    assert torch.equal(W4Linear(*w, k=100, group=32)(x, out_dtype=torch.float32).double(),
+                       x.double() @ dequantize_w4(*w, 100, 32).double().T)
+
+
 def test_linear_no_tokens_and_refusals():
     w = quantize_w4(torch.randn(32, 64, generator=gen(0), device=DEV).to(torch.bfloat16), 32)
     lin = W4Linear(*w, k=64, group=32)

@@ -33,6 +33,13 @@ def test_quantize_zero_group_decodes_to_zero():
         assert (scales == 0).all() and (dequantize_w4(codes, scales, zeros, 64, 32) == 0).all()
 
 
+def test_quantize_past_the_scale_range_saturates():
+    w = torch.tensor([[3e6, -1e6] + [0.0] * 30])
+    codes, scales, zeros = quantize_w4(w, 32, dtype=torch.float16)
+    back = dequantize_w4(codes, scales, zeros, 32, 32)
+    assert scales.item() == 65504 and back.isfinite().all() and back[0, 0] == 7 * 65504
+
+
 def decode_layout(q, s, z, N, k, group, gate_up):
     """W [E, N, k] from the laid-out tensors, word by word as csrc/mk_w4.cuh states the order."""
     q, s = q.numpy(), s.float().numpy()
