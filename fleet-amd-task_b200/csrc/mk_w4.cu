@@ -15,7 +15,7 @@
 // 8 columns; 71 and 74 at 16): an SM partition issues nothing beside an mma.sync. The codes of a step
 // take 44 cycles at 6.5 TB/s, so a head of 102400 x 2048 reads at 5.3 TB/s within its 25.6 us (107 MB;
 // about 5 us are the launch, the first instructions and loads, and the end), 16 tokens take 37 us and
-// 32 tokens 59, bound by issue. tcgen05 was built beside it (codes decoded into tensor memory, 128 rows a
+// 32 tokens 54, bound by issue. tcgen05 was built beside it (codes decoded into tensor memory, 128 rows a
 // tile, 16 or 32 columns): 48 to 62 us for 9 to 32 tokens, bound by the chain of a tile (decode, store,
 // barrier, MMA, commit, read back), and not kept.
 //
@@ -224,8 +224,8 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   a.x = static_cast<const uint16_t*>(x);
   a.ldx = ldx;
   a.x_vec = aligned16(x, ldx);
-  // even blocks of at most 16 tokens, or 32 if their activations fit (102400 x 2048, 32 tokens: 59 us, two
-  // blocks of 16 63)
+  // even blocks of at most 16 tokens, or 32 if their activations fit (102400 x 2048, 32 tokens: 54 us, two
+  // blocks of 16 60)
   const int most = t > MAX_COLS && fits(a.units.d, 2 * MAX_COLS) ? 2 * MAX_COLS : MAX_COLS;
   const int blocks = (t + most - 1) / most;
   a.tb = (t + blocks - 1) / blocks;

@@ -235,8 +235,8 @@ struct Kernel {
 #pragma unroll
     for (int r = 0; r < RT; ++r) n.w[r][0] = ldg128(code + r * TILE_UNIT_BYTES);
   }
-  // the next unit; rest: without that half
-  __device__ __forceinline__ void load(Unit& n, bool rest) {
+  // the next unit's codes, scales and zero points; rest: without that half
+  __device__ __forceinline__ void load_weights(Unit& n, bool rest) {
     if (cp >= cp_end) return;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -248,6 +248,10 @@ struct Kernel {
         else ldg_words<ZP ? ZWORDS : 1>(zero + r * (GROUPS * 16), n.z[r]);
       }
     }
+  }
+  // its activations, and the cursor on to the unit after it
+  __device__ __forceinline__ void load_rest(Unit& n) {
+    if (cp >= cp_end) return;
     if (XR) {
 #pragma unroll
       for (int h = 0; h < 4; ++h)
@@ -310,13 +314,14 @@ struct Kernel {
         // 16-bit output 1.4 times that of one rounding (0.0024 against 0.0017 of the norm in BF16).
         const uint32_t two = transpose8(D::round2(v[0], v[1]));
         const int col = n * 8 + g, j = (strip * RT + r) * 8 + 2 * t;
-        if (col >= item_count || j >= I) continue;
-        if (a.mode == GATEUP) {      // (the place after an odd last j is padding)
-          *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (int64_t)(item_start + col) * a.ldo + j) = two;
-        } else {
-          const uint32_t w = plan->tokens[item] >> col & 1 ? two : 0u;
-          if (j + 1 < I) *reinterpret_cast<uint32_t*>(&act_at(item, col, j)) = w;
-          else act_at(item, col, j) = (uint16_t)w;
+        if (col < item_count && j < I) {
+          if (a.mode == GATEUP) {      // (the place after an odd last j is padding)
+            *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (int64_t)(item_start + col) * a.ldo + j) = two;
+          } else {
+            const uint32_t w = plan->tokens[item] >> col & 1 ? two : 0u;
+            if (j + 1 < I) *reinterpret_cast<uint32_t*>(&act_at(item, col, j)) = w;
+            else act_at(item, col, j) = (uint16_t)w;
+          }
         }
       }
   }
@@ -433,7 +438,8 @@ struct Kernel {
         for (int i = 0; i < AHEAD; ++i) {
           if (next == i && left > 0) {
             multiply(un[i], xl, x_off, x_h, w2, tot);
-            load(un[i], AHEAD == 1);
+            load_weights(un[i], AHEAD == 1);
+            load_rest(un[i]);
             next = i + 1 == AHEAD ? 0 : i + 1;
             --left;
             x_off += x_h * 4;
@@ -505,7 +511,6 @@ struct Kernel {
     // the CTA's strips: the first total % grid CTAs have one more
     const int total = n_items * a.strips.d, each = total / (int)gridDim.x, more = total - each * (int)gridDim.x;
     const int lo = each * (int)blockIdx.x + min((int)blockIdx.x, more), hi = lo + each + ((int)blockIdx.x < more);
-    if (SMALL2 && a.follows) wait_predecessor();   // its activations; the plan came from the call's inputs
     start_dependents();
     if (SMALL2 && U == 0) {   // no slot selects an expert
       for (int strip = lo + warp; strip < hi; strip += WARPS) {
@@ -536,10 +541,14 @@ struct Kernel {
       run = 0;
       if (p < p_end) locate();
       if (staged) __syncthreads();   // every warp is done with the last phase's activations and parts
-      if (!XR) stage_x(a, xs, item_start, item_count);
       Unit un[AHEAD];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) load(un[i], false);
+      for (int i = 0; i < AHEAD; ++i) {
+        load_weights(un[i], false);
+        if (SMALL2 && i == 0 && a.follows) wait_predecessor();   // its activations: the plan and the weights are not
+        load_rest(un[i]);
+      }
+      if (!XR) stage_x(a, xs, item_start, item_count);
       if (!XR) {
         cp_wait_all();
         __syncthreads();
