@@ -14,7 +14,7 @@
 // parts left out, a step takes instructions / 4 + 2 cycles an MMA (49 cycles modelled, 52 measured at
 // 8 columns; 71 and 74 at 16): an SM partition issues nothing beside an mma.sync. The codes of a step
 // take 44 cycles at 6.5 TB/s, so a head of 102400 x 2048 reads at 5.3 TB/s within its 25.6 us (107 MB;
-// about 5 us are the launch, the first instructions and loads, and the end), 16 tokens take 37 us and
+// about 5 us are the launch, the first instructions and loads, and the end), 16 tokens take 35 us and
 // 32 tokens 54, bound by issue. tcgen05 was built beside it (codes decoded into tensor memory, 128 rows a
 // tile, 16 or 32 columns): 48 to 62 us for 9 to 32 tokens, bound by the chain of a tile (decode, store,
 // barrier, MMA, commit, read back), and not kept.
@@ -37,7 +37,7 @@
 // are added afterwards in slot order (combine_kernel). The launches of one call overlap
 // (programmatic dependent launches): 24 us instead of 30 for a small layer's four.
 // Measured, a layer of 66 experts of 2048 x 1408, 8 slots a token: 1 token 20.6 us (36 MB, 5.4 us at the
-// copy rate), 8 tokens 50 (165 MB of distinct experts, 25 us), 64 tokens 97 (295 MB, 45 us).
+// copy rate), 8 tokens 47 (165 MB of distinct experts, 25 us), 64 tokens 95 (295 MB, 45 us).
 #include <algorithm>
 
 #include "mk_w4_kernel.cuh"
