@@ -331,7 +331,9 @@ int mk_mla_decode_noalloc(const void* ql_nope, const void* q_pe, const void* c_k
 
 /* ---- Serving a batch of sequences with 4-bit weights (no counterpart in the reference, whose path
    decodes one sequence in BF16). Each call launches its kernels on `stream` and returns; nothing is
-   allocated, so the calls may be captured in a CUDA graph. Tensors are on the current device.
+   allocated, so the calls may be captured in a CUDA graph (a first call of the same shapes, which sets
+   the kernels' shared-memory limits on the device, should come before the capture). Tensors are on
+   the current device.
    ---- */
 
 /* Routing of t tokens to experts (csrc/mk_route.cu has the formulas and the rules for ties, -inf and
