@@ -94,8 +94,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const int* __restrict__ ids,
 
 // out[t] = (residual[t] +) sum over slots, in slot order, of w[t, s] y[column of the slot]
 template <class D>
-__global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ y, const int* __restrict__ slot_col,
-                                                      const float* __restrict__ weights, int s, int h,
+__global__ void __launch_bounds__(256) combine_kernel(const float* y, const int* slot_col, const float* weights, int s, int h,
                                                       const uint16_t* residual, int64_t ldr, uint16_t* out, int64_t ldo) {
   const int tok = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
   wait_predecessor();

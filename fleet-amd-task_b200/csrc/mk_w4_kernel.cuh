@@ -78,7 +78,9 @@ struct Args {
 };
 
 // The launches of one call overlap: each lets the next one start while it runs (the next's blocks take
-// SMs as this one's leave them) and waits for its predecessor's results before it reads them.
+// SMs as this one's leave them) and waits for its predecessor's results before it reads them. What an
+// earlier launch of the call writes changes during the life of the kernel that reads it, so no kernel that
+// waits takes it through const __restrict__ (loads that may be non-coherent, or moved before the wait).
 __device__ __forceinline__ void wait_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void start_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
