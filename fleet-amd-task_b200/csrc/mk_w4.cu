@@ -302,7 +302,10 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   int* items_n = reinterpret_cast<int*>(ws + p.items_n);
   int* col_token = reinterpret_cast<int*>(ws + p.col_token);
   int* slot_col = reinterpret_cast<int*>(ws + p.slot_col);
-  plan_kernel<<<1, 1024, 0, st>>>(ids, t, slots, w13->experts, p.cols, items, items_n, col_token, slot_col);
+  // the launches after it take counts and indices from its output: none without it
+  cudaError_t e = launch_behind(plan_kernel, dim3(1), 1024, 0, st, false, ids, (int)t, (int)slots, (int)w13->experts, p.cols, items,
+                                items_n, col_token, slot_col);
+  if (e != cudaSuccess) return fail(MK_ECUDA, cudaGetErrorString(e));
   a.mode = GATEUP;
   a.follows = b.follows = 1;
   a.items = b.items = items;
@@ -317,7 +320,7 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   if (int rc = launch_weight(b, w2, items_about, false, false, sms, st)) return rc;
   const dim3 grid((unsigned)((w2->n + 255) / 256), (unsigned)t);
   const float* y = reinterpret_cast<const float*>(ws + p.y);
-  const cudaError_t e = launch_behind(
+  e = launch_behind(
       w2->dtype == MK_W4_BF16 ? combine_kernel<Bf16> : combine_kernel<Fp16>, grid, 256, 0, st, true, y, (const int*)slot_col, weights, (int)slots,
       (int)w2->n, static_cast<const uint16_t*>(residual), ldr, static_cast<uint16_t*>(out), ldo);
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));

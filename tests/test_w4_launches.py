@@ -1,9 +1,18 @@
 """The launches of the batch operators' host code, without a GPU: rules that their kernels' sources keep, and
 the host code itself over a CUDA runtime that records launches and fails the ones it is told to."""
+import ctypes
 import re
+import shutil
+import subprocess
 from pathlib import Path
 
+import pytest
+
+from fleet import mk
+
 CSRC = Path(__file__).resolve().parent.parent / "fleet-amd-task_b200" / "csrc"
+OBJ = CSRC.parent / "lib" / "obj"
+CUDA = Path(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc").resolve().parent.parent / "include"
 
 
 def kernels(text):
@@ -24,3 +33,51 @@ def test_a_kernel_that_waits_for_its_predecessor_has_no_restrict():
     for name in waiting:
         assert "__restrict__" not in of[name][0], name
     assert not re.search(r"\*\s*__restrict__", (CSRC / "mk_w4_kernel.cuh").read_text())
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    """The host code of mk_w4.cu and mk_route.cu as built, linked with the recording runtime."""
+    objects = [OBJ / "mk_w4.o", OBJ / "mk_route.o"]
+    if not all(o.exists() for o in objects) or not (CUDA / "cuda_runtime.h").exists() or not shutil.which("g++"):
+        pytest.skip("needs the built objects, the CUDA headers and g++")
+    so = tmp_path_factory.mktemp("fake") / "host.so"
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-Wl,-Bsymbolic", f"-I{CUDA}", "-o", str(so),
+                    str(Path(__file__).with_name("fake_cudart.cpp")), *map(str, objects)], check=True)
+    L = ctypes.CDLL(str(so))
+    vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+    L.mk_w4_experts.argtypes = [vp, vp, vp, i64, vp, vp, i32, i32, vp, i64, vp, i64, vp, i64, vp]
+    L.mk_w4_experts_workspace.argtypes = [vp, vp, i32, i32, ctypes.POINTER(i64)]
+    L.mk_w4_linear.argtypes = [vp, vp, i64, i32, vp, i64, vp, i64, i32, vp]
+    L.mk_route.argtypes = [vp, vp, i64, i32, vp, vp, vp, vp]
+    L.fake_launches.restype = L.fake_message.restype = ctypes.c_char_p
+    return L
+
+
+def launched(host):
+    return host.fake_launches().decode().splitlines()
+
+
+def experts(host, T, S, E=4, H=64, inter=96, fail=-1):
+    """mk_w4_experts' code; nothing of what the pointers name is touched."""
+    a, b = (mk.MkW4(4096, 4096, None, n, k, 32, 0, E, 0) for n, k in ((2 * inter, H), (H, inter)))
+    need = ctypes.c_int64()
+    pa, pb = ctypes.addressof(a), ctypes.addressof(b)
+    assert host.mk_w4_experts_workspace(pa, pb, T, S, ctypes.byref(need)) == mk.MK_OK
+    host.fake_begin(fail, 0)
+    return host.mk_w4_experts(pa, pb, 4096, H, 4096, 4096, T, S, None, 0, 8192, H, 1 << 20, need.value, None)
+
+
+def test_experts_launches(host):
+    assert experts(host, 3, 2) == mk.MK_OK and len(launched(host)) == 2
+    assert experts(host, 20, 2) == mk.MK_OK
+    plan, gate_up, down, combine = launched(host)
+    assert "plan_kernel" in plan and "combine_kernel" in combine
+    assert "overlaps" not in plan and "overlaps" in combine      # what precedes the call is not waited for otherwise
+
+
+@pytest.mark.parametrize("fail", [0, 1, 2, 3])
+def test_experts_stop_at_a_launch_that_fails(host, fail):
+    """The launches after the plan take counts and indices from its output."""
+    assert experts(host, 20, 2, fail=fail) == mk.MK_ECUDA
+    assert len(launched(host)) == fail + 1 and host.fake_message()
