@@ -153,7 +153,7 @@ int launch_weight(Args& a, const MkW4* w, int64_t items, bool known, bool xr, in
   const int strips = (w->n + STRIP_ROWS - 1) / STRIP_ROWS;
   // Two tiles a warp share its activations and its loop, one tile spreads few strips over more CTAs (K 2048,
   // one / two tiles: 2048 rows 6.2 / 8.3 us, 8192 rows 8.3 / 9.3, 20000 rows of 8 tokens 14.1 / 13.0)
-  const bool two = items * strips >= 2 * sms && !(xr && a.cols > 8) && a.cols <= MAX_COLS;
+  const bool two = items * strips >= 2 * sms && !(xr && (a.cols > 8 || a.mode == DOWN || a.mode == DOWN_SMALL)) && a.cols <= MAX_COLS;
   a.strips = div_by(two ? strips : 2 * strips);
   const int grid = (int)(known ? std::min<int64_t>(sms, items * a.strips.d) : sms);
   return w->dtype == MK_W4_BF16 ? launch_bf16(a, w->group, two, xr, grid, s)
@@ -167,7 +167,7 @@ bool aligned16(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && l
 struct Plan {   // the workspace of mk_w4_experts, in bytes from its start
   int64_t items, items_n, col_token, slot_col, act, y, bytes;
   int cols, ldact;
-  bool small;
+  bool small, xr2;      // xr2: the down projection's activations come with its units
 };
 
 const char* plan_experts(const MkW4* w13, const MkW4* w2, int64_t t, int64_t s, Plan* p) {
@@ -181,22 +181,23 @@ const char* plan_experts(const MkW4* w13, const MkW4* w2, int64_t t, int64_t s, 
   if (t < 0 || s < 0 || t * s >= (1 << 24)) return "slots (tokens x slots per token) are from 0 to 2^24 - 1";
   p->small = t <= SMALL_T && t * s <= SMALL_SLOTS && fits(units_of(w13), (int)std::max<int64_t>(t, 1));
   p->cols = (int)std::min<int64_t>(std::max<int64_t>(t, 1), GROUPED_COLS);
-  while (p->cols > 1 && !(fits(units_of(w13), p->cols) && (p->small || fits(units_of(w2), p->cols)))) --p->cols;
-  if (!fits(units_of(w13), p->cols) || (!p->small && !fits(units_of(w2), p->cols))) return "rows are too long for the shared memory";
+  while (p->cols > 1 && !fits(units_of(w13), p->cols)) --p->cols;
+  if (!fits(units_of(w13), p->cols)) return "rows are too long for the shared memory";
+  p->xr2 = p->small || !fits(units_of(w2), 2 * p->cols);
   const int64_t n = std::max<int64_t>(t * s, 1), items = w13->experts + n / p->cols + 1;
   const int64_t most = std::max((std::max(w13->n, w2->n) / 16 + 2) * std::max<int64_t>(units_of(w13), units_of(w2)), (int64_t)1);
   if (items * most > INT32_MAX / 2) return "too many slots times rows";
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t r = at; at += (bytes + 255) / 256 * 256; return r; };
   if (p->small) {
-    p->act = take(2 * n * t * units_of(w2) * UNIT_K);
+    p->act = take(2 * 2 * n * t * units_of(w2) * UNIT_K);
   } else {
     p->ldact = (w2->k + 7) / 8 * 8;
     p->items_n = take(4);
     p->items = take(16 * items);
     p->col_token = take(4 * n);
     p->slot_col = take(4 * n);
-    p->act = take(2 * n * p->ldact);
+    p->act = take(2 * 2 * n * p->ldact);
     p->y = take(4 * n * w2->n);
   }
   p->bytes = std::max<int64_t>(at, 256);
@@ -296,7 +297,7 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
     b.out = out;
     b.ldo = ldo;
     b.pairs = aligned4(out, ldo) && (!residual || aligned4(residual, ldr));
-    return launch_weight(b, w2, 1, true, true, sms, st);
+    return launch_weight(b, w2, 1, true, p.xr2, sms, st);
   }
   int4* items = reinterpret_cast<int4*>(ws + p.items);
   int* items_n = reinterpret_cast<int*>(ws + p.items_n);
@@ -311,13 +312,13 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   a.items = b.items = items;
   a.items_n = b.items_n = items_n;
   a.col_token = col_token;
-  a.ldo = b.ldx = p.ldact;
+  a.ldo = b.ldx = 2 * p.ldact;
   if (int rc = launch_weight(a, w13, items_about, false, false, sms, st)) return rc;
   b.mode = DOWN;
   b.out = ws + p.y;
   b.ldo = w2->n;
   b.out_f32 = 1;
-  if (int rc = launch_weight(b, w2, items_about, false, false, sms, st)) return rc;
+  if (int rc = launch_weight(b, w2, items_about, false, p.xr2, sms, st)) return rc;
   const dim3 grid((unsigned)((w2->n + 255) / 256), (unsigned)t);
   const float* y = reinterpret_cast<const float*>(ws + p.y);
   e = launch_behind(

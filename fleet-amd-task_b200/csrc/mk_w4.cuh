@@ -5,7 +5,7 @@
 // points. Products sum exactly that: q - z is an integer of at most 5 bits (exact in BF16 and FP16),
 // its product with a 16-bit activation is exact in FP32, a group is summed by the tensor cores in
 // FP32 and the group's sum is multiplied by its scale in FP32. Nothing is rounded to 16 bits before
-// the result.
+// the result: the experts' intermediate silu(g) u goes to the down projection as the sum of two BF16 values.
 //
 // The laid-out form (fleet/w4.py lay_out) is the order in which the lanes of a warp want the codes
 // for mma.sync m16n8k16 with the weights as the 16-row operand and the tokens as its 8 columns. A
@@ -87,6 +87,15 @@ struct Fp16 {
   }
 };
 
+// v = hi + lo to 16 significant bits (2^-16 of v at most), in FP32's range: both are BF16. An infinity is
+// hi alone, and so is what would round to one.
+__device__ __forceinline__ void split_bf16(float v, uint32_t& hi, uint32_t& lo) {
+  hi = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  if ((hi & 0x7F80u) == 0x7F80u) hi = __float_as_uint(v) >> 16;
+  const float rest = v - __uint_as_float(hi << 16);
+  lo = isinf(v) ? 0u : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(rest));
+}
+
 // weights are read once: past L1
 __device__ __forceinline__ uint4 ldg128(const void* p) {
   uint4 v;
@@ -157,21 +166,25 @@ __device__ __forceinline__ void decode(uint32_t magic, uint32_t w, uint32_t z0, 
   a[3] = D::sub2(and_or(w >> 12, magic), z1);
 }
 
-// 32 values of K: two words against each column tile's 16 bytes of activations; FIRST: acc = instead
-// of acc +=
-template <class D, int NT, bool FIRST>
-__device__ __forceinline__ void half_chunk(uint32_t magic, uint32_t w0, uint32_t w1, uint32_t z0, uint32_t z1, const uint4 (&xb)[NT],
-                                           float (&acc)[NT][4]) {
+// 32 values of K: two words against each column tile's 16 bytes of activations (of every plane: an
+// activation is the sum of its planes); FIRST: acc = instead of acc +=
+template <class D, int NT, int PLANES, bool FIRST>
+__device__ __forceinline__ void half_chunk(uint32_t magic, uint32_t w0, uint32_t w1, uint32_t z0, uint32_t z1,
+                                           const uint4 (&xb)[PLANES][NT], float (&acc)[NT][4]) {
   uint32_t a[4];
   decode<D>(magic, w0, z0, z1, a);
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    if (FIRST) D::mma0(acc[n], a[0], a[1], a[2], a[3], xb[n].x, xb[n].y);
-    else D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].x, xb[n].y);
-  }
+  for (int p = 0; p < PLANES; ++p)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (FIRST && p == 0) D::mma0(acc[n], a[0], a[1], a[2], a[3], xb[p][n].x, xb[p][n].y);
+      else D::mma(acc[n], a[0], a[1], a[2], a[3], xb[p][n].x, xb[p][n].y);
+    }
   decode<D>(magic, w1, z0, z1, a);
 #pragma unroll
-  for (int n = 0; n < NT; ++n) D::mma(acc[n], a[0], a[1], a[2], a[3], xb[n].z, xb[n].w);
+  for (int p = 0; p < PLANES; ++p)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) D::mma(acc[n], a[0], a[1], a[2], a[3], xb[p][n].z, xb[p][n].w);
 }
 
 // tot += scale (rows g, g + 8) * acc (* cw, the columns' weights)

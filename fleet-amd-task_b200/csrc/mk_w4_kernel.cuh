@@ -3,6 +3,7 @@
 #pragma once
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/fleet_mk.h"
 #include "mk_w4.cuh"
@@ -26,7 +27,7 @@ constexpr int SMALL_SLOTS = 256;
 // what a launch computes and where its columns and outputs are
 enum Mode {
   LINEAR = 0,        // items: blocks of tb tokens
-  GATEUP = 1,        // items: the plan's; columns: an item's slots; out: act [column][ldo]
+  GATEUP = 1,        // items: the plan's; columns: an item's slots; out: act [column][2 planes][ldo / 2]
   DOWN = 2,          // items: the plan's; x: act; out: y [column][ldo] FP32
   GATEUP_SMALL = 3,  // items: the selected experts; columns: the tokens; out: act in the MMA's order
   DOWN_SMALL = 4     // one item; a strip's units run over all selected experts; x: act as above
@@ -142,15 +143,17 @@ __device__ __forceinline__ void plan_small(const Args& a, SmallPlan& p) {
   __syncthreads();
 }
 
-// the item's activations in the MMA's order: [K / 32][columns][4] 16-byte vectors
+// the item's activations in the MMA's order: [K / 32][planes][columns][4] 16-byte vectors
+template <int PLANES>
 __device__ __forceinline__ void stage_x(const Args& a, uint4* xs, int start, int count) {
   const int nv = a.nv.d;
   const uint32_t xs_s = (uint32_t)__cvta_generic_to_shared(xs);
-  for (int i = threadIdx.x; i < count * nv; i += blockDim.x) {
-    const int col = i / a.nv, v = i - col * nv;
+  for (int i = threadIdx.x; i < PLANES * count * nv; i += blockDim.x) {
+    const int pc = i / a.nv, v = i - pc * nv;
+    const int plane = PLANES > 1 && pc >= count, col = pc - plane * count;
     const int row = a.mode == GATEUP ? a.col_token[start + col] : start + col;
-    const uint16_t* src = a.x + (int64_t)row * a.ldx + 8 * v;
-    const int at = ((v >> 2) * count + col) * 4 + (v & 3);
+    const uint16_t* src = a.x + (int64_t)row * a.ldx + (plane ? a.ldx / 2 : 0) + 8 * v;
+    const int at = ((v >> 2) * PLANES * count + pc) * 4 + (v & 3);
     if (a.x_vec && 8 * v + 8 <= a.k) {
       cp16(xs_s + at * 16, src);
     } else {
@@ -163,9 +166,12 @@ __device__ __forceinline__ void stage_x(const Args& a, uint4* xs, int start, int
 }
 
 // RT, NT: tiles of 16 rows and 8 columns a warp computes at a time. XR: the activations are loaded with
-// each unit instead of staged. SMALL2: DOWN_SMALL.
-template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2>
+// each unit instead of staged. SMALL2: DOWN_SMALL. WIDE: an activation is the sum of two BF16 planes (DOWN,
+// DOWN_SMALL), whatever the type of the scales and outputs.
+template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2, bool WIDE>
 struct Kernel {
+  using M = std::conditional_t<WIDE, Bf16, D>;    // the MMAs' type
+  static constexpr int PLANES = WIDE ? 2 : 1;
   // Warps and the units each has in flight. 8 columns: 24 warps of 80 registers, one unit each, its halves
   // reloaded as they are used (the 1-token head 25.6 us; 16 warps two units ahead 28.3). More columns, or
   // too few rows for two tiles a warp: 16 warps of 128 registers
@@ -178,7 +184,7 @@ struct Kernel {
     uint4 w[RT][2];
     uint32_t sc[RT][GROUPS];
     uint32_t z[RT][ZP ? ZWORDS : 1];
-    uint4 x[XR ? 4 : 1][XR ? NT : 1];
+    uint4 x[XR ? 4 : 1][PLANES][XR ? NT : 1];
   };
 
   const Args& a;
@@ -226,7 +232,7 @@ struct Kernel {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {   // a lane past the columns takes the last one's: its sums are not used
         const int col = min(i * 8 + g, item_count - 1);
-        x_at[i] = SMALL2 ? a.x + (((int64_t)(item * a.units.d + u) * 4 * item_count + col) * 4 + t) * 8
+        x_at[i] = SMALL2 ? a.x + (((int64_t)(item * a.units.d + u) * 4 * PLANES * item_count + col) * 4 + t) * 8
                          : a.x + (int64_t)(item_start + col) * a.ldx + x_k;
       }
     }
@@ -258,13 +264,15 @@ struct Kernel {
 #pragma unroll
       for (int h = 0; h < 4; ++h)
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          if (SMALL2) n.x[h][i] = ldg128_x(x_at[i] + h * item_count * 32);
-          else if (x_k + 32 * h < a.k) n.x[h][i] = ldg128_x(x_at[i] + 32 * h);
-          else n.x[h][i] = make_uint4(0, 0, 0, 0);
-        }
+        for (int p = 0; p < PLANES; ++p)
 #pragma unroll
-      for (int i = 0; i < NT; ++i) x_at[i] += SMALL2 ? item_count * 128 : UNIT_K;
+          for (int i = 0; i < NT; ++i) {
+            if (SMALL2) n.x[h][p][i] = ldg128_x(x_at[i] + (h * PLANES + p) * item_count * 32);
+            else if (x_k + 32 * h < a.k) n.x[h][p][i] = ldg128_x(x_at[i] + 32 * h + (p ? a.ldx / 2 : 0));
+            else n.x[h][p][i] = make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) x_at[i] += SMALL2 ? PLANES * item_count * 128 : UNIT_K;
       x_k += UNIT_K;
     }
     code += 2 * TILE_UNIT_BYTES;
@@ -277,10 +285,12 @@ struct Kernel {
   static __device__ __forceinline__ int part_of(int p0, int n, int w) {
     return p0 + (n / WARPS) * w + n % WARPS * w / WARPS;
   }
-  // GATEUP_SMALL: act [expert of the plan][unit][32-value part][token][4][8]
-  __device__ __forceinline__ uint16_t& act_at(int item, int col, int j) {
+  // GATEUP_SMALL: act [expert of the plan][unit][32-value part][2 planes][token][4][8]
+  __device__ __forceinline__ uint16_t& act_at(int item, int plane, int col, int j) {
+    uint16_t* act = static_cast<uint16_t*>(a.out);
+    if (a.mode == GATEUP) return act[(int64_t)(item_start + col) * a.ldo + (plane ? a.ldo / 2 : 0) + j];
     const int64_t part = ((int64_t)item * a.ldo + (j >> 7)) * 4 + (j >> 5 & 3);
-    return static_cast<uint16_t*>(a.out)[((part * item_count + col) * 4 + (j >> 3 & 3)) * 8 + (j & 7)];
+    return act[(((part * 2 + plane) * item_count + col) * 4 + (j >> 3 & 3)) * 8 + (j & 7)];
   }
 
   // a barrier that warps meet at from two places
@@ -294,35 +304,37 @@ struct Kernel {
     else if (a.pairs) finish_pairs(strip, tot);
     else finish_single(strip, tot);
   }
-  // gate and up rows: a tile's rows g and g + 8
+  // Gate and up rows: a tile's rows g and g + 8. silu(g) u is kept as two BF16 values, hi + lo: the down
+  // projection's tensor-core operands, in FP32's range (an FP16 one would end at 65504) and off by at most 2^-16 of
+  // itself, so that the results are those of an FP32 activation but for their own rounding.
   __device__ __forceinline__ void finish_act(int item, int strip, const float (&tot)[RT][NT][4]) {
     const int I = a.rows / 2;
-    if (a.mode == GATEUP_SMALL && strip == a.strips.d - 1) {   // act's padding to whole units is zero
-      const int pad = (int)a.ldo * UNIT_K - I;
-      for (int i = lane; i < pad * item_count; i += 32) act_at(item, i / pad, I + i % pad) = 0;
+    if (strip == a.strips.d - 1) {   // act's padding is zero (to whole units, or to the row's end)
+      const int pad = (a.mode == GATEUP ? (int)a.ldo / 2 : (int)a.ldo * UNIT_K) - I;
+      for (int i = lane; i < 2 * pad * item_count; i += 32) {
+        const int pc = i / pad;
+        act_at(item, pc & 1, pc >> 1, I + i % pad) = 0;
+      }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        float v[2];
+        uint32_t hi[2], lo[2];
 #pragma unroll
         for (int ci = 0; ci < 2; ++ci) {
           const float gt = tot[r][n][ci], up = tot[r][n][2 + ci];
-          v[ci] = __fdiv_rn(gt, 1.0f + expf(-gt)) * up;
+          split_bf16(__fdiv_rn(gt, 1.0f + expf(-gt)) * up, hi[ci], lo[ci]);
         }
-        // Rounded to the activations' type: it is the down projection's tensor-core operand, and the rounding
-        // point of the persistent kernel's experts. With the result's own rounding this makes the error of a
-        // 16-bit output 1.4 times that of one rounding (0.0024 against 0.0017 of the norm in BF16).
-        const uint32_t two = transpose8(D::round2(v[0], v[1]));
+        const uint32_t planes[2] = {transpose8(hi[0] | hi[1] << 16), transpose8(lo[0] | lo[1] << 16)};
         const int col = n * 8 + g, j = (strip * RT + r) * 8 + 2 * t;
         if (col < item_count && j < I) {
-          if (a.mode == GATEUP) {      // (the place after an odd last j is padding)
-            *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (int64_t)(item_start + col) * a.ldo + j) = two;
-          } else {
-            const uint32_t w = plan->tokens[item] >> col & 1 ? two : 0u;
-            if (j + 1 < I) *reinterpret_cast<uint32_t*>(&act_at(item, col, j)) = w;
-            else act_at(item, col, j) = (uint16_t)w;
+          const bool selected = a.mode == GATEUP || plan->tokens[item] >> col & 1;
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const uint32_t two = selected ? planes[p] : 0u;
+            if (j + 1 < I) *reinterpret_cast<uint32_t*>(&act_at(item, p, col, j)) = two;
+            else act_at(item, p, col, j) = (uint16_t)two;
           }
         }
       }
@@ -377,27 +389,29 @@ struct Kernel {
       }
   }
 
-  // tot += the unit's products; staged activations at shared address xl + x_off
-  __device__ __forceinline__ void multiply(Unit& n, const uint32_t (&xl)[NT], uint32_t x_off, uint32_t x_h,
+  // tot += the unit's products; staged activations at shared address xl + x_off, x_p to the next plane
+  __device__ __forceinline__ void multiply(Unit& n, const uint32_t (&xl)[NT], uint32_t x_off, uint32_t x_p,
                                            const float2 (&w2)[NT], float (&tot)[RT][NT][4]) {
     float acc[RT][NT][4];
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      uint4 xb[NT];
+      uint4 xb[PLANES][NT];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) xb[i] = XR ? n.x[XR ? h : 0][XR ? i : 0] : lds128(xl[i] + x_off + h * x_h);
+      for (int p = 0; p < PLANES; ++p)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) xb[p][i] = XR ? n.x[XR ? h : 0][p][XR ? i : 0] : lds128(xl[i] + x_off + (h * PLANES + p) * x_p);
       const int i = h * 32 / G;
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        uint32_t z0 = D::MAGIC + 0x00080008u, z1 = z0;
+        uint32_t z0 = M::MAGIC + 0x00080008u, z1 = z0;
         if (ZP) {   // rows g and g + 8 of group i: two bytes
           const uint32_t z = n.z[r][i / 2] >> (i % 2 * 16);
-          z0 = (z & 0xFFu) * 0x00010001u | D::MAGIC;
-          z1 = (z >> 8 & 0xFFu) * 0x00010001u | D::MAGIC;
+          z0 = (z & 0xFFu) * 0x00010001u | M::MAGIC;
+          z1 = (z >> 8 & 0xFFu) * 0x00010001u | M::MAGIC;
         }
         const uint4& v = n.w[r][h >> 1];
-        if (h * 32 % G == 0) half_chunk<D, NT, true>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
-        else half_chunk<D, NT, false>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
+        if (h * 32 % G == 0) half_chunk<M, NT, PLANES, true>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
+        else half_chunk<M, NT, PLANES, false>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
         if ((h + 1) * 32 % G == 0) fold<D, NT, SMALL2>(n.sc[r][i], w2, acc[r], tot[r]);
       }
       if (AHEAD == 1 && h == 1) load_half(n);
@@ -414,7 +428,7 @@ struct Kernel {
 #pragma unroll
     for (int i = 0; i < NT; ++i)
       xl[i] = XR ? 0 : (uint32_t)__cvta_generic_to_shared(xs) + (min(i * 8 + g, item_count - 1) * 4 + t) * 16;
-    const uint32_t x_h = item_count * 64;
+    const uint32_t x_p = item_count * 64, x_u = 4 * PLANES * x_p;
     bool met = false;                     // this warp has been at the barrier
     int next = 0;                         // the place in un of the next unit
     while (p < p_end) {
@@ -422,7 +436,7 @@ struct Kernel {
       const int q0 = p - strip_flat * U, q1 = min(U, q0 + p_end - p);
 #pragma unroll
       for (int i = 0; i < WORDS; ++i) (&tot[0][0][0])[i] = 0.0f;
-      uint32_t x_off = q0 * x_h * 4;
+      uint32_t x_off = q0 * x_u;
       float2 w2[NT];
       int to_expert = 0, expert = 0;      // SMALL2: units to the next expert, its place in the plan
       auto weigh = [&]() {
@@ -439,12 +453,12 @@ struct Kernel {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
           if (next == i && left > 0) {
-            multiply(un[i], xl, x_off, x_h, w2, tot);
+            multiply(un[i], xl, x_off, x_p, w2, tot);
             load_weights(un[i], AHEAD == 1);
             load_rest(un[i]);
             next = i + 1 == AHEAD ? 0 : i + 1;
             --left;
-            x_off += x_h * 4;
+            x_off += x_u;
             if (SMALL2 && --to_expert == 0 && left > 0) {
               to_expert = a.units.d;
               ++expert;
@@ -478,7 +492,7 @@ struct Kernel {
 
   __device__ __forceinline__ void run_all(uint8_t* smem, SmallPlan& sp) {
     warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    magic = magic_register<D>();
+    magic = magic_register<M>();
     uint8_t* after = smem;
     slots = reinterpret_cast<float*>(after);
     after += WARPS * RT * NT * 4 * 32 * 4;
@@ -550,7 +564,7 @@ struct Kernel {
         if (SMALL2 && i == 0 && a.follows) wait_predecessor();   // its activations: the plan and the weights are not
         load_rest(un[i]);
       }
-      if (!XR) stage_x(a, xs, item_start, item_count);
+      if (!XR) stage_x<PLANES>(a, xs, item_start, item_count);
       if (!XR) {
         cp_wait_all();
         __syncthreads();
@@ -562,11 +576,11 @@ struct Kernel {
   }
 };
 
-template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2>
-__global__ void __launch_bounds__(Kernel<D, RT, NT, G, ZP, XR, SMALL2>::THREADS, 1) w4_kernel(const Args a) {
+template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2, bool WIDE>
+__global__ void __launch_bounds__(Kernel<D, RT, NT, G, ZP, XR, SMALL2, WIDE>::THREADS, 1) w4_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ SmallPlan plan;
-  Kernel<D, RT, NT, G, ZP, XR, SMALL2> k(a);
+  Kernel<D, RT, NT, G, ZP, XR, SMALL2, WIDE> k(a);
   k.run_all(smem, plan);
 }
 
@@ -595,13 +609,13 @@ cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, int threads, int smem
   return cudaLaunchKernelEx(&c, kernel, args...);
 }
 
-template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2>
+template <class D, int RT, int NT, int G, bool ZP, bool XR, bool SMALL2, bool WIDE>
 static int launch(const Args& a, int grid, cudaStream_t s) {
-  using K = Kernel<D, RT, NT, G, ZP, XR, SMALL2>;
+  using K = Kernel<D, RT, NT, G, ZP, XR, SMALL2, WIDE>;
   constexpr int parts = K::WARPS * RT * NT * 4 * 32 * 4;
   static_assert(parts <= PARTS_BYTES, "the parts of strips");
-  const int smem = parts + (SMALL2 ? CW_BYTES : XR ? 0 : a.cols * a.units.d * UNIT_K * 2);
-  const auto kernel = w4_kernel<D, RT, NT, G, ZP, XR, SMALL2>;
+  const int smem = parts + (SMALL2 ? CW_BYTES : XR ? 0 : K::PLANES * a.cols * a.units.d * UNIT_K * 2);
+  const auto kernel = w4_kernel<D, RT, NT, G, ZP, XR, SMALL2, WIDE>;
   static std::atomic<bool> ready[MAX_DEVICES];   // the kernel may use that much shared memory on the device
   cudaError_t e = cudaSuccess;
   if (!ready[a.device].load(std::memory_order_acquire)) {
@@ -612,17 +626,22 @@ static int launch(const Args& a, int grid, cudaStream_t s) {
   return e == cudaSuccess ? MK_OK : mk::set_last_error(MK_ECUDA, cudaGetErrorString(e));
 }
 
-// two: two tiles a warp; xr: the activations come with the units (one tile a warp if over 8 columns)
+// two: two tiles a warp; xr: the activations come with the units (of more than 8 columns, or in two planes: one
+// tile a warp, for its registers)
 template <class D, int G, bool ZP>
 static int launch_form(const Args& a, bool two, bool xr, int grid, cudaStream_t s) {
-  if (a.cols <= 8) {
-    if (a.mode == DOWN_SMALL) return two ? launch<D, 2, 1, G, ZP, true, true>(a, grid, s) : launch<D, 1, 1, G, ZP, true, true>(a, grid, s);
-    if (xr) return two ? launch<D, 2, 1, G, ZP, true, false>(a, grid, s) : launch<D, 1, 1, G, ZP, true, false>(a, grid, s);
-    return two ? launch<D, 2, 1, G, ZP, false, false>(a, grid, s) : launch<D, 1, 1, G, ZP, false, false>(a, grid, s);
+  if (a.mode == DOWN_SMALL) return launch<D, 1, 1, G, ZP, true, true, true>(a, grid, s);
+  if (a.mode == DOWN) {
+    if (xr) return launch<D, 1, 1, G, ZP, true, false, true>(a, grid, s);
+    return two ? launch<D, 2, 1, G, ZP, false, false, true>(a, grid, s) : launch<D, 1, 1, G, ZP, false, false, true>(a, grid, s);
   }
-  if (xr) return launch<D, 1, 2, G, ZP, true, false>(a, grid, s);
-  if (a.cols > MAX_COLS) return launch<D, 1, 4, G, ZP, false, false>(a, grid, s);
-  return two ? launch<D, 2, 2, G, ZP, false, false>(a, grid, s) : launch<D, 1, 2, G, ZP, false, false>(a, grid, s);
+  if (a.cols <= 8) {
+    if (xr) return two ? launch<D, 2, 1, G, ZP, true, false, false>(a, grid, s) : launch<D, 1, 1, G, ZP, true, false, false>(a, grid, s);
+    return two ? launch<D, 2, 1, G, ZP, false, false, false>(a, grid, s) : launch<D, 1, 1, G, ZP, false, false, false>(a, grid, s);
+  }
+  if (xr) return launch<D, 1, 2, G, ZP, true, false, false>(a, grid, s);
+  if (a.cols > MAX_COLS) return launch<D, 1, 4, G, ZP, false, false, false>(a, grid, s);
+  return two ? launch<D, 2, 2, G, ZP, false, false, false>(a, grid, s) : launch<D, 1, 2, G, ZP, false, false, false>(a, grid, s);
 }
 
 template <class D>

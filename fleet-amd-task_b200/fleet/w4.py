@@ -174,8 +174,8 @@ class W4Experts:
 
     w13, w2: (codes, scales, zeros or None) of W13 [E, 2 I, H] (gate/up rows interleaved as
     pack_weights packs them) and W2 [E, H, I] (`inter` = I). ids [T, S] int32 and weights [T, S] float32 as
-    route_experts returns them; a slot whose id is outside [0, E) is empty. The activation silu(g) u
-    is rounded to the type of x (the down projection's tensor-core operand), all sums are FP32. Runs on
+    route_experts returns them; a slot whose id is outside [0, E) is empty. The intermediate
+    silu(g) u is held to 16 significant bits in FP32's range, all sums are FP32, rounded once. Runs on
     `stream` (default: the current stream); the workspace comes from torch's allocator for each call,
     so calls on several streams do not share one."""
 

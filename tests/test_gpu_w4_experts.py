@@ -1,0 +1,111 @@
+"""W4Experts where its intermediate, the order of its sums and its forms can go wrong, against 64 bits.
+
+The bounds are those of a computation in FP32 that rounds once, at the end. The intermediate a = silu(g) u goes
+to the down projection as two BF16 values: the second holds the first one's remainder to 8 significant
+bits, so a is off by at most 2^-16 of itself. An MMA rounds or truncates its sum by at most 2^-23 of the terms'
+magnitudes; a group has at most 8 of them for the gate and up rows and 16 for the down projection (8 for
+each value), each with two such roundings, then one for the scale and one for the sum per group and 18
+across the warps, the residual and the result, as for the linear."""
+import pytest
+import torch
+
+from fleet.pack_weights import dequantize_w4
+from fleet.w4 import W4Experts
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U16 = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}   # half a step of 8 and 11 significant bits
+SUBNORMAL = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}   # half a step below the normal range
+U = 2.0 ** -24
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def weight_of(g, shape, k, group, zeros, dtype, scale=0.01):
+    n = -(-k // group)
+    codes = torch.randint(0, 256, (*shape, (k + 1) // 2), generator=g, device=DEV, dtype=torch.uint8)
+    scales = (torch.rand(*shape, n, generator=g, device=DEV) * scale + scale / 10).to(dtype)
+    return codes, scales, torch.randint(0, 16, (*shape, n), generator=g, device=DEV, dtype=torch.uint8) if zeros else None
+
+
+def reference(x, ids, weights, w13, w2, H, I, group, res, dtype):
+    """(want, bound) in 64 bits; empty slots are ids outside the experts."""
+    E = w13[0].shape[0]
+    sums = lambda mmas, k: (2 * mmas + 2 * -(-k // group) + 18) * 2 * U  # noqa: E731
+    want = torch.zeros(x.shape[0], H, dtype=torch.float64, device=DEV) if res is None else res.double().clone()
+    err, mag = torch.zeros_like(want), want.abs()
+    part = lambda w, e: [None if v is None else v[e] for v in w]  # noqa: E731
+    for e in ids.unique().tolist():
+        if not 0 <= e < E:
+            continue
+        W13, W2 = dequantize_w4(*part(w13, e), H, group).double(), dequantize_w4(*part(w2, e), I, group).double()
+        t, s = (ids == e).nonzero(as_tuple=True)
+        xe = x[t].double()
+        gu, m = xe @ W13.T, (xe.abs() @ W13.abs().T) * sums(8, H)
+        gt, up = gu[:, 0::2], gu[:, 1::2]
+        silu = gt * torch.sigmoid(gt)
+        a = silu * up
+        # |silu'| <= 1.1; expf, the addition, the division and the product round by at most 6 units
+        ea = 1.1 * m[:, 0::2] * (up.abs() + m[:, 1::2]) + silu.abs() * m[:, 1::2] + a.abs() * (2.0 ** -16 + 6 * U)
+        ey = ea @ W2.abs().T + ((a.abs() + ea) @ W2.abs().T) * sums(16, I)
+        f, y = weights[t, s].double()[:, None], a @ W2.T
+        want.index_add_(0, t, f * y)
+        err.index_add_(0, t, f.abs() * ey)
+        mag.index_add_(0, t, f.abs() * (y.abs() + ey))
+    err = err + mag * (ids.shape[1] + 2) * 2 * U
+    return want, err + (want.abs() + err) * U16[dtype] + SUBNORMAL[dtype]
+
+
+def routed(g, T, E, S):
+    ids = torch.rand(T, E, generator=g, device=DEV).argsort(1)[:, :S].to(torch.int32).contiguous()
+    return ids, torch.rand(T, S, generator=g, device=DEV)
+
+
+def check(T, H, I, E, S, group, zeros, residual, dtype, scale=0.01, x_scale=1.0, w2_scale=None):
+    g = gen(T * 37 + H)
+    w13 = weight_of(g, (E, 2 * I), H, group, zeros, dtype, scale)
+    w2 = weight_of(g, (E, H), I, group, zeros, dtype, w2_scale or scale)
+    x = (torch.randn(T, H, generator=g, device=DEV) * x_scale).to(dtype)
+    ids, weights = routed(g, T, E, S)
+    res = torch.randn(T, H, generator=g, device=DEV).to(dtype) if residual else None
+    op = W4Experts(w13, w2, group=group, inter=I)
+    got = op(x, ids, weights, residual=res)
+    want, bound = reference(x, ids, weights, w13, w2, H, I, group, res, dtype)
+    assert ((got.double() - want).abs() <= bound).all()
+    return op, x, ids, weights, res, got, want
+
+
+DTYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+
+
+@DTYPES
+@pytest.mark.parametrize("T,H,I,E,S,group,zeros,residual", [
+    (1, 256, 512, 4, 4, 128, False, False), (6, 512, 640, 8, 3, 32, True, True), (8, 192, 330, 16, 8, 64, True, False),
+    (24, 256, 512, 6, 3, 64, False, False), (50, 384, 523, 4, 2, 32, True, True), (30, 9500, 48, 3, 2, 64, False, True),
+])
+def test_one_rounding(T, H, I, E, S, group, zeros, residual, dtype):
+    """No rounding to 16 bits but the result's: the bound has none, and where the result does not cancel the
+    errors are those of one rounding."""
+    got, want = check(T, H, I, E, S, group, zeros, residual, dtype)[-2:]
+    once = (want.to(dtype).double() - want).norm()
+    assert (got.double() - want).norm() <= 1.05 * once
+
+
+@pytest.mark.parametrize("T", [1, 5, 20])
+def test_fp16_intermediate_past_its_types_range(T):
+    """silu(g) u past 65504 with results inside FP16's range."""
+    op, x, ids, weights, res, got, want = check(T, 64, 96, 4, 2, 32, True, True, torch.float16, scale=0.5, x_scale=40.0,
+                                                w2_scale=2e-6)
+    g = gen(T * 37 + 64)
+    w13 = weight_of(g, (4, 192), 64, 32, True, torch.float16, 0.5)
+    gu = torch.einsum("tk,enk->ten", x.float(), dequantize_w4(*w13, 64, 32))
+    assert (torch.nn.functional.silu(gu[..., 0::2]) * gu[..., 1::2]).abs().max() > 4 * 65504
+    assert want.abs().max() < 65504 and got.isfinite().all()
+
+
+@DTYPES
+@pytest.mark.parametrize("T", [1, 9])
+def test_rows_of_the_down_projection_too_long_to_stage(T, dtype):
+    check(T, 64, 50011, 2, 1, 64, False, True, dtype)
