@@ -46,26 +46,44 @@ using namespace w4;
 
 namespace {
 
-// The slots grouped by expert: columns (slots in expert order), col_token, slot_col (a slot's
-// column, -1 if empty), and the items of at most tb columns of one expert. One CTA. A slot's place
-// among its expert's columns depends on the order of the counting and changes no result: a column's
-// sums do not depend on its place.
-__global__ void __launch_bounds__(1024) plan_kernel(const int* __restrict__ ids, int t, int s, int experts, int tb,
+constexpr int PLAN_COUNTS = 10240;   // 40 KB: all 32 warps count for up to 320 experts, 10 for 1024
+
+// The slots grouped by expert: columns (slots in expert order, an expert's in slot order), col_token,
+// slot_col (a slot's column, -1 if empty), and the items of at most tb columns of one expert. One CTA. A
+// column's sums are split where its item lies in the CTAs' ranges, so a slot's place among its expert's columns
+// has to be the same on every run: each warp counts the experts of a run of consecutive slots, and the
+// places are the counts of the warps before it and of the slots before in its own run. (Places in the order
+// of atomics: 162 of 200 runs of 64 tokens of 66 experts differed from the first in some results.) The first
+// `warps` warps take `chunk` slots each, a multiple of 32.
+__global__ void __launch_bounds__(1024) plan_kernel(const int* __restrict__ ids, int n, int s, int experts, int tb, int warps, int chunk,
                                                     int4* items, int* items_n, int* col_token, int* slot_col) {
-  __shared__ int cnt[MAX_EXPERTS], first[MAX_EXPERTS];
+  extern __shared__ int cnt[];           // [warps][experts]
+  __shared__ int first[MAX_EXPERTS];
   start_dependents();
-  const int n = t * s;
-  for (int e = threadIdx.x; e < MAX_EXPERTS; e += blockDim.x) cnt[e] = 0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lo = warp < warps ? min(warp * chunk, n) : n, hi = min(lo + chunk, n);
+  int* mine = cnt + warp * experts;      // (of warps past the last one: not used)
+  for (int i = threadIdx.x; i < warps * experts; i += blockDim.x) cnt[i] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+  for (int i = lo + lane; i < hi; i += 32) {
     const int e = ids[i];
-    if ((unsigned)e < (unsigned)experts) atomicAdd(&cnt[e], 1);
+    if ((unsigned)e < (unsigned)experts) atomicAdd(&mine[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+    int sum = 0;
+    for (int w = 0; w < warps; ++w) {
+      const int c = cnt[w * experts + e];
+      cnt[w * experts + e] = sum;
+      sum += c;
+    }
+    first[e] = sum;
   }
   __syncthreads();
   if (threadIdx.x < 32) {
     int cols = 0, its = 0;
     for (int e0 = 0; e0 < experts; e0 += 32) {
-      const int e = e0 + threadIdx.x, c = e < experts ? cnt[e] : 0, b = (c + tb - 1) / tb;
+      const int e = e0 + threadIdx.x, c = e < experts ? first[e] : 0, b = (c + tb - 1) / tb;
       int ci = c, bi = b;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -81,14 +99,19 @@ __global__ void __launch_bounds__(1024) plan_kernel(const int* __restrict__ ids,
     if (threadIdx.x == 0) *items_n = its;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int e = ids[i];
+  for (int i0 = lo; i0 < hi; i0 += 32) {
+    const int i = i0 + lane, e = i < hi ? ids[i] : -1;
+    const bool valid = (unsigned)e < (unsigned)experts;
+    const uint32_t same = __match_any_sync(~0u, valid ? e : -1), before = same & ((1u << lane) - 1);
     int col = -1;
-    if ((unsigned)e < (unsigned)experts) {
-      col = atomicAdd(&first[e], 1);
+    if (valid) {
+      col = first[e] + mine[e] + __popc(before);
       col_token[col] = i / s;
     }
-    slot_col[i] = col;
+    if (i < hi) slot_col[i] = col;
+    __syncwarp();
+    if (valid && before == 0) mine[e] += __popc(same);
+    __syncwarp();
   }
 }
 
@@ -304,8 +327,10 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   int* col_token = reinterpret_cast<int*>(ws + p.col_token);
   int* slot_col = reinterpret_cast<int*>(ws + p.slot_col);
   // the launches after it take counts and indices from its output: none without it
-  cudaError_t e = launch_behind(plan_kernel, dim3(1), 1024, 0, st, false, ids, (int)t, (int)slots, (int)w13->experts, p.cols, items,
-                                items_n, col_token, slot_col);
+  const int n = t * slots, warps = std::min({32, PLAN_COUNTS / w13->experts, (n + 31) / 32});
+  const int chunk = warps ? ((n + warps - 1) / warps + 31) / 32 * 32 : 0;
+  cudaError_t e = launch_behind(plan_kernel, dim3(1), 1024, warps * w13->experts * 4, st, false, ids, n, (int)slots, (int)w13->experts,
+                                p.cols, warps, chunk, items, items_n, col_token, slot_col);
   if (e != cudaSuccess) return fail(MK_ECUDA, cudaGetErrorString(e));
   a.mode = GATEUP;
   a.follows = b.follows = 1;

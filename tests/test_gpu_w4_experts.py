@@ -109,3 +109,32 @@ def test_fp16_intermediate_past_its_types_range(T):
 @pytest.mark.parametrize("T", [1, 9])
 def test_rows_of_the_down_projection_too_long_to_stage(T, dtype):
     check(T, 64, 50011, 2, 1, 64, False, True, dtype)
+
+
+@DTYPES
+@pytest.mark.parametrize("T,S,E,H,I", [(64, 8, 66, 512, 200), (256, 2, 4, 512, 512), (1000, 4, 8, 1024, 256), (300, 1, 1, 256, 300)])
+def test_experts_of_several_items_are_the_same_on_every_run(T, S, E, H, I, dtype):
+    """More slots an expert than an item has columns: which of them share an item must not depend on timing."""
+    op, x, ids, weights, res, got, want = check(T, H, I, E, S, 64, True, False, dtype)
+    for _ in range(30):
+        assert torch.equal(op(x, ids, weights), got)
+
+
+@pytest.mark.parametrize("T,S,E", [(9, 1, 1024), (2000, 16, 1024), (3000, 32, 700), (5000, 2, 321), (40, 8, 320), (20000, 3, 5)])
+def test_every_slot_has_its_place(T, S, E):
+    """Empty slots between the others, an expert's slots spread over all warps of the plan, repeated slots, more
+    experts than all of its warps can count."""
+    g = gen(T + E)
+    H, I = 32, 16
+    w13 = torch.randint(0, 256, (E, 2 * I, H // 2), generator=g, device=DEV, dtype=torch.uint8)
+    w2 = torch.randint(0, 256, (E, H, I // 2), generator=g, device=DEV, dtype=torch.uint8)
+    one = torch.ones(E, 2 * I, 1, device=DEV, dtype=torch.bfloat16)
+    op = W4Experts((w13, one / 64, None), (w2, one[:, :H], None), group=32, inter=I)
+    x = torch.randn(T, H, generator=g, device=DEV).bfloat16()
+    ids = torch.randint(0, E, (T, S), generator=g, device=DEV, dtype=torch.int32)
+    ids[torch.rand(T, S, generator=g, device=DEV) < 0.2] = -1
+    weights = torch.randint(-2, 3, (T, S), generator=g, device=DEV).float()
+    got = op(x, ids, weights)
+    want, bound = reference(x, ids, weights, (w13, one / 64, None), (w2, one[:, :H], None), H, I, 32, None, torch.bfloat16)
+    assert ((got.double() - want).abs() <= bound).all()
+    assert torch.equal(op(x, ids, weights), got)
