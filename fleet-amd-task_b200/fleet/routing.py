@@ -55,7 +55,8 @@ def route_experts(logits, topk, *, score="softmax", bias=None, n_group=1, topk_g
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError(f"logits [T, E] with unit stride along E expected, got {tuple(logits.shape)}, strides {logits.stride()}")
     T, E = logits.shape
-    params = _params(E, topk, n_forced, n_group, topk_group, group_score, score, renormalize, logits.dtype, scaling)[1]
+    # held until the call is over: the cache may drop it meanwhile
+    params = _params(E, topk, n_forced, n_group, topk_group, group_score, score, renormalize, logits.dtype, scaling)
     call, device, current_stream, context = mk.entry("mk_route")
     index = logits.get_device()
     if index < 0 or device() != index:
@@ -77,7 +78,7 @@ def route_experts(logits, topk, *, score="softmax", bias=None, n_group=1, topk_g
         weights = torch.empty_strided(shape, (k, 1), dtype=torch.float32, device=logits.device)
     else:
         _given(weights, shape, torch.float32, logits.device, "weights")
-    rc = call(params, logits.data_ptr(), logits.stride(0), T, b, ids.data_ptr(), weights.data_ptr(), current_stream(index))
+    rc = call(params[1], logits.data_ptr(), logits.stride(0), T, b, ids.data_ptr(), weights.data_ptr(), current_stream(index))
     if rc:
         mk._check(rc, "mk_route")
     return ids, weights

@@ -1,0 +1,66 @@
+"""route_experts' host side without a GPU: what the library is handed, with its entry point replaced."""
+import ctypes
+import gc
+import weakref
+
+import pytest
+import torch
+
+from fleet import mk, routing
+
+
+class OnDevice:
+    """Logits [4, 64] that say they are on CUDA device 0."""
+    shape, dtype, device = torch.Size((4, 64)), torch.float32, torch.device("cpu")
+
+    def dim(self):
+        return 2
+
+    def stride(self, i=None):
+        return (64, 1) if i is None else (64, 1)[i]
+
+    def get_device(self):
+        return 0
+
+    def data_ptr(self):
+        return 4096
+
+
+class Handed:
+    """The library's calls: what `during` made of each call's parameters (a copy of them)."""
+
+    def __init__(self):
+        self.calls = []
+        self.during = lambda p: mk.MkRoute.from_buffer_copy(ctypes.string_at(p, ctypes.sizeof(mk.MkRoute)))
+
+    def __call__(self, params, *_):
+        self.calls.append(self.during(params))
+        return 0
+
+
+@pytest.fixture
+def handed(monkeypatch):
+    h = Handed()
+    monkeypatch.setattr(mk, "entry", lambda name: (h, lambda: 0, lambda index: 0, None))
+    routing._params.cache_clear()
+    return h
+
+
+def test_parameters_live_as_long_as_the_call(handed, monkeypatch):
+    """Another thread may route with so many other parameters during a call that the cache drops this call's."""
+    made = []
+
+    class Watched(mk.MkRoute):
+        def __init__(self, *a):
+            super().__init__(*a)
+            made.append(weakref.ref(self))
+    monkeypatch.setattr(mk, "MkRoute", Watched)
+
+    def others(params):
+        for k in range(1, 400):
+            routing._params(64, 1, 0, 1, 1, "max", "softmax", False, torch.float32, float(k))
+        gc.collect()
+        return made[0]() is not None
+    handed.during = others
+    routing.route_experts(OnDevice(), 6)
+    assert handed.calls == [True]
