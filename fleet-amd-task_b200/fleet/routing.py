@@ -6,6 +6,7 @@ their configurations. Its ids and weights are what fleet.w4.W4Experts takes.
 """
 import ctypes
 from functools import lru_cache
+from operator import index as index_of
 
 import torch
 
@@ -55,8 +56,11 @@ def route_experts(logits, topk, *, score="softmax", bias=None, n_group=1, topk_g
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError(f"logits [T, E] with unit stride along E expected, got {tuple(logits.shape)}, strides {logits.stride()}")
     T, E = logits.shape
-    # held until the call is over: the cache may drop it meanwhile
-    params = _params(E, topk, n_forced, n_group, topk_group, group_score, score, renormalize, logits.dtype, scaling)
+    topk, n_forced = index_of(topk), index_of(n_forced)
+    # plain numbers (a tensor would be cached by its identity), held until the call is over: the cache may drop
+    # them meanwhile
+    params = _params(E, topk, n_forced, index_of(n_group), index_of(topk_group), group_score, score, bool(renormalize),
+                     logits.dtype, float(scaling))
     call, device, current_stream, context = mk.entry("mk_route")
     index = logits.get_device()
     if index < 0 or device() != index:

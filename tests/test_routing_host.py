@@ -64,3 +64,21 @@ def test_parameters_live_as_long_as_the_call(handed, monkeypatch):
     handed.during = others
     routing.route_experts(OnDevice(), 6)
     assert handed.calls == [True]
+
+
+def test_scaling_is_a_number_not_an_object(handed):
+    """A tensor hashes by its identity: the call after it changed must not get the first one's value."""
+    scaling = torch.tensor(2.0)
+    routing.route_experts(OnDevice(), 6, scaling=scaling)
+    scaling.fill_(3.0)
+    routing.route_experts(OnDevice(), 6, scaling=scaling)
+    assert [p.scaling for p in handed.calls] == [2.0, 3.0]
+
+
+def test_counts_are_integers(handed):
+    import numpy as np
+    ids, weights = routing.route_experts(OnDevice(), np.int64(6), n_forced=torch.tensor(2), renormalize=np.bool_(True))
+    assert ids.shape == weights.shape == (4, 8)
+    assert (handed.calls[0].topk, handed.calls[0].n_forced, handed.calls[0].renormalize) == (6, 2, 1)
+    with pytest.raises(TypeError):
+        routing.route_experts(OnDevice(), 6.0)
