@@ -169,8 +169,12 @@ def on_stream(t, stream):
     """A context with `stream` (a torch stream, or a raw handle on tensor t's device) current, so that
     what a call allocates belongs to the stream that uses it."""
     import torch
+    if t.device.type != "cuda":
+        raise MkError(MK_EINVAL, f"a stream is given, but the tensors are on {t.device}")
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=t.device)
+    elif stream.device != t.device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors are on {t.device}")
     return torch.cuda.stream(stream)
 
 

@@ -82,3 +82,14 @@ def test_counts_are_integers(handed):
     assert (handed.calls[0].topk, handed.calls[0].n_forced, handed.calls[0].renormalize) == (6, 2, 1)
     with pytest.raises(TypeError):
         routing.route_experts(OnDevice(), 6.0)
+
+
+def test_a_stream_of_another_device_is_refused():
+    """It would otherwise be ignored: the call runs on its tensors' device, on that device's current stream."""
+    from types import SimpleNamespace
+    on = SimpleNamespace(device=torch.device("cuda", 0))
+    with pytest.raises(ValueError):
+        mk.on_stream(on, SimpleNamespace(cuda_stream=64, device=torch.device("cuda", 1)))
+    for stream in (64, SimpleNamespace(cuda_stream=64, device=torch.device("cuda", 0))):
+        with pytest.raises(mk.MkError):
+            mk.on_stream(SimpleNamespace(device=torch.device("cpu")), stream)
