@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const int* __restrict__ ids,
 template <class D>
 __global__ void __launch_bounds__(256) combine_kernel(const float* y, const int* slot_col, const float* weights, int s, int h,
                                                       const uint16_t* residual, int64_t ldr, uint16_t* out, int64_t ldo) {
-  const int tok = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
+  const int tok = blockIdx.x, j = blockIdx.y * 256 + threadIdx.x;
   wait_predecessor();
   if (j >= h) return;
   float v = residual ? D::one_to_f32(residual[(int64_t)tok * ldr + j]) : 0.0f;
@@ -286,7 +286,6 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   if (((uintptr_t)x & 1) || ((uintptr_t)residual & 1) || ((uintptr_t)out & 1)) return fail(MK_EINVAL, "misaligned x, residual or out");
   if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255))
     return fail(MK_EINVAL, "the workspace is missing, too small (mk_w4_experts_workspace) or not at a 256-byte boundary");
-  if (t > 65535) return fail(MK_EINVAL, "at most 65535 tokens a call");
   int sms = 0;
   Args a{}, b{};
   if (int rc = device_sms(&a.device, &sms)) return rc;
@@ -344,7 +343,7 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   b.ldo = w2->n;
   b.out_f32 = 1;
   if (int rc = launch_weight(b, w2, items_about, false, p.xr2, sms, st)) return rc;
-  const dim3 grid((unsigned)((w2->n + 255) / 256), (unsigned)t);
+  const dim3 grid((unsigned)t, (unsigned)((w2->n + 255) / 256));
   const float* y = reinterpret_cast<const float*>(ws + p.y);
   e = launch_behind(
       w2->dtype == MK_W4_BF16 ? combine_kernel<Bf16> : combine_kernel<Fp16>, grid, 256, 0, st, true, y, (const int*)slot_col, weights, (int)slots,

@@ -378,7 +378,9 @@ int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t, const voi
    of its tiles holding 8 gate rows, then their 8 up rows (lay_out(..., gate_up=True)); w2 [E, H, I].
    ids [t, slots] int32 and weights [t, slots] FP32, contiguous; a slot whose id is outside [0, E) is
    empty. The workspace (mk_w4_experts_workspace bytes, 256-byte aligned) holds nothing between
-   calls; calls that overlap on the GPU need one each. */
+   calls; calls that overlap on the GPU need one each. Limits, which both functions refuse alike: 1024
+   experts, 2^24 - 1 slots (t x slots), H of 95232, and slots / 8 x the rows and values of an expert in
+   tiles of 16 x 128 within 2^30 (3 million slots of 2048 x 1408). */
 int mk_w4_experts_workspace(const MkW4* w13, const MkW4* w2, int32_t t, int32_t slots, int64_t* bytes);
 int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int64_t ldx, const int32_t* ids, const float* weights,
                   int32_t t, int32_t slots, const void* residual, int64_t ldr, void* out, int64_t ldo, void* workspace,

@@ -138,3 +138,7 @@ def test_every_slot_has_its_place(T, S, E):
     want, bound = reference(x, ids, weights, (w13, one / 64, None), (w2, one[:, :H], None), H, I, 32, None, torch.bfloat16)
     assert ((got.double() - want).abs() <= bound).all()
     assert torch.equal(op(x, ids, weights), got)
+
+
+def test_more_tokens_than_a_grid_has_rows():
+    check(70000, 16, 8, 3, 1, 32, False, True, torch.bfloat16)

@@ -81,3 +81,12 @@ def test_experts_stop_at_a_launch_that_fails(host, fail):
     """The launches after the plan take counts and indices from its output."""
     assert experts(host, 20, 2, fail=fail) == mk.MK_ECUDA
     assert len(launched(host)) == fail + 1 and host.fake_message()
+
+
+@pytest.mark.parametrize("T,H", [(65536, 64), (1 << 21, 64), (9, 4096)])
+def test_experts_of_any_number_of_tokens(host, T, H):
+    """What the workspace query accepts the call accepts, in grids that a device takes."""
+    assert experts(host, T, 2, H=H) == mk.MK_OK, host.fake_message()
+    for line in launched(host):
+        x, y = map(int, re.search(r" (\d+) (\d+) \d+(?: overlaps)?$", line).groups())
+        assert 1 <= x < 2 ** 31 and 1 <= y <= 65535, line
