@@ -284,6 +284,7 @@ extern "C" int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int
   if (t == 0) return MK_OK;
   if (!x || !out || (slots && (!ids || !weights))) return fail(MK_EINVAL, "null pointer");
   if (((uintptr_t)x & 1) || ((uintptr_t)residual & 1) || ((uintptr_t)out & 1)) return fail(MK_EINVAL, "misaligned x, residual or out");
+  if (((uintptr_t)ids & 3) || ((uintptr_t)weights & 3)) return fail(MK_EINVAL, "misaligned ids or weights");
   if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255))
     return fail(MK_EINVAL, "the workspace is missing, too small (mk_w4_experts_workspace) or not at a 256-byte boundary");
   int sms = 0;

@@ -90,3 +90,13 @@ def test_experts_of_any_number_of_tokens(host, T, H):
     for line in launched(host):
         x, y = map(int, re.search(r" (\d+) (\d+) \d+(?: overlaps)?$", line).groups())
         assert 1 <= x < 2 ** 31 and 1 <= y <= 65535, line
+
+
+@pytest.mark.parametrize("ids,weights", [(4097, 4096), (4098, 4096), (4096, 4098)])
+def test_experts_refuse_misaligned_routing(host, ids, weights):
+    a, b = (mk.MkW4(4096, 4096, None, n, k, 32, 0, 4, 0) for n, k in ((192, 64), (64, 96)))
+    for t in (3, 20):
+        host.fake_begin(-1, 0)
+        assert host.mk_w4_experts(ctypes.addressof(a), ctypes.addressof(b), 4096, 64, ids, weights, t, 2, None, 0, 8192, 64, 1 << 20,
+                                  1 << 30, None) == mk.MK_EINVAL
+        assert not launched(host)
