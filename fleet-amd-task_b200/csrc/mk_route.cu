@@ -291,7 +291,7 @@ cudaError_t launch_width(Args a, cudaStream_t s) {
   if (a.gsize % V == 0)
     for (int l = 0; l <= 5; ++l)
       if (a.gsize / V == 1 << l) a.lanes = l;
-  route_kernel<L, V><<<(unsigned)((a.t + WARPS - 1) / WARPS), WARPS * 32, 0, s>>>(a);
+  route_kernel<L, V><<<((unsigned)a.t + WARPS - 1) / WARPS, WARPS * 32, 0, s>>>(a);
   return cudaGetLastError();
 }
 

@@ -135,6 +135,7 @@ int fail(int code, const char* msg) { return mk::set_last_error(code, msg); }
 const char* bad_weight(const MkW4* w) {
   if (!w || !w->codes || !w->scales) return "null 4-bit weight";
   if (w->n < 1 || w->k < 1 || w->experts < 1) return "a 4-bit weight has at least one row, value and expert";
+  if (w->n > INT32_MAX - UNIT_K || w->k > INT32_MAX - UNIT_K) return "a 4-bit weight's padded rows and values are below 2^31";
   if (w->group != 32 && w->group != 64 && w->group != 128) return "the group size is 32, 64 or 128";
   if (w->dtype != MK_W4_BF16 && w->dtype != MK_W4_FP16) return "the activations are BF16 or FP16";
   if (((uintptr_t)w->codes & 15) || ((uintptr_t)w->scales & 15) || ((uintptr_t)w->zeros & 15))
@@ -250,13 +251,13 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   // even blocks of at most 16 tokens, or 32 if their activations fit (102400 x 2048, 32 tokens: 54 us, two
   // blocks of 16 60)
   const int most = t > MAX_COLS && fits(a.units.d, 2 * MAX_COLS) ? 2 * MAX_COLS : MAX_COLS;
-  const int blocks = (t + most - 1) / most;
-  a.tb = (t + blocks - 1) / blocks;
+  const int64_t blocks = ((int64_t)t + most - 1) / most;
+  a.tb = (int)((t + blocks - 1) / blocks);
   const bool xr = a.x_vec && w->k % 8 == 0 && !fits(a.units.d, a.tb);
   if (!xr)
     while (a.tb > 1 && !fits(a.units.d, a.tb)) --a.tb;
   if (!xr && !fits(a.units.d, a.tb)) return fail(MK_EINVAL, "rows that are not 16-byte aligned are too long for the shared memory");
-  a.n_items = (t + a.tb - 1) / a.tb;
+  a.n_items = (int)(((int64_t)t + a.tb - 1) / a.tb);
   a.cols = a.tb;
   a.residual = static_cast<const uint16_t*>(residual);
   a.ldr = ldr;

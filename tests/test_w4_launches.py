@@ -100,3 +100,31 @@ def test_experts_refuse_misaligned_routing(host, ids, weights):
         assert host.mk_w4_experts(ctypes.addressof(a), ctypes.addressof(b), 4096, 64, ids, weights, t, 2, None, 0, 8192, 64, 1 << 20,
                                   1 << 30, None) == mk.MK_EINVAL
         assert not launched(host)
+
+
+INT_MAX = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("n,k", [(32, INT_MAX), (32, INT_MAX - 100), (INT_MAX, 32), (INT_MAX - 20, 32)])
+def test_weights_whose_padded_sizes_pass_32_bits_are_refused(host, n, k):
+    w = mk.MkW4(4096, 4096, None, n, k, 32, 0, 1, 0)
+    host.fake_begin(-1, 0)
+    assert host.mk_w4_linear(ctypes.addressof(w), 4096, k, 1, None, 0, 4096, n, 0, None) == mk.MK_EINVAL
+    assert not launched(host)
+    if n == 32:       # as a down projection, whose rows are the gate and up rows' number
+        w13, w2 = mk.MkW4(4096, 4096, None, 2, k, 32, 0, 1, 0), mk.MkW4(4096, 4096, None, k, 1, 32, 0, 1, 0)
+        need = ctypes.c_int64()
+        assert host.mk_w4_experts_workspace(ctypes.addressof(w13), ctypes.addressof(w2), 1, 1, ctypes.byref(need)) == mk.MK_EINVAL
+
+
+@pytest.mark.parametrize("t", [INT_MAX, INT_MAX - 8, INT_MAX - 31])
+def test_token_counts_near_the_end_of_32_bits(host, t):
+    """Row blocks are counted without wrapping around."""
+    w = mk.MkW4(4096, 4096, None, 1, 64, 32, 0, 1, 0)
+    host.fake_begin(-1, 0)
+    assert host.mk_w4_linear(ctypes.addressof(w), 4096, 0, t, None, 0, 4096, 1, 0, None) == mk.MK_OK
+    r = mk.MkRoute(64, 6, 0, 1, 1, 0, 0, 0, 0, 1.0)
+    assert host.mk_route(ctypes.addressof(r), 4096, 0, t, None, 4096, 4096, None) == mk.MK_OK
+    product, route = launched(host)
+    assert product.split()[:2] == ["bf16", "one"]
+    assert int(re.search(r" (\d+) 1 256$", route)[1]) == -(-t // 8)
