@@ -291,8 +291,12 @@ cudaError_t launch_width(Args a, cudaStream_t s) {
   if (a.gsize % V == 0)
     for (int l = 0; l <= 5; ++l)
       if (a.gsize / V == 1 << l) a.lanes = l;
-  route_kernel<L, V><<<((unsigned)a.t + WARPS - 1) / WARPS, WARPS * 32, 0, s>>>(a);
-  return cudaGetLastError();
+  // (the launch's own result: the last error may be another call's)
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(((unsigned)a.t + WARPS - 1) / WARPS);
+  c.blockDim = dim3(WARPS * 32);
+  c.stream = s;
+  return cudaLaunchKernelEx(&c, route_kernel<L, V>, a);
 }
 
 template <typename L>

@@ -128,3 +128,15 @@ def test_token_counts_near_the_end_of_32_bits(host, t):
     product, route = launched(host)
     assert product.split()[:2] == ["bf16", "one"]
     assert int(re.search(r" (\d+) 1 256$", route)[1]) == -(-t // 8)
+
+
+def test_route_answers_for_its_own_launch(host):
+    """An error that another call left behind is not the router's; its own is."""
+    r = mk.MkRoute(64, 6, 0, 1, 1, 0, 0, 0, 0, 1.0)
+    call = lambda: host.mk_route(ctypes.addressof(r), 4096, 64, 9, None, 4096, 4096, None)  # noqa: E731
+    host.fake_begin(-1, 2)          # out of memory, of an allocation that failed before
+    assert call() == mk.MK_OK and len(launched(host)) == 1
+    host.fake_begin(0, 0)
+    assert call() == mk.MK_ECUDA
+    host.fake_begin(-1, 0)
+    assert call() == mk.MK_OK
