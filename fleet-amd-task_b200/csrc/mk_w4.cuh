@@ -187,16 +187,22 @@ __device__ __forceinline__ void half_chunk(uint32_t magic, uint32_t w0, uint32_t
     for (int n = 0; n < NT; ++n) D::mma(acc[n], a[0], a[1], a[2], a[3], xb[p][n].z, xb[p][n].w);
 }
 
-// tot += scale (rows g, g + 8) * acc (* cw, the columns' weights)
+// tot += scale (rows g, g + 8) * acc (CW: * cw, the columns' weights, of the columns that take part: an
+// infinite scale or a NaN is not the others')
 template <class D, int NT, bool CW>
-__device__ __forceinline__ void fold(uint32_t scale, const float2 (&cw)[NT], const float (&acc)[NT][4], float (&tot)[NT][4]) {
+__device__ __forceinline__ void fold(uint32_t scale, const float2 (&cw)[NT], const bool (&part)[NT][2], const float (&acc)[NT][4],
+                                     float (&tot)[NT][4]) {
   const float2 s = D::to_f32(scale);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    tot[n][0] = fmaf(CW ? s.x * cw[n].x : s.x, acc[n][0], tot[n][0]);
-    tot[n][1] = fmaf(CW ? s.x * cw[n].y : s.x, acc[n][1], tot[n][1]);
-    tot[n][2] = fmaf(CW ? s.y * cw[n].x : s.y, acc[n][2], tot[n][2]);
-    tot[n][3] = fmaf(CW ? s.y * cw[n].y : s.y, acc[n][3], tot[n][3]);
+    if (!CW || part[n][0]) {
+      tot[n][0] = fmaf(CW ? s.x * cw[n].x : s.x, acc[n][0], tot[n][0]);
+      tot[n][2] = fmaf(CW ? s.y * cw[n].x : s.y, acc[n][2], tot[n][2]);
+    }
+    if (!CW || part[n][1]) {
+      tot[n][1] = fmaf(CW ? s.x * cw[n].y : s.x, acc[n][1], tot[n][1]);
+      tot[n][3] = fmaf(CW ? s.y * cw[n].y : s.y, acc[n][3], tot[n][3]);
+    }
   }
 }
 

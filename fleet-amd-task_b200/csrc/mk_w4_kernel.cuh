@@ -391,7 +391,7 @@ struct Kernel {
 
   // tot += the unit's products; staged activations at shared address xl + x_off, x_p to the next plane
   __device__ __forceinline__ void multiply(Unit& n, const uint32_t (&xl)[NT], uint32_t x_off, uint32_t x_p,
-                                           const float2 (&w2)[NT], float (&tot)[RT][NT][4]) {
+                                           const float2 (&w2)[NT], const bool (&part)[NT][2], float (&tot)[RT][NT][4]) {
     float acc[RT][NT][4];
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
@@ -412,7 +412,7 @@ struct Kernel {
         const uint4& v = n.w[r][h >> 1];
         if (h * 32 % G == 0) half_chunk<M, NT, PLANES, true>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
         else half_chunk<M, NT, PLANES, false>(magic, h & 1 ? v.z : v.x, h & 1 ? v.w : v.y, z0, z1, xb, acc[r]);
-        if ((h + 1) * 32 % G == 0) fold<D, NT, SMALL2>(n.sc[r][i], w2, acc[r], tot[r]);
+        if ((h + 1) * 32 % G == 0) fold<D, NT, SMALL2>(n.sc[r][i], w2, part, acc[r], tot[r]);
       }
       if (AHEAD == 1 && h == 1) load_half(n);
     }
@@ -438,10 +438,16 @@ struct Kernel {
       for (int i = 0; i < WORDS; ++i) (&tot[0][0][0])[i] = 0.0f;
       uint32_t x_off = q0 * x_u;
       float2 w2[NT];
+      bool part[NT][2];
       int to_expert = 0, expert = 0;      // SMALL2: units to the next expert, its place in the plan
       auto weigh = [&]() {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) w2[i] = *reinterpret_cast<const float2*>(cw + expert * SMALL_T + i * 8 + 2 * t);
+        for (int i = 0; i < NT; ++i) {
+          w2[i] = *reinterpret_cast<const float2*>(cw + expert * SMALL_T + i * 8 + 2 * t);
+          const uint32_t tokens = plan->tokens[expert] >> (i * 8 + 2 * t);
+          part[i][0] = tokens & 1;
+          part[i][1] = tokens & 2;
+        }
       };
       if (SMALL2) {
         expert = q0 / a.units;
@@ -453,7 +459,7 @@ struct Kernel {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
           if (next == i && left > 0) {
-            multiply(un[i], xl, x_off, x_p, w2, tot);
+            multiply(un[i], xl, x_off, x_p, w2, part, tot);
             load_weights(un[i], AHEAD == 1);
             load_rest(un[i]);
             next = i + 1 == AHEAD ? 0 : i + 1;

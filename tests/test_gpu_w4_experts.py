@@ -142,3 +142,23 @@ def test_every_slot_has_its_place(T, S, E):
 
 def test_more_tokens_than_a_grid_has_rows():
     check(70000, 16, 8, 3, 1, 32, False, True, torch.bfloat16)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("T", [5, 8, 20])
+def test_scales_that_are_not_finite_stay_with_their_expert(T, bad):
+    """Tokens that do not select the expert have the results they have without its scales."""
+    g = gen(T)
+    H, I, E = 96, 200, 6
+    for k in (0, 1):
+        ws = [weight_of(g, (E, 2 * I), H, 32, True, torch.bfloat16), weight_of(g, (E, H), I, 32, True, torch.bfloat16)]
+        x = torch.randn(T, H, generator=g, device=DEV).bfloat16()
+        ids, weights = routed(g, T, E, 2)
+        ids[0] = torch.tensor([1, 4])
+        weights[0, 1] = 0.0                      # expert 4 with weight 0: 0 x an infinity is NaN
+        clean = W4Experts(*ws, group=32, inter=I)(x, ids, weights)
+        ws[k][1][4] = bad
+        got = W4Experts(*ws, group=32, inter=I)(x, ids, weights)
+        selects = (ids == 4).any(1)
+        assert 0 < selects.sum() < T and torch.equal(got[~selects], clean[~selects])
+        assert got[0].isnan().any()
