@@ -75,6 +75,8 @@ class W4Weight:
             raise ValueError(f"gate and up rows come in pairs, got {N} rows")
         if any(v is not None and v.device != codes.device for v in (scales, zeros)):
             raise ValueError("codes, scales and zeros are on one device")
+        if zeros is not None and int(zeros.max()) > 15:
+            raise ValueError("zero points are in 0..15")
         self.n, self.k, self.group, self.experts, self.dtype, self.device = N, k, group, E, scales.dtype, codes.device
         self.index = -1 if codes.device.index is None else codes.device.index
         self.codes, self.scales, self.zeros = lay_out(codes, scales, zeros, k, group, gate_up)
