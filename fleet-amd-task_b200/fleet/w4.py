@@ -118,7 +118,7 @@ def _out(out, shape, dtypes, device, x, residual):
     if not apart(x):
         raise ValueError("out overlaps x")
     if residual is not None and not apart(residual) and not (
-            residual.data_ptr() == lo and residual.stride(0) == ld and residual.dtype == out.dtype):
+            residual.data_ptr() == lo and (shape[0] == 1 or residual.stride(0) == ld) and residual.dtype == out.dtype):
         raise ValueError("out is the residual itself or apart from it")
     return ld
 
