@@ -244,8 +244,6 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   if (int rc = device_sms(&a.device, &sms)) return rc;
   fill(a, w);
   a.mode = LINEAR;
-  a.t = t;
-  a.x = static_cast<const uint16_t*>(x);
   a.ldx = ldx;
   a.x_vec = aligned16(x, ldx);
   // even blocks of at most 16 tokens, or 32 if their activations fit (102400 x 2048, 32 tokens: 54 us, two
@@ -257,16 +255,23 @@ extern "C" int mk_w4_linear(const MkW4* w, const void* x, int64_t ldx, int32_t t
   if (!xr)
     while (a.tb > 1 && !fits(a.units.d, a.tb)) --a.tb;
   if (!xr && !fits(a.units.d, a.tb)) return fail(MK_EINVAL, "rows that are not 16-byte aligned are too long for the shared memory");
-  a.n_items = (int)(((int64_t)t + a.tb - 1) / a.tb);
   a.cols = a.tb;
-  a.residual = static_cast<const uint16_t*>(residual);
   a.ldr = ldr;
-  a.out = out;
   a.ldo = ldo;
   a.out_f32 = out_f32;
   a.pairs = !out_f32 && aligned4(out, ldo) && (!residual || aligned4(residual, ldr));
-  if ((int64_t)a.n_items * (w->n / 16 + 2) * a.units.d > INT32_MAX / 2) return fail(MK_EINVAL, "too many tokens times weights");
-  return launch_weight(a, w, a.n_items, true, xr, sms, static_cast<cudaStream_t>(stream));
+  // a launch counts units of all its items in 32 bits: as many blocks at a time
+  const int64_t most_items = INT32_MAX / 2 / ((int64_t)(w->n / 16 + 2) * a.units.d);
+  if (!most_items) return fail(MK_EINVAL, "the weight is too large");
+  for (int64_t at = 0; at < t; at += a.t) {
+    a.t = (int)std::min(t - at, most_items * a.tb);
+    a.n_items = (int)(((int64_t)a.t + a.tb - 1) / a.tb);
+    a.x = static_cast<const uint16_t*>(x) + at * ldx;
+    a.residual = residual ? static_cast<const uint16_t*>(residual) + at * ldr : nullptr;
+    a.out = static_cast<uint8_t*>(out) + at * ldo * (out_f32 ? 4 : 2);
+    if (int rc = launch_weight(a, w, a.n_items, true, xr, sms, static_cast<cudaStream_t>(stream))) return rc;
+  }
+  return MK_OK;
 }
 
 extern "C" int mk_w4_experts_workspace(const MkW4* w13, const MkW4* w2, int32_t t, int32_t slots, int64_t* bytes) {

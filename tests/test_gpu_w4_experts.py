@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from fleet.pack_weights import dequantize_w4
-from fleet.w4 import W4Experts
+from fleet.w4 import W4Experts, W4Linear
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -162,3 +162,16 @@ def test_scales_that_are_not_finite_stay_with_their_expert(T, bad):
         selects = (ids == 4).any(1)
         assert 0 < selects.sum() < T and torch.equal(got[~selects], clean[~selects])
         assert got[0].isnan().any()
+
+
+def test_linear_of_more_tokens_than_a_launch_counts():
+    """Two launches of one call: the rows on either side of where they part, and the last ones (small integers, exact)."""
+    g, T, N, K, group = gen(6), 16 * 10715 + 300, 16000, 12800, 64
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, device=DEV, dtype=torch.uint8)
+    scales = (2.0 ** torch.randint(-1, 1, (N, K // group), generator=g, device=DEV).float()).bfloat16()
+    x = torch.randint(-1, 2, (8 * T + K,), generator=g, device=DEV).bfloat16().as_strided((T, K), (8, 1))   # a row every 8 values
+    got = W4Linear(codes, scales, group=group)(x)
+    W = dequantize_w4(codes, scales, None, K, group)
+    for rows in (slice(0, 20), slice(16 * 10715 - 20, 16 * 10715 + 20), slice(T - 20, T)):
+        want = x[rows].double() @ W.double().T
+        assert want.abs().max() * 2 < 2 ** 24 and torch.equal(got[rows], want.bfloat16())

@@ -140,3 +140,15 @@ def test_route_answers_for_its_own_launch(host):
     assert call() == mk.MK_ECUDA
     host.fake_begin(-1, 0)
     assert call() == mk.MK_OK
+
+
+def test_linear_of_more_tokens_than_a_launch_counts(host):
+    """Units of weights times blocks of tokens are 32-bit counts of one launch: more of them are more launches."""
+    w = mk.MkW4(4096, 4096, None, 16000, 12800, 64, 0, 1, 0)
+    for t, launches in ((16 * 10715, 1), (16 * 10715 + 1, 2), (10 ** 6, 6)):
+        host.fake_begin(-1, 0)
+        assert host.mk_w4_linear(ctypes.addressof(w), 4096, 8, t, None, 0, 4096, 16000, 0, None) == mk.MK_OK, host.fake_message()
+        assert len(launched(host)) == launches
+    host.fake_begin(1, 0)
+    assert host.mk_w4_linear(ctypes.addressof(w), 4096, 8, 10 ** 6, None, 0, 4096, 16000, 0, None) == mk.MK_ECUDA
+    assert len(launched(host)) == 2
