@@ -165,9 +165,10 @@ def _ptr(t):
     return t.data_ptr()
 
 
-def on_stream(t, stream):
+def on_stream(t, stream, *used):
     """A context with `stream` (a torch stream, or a raw handle on tensor t's device) current, so that
-    what a call allocates belongs to the stream that uses it."""
+    what a call allocates belongs to the stream that uses it. The tensors `used` may be dropped before
+    `stream` has come to them: their memory is not used again until it has."""
     import torch
     if t.device.type != "cuda":
         raise MkError(MK_EINVAL, f"a stream is given, but the tensors are on {t.device}")
@@ -175,6 +176,9 @@ def on_stream(t, stream):
         stream = torch.cuda.ExternalStream(int(stream), device=t.device)
     elif stream.device != t.device:
         raise ValueError(f"the stream is on {stream.device}, the tensors are on {t.device}")
+    for u in (t, *used):
+        if u is not None and u.device == t.device:
+            u.record_stream(stream)
     return torch.cuda.stream(stream)
 
 

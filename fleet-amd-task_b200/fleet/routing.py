@@ -49,7 +49,7 @@ def route_experts(logits, topk, *, score="softmax", bias=None, n_group=1, topk_g
     `stream` (default: the current stream of the tensors' device); `ids` / `weights` are written if
     given."""
     if stream is not None:
-        with mk.on_stream(logits, stream):
+        with mk.on_stream(logits, stream, bias, ids, weights):
             return route_experts(logits, topk, score=score, bias=bias, n_group=n_group, topk_group=topk_group,
                                  group_score=group_score, renormalize=renormalize, scaling=scaling, n_forced=n_forced,
                                  ids=ids, weights=weights)

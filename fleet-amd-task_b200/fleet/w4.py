@@ -83,6 +83,7 @@ class W4Weight:
         self.c = mk.MkW4(self.codes.data_ptr(), self.scales.data_ptr(), mk._ptr(self.zeros), N, k, group,
                          DTYPES[scales.dtype], E, 0)
         self.ptr = ctypes.addressof(self.c)
+        self.tensors = self.codes, self.scales, self.zeros
 
 
 def _fits(t, shape, dtype, index):
@@ -136,7 +137,7 @@ class W4Linear:
 
     def __call__(self, x, out=None, residual=None, out_dtype=None, stream=None):
         if stream is not None:
-            with mk.on_stream(x, stream):
+            with mk.on_stream(x, stream, out, residual, *self.w.tensors):
                 return self(x, out, residual, out_dtype)
         w = self.w
         call, device, current_stream, context = mk.entry("mk_w4_linear")
@@ -206,7 +207,7 @@ class W4Experts:
 
     def __call__(self, x, ids, weights, residual=None, out=None, stream=None):
         if stream is not None:
-            with mk.on_stream(x, stream):
+            with mk.on_stream(x, stream, ids, weights, residual, out, *self.w13.tensors, *self.w2.tensors):
                 return self(x, ids, weights, residual, out)
         w = self.w13
         call, device, current_stream, context = mk.entry("mk_w4_experts")

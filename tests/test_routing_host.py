@@ -93,3 +93,13 @@ def test_a_stream_of_another_device_is_refused():
     for stream in (64, SimpleNamespace(cuda_stream=64, device=torch.device("cuda", 0))):
         with pytest.raises(mk.MkError):
             mk.on_stream(SimpleNamespace(device=torch.device("cpu")), stream)
+
+
+def test_tensors_of_a_call_on_a_stream_are_recorded(monkeypatch):
+    from types import SimpleNamespace
+    dev, stream = torch.device("cuda", 0), SimpleNamespace(cuda_stream=64, device=torch.device("cuda", 0))
+    seen = []
+    t = lambda name, device=dev: SimpleNamespace(device=device, record_stream=lambda s: seen.append((name, s)))  # noqa: E731
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: s)
+    assert mk.on_stream(t("x"), stream, None, t("ids"), t("other", torch.device("cpu"))) is stream
+    assert seen == [("x", stream), ("ids", stream)]
