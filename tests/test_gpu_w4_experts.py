@@ -175,3 +175,44 @@ def test_linear_of_more_tokens_than_a_launch_counts():
     for rows in (slice(0, 20), slice(16 * 10715 - 20, 16 * 10715 + 20), slice(T - 20, T)):
         want = x[rows].double() @ W.double().T
         assert want.abs().max() * 2 < 2 ** 24 and torch.equal(got[rows], want.bfloat16())
+
+
+@DTYPES
+@pytest.mark.parametrize("T,H,I,E,S,group,zeros,residual", [
+    # odd values and rows: the last store of an intermediate, its padding, results in single stores
+    (1, 131, 51, 4, 2, 32, True, True), (3, 131, 51, 5, 3, 64, False, False), (8, 33, 1, 3, 2, 128, True, True),
+    (7, 1, 77, 4, 4, 32, False, True), (2, 255, 129, 6, 2, 128, True, False), (20, 131, 51, 5, 3, 32, True, True),
+    (33, 65, 127, 3, 1, 64, False, False),
+    # plans near their limits: 256 slots of a small batch, more slots than lanes, many experts
+    (8, 64, 24, 40, 32, 32, False, True), (5, 48, 40, 60, 50, 64, True, False), (1, 32, 16, 300, 256, 32, False, True),
+    (8, 32, 16, 1024, 32, 32, True, False), (9, 32, 16, 1024, 40, 32, False, True),
+])
+def test_odd_sizes_and_plans_near_their_limits(T, H, I, E, S, group, zeros, residual, dtype):
+    op, x, ids, weights, res, got, want = check(T, H, I, E, S, group, zeros, residual, dtype)
+    assert torch.equal(op(x, ids, weights, residual=res), got)
+
+
+@pytest.mark.parametrize("T", [1, 5, 20])
+@pytest.mark.parametrize("H", [96, 97])
+def test_strides_and_alignment(T, H):
+    """x, residual and out at odd places of wider rows; nothing outside the results is written."""
+    g = gen(T + H)
+    I, E, dtype = 40, 6, torch.bfloat16
+    w13, w2 = weight_of(g, (E, 2 * I), H, 32, True, dtype), weight_of(g, (E, H), I, 32, True, dtype)
+    op, (ids, weights) = W4Experts(w13, w2, group=32, inter=I), routed(g, T, E, 2)
+    wide = torch.randn(T + 1, H + 13, generator=g, device=DEV).to(dtype)
+    wide_res = torch.randn(T, H + 7, generator=g, device=DEV).to(dtype)
+    for x0, r0, o0, extra in ((0, 0, 0, 8), (3, 1, 5, 9), (8, 2, 4, 10), (1, 7, 3, 6)):
+        x, res = wide[1:, x0:x0 + H], wide_res[:, r0:r0 + H]
+        out = torch.full((T, H + extra), 7.0, device=DEV, dtype=dtype)
+        view = out[:, o0:o0 + H]
+        assert op(x, ids, weights, residual=res, out=view) is view
+        want, bound = reference(x, ids, weights, w13, w2, H, I, 32, res, dtype)
+        assert ((view.double() - want).abs() <= bound).all()
+        assert (out[:, :o0] == 7).all() and (out[:, o0 + H:] == 7).all()
+        first = op(x, ids, weights, residual=res)
+        assert torch.equal(first, view)
+        assert op(x, ids, weights, residual=res, out=res) is res and torch.equal(res, first)     # in place
+    one = wide[:1, 2:H + 2].expand(T, H)                                                         # one row for every token
+    want, bound = reference(one, ids, weights, w13, w2, H, I, 32, None, dtype)
+    assert ((op(one, ids, weights).double() - want).abs() <= bound).all()
