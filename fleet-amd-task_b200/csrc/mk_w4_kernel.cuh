@@ -174,10 +174,12 @@ struct Kernel {
   static constexpr int PLANES = WIDE ? 2 : 1;
   // Warps and the units each has in flight. 8 columns: 24 warps of 80 registers, one unit each, its halves
   // reloaded as they are used (the 1-token head 25.6 us; 16 warps two units ahead 28.3). More columns, or
-  // too few rows for two tiles a warp: 16 warps of 128 registers
-  static constexpr bool NARROW = NT == 1 && (RT == 2 || XR);
+  // too few rows for two tiles a warp: 16 warps of 128 registers. Both planes with each unit (32 registers): 16
+  // warps, one unit each (experts of 1 / 8 tokens 21.1 / 58.3 us; 24 warps, which spill, 22.5 / 61.1; 20 warps 22.5 /
+  // 59.3; 16 warps two units ahead 22.5 / 62.9)
+  static constexpr bool BOTH = XR && WIDE, NARROW = NT == 1 && (RT == 2 || XR) && !BOTH;
   static constexpr int WARPS = NARROW ? 24 : 16, THREADS = WARPS * 32;
-  static constexpr int AHEAD = NARROW ? 1 : RT == 2 || NT > 1 ? 2 : 3;
+  static constexpr int AHEAD = NARROW || BOTH ? 1 : RT == 2 || NT > 1 ? 2 : 3;
   static constexpr int GROUPS = UNIT_K / G, ZWORDS = GROUPS / 2 > 0 ? GROUPS / 2 : 1;
   // a unit of RT tiles in registers
   struct Unit {
