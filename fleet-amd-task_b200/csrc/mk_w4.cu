@@ -35,9 +35,12 @@
 // experts' activations, each expert's part scaled by the tokens' weights for it. A larger batch is
 // grouped by expert first (plan_kernel), each expert's slots being its columns, and the slots' outputs
 // are added afterwards in slot order (combine_kernel). The launches of one call overlap
-// (programmatic dependent launches): 24 us instead of 30 for a small layer's four.
-// Measured, a layer of 66 experts of 2048 x 1408, 8 slots a token: 1 token 20.6 us (36 MB, 5.4 us at the
-// copy rate), 8 tokens 47 (165 MB of distinct experts, 25 us), 64 tokens 95 (295 MB, 45 us).
+// (programmatic dependent launches): 24 us instead of 30 for a small layer's four. The intermediate is the sum
+// of two BF16 values, which the down projection multiplies one after the other with the same decoded codes: twice its
+// MMAs and activations, 4 to 10 % of a call (one 16-bit value: 20.5, 53 and 95 us below).
+// Measured, a layer of 66 experts of 2048 x 1408, 8 slots a token: 1 token 21.3 us (36 MB, 5.4 us at the
+// copy rate), 8 tokens in groups of 64 with zero points 58 (172 MB of distinct experts, 26 us), 64 tokens 105
+// (295 MB, 45 us).
 #include <algorithm>
 
 #include "mk_w4_kernel.cuh"

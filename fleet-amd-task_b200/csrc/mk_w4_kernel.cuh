@@ -19,8 +19,9 @@ constexpr int SMEM_LIMIT = 227 * 1024;
 constexpr int MAX_EXPERTS = 1024;
 constexpr int MAX_DEVICES = 64;
 constexpr int MAX_COLS = 16;           // columns of an item (of a LINEAR: 32)
-constexpr int GROUPED_COLS = 8;        // of an expert's item (64 tokens of 66 experts: 101 us; 12: 111, 16: 109)
-// most tokens and slots of the two-launch experts (12 tokens: 80 us, grouped 68)
+// of an expert's item (64 tokens of 66 experts: 101 us; 12: 111, 16: 109; with the intermediate in one value)
+constexpr int GROUPED_COLS = 8;
+// most tokens and slots of the two-launch experts (12 tokens: 80 us, grouped 68; with the intermediate in one value)
 constexpr int SMALL_T = 8;
 constexpr int SMALL_SLOTS = 256;
 

@@ -10,6 +10,9 @@ A 4-bit weight W [..., N, K] is
 with W[n, k] = scales[n, k // group] * (code[n, k] - zeros[n, k // group]) and group 32, 64 or 128
 (pack_weights.quantize_w4 makes one from a BF16 weight). The constructors lay the codes out once in
 the order the kernels stream them (csrc/mk_w4.cuh) and keep only that form.
+
+A call repeated gives the same bits. A token's sums are split by where its block of tokens or its expert's slots
+lie, so its last bits may differ between batches of other sizes or routing.
 """
 import ctypes
 
