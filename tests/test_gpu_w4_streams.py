@@ -90,3 +90,32 @@ def test_inputs_change_from_call_to_call(T):
         assert not torch.equal(want[0], want[i])
     got = [experts(*sets[i % 8]) for i in range(400)]
     assert all(torch.equal(v, want[i % 8]) for i, v in enumerate(got))
+
+
+@pytest.mark.parametrize("T", [4, 20])
+def test_calls_on_a_stream_in_a_captured_graph(T):
+    """stream= while a graph is captured: the capturing stream itself, and one that it forks to and joins."""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    w = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()  # noqa: E731
+    lin = W4Linear(*quantize_w4(w(256, 512), 64), group=64)
+    experts = W4Experts(quantize_w4(w(4, 256, 512), 64), quantize_w4(w(4, 512, 128), 64), group=64)
+    static, logits = w(T, 512), torch.randn(T, 4, generator=g, device=DEV)
+
+    def step(x, **kw):
+        ids, weights = route_experts(logits, 2, **kw)
+        return lin(experts(x, ids, weights, residual=x, **kw), **kw)
+    inputs = [w(T, 512) for _ in range(3)]
+    want = [step(x) for x in inputs]
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        a = step(static, stream=here)
+        side.wait_stream(here)
+        b = step(static, stream=side)
+        here.wait_stream(side)
+    for x, v in zip(inputs, want):
+        static.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, v) and torch.equal(b, v)
