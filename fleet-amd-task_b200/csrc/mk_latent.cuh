@@ -1,0 +1,143 @@
+// mk_latent.cuh -- the latent cache in 8 bits: format, and what its kernels share.
+//
+// A cache is `pages` pages of `page` tokens (16, 32, 64 or 128). A token is d_c latent values (key and value of every
+// head) and d_r rotary key values (of every head's key), E4M3 codes in rows of ld_c = d_c rounded up to 128 and
+// ld_r = 64 bytes; the bytes behind a row's values are zero and stay so. scales [pages, 2] FP32: a page's
+// latents and rotary keys stand for code x scale.
+//
+// Scales are powers of two, the smallest 2^e with |x| <= 448 2^e for what the page holds, e from -32 to 32: E4M3
+// keeps the same relative precision at any scale, so nothing is lost by it, codes x scale are exact in
+// BF16, and where a page's scale grows its earlier codes are only shifted (exact down to E4M3's subnormals).
+//
+// A batch is a table of pages, the sequences' lengths (this step's tokens included) and, if not one row each,
+// the starts of their rows. What these arrays hold is not known on the host, so kernels take nothing of it on trust: a
+// length is cut to the table's width and not below 0, rows to the call's tokens, and a page outside the cache holds
+// no token.
+#ifndef MK_LATENT_CUH
+#define MK_LATENT_CUH
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/fleet_mk.h"
+
+namespace mk {
+int set_last_error(int code, const char* msg);   // mk_runtime.cu: the message mk_last_error() returns
+}
+
+namespace latent {
+
+constexpr int MAX_DC = 512, LD_R = 64, MAX_PAGE = 128;
+
+struct Cache {
+  uint8_t *c, *r;
+  float* scales;
+  int pages, page, shift, d_c, d_r, ld_c;      // page = 1 << shift
+};
+
+struct Batch {
+  const int32_t *table, *lens, *starts;
+  int64_t ldt;
+  int n, capacity;                             // capacity: tokens that a table's row can name
+  int rows;                                    // the call's rows
+};
+
+// One sequence: its rows [row, row + n) of the call are its tokens [len - n, len), len as the caller has it.
+struct Seq {
+  int row, n, len;
+};
+
+__device__ __forceinline__ Seq sequence(const Batch& b, int s) {
+  Seq q;
+  q.len = max(b.lens[s], 0);
+  if (!b.starts) {
+    q.row = s;
+    q.n = s < b.rows ? 1 : 0;
+  } else {
+    q.row = min(max(b.starts[s], 0), b.rows);
+    q.n = max(min(b.starts[s + 1], b.rows) - q.row, 0);
+  }
+  return q;
+}
+
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ float2 decode2(uint16_t codes) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(codes, __NV_E4M3)));
+}
+__device__ __forceinline__ uint16_t encode2(float a, float b) {      // NaN stays NaN, finite values saturate
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+// The item (of n with count(i) >= 0 parts each) that holds part `at` of all, and the part's place in it; every thread of
+// the block calls it. Returns the number of all parts; item is n if `at` lies past them.
+template <int THREADS, typename Count>
+__device__ __forceinline__ int64_t locate(int n, int64_t at, Count count, int& item, int64_t& place) {
+  __shared__ int64_t warps[THREADS / 32];
+  __shared__ int64_t found_place;
+  __shared__ int found_item;
+  const int per = (n + THREADS - 1) / THREADS, lo = min((int)threadIdx.x * per, n), hi = min(lo + per, n);
+  int64_t mine = 0;
+  for (int i = lo; i < hi; ++i) mine += count(i);
+  int64_t upto = mine;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (threadIdx.x == 0) found_item = n;
+  if (lane == 31) warps[warp] = upto;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) upto += warps[w];
+    total += warps[w];
+  }
+  if (at >= upto - mine && at < upto) {
+    int64_t left = at - (upto - mine);
+    int i = lo;
+    for (int64_t c; left >= (c = count(i)); ++i) left -= c;
+    found_item = i;
+    found_place = left;
+  }
+  __syncthreads();
+  item = found_item;
+  place = found_place;
+  return total;
+}
+
+inline int fail(int code, const char* msg) { return mk::set_last_error(code, msg); }
+
+// The host's checks of what every call is handed; MK_OK and the kernels' structs, or the error.
+inline int check(const MkLatent* l, const MkLatentBatch* b, int32_t rows, int32_t dtype, Cache& cache, Batch& batch) {
+  if (!l || !b) return fail(MK_EINVAL, "null cache or batch");
+  if (l->page != 16 && l->page != 32 && l->page != 64 && l->page != 128) return fail(MK_EINVAL, "a page holds 16, 32, 64 or 128 tokens");
+  if (l->d_c < 8 || l->d_c > MAX_DC || l->d_c % 8 || l->d_r < 8 || l->d_r > LD_R || l->d_r % 8)
+    return fail(MK_EINVAL, "d_c is from 8 to 512, d_r from 8 to 64, both multiples of 8");
+  if (l->pages < 1 || (int64_t)l->pages * l->page > INT32_MAX) return fail(MK_EINVAL, "a cache holds from 1 page to 2^31 - 1 tokens");
+  if (b->n < 0 || b->pages < 1 || (int64_t)b->pages * l->page > INT32_MAX || b->ldt < 0)
+    return fail(MK_EINVAL, "a batch has 0 or more sequences of 1 page to 2^31 - 1 tokens each");
+  if (rows < 0 || (!b->starts && rows != b->n)) return fail(MK_EINVAL, "without starts a batch has one row for each sequence");
+  if (dtype != MK_BF16 && dtype != MK_FP16) return fail(MK_EINVAL, "values are BF16 or FP16");
+  if (!l->c || !l->r || !l->scales || (b->n && (!b->table || !b->lens))) return fail(MK_EINVAL, "null pointer");
+  if (((uintptr_t)l->c | (uintptr_t)l->r) % 128 || (uintptr_t)l->scales % 8 ||
+      ((uintptr_t)b->table | (uintptr_t)b->lens | (uintptr_t)b->starts) % 4)
+    return fail(MK_EINVAL, "misaligned codes (128 bytes), scales (8), table, lens or starts (4)");
+  cache = {static_cast<uint8_t*>(l->c), static_cast<uint8_t*>(l->r), l->scales, l->pages, l->page,
+           l->page == 16 ? 4 : l->page == 32 ? 5 : l->page == 64 ? 6 : 7, l->d_c, l->d_r, (l->d_c + 127) / 128 * 128};
+  batch = {b->table, b->lens, b->starts, b->ldt, b->n, b->pages * l->page, rows};
+  return MK_OK;
+}
+
+}  // namespace latent
+#endif

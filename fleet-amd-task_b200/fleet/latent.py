@@ -1,0 +1,201 @@
+"""The latent attention of a batch of sequences over a paged cache in 8 bits: LatentCache (append, read,
+attend) and LatentBatch, over mk_latent_* (csrc/mk_latent.cu, csrc/mk_latent_attend.cu).
+
+The persistent kernel decodes one sequence over a BF16 cache of its own; this is the cache and the
+attention of a batch. A token of the cache is a latent of d_c values, which is the key and the value of
+every head, and a rotary key of d_r values that all heads share (the absorbed form of the model's
+attention). Codes are E4M3 bytes, and each page has one scale for its latents and one for its rotary
+keys: the smallest power of two 2^e with |x| <= 448 2^e for what the page holds, e from -32 to 32. It is
+anew where a page's first token is written and grows with later ones otherwise, its earlier codes being
+rounded to it.
+"""
+import ctypes
+
+import torch
+
+from fleet import mk
+from fleet.rope import _apart, overlap
+
+DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+PAGES = (16, 32, 64, 128)
+
+
+def _beside(a, b):
+    """Whether the rows of two 2-D tensors are side by side in longer rows."""
+    ld, at = a.stride(0), (b.data_ptr() - a.data_ptr()) // a.element_size()
+    return b.stride(0) == ld and ld > 0 and a.shape[1] <= at % ld <= ld - b.shape[1]
+
+
+class LatentBatch:
+    """The sequences of a call: `table` [B, P] int32, the pages of each; `lens` [B] int32, the tokens of
+    each, the ones of this step included; `starts` [B + 1] int32, where the rows of each begin in the
+    call's tensors (ascending; rows from starts[B] on belong to nobody), or None for one row each, row b
+    being sequence b's. Row i of the n of a sequence is its token lens - n + i.
+
+    The tensors are held and may change between calls (a captured graph reads what they hold then).
+    What they say is the device's: a length counts as at most the P pages and at least 0, and a page
+    outside the cache holds no token."""
+
+    def __init__(self, table, lens, starts=None):
+        B = lens.shape[0] if lens.dim() == 1 else -1
+        if lens.dtype != torch.int32 or B < 0 or not lens.is_contiguous():
+            raise ValueError(f"lens: contiguous int32 [B] expected, got {lens.dtype} {tuple(lens.shape)}")
+        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1 or \
+                (table.shape[1] > 1 and table.stride(1) != 1):
+            raise ValueError(f"table: int32 [{B}, P] with unit stride along P expected, got {table.dtype} {tuple(table.shape)}, strides {table.stride()}")
+        if starts is not None and (starts.dtype != torch.int32 or tuple(starts.shape) != (B + 1,) or not starts.is_contiguous()):
+            raise ValueError(f"starts: contiguous int32 [{B + 1}] expected, got {starts.dtype} {tuple(starts.shape)}")
+        if any(v is not None and v.device != lens.device for v in (table, starts)):
+            raise ValueError("table, lens and starts are on one device")
+        self.table, self.lens, self.starts = table, lens, starts
+        self.n, self.index = B, lens.get_device()
+        self.c = mk.MkLatentBatch(table.data_ptr(), lens.data_ptr(), mk._ptr(starts), table.stride(0), B, table.shape[1])
+        self.ptr = ctypes.addressof(self.c)
+        self.tensors = table, lens, starts
+
+
+class LatentCache:
+    """A cache of `pages` pages of `page` tokens (16, 32, 64 or 128), d_c and d_r multiples of 8 up to 512 and 64.
+
+    `c_codes` [pages, page, d_c] and `r_codes` [pages, page, d_r] uint8 and `scales` [pages, 2] float32
+    are the cache's own memory, zero at first; a program may copy, save and fill them."""
+
+    def __init__(self, pages, page, d_c, d_r, device="cuda"):
+        if page not in PAGES:
+            raise ValueError(f"page {page} is one of {PAGES}")
+        if not 8 <= d_c <= 512 or d_c % 8 or not 8 <= d_r <= 64 or d_r % 8:
+            raise ValueError(f"d_c from 8 to 512 and d_r from 8 to 64, multiples of 8, expected, got {d_c} and {d_r}")
+        if pages < 1 or pages * page >= 2 ** 31:
+            raise ValueError(f"from 1 page to 2^31 - 1 tokens expected, got {pages} pages of {page}")
+        self.pages, self.page, self.d_c, self.d_r = pages, page, d_c, d_r
+        self._c = torch.zeros(pages, page, -(-d_c // 128) * 128, dtype=torch.uint8, device=device)
+        self._r = torch.zeros(pages, page, 64, dtype=torch.uint8, device=device)
+        self.scales = torch.zeros(pages, 2, dtype=torch.float32, device=device)
+        self.c_codes, self.r_codes = self._c[..., :d_c], self._r[..., :d_r]
+        self.device, self.index = self._c.device, self._c.get_device()
+        self.c = mk.MkLatent(self._c.data_ptr(), self._r.data_ptr(), self.scales.data_ptr(), pages, page, d_c, d_r)
+        self.ptr = ctypes.addressof(self.c)
+        self.tensors = self._c, self._r, self.scales
+        self._need = {}            # (sequences, rows, heads) -> workspace bytes
+
+    def _batch(self, batch, rows):
+        if batch.index != self.index:
+            raise ValueError(f"the batch is on {batch.lens.device}, the cache on {self.device}")
+        if batch.starts is None and rows != batch.n:
+            raise ValueError(f"without starts a batch has one row for each of its {batch.n} sequences, got {rows} rows")
+
+    def _rows(self, t, d, name, dtype=None, T=None):
+        if t.dim() != 2 or t.shape[1] != d or t.stride(1) != 1 or t.get_device() != self.index or \
+                (t.dtype not in DTYPES if dtype is None else t.dtype is not dtype) or (T is not None and t.shape[0] != T):
+            raise ValueError(f"{name}: {dtype or 'bfloat16 or float16'} [{'rows' if T is None else T}, {d}] with unit stride along its rows on "
+                             f"{self.device} expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()} on {t.device}")
+
+    def append(self, c_kv, k_pe, batch, stream=None):
+        """Write the rows' latents c_kv [rows, d_c] (after their norm) and rotary keys k_pe [rows, d_r] (after
+        their turn) into the batch's pages, bfloat16 or float16 with any row strides. What is not finite
+        becomes NaN and does not count for a scale; values past 448 2^32 saturate. Rows before a sequence's first
+        token (more rows than tokens), past its table or in a page outside the cache are left out, and so
+        are rows of no sequence. A page is written by one sequence of a call at most; writing tokens again
+        (rejected drafts) is an append with shorter lens."""
+        if stream is not None:
+            with mk.on_stream(c_kv, stream, k_pe, *batch.tensors, *self.tensors):
+                return self.append(c_kv, k_pe, batch)
+        call, device, current_stream, context = mk.entry("mk_latent_append")
+        index = self.index
+        if index < 0 or device() != index:
+            return mk.off_device("mk_latent_append", index, context, lambda: self.append(c_kv, k_pe, batch))
+        self._rows(c_kv, self.d_c, "c_kv")
+        rows = c_kv.shape[0]
+        self._rows(k_pe, self.d_r, "k_pe", c_kv.dtype, rows)
+        self._batch(batch, rows)
+        rc = call(self.ptr, batch.ptr, c_kv.data_ptr(), c_kv.stride(0), k_pe.data_ptr(), k_pe.stride(0), rows, DTYPES[c_kv.dtype],
+                  current_stream(index))
+        if rc:
+            mk._check(rc, "mk_latent_append")
+
+    def read(self, batch, rows, dtype=torch.bfloat16, out=None, stream=None):
+        """(latents [rows, d_c], rotary keys [rows, d_r]) of the batch's rows, code x scale rounded once
+        (exact in bfloat16). A whole sequence is lens rows. Tokens that are in no page of the cache read as zeros;
+        rows of no sequence are zeros too, or stay as they were in the pair `out`."""
+        if stream is not None:
+            with mk.on_stream(self._c, stream, *batch.tensors, *self.tensors, *(out or ())):
+                return self.read(batch, rows, dtype, out)
+        call, device, current_stream, context = mk.entry("mk_latent_read")
+        index = self.index
+        if index < 0 or device() != index:
+            return mk.off_device("mk_latent_read", index, context, lambda: self.read(batch, rows, dtype, out))
+        if dtype not in DTYPES:
+            raise TypeError(f"dtype is bfloat16 or float16, not {dtype}")
+        self._batch(batch, rows)
+        fill = out is None
+        if fill:
+            out = (torch.empty_strided((rows, self.d_c), (self.d_c, 1), dtype=dtype, device=self.device),
+                   torch.empty_strided((rows, self.d_r), (self.d_r, 1), dtype=dtype, device=self.device))
+        c, r = out
+        if not fill:
+            self._rows(c, self.d_c, "out[0]", dtype, rows)
+            self._rows(r, self.d_r, "out[1]", dtype, rows)
+            if rows > 1 and (c.stride(0) < self.d_c or r.stride(0) < self.d_r):
+                raise ValueError(f"out: rows overlap (strides {c.stride(0)} and {r.stride(0)})")
+            if (overlap(c, r) and not _beside(c, r)) or any(t is not None and overlap(o, t) for o in out for t in (*self.tensors, *batch.tensors)):
+                raise ValueError("out: its tensors are apart from one another, the cache and the batch")
+        rc = call(self.ptr, batch.ptr, c.data_ptr(), c.stride(0), r.data_ptr(), r.stride(0), rows, DTYPES[dtype], fill,
+                  current_stream(index))
+        if rc:
+            mk._check(rc, "mk_latent_read")
+        return c, r
+
+    def workspace_bytes(self, n, rows, heads):
+        got = self._need.get((n, rows, heads))
+        if got is None:
+            need = ctypes.c_int64()
+            mk._check(mk.lib().mk_latent_attend_workspace(self.ptr, n, rows, heads, ctypes.byref(need)), "mk_latent_attend_workspace")
+            if len(self._need) > 4096:
+                self._need.clear()
+            got = self._need[(n, rows, heads)] = need.value
+        return got
+
+    def attend(self, q, batch, scale, out=None, return_lse=False, stream=None):
+        """out [rows, heads, d_c] of q [rows, heads, d_c + d_r] (bfloat16 or float16; the absorbed query, then its
+        rotary part): softmax over the tokens up to the row's own of scale x (q . (latent, rotary key)), times the
+        latents. With return_lse also the log of the sum of the scores' exponentials [rows, heads] float32.
+        A row that sees no token gives zeros and -inf. Rows of no sequence stay as they were in `out`
+        (undefined in a new tensor). A NaN in a token stays with the rows that see it, an infinity or a NaN in q
+        with its row and head, which it makes NaN. Strides of rows and heads may be any. Runs on `stream` (default:
+        the current stream); the workspace comes from torch's allocator for each call."""
+        if stream is not None:
+            with mk.on_stream(q, stream, out, *batch.tensors, *self.tensors):
+                return self.attend(q, batch, scale, out, return_lse)
+        call, device, current_stream, context = mk.entry("mk_latent_attend")
+        index = self.index
+        if index < 0 or device() != index:
+            return mk.off_device("mk_latent_attend", index, context, lambda: self.attend(q, batch, scale, out, return_lse))
+        d = self.d_c + self.d_r
+        if q.dim() != 3 or q.shape[2] != d or q.stride(2) != 1 or q.get_device() != index or q.dtype not in DTYPES:
+            raise ValueError(f"q: bfloat16 or float16 [rows, heads, {d}] with unit stride along its values on {self.device} expected, got "
+                             f"{q.dtype} {tuple(q.shape)}, strides {q.stride()} on {q.device}")
+        rows, heads, _ = q.shape
+        self._batch(batch, rows)
+        shape = (rows, heads, self.d_c)
+        if out is None:
+            out = torch.empty_strided(shape, (heads * self.d_c, self.d_c, 1), dtype=q.dtype, device=self.device)
+        else:
+            if out.shape != shape or out.dtype != q.dtype or out.get_device() != index or out.stride(2) != 1:
+                raise ValueError(f"out: {q.dtype} {shape} with unit stride along its values on {self.device} expected, got "
+                                 f"{out.dtype} {tuple(out.shape)}, strides {out.stride()} on {out.device}")
+            if not _apart(shape, out.stride()):
+                raise ValueError(f"out: heads overlap (strides {out.stride()}, {self.d_c} values)")
+            if any(t is not None and overlap(out, t) for t in (q, *self.tensors, *batch.tensors)):
+                raise ValueError("out is apart from q, the cache and the batch")
+        lse = torch.empty_strided((rows, heads), (heads, 1), dtype=torch.float32, device=self.device) if return_lse else None
+        nbytes = self._need.get((batch.n, rows, heads))
+        if nbytes is None:
+            nbytes = self.workspace_bytes(batch.n, rows, heads)
+        ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=self.device)
+        qt, qh, _ = q.stride()
+        ot, oh, _ = out.stride()
+        rc = call(self.ptr, batch.ptr, q.data_ptr(), qt, qh, rows, heads, DTYPES[q.dtype], scale, out.data_ptr(), ot, oh,
+                  lse.data_ptr() if return_lse else None, ws.data_ptr(), nbytes, current_stream(index))
+        if rc:
+            mk._check(rc, "mk_latent_attend")
+        return (out, lse) if return_lse else out

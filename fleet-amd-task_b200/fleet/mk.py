@@ -94,12 +94,29 @@ class MkW4(ctypes.Structure):
                 ("experts", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
+class MkRope(ctypes.Structure):
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("dim", ctypes.c_int32), ("layout", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("pos64", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("reserved", ctypes.c_int32)]
+
+
+class MkLatent(ctypes.Structure):
+    _fields_ = [("c", ctypes.c_void_p), ("r", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("pages", ctypes.c_int32),
+                ("page", ctypes.c_int32), ("d_c", ctypes.c_int32), ("d_r", ctypes.c_int32)]
+
+
+class MkLatentBatch(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("starts", ctypes.c_void_p),
+                ("ldt", ctypes.c_int64), ("n", ctypes.c_int32), ("pages", ctypes.c_int32)]
+
+
 EXPORTS = ["mk_version", "mk_last_error", "mk_create", "mk_add_op", "mk_finalize", "mk_launch", "mk_decode_token",
            "mk_status",
            "mk_reset", "mk_trace", "mk_op_tasks", "mk_destroy", "mk_debug_block_op", "mk_selftest_math",
            "mk_mla_decode_noalloc", "mk_set_op_deps", "mk_ep_alloc", "mk_ep_free", "mk_ep_ipc_handle",
            "mk_ep_ipc_open", "mk_ep_ipc_close", "mk_route", "mk_w4_linear", "mk_w4_experts_workspace",
-           "mk_w4_experts"]
+           "mk_w4_experts", "mk_rope", "mk_latent_append", "mk_latent_read", "mk_latent_attend_workspace",
+           "mk_latent_attend"]
 
 _lib = None
 
@@ -146,6 +163,11 @@ def lib():
         L.mk_w4_linear.argtypes = [vp, vp, i64, i32, vp, i64, vp, i64, i32, vp]
         L.mk_w4_experts_workspace.argtypes = [vp, vp, i32, i32, ctypes.POINTER(i64)]
         L.mk_w4_experts.argtypes = [vp, vp, vp, i64, vp, vp, i32, i32, vp, i64, vp, i64, vp, i64, vp]
+        L.mk_rope.argtypes = [vp, vp, i32, vp, i64, i64, i32, i32, i32, vp, i64, i64, vp]
+        L.mk_latent_append.argtypes = [vp, vp, vp, i64, vp, i64, i32, i32, vp]
+        L.mk_latent_read.argtypes = [vp, vp, vp, i64, vp, i64, i32, i32, i32, vp]
+        L.mk_latent_attend_workspace.argtypes = [vp, i32, i32, i32, ctypes.POINTER(i64)]
+        L.mk_latent_attend.argtypes = [vp, vp, vp, i64, i64, i32, i32, i32, ctypes.c_float, vp, i64, i64, vp, vp, i64, vp]
         for name in EXPORTS:
             getattr(L, name).restype = ctypes.c_int if name != "mk_last_error" else ctypes.c_char_p
         _lib = L

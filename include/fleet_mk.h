@@ -386,6 +386,63 @@ int mk_w4_experts(const MkW4* w13, const MkW4* w2, const void* x, int64_t ldx, c
                   int32_t t, int32_t slots, const void* residual, int64_t ldr, void* out, int64_t ldo, void* workspace,
                   int64_t workspace_bytes, void* stream);
 
+/* ---- The latent attention of a batch of sequences (no counterpart in the reference): rotary positions, the latent
+   cache in 8 bits, the attention over it. As above: each call launches on `stream`, allocates nothing and may be
+   captured in a CUDA graph after a first call of the same shapes; tensors are on the current device.
+   ---- */
+#define MK_BF16 0
+#define MK_FP16 1
+
+/* x [t, heads, width] -> out (csrc/mk_rope.cu has the formulas): the values [start, start + dim) of each head turn by
+   position x inv_freq, the rest is copied where out is not x. Strides of tokens and heads in values; a head's values
+   are contiguous. out is x itself or apart from it. A token at a negative position is left out. */
+#define MK_ROPE_HALF 0
+#define MK_ROPE_INTERLEAVED 1
+#define MK_ROPE_PAIRS_TO_HALF 2
+typedef struct MkRope {
+  const double* inv_freq;   /* [dim / 2], radians a position */
+  int32_t dim, layout, dtype, pos64;   /* pos64: positions are int64, otherwise int32 */
+  float scale;              /* of cos and sin */
+  int32_t reserved;
+} MkRope;
+int mk_rope(const MkRope* r, const void* positions, int32_t t, const void* x, int64_t xt, int64_t xh, int32_t heads,
+            int32_t width, int32_t start, void* out, int64_t ot, int64_t oh, void* stream);
+
+/* A latent cache (csrc/mk_latent.cuh has the format): E4M3 codes c [pages, page, ld_c], ld_c = d_c rounded up to 128,
+   r [pages, page, 64], zero behind a row's values; scales [pages, 2] FP32 of each page's latents and rotary keys. */
+typedef struct MkLatent {
+  void* c;               /* 128-byte aligned */
+  void* r;
+  float* scales;
+  int32_t pages, page;   /* page: 16, 32, 64 or 128 tokens */
+  int32_t d_c, d_r;      /* multiples of 8: 8 to 512, 8 to 64 */
+} MkLatent;
+/* n sequences: table [n, pages] with row stride ldt, lens [n] (this step's tokens included) and starts [n + 1] of
+   their rows in a call, or NULL for one row each. Row i of a sequence's m is its token len - m + i. A length
+   past the table counts as the table's end, below 0 as 0; a page outside the cache holds no token. */
+typedef struct MkLatentBatch {
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* starts;
+  int64_t ldt;
+  int32_t n, pages;
+} MkLatentBatch;
+/* The rows' latents c [rows, d_c] and rotary keys r [rows, d_r] (MK_BF16 or MK_FP16, row strides in values) into
+   the cache. A page is written by one sequence of a call at most. */
+int mk_latent_append(const MkLatent* l, const MkLatentBatch* b, const void* c, int64_t ldc, const void* r, int64_t ldr,
+                     int32_t rows, int32_t dtype, void* stream);
+/* The rows' tokens back from the cache; a token that is in none is zeros, rows of no sequence stay as they were (fill:
+   become zeros). */
+int mk_latent_read(const MkLatent* l, const MkLatentBatch* b, void* c, int64_t ldc, void* r, int64_t ldr, int32_t rows,
+                   int32_t dtype, int32_t fill, void* stream);
+/* out [rows, heads, d_c] = the attention of q [rows, heads, d_c + d_r] (strides of rows and heads in values) over each
+   row's tokens; lse [rows, heads] FP32 or NULL. The workspace (mk_latent_attend_workspace bytes, 256-byte
+   aligned) holds nothing between calls; calls that overlap on the GPU need one each. */
+int mk_latent_attend_workspace(const MkLatent* l, int32_t n, int32_t rows, int32_t heads, int64_t* bytes);
+int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const void* q, int64_t qt, int64_t qh, int32_t rows,
+                     int32_t heads, int32_t dtype, float scale, void* out, int64_t ot, int64_t oh, float* lse, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
