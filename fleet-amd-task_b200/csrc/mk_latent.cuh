@@ -125,8 +125,8 @@ inline int check(const MkLatent* l, const MkLatentBatch* b, int32_t rows, int32_
   if (l->d_c < 8 || l->d_c > MAX_DC || l->d_c % 8 || l->d_r < 8 || l->d_r > LD_R || l->d_r % 8)
     return fail(MK_EINVAL, "d_c is from 8 to 512, d_r from 8 to 64, both multiples of 8");
   if (l->pages < 1 || (int64_t)l->pages * l->page > INT32_MAX) return fail(MK_EINVAL, "a cache holds from 1 page to 2^31 - 1 tokens");
-  if (b->n < 0 || b->pages < 1 || (int64_t)b->pages * l->page > INT32_MAX || b->ldt < 0)
-    return fail(MK_EINVAL, "a batch has 0 or more sequences of 1 page to 2^31 - 1 tokens each");
+  if (b->n < 0 || b->pages < 1 || (int64_t)b->pages * l->page > 1 << 30 || b->ldt < 0)
+    return fail(MK_EINVAL, "a batch has 0 or more sequences of 1 page to 2^30 tokens each");
   if (rows < 0 || (!b->starts && rows != b->n)) return fail(MK_EINVAL, "without starts a batch has one row for each sequence");
   if (dtype != MK_BF16 && dtype != MK_FP16) return fail(MK_EINVAL, "values are BF16 or FP16");
   if (!l->c || !l->r || !l->scales || (b->n && (!b->table || !b->lens))) return fail(MK_EINVAL, "null pointer");

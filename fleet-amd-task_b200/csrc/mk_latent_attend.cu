@@ -4,94 +4,784 @@
 //   s_j = scale (qc . c_j + qr . r_j), j = 0 .. P;  out = sum_j softmax(s)_j c_j;  lse = log sum_j exp(s_j).
 // A row that sees no token (an empty sequence, P < 0, pages outside the cache) gives zeros and lse -inf.
 //
-// A block takes one (row, head), a warp every fourth token.
+// Why E4M3 operands, and how nothing is lost by them. A token is 576 bytes and 16 heads do 35 thousand operations on
+// it: HBM brings an SM a tile of 128 tokens in 3200 clocks, which leaves no time to widen its codes to 16 bits (147 KB
+// of shared memory written and read back). So the codes go to tcgen05.mma (kind::f8f6f4) as they arrive by TMA, twice:
+// as the keys of S = K q^T (128 tokens x N, K-major) and, the same bytes, as the values of O = C^T P (128 latent
+// values x N, MN-major). What is not in 8 bits is split into pieces that are, each a column of its own, for the tensor core's
+// time goes by the 128 rows of the tile, not by N, up to 64 columns:
+//   q    = scale_q (q1 + q2 / 16 (+ q3 / 256)) in E4M3: each piece takes 4 bits and the remainder's sign one more, so
+//          two hold a BF16 value and three an FP16 value exactly, down to 2^-23 of the row's largest;
+//   p    = x 2^-7, x rounded to FP16 = x1 + x2 / 8 + x3 / 64 in E5M2: within 2^-11 (3, 4 and 4 bits are all of FP16's
+//          11), or 2^-30 of the row's largest where that is more.
+// A page's scales (keys: sc latent, sr rotary) multiply the scores' two accumulators in FP32. As the values' scale, sc
+// goes into the exponent: t = s + log2 sc, p = 2^(t - ref), so the pieces are relative to the largest p |c|, and the sum
+// of the weights takes p / sc. ref is a tile's maximum of t, taken anew (with O rescaled in tensor memory) only where some t
+// is more than 8 above it.
+//
+// The work is units of 64 tokens of a group of R rows (a row is a token's head) of a sequence; each block (one per SM)
+// takes an equal run of all units, whatever the lengths, as tiles of two. A group within one run is finished there, one
+// that several runs share leaves partial sums, which merge_kernel joins. Warps 0 to 3 hold a tile's 128 tokens (softmax),
+// warp 4 loads, one thread of warp 5 issues the products.
+#include <cuda.h>
+
+#include <atomic>
+#include <cfloat>
+
+#include "mk_device.cuh"
 #include "mk_latent.cuh"
 
 namespace latent {
 namespace {
 
-constexpr int WARPS = 4, PER = MAX_DC / 32;
+using mk::mbar_arrive;
+using mk::mbar_arrive_expect_tx;
+using mk::mbar_init;
+using mk::mbar_try_wait;
+using mk::smem_u32;
 
-struct Attend {
+constexpr int MAX_CTAS = 148, TILE = 128, UNIT = 64, THREADS = 192, SOFTMAX = 128;
+constexpr int SUB = TILE * 128, STAGE = 4 * SUB + TILE * LD_R;      // a tile: up to 4 x [128 tokens][128 B], then [128][64 B]
+constexpr uint64_t TIMEOUT_NS = 2000000000ull;
+constexpr float X_SCALE = 7.0f, RAISE = 8.0f;                       // x = 2^7 at ref, 2^15 at most
+
+template <typename T, int R_>
+struct Config {
+  static constexpr int R = R_, PIECES = sizeof(typename T::half_type) == 2 && T::exact3 ? 3 : 2;
+  static constexpr int NS = R * PIECES, NO = R * 3;
+  static constexpr int BUFS = 4 * NS + 4 * NO <= 512 ? 2 : 1;       // buffers of scores in tensor memory
+  static constexpr int O_COL = BUFS * 2 * NS;
+  static constexpr int QC = 2 * STAGE, QR = QC + 4 * NS * 128, PB = QR + NS * 64, SMEM = PB + 2 * NO * 128;
+  static_assert(O_COL + 4 * NO <= 512 && SMEM + 1024 + 2048 <= 232448, "tensor memory, shared memory");
+};
+struct Bf16 { using half_type = __nv_bfloat16; static constexpr bool exact3 = false; };
+struct Fp16 { using half_type = __half; static constexpr bool exact3 = true; };
+
+struct Meta {                   // where a block's run begins
+  int split, row, rows, pad;    // within a group: whose flat rows [row, row + rows)
+  int64_t lo, hi, total;        // the group's units, all units
+};
+
+struct Args {
   Cache k;
   Batch b;
   const void* q;
   void* out;
   float* lse;
   int64_t qt, qh, ot, oh;
-  int heads;
+  int heads, subs, box, wide;   // subs: 128-byte columns of a latent; box: rows of a TMA box; wide: 16-byte loads of q
   float scale;
+  Meta* meta;                   // [blocks]
+  float* stat;                  // [2 blocks][R][2]: ref, sum
+  float* part;                  // [2 blocks][R][128 subs]
 };
 
-template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) attend_kernel(const Attend a) {
-  __shared__ float part[WARPS][MAX_DC], stat[WARPS][2];
+// ---- a block's share of the units ----------------------------------------------------------
+template <int R>
+__device__ __forceinline__ int64_t groups_of(const Args& a, const Seq& q) { return ((int64_t)q.n * a.heads + R - 1) / R; }
+__device__ __forceinline__ int units_of(const Args& a, const Seq& q) { return max(1, (min(q.len, a.b.capacity) + UNIT - 1) / UNIT); }
+
+struct Work {
+  int b, u;
+  int64_t g, left;
+};
+struct Segment {
+  Seq q;
+  int s;                        // the sequence
+  int r0, rows;                 // rows [r0, r0 + rows) of the sequence's n x heads
+  int u0, u1, units;            // units [u0, u1) of the group's
+  int lim;                      // tokens that its last row sees
+  int end;                      // past the last token of this segment
+  int tiles;
+};
+
+template <int R>
+__device__ __forceinline__ bool next(const Args& a, Work& w, Segment& s) {
+  while (w.left > 0 && w.b < a.b.n) {
+    s.q = sequence(a.b, w.b);
+    if (w.g >= groups_of<R>(a, s.q)) {
+      ++w.b;
+      w.g = 0;
+      continue;
+    }
+    s.s = w.b;
+    s.units = units_of(a, s.q);
+    s.u0 = w.u;
+    s.u1 = (int)min((int64_t)s.units, w.u + w.left);
+    w.left -= s.u1 - s.u0;
+    s.r0 = (int)(w.g * R);
+    s.rows = min(R, s.q.n * a.heads - s.r0);
+    if (s.u1 == s.units) {
+      ++w.g;
+      w.u = 0;
+    } else {
+      w.u = s.u1;
+    }
+    s.lim = min(max(s.q.len - s.q.n + (s.r0 + s.rows - 1) / a.heads + 1, 0), a.b.capacity);
+    s.end = min(s.u1 * UNIT, s.lim);
+    s.tiles = max(0, (s.end - s.u0 * UNIT + TILE - 1) / TILE);
+    return true;
+  }
+  return false;
+}
+
+// ---- tcgen05 -------------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t descriptor(uint32_t addr, uint32_t lead, uint32_t stride, uint64_t swizzle) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | swizzle << 61;
+}
+constexpr uint64_t SWIZZLE_NONE = 0, SWIZZLE_128 = 2, SWIZZLE_64 = 4;
+// FP32 accumulators; types 0 E4M3, 1 E5M2; transposed: MN-major
+__host__ __device__ constexpr uint32_t instruction(uint32_t b_type, bool transposed, uint32_t n) {
+  return 1u << 4 | 0u << 7 | b_type << 10 | (transposed ? 3u << 15 : 0u) | (n >> 3) << 17 | (uint32_t)(TILE >> 4) << 24;
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// 16 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_store(uint32_t addr, const float (&v)[16]) {
+  const auto u = [&](int i) { return __float_as_uint(v[i]); };
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(u(0)), "r"(u(1)), "r"(u(2)), "r"(u(3)), "r"(u(4)), "r"(u(5)), "r"(u(6)), "r"(u(7)), "r"(u(8)), "r"(u(9)), "r"(u(10)),
+      "r"(u(11)), "r"(u(12)), "r"(u(13)), "r"(u(14)), "r"(u(15))
+      : "memory");
+}
+// (the loaded values may be used from here on)
+template <int N>
+__device__ __forceinline__ void tmem_wait_load(float (&v)[N][16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(v[n][i]));
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A wait with a limit: false where it ran out.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity & 1)) return true;
+  const uint64_t begin = mk::globaltimer();
+  while (!mbar_try_wait(bar, parity & 1))
+    if (mk::globaltimer() - begin > TIMEOUT_NS) return false;
+  return true;
+}
+
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool softmax_any(bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)v)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ float exp2_fast(float v) {      // within 2^-22; below 2^-126: 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// unsigned order of the key = order of the float
+__device__ __forceinline__ uint32_t key_of(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+template <int R>
+struct Shared {
+  uint64_t full[2], empty[2], scored[2], taken[2], weighed[2], summed[2], asked, drained;
+  uint32_t tmem;
+  volatile int lost;            // a softmax thread's wait ran out
+  float4 gran[2][TILE / 16];    // of each 16 tokens: sc, sr, log2 sc, 1 / sc (0: no such page)
+  float qc[R], qr[R];           // the rows' factors of the two accumulators, log2 e included
+  int sees[R];
+  int64_t at[R];                // the rows' outputs
+  float red[4][R];
+};
+
+// The pieces of 16 weights x (FP16, two a word) as bytes of E5M2, the upper byte of an FP16 value: x1 + x2 / 8 + x3 / 64.
+__device__ __forceinline__ void pieces_of(const float (&x)[16], uint4 (&p)[3]) {
+  uint32_t* out[3] = {&p[0].x, &p[1].x, &p[2].x};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[3][2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      __half2 v = __floats2half2_rn(x[4 * i + 2 * k], x[4 * i + 2 * k + 1]);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) {
+        uint32_t u;
+        memcpy(&u, &v, 4);
+        u += 0x00800080u;       // to nearest: magnitudes stay below 2^15.8, so nothing carries over
+        w[n][k] = u;
+        if (n < 2) {
+          u &= 0xFF00FF00u;
+          __half2 h;
+          memcpy(&h, &u, 4);
+          v = __hmul2(__hsub2(v, h), __float2half2_rn(8.0f));
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 3; ++n) out[n][i] = __byte_perm(w[n][0], w[n][1], 0x7531);
+  }
+}
+
+// A segment's queries: each row's scales, and its values' pieces in the order that the products read (K-major, swizzled as
+// TMA does it), zeros behind its values and in absent rows. What is not finite becomes NaN.
+template <typename T, int R>
+__device__ __forceinline__ void ask(const Args& a, const Segment& s, uint8_t* smem, Shared<R>& sh) {
+  using C = Config<T, R>;
+  using E = typename T::half_type;
+  constexpr int PER = SOFTMAX / R, CHUNKS = MAX_DC / 8 / PER;     // threads of a row, eights of values that each holds
+  const int row = threadIdx.x / PER, sub = threadIdx.x % PER, f = s.r0 + row, tok = f / a.heads;
+  const bool live = row < s.rows;
+  const E* q = static_cast<const E*>(a.q) + (s.q.row + tok) * a.qt + (f - tok * a.heads) * a.qh;
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    const int d = part ? a.k.d_r : a.k.d_c, from = part ? a.k.d_c : 0, chunks = part ? LD_R / 8 : a.subs * 16;
+    constexpr int N = CHUNKS;
+    union { uint4 u; E e[8]; } v[N];
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = sub + i * PER;
+      v[i].u = make_uint4(0, 0, 0, 0);
+      if (live && c * 8 < d) {
+        const E* p = q + from + c * 8;
+        if (a.wide) {
+          v[i].u = *reinterpret_cast<const uint4*>(p);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i].e[e] = p[e];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = fabsf(to_f32(v[i].e[e]));
+        amax = x < INFINITY ? fmaxf(amax, x) : amax;
+      }
+#pragma unroll
+    for (int o = PER / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
+    // the smallest power of two with amax <= 448 of it
+    const uint32_t u = __float_as_uint(amax);
+    const int e2 = max((int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0), -120);
+    const float up = __uint_as_float((uint32_t)(e2 + 127) << 23), inv = __uint_as_float((uint32_t)(127 - e2) << 23);
+    if (sub == 0) (part ? sh.qr : sh.qc)[row] = up * (a.scale * 1.44269504f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = sub + i * PER;
+      if (c >= chunks) continue;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = to_f32(v[i].e[e]);
+        x[e] = fabsf(x[e]) < INFINITY ? x[e] * inv : __int_as_float(0x7FC00000);
+      }
+#pragma unroll
+      for (int n = 0; n < C::PIECES; ++n) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = encode2(x[2 * e], x[2 * e + 1]);
+          const float2 back = decode2((uint16_t)w[e]);
+          x[2 * e] = (x[2 * e] - back.x) * 16.0f;
+          x[2 * e + 1] = (x[2 * e + 1] - back.y) * 16.0f;
+        }
+        const int at = n * R + row;     // the piece's row of the operand
+        uint8_t* to = part ? smem + C::QR + at * 64 + (((c >> 1) ^ (at >> 1 & 3)) << 4)
+                           : smem + C::QC + (c >> 4) * (C::NS * 128) + at * 128 + (((c >> 1 & 7) ^ (at & 7)) << 4);
+        *reinterpret_cast<uint2*>(to + (c & 1) * 8) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+      }
+    }
+  }
+}
+
+// ---- the attention -------------------------------------------------------------------------
+template <typename T, int R>
+__global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap map_c,
+                                                             const __grid_constant__ CUtensorMap map_r) {
+  using C = Config<T, R>;
+  using E = typename T::half_type;
+  extern __shared__ uint8_t raw[];
+  __shared__ Shared<R> sh;
+  uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  const uint32_t base = smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Cache& k = a.k;
-  const int row = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int s = row;
-  if (a.b.starts) {
-    int lo = 0, hi = a.b.n;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (a.b.starts[mid] <= row) lo = mid + 1;
-      else hi = mid;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+      mbar_init(&sh.scored[i], 1);
+      mbar_init(&sh.taken[i], 4);
+      mbar_init(&sh.weighed[i], 4);
+      mbar_init(&sh.summed[i], 1);
     }
-    s = lo - 1;
+    mbar_init(&sh.asked, 4);
+    mbar_init(&sh.drained, 1);
+    sh.lost = 0;
+    mk::fence_barrier_init();
   }
-  if (s < 0 || s >= a.b.n) return;
-  const Seq seq = sequence(a.b, s);
-  if (row < seq.row || row >= seq.row + seq.n) return;
-  const int sees = min(seq.len - seq.n + (row - seq.row) + 1, a.b.capacity);
-  const T* q = static_cast<const T*>(a.q) + row * a.qt + h * a.qh;
-  float qc[PER], qr[2], o[PER] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) qc[i] = lane + 32 * i < k.d_c ? to_f32(q[lane + 32 * i]) : 0.0f;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) qr[i] = lane + 32 * i < k.d_r ? to_f32(q[k.d_c + lane + 32 * i]) : 0.0f;
-  for (int j = warp; j < sees; j += WARPS) {
-    const int p = a.b.table[s * a.b.ldt + (j >> k.shift)];
-    if (p < 0 || p >= k.pages) continue;
-    const int64_t at = ((int64_t)p << k.shift) + (j & (k.page - 1));
-    const float sc = k.scales[2 * (int64_t)p], sr = k.scales[2 * (int64_t)p + 1];
-    float c[PER], dot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      c[i] = lane + 32 * i < k.d_c ? decode2(k.c[at * k.ld_c + lane + 32 * i]).x * sc : 0.0f;
-      dot += qc[i] * c[i];
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    fence_before();
+  }
+  // this block's run of the units
+  Work work{};
+  {
+    const auto count = [&](int i) {
+      const Seq q = sequence(a.b, i);
+      return groups_of<R>(a, q) * units_of(a, q);
+    };
+    int64_t place;
+    const int64_t total = locate<THREADS>(a.b.n, 0, count, work.b, place);
+    const int64_t lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
+    __syncthreads();
+    locate<THREADS>(a.b.n, lo, count, work.b, place);
+    work.left = hi - lo;
+    const bool any = work.b < a.b.n;
+    const Seq q = any ? sequence(a.b, work.b) : Seq{0, 0, 0};
+    const int units = units_of(a, q);
+    work.g = any ? place / units : 0;
+    work.u = any ? (int)(place - work.g * units) : 0;
+    if (threadIdx.x == 0) {
+      Meta m{};
+      m.split = any && work.u > 0;
+      m.row = q.row * a.heads + (int)(work.g * R);
+      m.rows = any ? min(R, q.n * a.heads - (int)(work.g * R)) : 0;
+      m.lo = lo - work.u;
+      m.hi = m.lo + units;
+      m.total = total;
+      a.meta[blockIdx.x] = m;
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (lane + 32 * i < k.d_r) dot += qr[i] * decode2(k.r[at * LD_R + lane + 32 * i]).x * sr;
-#pragma unroll
-    for (int e = 16; e > 0; e >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, e);
-    const float v = dot * a.scale, to = fmaxf(m, isnan(v) ? 0.0f : v);   // (a NaN is the weights', not the largest score's)
-    const float was = m == -INFINITY ? 0.0f : expf(m - to), is = expf(v - to);
-    m = to;
-    l = l * was + is;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = o[i] * was + is * c[i];
   }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = sh.tmem;
+  Segment s;
+  int it = 0;                   // tiles so far
+
+  if (warp == 4) {
+    // ---- loads: a tile's pages, and the scales of their tokens
+    bool ok = true;
+    while (ok && next<R>(a, work, s)) {
+      for (int t = 0; t < s.tiles; ++t, ++it) {
+        const int st = it & 1, pos0 = s.u0 * UNIT + t * TILE, pos = pos0 + 16 * lane;
+        int page = -1;
+        float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (lane < TILE / 16 && pos < s.end) {
+          page = a.b.table[s.s * a.b.ldt + (pos >> k.shift)];
+          if (page >= 0 && page < k.pages) {
+            g.x = k.scales[2 * (int64_t)page];
+            g.y = k.scales[2 * (int64_t)page + 1];
+            const float v = fmaxf(g.x, 5.42101086e-20f);        // 2^-64: a page that was never written has scale 0
+            g.z = log2f(v);
+            g.w = 1.0f / v;
+          } else {
+            page = -1;
+          }
+        }
+        if (it >= 2) ok = __all_sync(~0u, wait(&sh.empty[st], (it - 2) >> 1));
+        if (!ok) break;
+        if (lane < TILE / 16) sh.gran[st][lane] = g;
+        const int each = a.box / 16;                            // a box's first 16 tokens name its page
+        const bool loads = page >= 0 && lane % each == 0;
+        const int boxes = __popc(__ballot_sync(~0u, loads));
+        if (lane == 0) mbar_arrive_expect_tx(&sh.full[st], boxes * a.box * (a.subs * 128 + LD_R));
+        __syncwarp();
+        if (loads) {
+          const int y = (page << k.shift) + (pos & (k.page - 1));
+          uint8_t* to = smem + st * STAGE + lane * 16 * 128;
+          for (int j = 0; j < a.subs; ++j) mk::tma_load_2d(to + j * SUB, &map_c, j * 128, y, &sh.full[st]);
+          mk::tma_load_2d(smem + st * STAGE + 4 * SUB + lane * 16 * LD_R, &map_r, 0, y, &sh.full[st]);
+        }
+      }
+    }
+    for (int i = max(it - 2, 0); i < it; ++i) wait(&sh.full[i & 1], i >> 1);   // no copy outlives the block
+  } else if (warp == 5) {
+    // ---- products, issued by one thread
+    if (lane == 0) {
+      constexpr uint32_t ASK = instruction(0, false, C::NS), SUM = instruction(1, true, C::NO);
+      bool ok = true;
+      const auto sum = [&](int i, int n, bool first) {          // O of tile i, n of whose tokens count
+        const int st = i & 1;
+        ok = ok && wait(&sh.weighed[st], i >> 1);
+        if (!ok) return;
+        fence_after();
+        for (int j = 0; j < a.subs; ++j)
+          for (int kk = 0; kk < (n + 31) / 32; ++kk)
+            mma(tmem + C::O_COL + j * C::NO, descriptor(base + st * STAGE + j * SUB + kk * 4096, SUB, 1024, SWIZZLE_128),
+                descriptor(base + C::PB + st * C::NO * 128 + kk * 512, 128, 2048, SWIZZLE_NONE), SUM, !first || kk > 0);
+        commit(&sh.empty[st]);
+        commit(&sh.summed[st]);
+      };
+      int segments = 0;
+      while (ok && next<R>(a, work, s)) {
+        if (s.tiles == 0) continue;
+        ok = wait(&sh.asked, segments++);
+        int n = 0;
+        for (int t = 0; t < s.tiles && ok; ++t, ++it) {
+          const int st = it & 1, buf = it % C::BUFS;
+          ok = wait(&sh.full[st], it >> 1) && (it < C::BUFS || wait(&sh.taken[buf], it / C::BUFS - 1));
+          if (!ok) break;
+          fence_after();
+          const uint32_t d = tmem + buf * 2 * C::NS;
+          for (int j = 0; j < a.subs; ++j)
+            for (int kk = 0; kk < 4; ++kk)
+              mma(d, descriptor(base + st * STAGE + j * SUB + kk * 32, 16, 1024, SWIZZLE_128),
+                  descriptor(base + C::QC + j * C::NS * 128 + kk * 32, 16, 1024, SWIZZLE_128), ASK, j > 0 || kk > 0);
+          for (int kk = 0; kk < 2; ++kk)
+            mma(d + C::NS, descriptor(base + st * STAGE + 4 * SUB + kk * 32, 16, 512, SWIZZLE_64),
+                descriptor(base + C::QR + kk * 32, 16, 512, SWIZZLE_64), ASK, kk > 0);
+          commit(&sh.scored[buf]);
+          if (t > 0) sum(it - 1, n, t == 1);
+          n = min(TILE, s.end - (s.u0 * UNIT + t * TILE));
+        }
+        sum(it - 1, n, s.tiles == 1);
+      }
+      commit(&sh.drained);
+      wait(&sh.drained, 0);
+    }
+  } else {
+    // ---- softmax: this thread's token of each tile, and its latent value of each 128
+    const int tid = threadIdx.x;
+    const uint32_t lanes = tmem + ((uint32_t)warp * 32 << 16);
+    bool dead = false;
+    while (next<R>(a, work, s)) {
+      softmax_sync();           // the last segment's factors are read
+      const int last_row = s.q.len - s.q.n + 1;
+      const int first_sees = min(max(last_row + s.r0 / a.heads, 0), a.b.capacity);
+      if (tid < R) {
+        const int f = s.r0 + tid, tok = f / a.heads;
+        sh.sees[tid] = tid < s.rows ? min(max(last_row + tok, 0), a.b.capacity) : INT32_MAX;
+        sh.at[tid] = (s.q.row + tok) * a.ot + (f - tok * a.heads) * a.oh;
+      }
+      if (s.tiles > 0 && !dead) {
+        ask<T, R>(a, s, smem, sh);
+        mk::fence_proxy_async_smem();
+      }
+      softmax_sync();
+      if (s.tiles > 0 && !dead && lane == 0) mbar_arrive(&sh.asked);
+      float ref[R], l[R];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) part[warp][lane + 32 * i] = o[i];
-  if (lane == 0) {
-    stat[warp][0] = m;
-    stat[warp][1] = l;
+      for (int h = 0; h < R; ++h) {
+        ref[h] = -FLT_MAX;
+        l[h] = 0.0f;
+      }
+      for (int t = 0; t < s.tiles && !dead; ++t, ++it) {
+        const int st = it & 1, buf = it % C::BUFS, pos0 = s.u0 * UNIT + t * TILE, pos = pos0 + tid;
+        bool ok = wait(&sh.full[st], it >> 1) && wait(&sh.scored[buf], it / C::BUFS);
+        fence_after();
+        const float4 g = sh.gran[st][tid >> 4];
+        const bool none = pos >= s.end || g.w == 0.0f;
+        float v[R];
+        bool rises = false;
+#pragma unroll
+        for (int c = 0; c < R / 16; ++c) {
+          float sc[2 * C::PIECES][16];
+#pragma unroll
+          for (int p = 0; p < 2 * C::PIECES; ++p) tmem_load(lanes + buf * 2 * C::NS + p * R + c * 16, sc[p]);
+          tmem_wait_load(sc);
+#pragma unroll
+          for (int h = 0; h < 16; ++h) {
+            float x = sc[1][h], y = sc[C::PIECES + 1][h];
+            if (C::PIECES == 3) {
+              x = fmaf(sc[2][h], 0.0625f, x);
+              y = fmaf(sc[C::PIECES + 2 * (C::PIECES == 3)][h], 0.0625f, y);
+            }
+            x = fmaf(x, 0.0625f, sc[0][h]) * g.x;
+            y = fmaf(y, 0.0625f, sc[C::PIECES][h]) * g.y;
+            v[c * 16 + h] = fmaf(x, sh.qc[c * 16 + h], fmaf(y, sh.qr[c * 16 + h], g.z));
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.taken[buf]);
+        if (none) {
+#pragma unroll
+          for (int h = 0; h < R; ++h) v[h] = -INFINITY;
+        } else if (pos >= first_sees) {
+#pragma unroll
+          for (int h = 0; h < R; ++h)
+            if (pos >= sh.sees[h]) v[h] = -INFINITY;
+        }
+#pragma unroll
+        for (int h = 0; h < R; ++h) rises |= v[h] > ref[h] + RAISE;
+        if (!ok) sh.lost = 1;
+        rises = softmax_any(rises);
+        if (sh.lost) {
+          dead = true;
+          break;
+        }
+        if (rises) {
+#pragma unroll
+          for (int h = 0; h < R; ++h) {
+            const uint32_t m = __reduce_max_sync(~0u, key_of(fmaxf(v[h], -INFINITY)));     // (a NaN is no largest value)
+            if (lane == h) sh.red[warp][h] = of_key(m);
+          }
+          softmax_sync();
+          float f[R];
+#pragma unroll
+          for (int h = 0; h < R; ++h) {
+            const float m = fmaxf(ref[h], fmaxf(fmaxf(sh.red[0][h], sh.red[1][h]), fmaxf(sh.red[2][h], sh.red[3][h])));
+            f[h] = exp2_fast(ref[h] - m);
+            l[h] *= f[h];
+            ref[h] = m;
+          }
+          if (t > 0) {
+            ok = wait(&sh.summed[st ^ 1], (it - 1) >> 1);
+            fence_after();
+            for (int j = 0; j < a.subs; ++j)
+#pragma unroll
+              for (int c = 0; c < R / 16; ++c) {
+                float o[3][16];
+#pragma unroll
+                for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R + c * 16, o[p]);
+                tmem_wait_load(o);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+#pragma unroll
+                  for (int h = 0; h < 16; ++h) o[p][h] *= f[c * 16 + h];
+                  tmem_store(lanes + C::O_COL + j * C::NO + p * R + c * 16, o[p]);
+                }
+              }
+            tmem_wait_store();
+          }
+        }
+        if (it >= 2) ok = wait(&sh.summed[st], (it - 2) >> 1) && ok;    // its weights have been used
+        if (!ok) sh.lost = 1;
+        uint8_t* w = smem + C::PB + st * C::NO * 128 + tid * 16;
+#pragma unroll
+        for (int c = 0; c < R / 16; ++c) {
+          float x[16];
+          uint4 p[3];
+#pragma unroll
+          for (int h = 0; h < 16; ++h) {
+            x[h] = exp2_fast(v[c * 16 + h] - (ref[c * 16 + h] - X_SCALE));
+            l[c * 16 + h] = fmaf(x[h], g.w, l[c * 16 + h]);
+          }
+          pieces_of(x, p);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4*>(w + (i * (R / 16) + c) * 2048) = p[i];
+        }
+        // 0 x NaN is NaN: what no row sees becomes zero, a NaN that only later rows see (their scores are NaN) too
+        if (none || pos >= first_sees) {
+          for (int j = 0; j < a.subs; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              uint4* at = reinterpret_cast<uint4*>(smem + st * STAGE + j * SUB + tid * 128 + i * 16);
+              uint4 u = make_uint4(0, 0, 0, 0);
+              if (!none) {
+                u = *at;
+                const auto clean = [](uint32_t x) { return x & ~((((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) / 128 * 255); };
+                u = make_uint4(clean(u.x), clean(u.y), clean(u.z), clean(u.w));
+              }
+              *at = u;
+            }
+        }
+        mk::fence_proxy_async_smem();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.weighed[st]);
+      }
+      // ---- the segment's end: whole groups are finished, others leave their sums
+      if (s.tiles > 0 && !dead && !wait(&sh.summed[(it - 1) & 1], (it - 1) >> 1)) sh.lost = 1;
+      fence_after();
+#pragma unroll
+      for (int h = 0; h < R; ++h) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l[h] += __shfl_xor_sync(~0u, l[h], o);
+        if (lane == h % 32) sh.red[warp][h] = l[h];
+      }
+      softmax_sync();
+      if (sh.lost) dead = true;
+      const bool whole = s.u0 == 0 && s.u1 == s.units;
+      const int64_t slot = (2 * (int64_t)blockIdx.x + (s.u0 == 0)) * R;
+      const float nan = __int_as_float(0x7FC00000);
+#pragma unroll
+      for (int h = 0; h < R; ++h) {
+        l[h] = dead ? nan : sh.red[0][h] + sh.red[1][h] + sh.red[2][h] + sh.red[3][h];
+        if (tid == h && h < s.rows) {
+          if (!whole) {
+            a.stat[(slot + h) * 2] = ref[h];
+            a.stat[(slot + h) * 2 + 1] = l[h];
+          } else if (a.lse) {
+            a.lse[(int64_t)s.q.row * a.heads + s.r0 + h] = l[h] == 0.0f ? -INFINITY : (ref[h] - X_SCALE + log2f(l[h])) * 0.693147181f;
+          }
+        }
+        if (whole) l[h] = l[h] == 0.0f ? 0.0f : 1.0f / l[h];
+      }
+      for (int j = 0; j < a.subs; ++j) {
+        const int dim = j * 128 + tid;
+#pragma unroll
+        for (int c = 0; c < R / 16; ++c) {
+          float o[3][16] = {};
+          if (s.tiles > 0) {
+#pragma unroll
+            for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R + c * 16, o[p]);
+            tmem_wait_load(o);
+          }
+#pragma unroll
+          for (int h = 0; h < 16; ++h) {
+            const int row = c * 16 + h;
+            const float x = fmaf(fmaf(o[2][h], 0.125f, o[1][h]), 0.125f, o[0][h]);
+            if (row < s.rows) {
+              if (!whole) a.part[(slot + row) * (a.subs * 128) + dim] = x;
+              else if (dim < k.d_c) static_cast<E*>(a.out)[sh.at[row] + dim] = from_f32<E>(l[row] == 0.0f ? 0.0f : x * l[row]);
+            }
+          }
+        }
+      }
+      fence_before();
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// One row of each group that several blocks' runs share, by the block whose run is the second of them: the partial sums
+// of all, in their order.
+template <typename T, int R>
+__global__ void __launch_bounds__(128) merge_kernel(const Args a, int blocks) {
+  using E = typename T::half_type;
+  __shared__ float weight[MAX_CTAS];
+  __shared__ int slots[MAX_CTAS];
+  __shared__ float top[4], all[4];
+  const int i = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Meta m = a.meta[i];
+  if (!m.split || row >= m.rows) return;
+  if (i == 0 || m.total * (i - 1) / blocks > m.lo) return;             // an earlier block's run splits it too
+  // the runs that hold some of it: with fewer units than blocks one for each unit, otherwise i - 1, i, ...
+  const auto holds = [&](int64_t unit) { return (int)(((unit + 1) * blocks - 1) / m.total); };
+  const int n = m.total < blocks ? (int)(m.hi - m.lo) : holds(m.hi - 1) - i + 2;
+  for (int p = tid; p < n; p += 128) {
+    const int b = m.total < blocks ? holds(m.lo + p) : i - 1 + p;
+    slots[p] = 2 * b + (p == 0);        // the first part begins it, the others continue it
   }
   __syncthreads();
-  float top = -INFINITY, total = 0.0f, w[WARPS];
-  for (int i = 0; i < WARPS; ++i) top = fmaxf(top, stat[i][0]);
-  for (int i = 0; i < WARPS; ++i) {
-    w[i] = stat[i][0] == -INFINITY ? 0.0f : expf(stat[i][0] - top);
-    total += w[i] * stat[i][1];
+  float ref = -FLT_MAX;
+  for (int p = tid; p < n; p += 128) ref = fmaxf(ref, a.stat[((int64_t)slots[p] * R + row) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(~0u, ref, o));
+  if (tid % 32 == 0) top[tid / 32] = ref;
+  __syncthreads();
+  ref = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  float l = 0.0f;
+  for (int p = tid; p < n; p += 128) {
+    const float* st = a.stat + ((int64_t)slots[p] * R + row) * 2;
+    weight[p] = exp2_fast(st[0] - ref);
+    l += weight[p] * st[1];
   }
-  T* out = static_cast<T*>(a.out) + row * a.ot + h * a.oh;
-  for (int c = threadIdx.x; c < k.d_c; c += WARPS * 32) {
-    float v = 0.0f;
-    for (int i = 0; i < WARPS; ++i) v += w[i] * part[i][c];
-    out[c] = from_f32<T>(top == -INFINITY ? 0.0f : v / total);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+  if (tid % 32 == 0) all[tid / 32] = l;
+  __syncthreads();
+  l = all[0] + all[1] + all[2] + all[3];
+  const int f = m.row + row, tok = f / a.heads;
+  if (a.lse && tid == 0) a.lse[f] = l == 0.0f ? -INFINITY : (ref - X_SCALE + log2f(l)) * 0.693147181f;
+  E* out = static_cast<E*>(a.out) + tok * a.ot + (f - tok * a.heads) * a.oh;
+  const int ld = a.subs * 128, dim = tid * 4;
+  if (dim >= ld) return;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+  for (int p = 0; p < n; ++p) {
+    const float4 v = *reinterpret_cast<const float4*>(a.part + ((int64_t)slots[p] * R + row) * ld + dim);
+    const float w = weight[p];
+    o.x = fmaf(w, v.x, o.x);
+    o.y = fmaf(w, v.y, o.y);
+    o.z = fmaf(w, v.z, o.z);
+    o.w = fmaf(w, v.w, o.w);
   }
-  if (a.lse && threadIdx.x == 0) a.lse[(int64_t)row * a.heads + h] = top == -INFINITY ? top : top + logf(total);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l, v[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (dim + e < a.k.d_c) out[dim + e] = from_f32<E>(l == 0.0f ? 0.0f : v[e] * inv);
 }
+
+// ---- the host's side -----------------------------------------------------------------------
+int tensor_map(CUtensorMap* map, void* base, uint64_t cols, uint64_t rows, uint32_t box, CUtensorMapSwizzle swizzle) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<Encode> known{nullptr};
+  Encode encode = known.load(std::memory_order_acquire);
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || !fn || q != cudaDriverEntryPointSuccess)
+      return fail(MK_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    encode = reinterpret_cast<Encode>(fn);
+    known.store(encode, std::memory_order_release);
+  }
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols};
+  const cuuint32_t boxes[2] = {cols < 128 ? (cuuint32_t)cols : 128, box}, ones[2] = {1, 1};
+  if (encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return fail(MK_EINVAL, "the codes make no tensor map");
+  return MK_OK;
+}
+
+constexpr int MAX_DEVICES = 64;
+
+template <typename T, int R>
+int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device, int blocks, cudaStream_t s) {
+  static std::atomic<bool> ready[MAX_DEVICES];   // the kernel may use that much shared memory on the device
+  cudaError_t e = cudaSuccess;
+  if (!ready[device].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(attend_kernel<T, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, Config<T, R>::SMEM + 1024);
+    if (e == cudaSuccess) ready[device].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = Config<T, R>::SMEM + 1024;
+  cfg.stream = s;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, attend_kernel<T, R>, a, c, r);
+  if (e == cudaSuccess) {
+    cudaLaunchAttribute overlap[1];
+    overlap[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)blocks, R);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    cfg.attrs = overlap;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, merge_kernel<T, R>, a, blocks);
+  }
+  return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
+}
+
+constexpr int64_t META_BYTES = (MAX_CTAS * sizeof(Meta) + 255) / 256 * 256;
+int64_t workspace(int rows, int subs) { return META_BYTES + (int64_t)2 * MAX_CTAS * rows * (2 + subs * 128) * 4; }
 
 }  // namespace
 }  // namespace latent
@@ -100,19 +790,26 @@ using namespace latent;
 
 extern "C" int mk_latent_attend_workspace(const MkLatent* l, int32_t n, int32_t rows, int32_t heads, int64_t* bytes) {
   if (!l || !bytes || n < 0 || rows < 0 || heads < 1) return fail(MK_EINVAL, "null pointer or a negative size");
-  *bytes = 0;
+  *bytes = workspace(16, (l->d_c + 127) / 128);
   return MK_OK;
 }
 
 extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const void* q, int64_t qt, int64_t qh, int32_t rows,
                                 int32_t heads, int32_t dtype, float scale, void* out, int64_t ot, int64_t oh, float* lse,
                                 void* workspace, int64_t workspace_bytes, void* stream) {
-  Attend a{};
+  Args a{};
   if (const int e = check(l, b, rows, dtype, a.k, a.b)) return e;
-  if (heads < 1 || heads > 1024) return fail(MK_EINVAL, "heads are from 1 to 1024");
+  if (heads < 1 || heads > 1024 || (int64_t)rows * heads > INT32_MAX) return fail(MK_EINVAL, "heads are from 1 to 1024, rows x heads below 2^31");
   if (rows == 0 || b->n == 0) return MK_OK;
-  if (!q || !out) return fail(MK_EINVAL, "null pointer");
-  if (((uintptr_t)q | (uintptr_t)out) & 1 || (uintptr_t)lse & 3) return fail(MK_EINVAL, "misaligned q, out or lse");
+  if (!q || !out || !workspace) return fail(MK_EINVAL, "null pointer");
+  if (((uintptr_t)q | (uintptr_t)out) & 1 || (uintptr_t)lse & 3 || (uintptr_t)workspace & 255)
+    return fail(MK_EINVAL, "misaligned q, out, lse or workspace (256 bytes)");
+  a.subs = a.k.ld_c / 128;
+  if (workspace_bytes < latent::workspace(16, a.subs)) return fail(MK_EINVAL, "the workspace is too small");
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= MAX_DEVICES ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    return fail(MK_ECUDA, "cudaGetDevice failed or device ordinal out of range");
   a.q = q;
   a.out = out;
   a.lse = lse;
@@ -122,11 +819,16 @@ extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const
   a.oh = oh;
   a.heads = heads;
   a.scale = scale;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)rows, (unsigned)heads);
-  cfg.blockDim = dim3(WARPS * 32);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == MK_BF16 ? cudaLaunchKernelEx(&cfg, attend_kernel<__nv_bfloat16>, a)
-                                          : cudaLaunchKernelEx(&cfg, attend_kernel<__half>, a);
-  return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
+  a.box = a.k.page < UNIT ? a.k.page : UNIT;
+  a.wide = (uintptr_t)q % 16 == 0 && qt % 8 == 0 && qh % 8 == 0;
+  a.meta = static_cast<Meta*>(workspace);
+  a.stat = reinterpret_cast<float*>(static_cast<char*>(workspace) + META_BYTES);
+  a.part = a.stat + (int64_t)2 * MAX_CTAS * 16 * 2;
+  CUtensorMap c, r;
+  const uint64_t tokens = (uint64_t)a.k.pages * a.k.page;
+  if (const int e = tensor_map(&c, a.k.c, a.k.ld_c, tokens, a.box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+  if (const int e = tensor_map(&r, a.k.r, LD_R, tokens, a.box, CU_TENSOR_MAP_SWIZZLE_64B)) return e;
+  const int blocks = sms < MAX_CTAS ? sms : MAX_CTAS;
+  return dtype == MK_BF16 ? launch<Bf16, 16>(a, c, r, device, blocks, static_cast<cudaStream_t>(stream))
+                          : launch<Fp16, 16>(a, c, r, device, blocks, static_cast<cudaStream_t>(stream));
 }
