@@ -77,7 +77,8 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Write a) {
   int s = blockIdx.x, first;
   int64_t nth = 0;
   if (a.b.starts)
-    locate<THREADS>(a.b.n, blockIdx.x, [&](int i) { int f; return pages_of(k, a.b, sequence(a.b, i), f); }, s, nth);
+    locate<THREADS>(a.b.n, [&](int i) { int f; return pages_of(k, a.b, sequence(a.b, i), f); },
+                    [](int64_t) { return (int64_t)blockIdx.x; }, s, nth);
   if (s >= a.b.n) return;
   const Seq q = sequence(a.b, s);
   if (nth >= pages_of(k, a.b, q, first)) return;

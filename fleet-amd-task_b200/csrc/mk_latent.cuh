@@ -77,10 +77,10 @@ __device__ __forceinline__ uint16_t encode2(float a, float b) {      // NaN stay
   return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 
-// The item (of n with count(i) >= 0 parts each) that holds part `at` of all, and the part's place in it; every thread of
-// the block calls it. Returns the number of all parts; item is n if `at` lies past them.
-template <int THREADS, typename Count>
-__device__ __forceinline__ int64_t locate(int n, int64_t at, Count count, int& item, int64_t& place) {
+// The item (of n with count(i) >= 0 parts each) that holds part which(all parts) of them, and the part's place in it; every
+// thread of the block calls it, once. item is n if there is no such part.
+template <int THREADS, typename Count, typename Which>
+__device__ __forceinline__ void locate(int n, Count count, Which which, int& item, int64_t& place) {
   __shared__ int64_t warps[THREADS / 32];
   __shared__ int64_t found_place;
   __shared__ int found_item;
@@ -103,6 +103,7 @@ __device__ __forceinline__ int64_t locate(int n, int64_t at, Count count, int& i
     if (w < warp) upto += warps[w];
     total += warps[w];
   }
+  const int64_t at = which(total);
   if (at >= upto - mine && at < upto) {
     int64_t left = at - (upto - mine);
     int i = lo;
@@ -113,7 +114,6 @@ __device__ __forceinline__ int64_t locate(int n, int64_t at, Count count, int& i
   __syncthreads();
   item = found_item;
   place = found_place;
-  return total;
 }
 
 inline int fail(int code, const char* msg) { return mk::set_last_error(code, msg); }

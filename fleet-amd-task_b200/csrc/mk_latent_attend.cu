@@ -21,8 +21,8 @@
 //
 // The work is units of 64 tokens of a group of R rows (a row is a token's head) of a sequence; each block (one per SM)
 // takes an equal run of all units, whatever the lengths, as tiles of two. A group within one run is finished there, one
-// that several runs share leaves partial sums, which merge_kernel joins. Warps 0 to 3 hold a tile's 128 tokens (softmax),
-// warp 4 loads, one thread of warp 5 issues the products.
+// that several runs share leaves partial sums, which merge_kernel joins. Warps 0 to 7 are the softmax: a warp holds 32 of a
+// tile's 128 tokens (the lanes of tensor memory that it may read) for half of the rows. Warp 8 loads, warp 9 issues the products.
 #include <cuda.h>
 
 #include <atomic>
@@ -40,14 +40,14 @@ using mk::mbar_init;
 using mk::mbar_try_wait;
 using mk::smem_u32;
 
-constexpr int MAX_CTAS = 148, TILE = 128, UNIT = 64, THREADS = 192, SOFTMAX = 128;
+constexpr int MAX_CTAS = 148, TILE = 128, UNIT = 64, THREADS = 320, SOFTMAX = 256;
 constexpr int SUB = TILE * 128, STAGE = 4 * SUB + TILE * LD_R;      // a tile: up to 4 x [128 tokens][128 B], then [128][64 B]
 constexpr uint64_t TIMEOUT_NS = 2000000000ull;
 constexpr float X_SCALE = 7.0f, RAISE = 8.0f;                       // x = 2^7 at ref, 2^15 at most
 
 template <typename T, int R_>
 struct Config {
-  static constexpr int R = R_, PIECES = sizeof(typename T::half_type) == 2 && T::exact3 ? 3 : 2;
+  static constexpr int R = R_, H = R_ / 2, PIECES = sizeof(typename T::half_type) == 2 && T::exact3 ? 3 : 2;
   static constexpr int NS = R * PIECES, NO = R * 3;
   static constexpr int BUFS = 4 * NS + 4 * NO <= 512 ? 2 : 1;       // buffers of scores in tensor memory
   static constexpr int O_COL = BUFS * 2 * NS;
@@ -59,7 +59,7 @@ struct Fp16 { using half_type = __half; static constexpr bool exact3 = true; };
 
 struct Meta {                   // where a block's run begins
   int split, row, rows, pad;    // within a group: whose flat rows [row, row + rows)
-  int64_t lo, hi, total;        // the group's units, all units
+  int64_t lo, hi, total;        // the places of the group's units, of all
 };
 
 struct Args {
@@ -81,9 +81,24 @@ template <int R>
 __device__ __forceinline__ int64_t groups_of(const Args& a, const Seq& q) { return ((int64_t)q.n * a.heads + R - 1) / R; }
 __device__ __forceinline__ int units_of(const Args& a, const Seq& q) { return max(1, (min(q.len, a.b.capacity) + UNIT - 1) / UNIT); }
 
+// Runs are cut by cost: a group costs its units and FIXED more (its queries, its first tile's maximum, its outputs).
+constexpr int FIXED = 3;
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {      // of values above -1
+  return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+__device__ __forceinline__ int64_t begin_of(int64_t total, int block, int blocks) {
+  const int64_t each = quotient(total, blocks), more = total - each * blocks;
+  return each * block + (block < more ? block : more);
+}
+// the block whose run holds place `at` < total
+__device__ __forceinline__ int holder_of(int64_t total, int64_t at, int blocks) {
+  const int64_t each = quotient(total, blocks), more = total - each * blocks;
+  return (int)(at < more * (each + 1) ? quotient(at, each + 1) : more + quotient(at - more * (each + 1), each));
+}
+
 struct Work {
-  int b, u;
-  int64_t g, left;
+  int b, at;                    // the sequence, the place in its group's cost
+  int64_t g, left;              // the group, what is left of the run
 };
 struct Segment {
   Seq q;
@@ -106,17 +121,18 @@ __device__ __forceinline__ bool next(const Args& a, Work& w, Segment& s) {
     }
     s.s = w.b;
     s.units = units_of(a, s.q);
-    s.u0 = w.u;
-    s.u1 = (int)min((int64_t)s.units, w.u + w.left);
-    w.left -= s.u1 - s.u0;
+    const int to = (int)min((int64_t)s.units + FIXED, w.at + w.left);
+    s.u0 = max(w.at - FIXED, 0);
+    s.u1 = max(to - FIXED, 0);
+    w.left -= to - w.at;
     s.r0 = (int)(w.g * R);
     s.rows = min(R, s.q.n * a.heads - s.r0);
+    w.at = to;
     if (s.u1 == s.units) {
       ++w.g;
-      w.u = 0;
-    } else {
-      w.u = s.u1;
+      w.at = 0;
     }
+    if (s.u1 == s.u0) continue;
     s.lim = min(max(s.q.len - s.q.n + (s.r0 + s.rows - 1) / a.heads + 1, 0), a.b.capacity);
     s.end = min(s.u1 * UNIT, s.lim);
     s.tiles = max(0, (s.end - s.u0 * UNIT + TILE - 1) / TILE);
@@ -134,47 +150,72 @@ constexpr uint64_t SWIZZLE_NONE = 0, SWIZZLE_128 = 2, SWIZZLE_64 = 4;
 __host__ __device__ constexpr uint32_t instruction(uint32_t b_type, bool transposed, uint32_t n) {
   return 1u << 4 | 0u << 7 | b_type << 10 | (transposed ? 3u << 15 : 0u) | (n >> 3) << 17 | (uint32_t)(TILE >> 4) << 24;
 }
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+// The whole warp calls these with the same operands and its elected lane issues: operands that the compiler has to make
+// uniform out of one lane's branch cost 80 to 130 clocks a product, more than the product (32 + N / 4).
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t elected) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(elected)
       : "memory");
 }
-__device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(elected)
+      : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// 16 columns of this warp's 32 lanes
+// 8 or 16 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(addr));
+}
 __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[16]) {
-  uint32_t r[16];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+        "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
       : "r"(addr));
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_store(uint32_t addr, const float (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "f"(v[0]), "f"(v[1]),
+               "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_store(uint32_t addr, const float (&v)[16]) {
-  const auto u = [&](int i) { return __float_as_uint(v[i]); };
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
-      "r"(u(0)), "r"(u(1)), "r"(u(2)), "r"(u(3)), "r"(u(4)), "r"(u(5)), "r"(u(6)), "r"(u(7)), "r"(u(8)), "r"(u(9)), "r"(u(10)),
-      "r"(u(11)), "r"(u(12)), "r"(u(13)), "r"(u(14)), "r"(u(15))
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
+      "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
       : "memory");
 }
 // (the loaded values may be used from here on)
-template <int N>
-__device__ __forceinline__ void tmem_wait_load(float (&v)[N][16]) {
+template <int N, int M>
+__device__ __forceinline__ void tmem_wait_load(float (&v)[N][M]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(v[n][i]));
+    for (int i = 0; i < M; ++i) asm volatile("" : "+f"(v[n][i]));
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ bool reached_yet(uint64_t* bar, uint32_t parity) {      // (mbarrier.try_wait may wait a while itself)
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity & 1)
+      : "memory");
+  return ok != 0;
+}
 // A wait with a limit: false where it ran out.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
   for (int i = 0; i < 64; ++i)
@@ -185,11 +226,11 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
   return true;
 }
 
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ bool softmax_any(bool v) {
   uint32_t r;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
       : "r"((uint32_t)v)
       : "memory");
@@ -200,12 +241,26 @@ __device__ __forceinline__ float exp2_fast(float v) {      // within 2^-22; belo
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// unsigned order of the key = order of the float
-__device__ __forceinline__ uint32_t key_of(float v) {
-  const uint32_t u = __float_as_uint(v);
-  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+// Of 32 lanes' v[N], lane l gets the whole of v[l % N].
+template <int N, typename Op>
+__device__ __forceinline__ float across(float (&v)[N], Op op) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int n = N / 2; n >= 1; n /= 2)
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const bool up = lane & n;
+      const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+      v[i] = op(keep, __shfl_xor_sync(~0u, give, n));
+    }
+#pragma unroll
+  for (int o = N; o < 32; o *= 2) v[0] = op(v[0], __shfl_xor_sync(~0u, v[0], o));
+  return v[0];
 }
-__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+__device__ __forceinline__ float lse_of(float ref, float sum) {
+  return sum == 0.0f ? -INFINITY : (ref - X_SCALE + log2f(sum)) * 0.693147181f;
+}
 
 template <int R>
 struct Shared {
@@ -216,14 +271,15 @@ struct Shared {
   float qc[R], qr[R];           // the rows' factors of the two accumulators, log2 e included
   int sees[R];
   int64_t at[R];                // the rows' outputs
-  float red[4][R];
+  float red[4][R];              // of each 32 tokens
+  float ref[R], inv[R];
 };
 
-// The pieces of 16 weights x (FP16, two a word) as bytes of E5M2, the upper byte of an FP16 value: x1 + x2 / 8 + x3 / 64.
-__device__ __forceinline__ void pieces_of(const float (&x)[16], uint4 (&p)[3]) {
-  uint32_t* out[3] = {&p[0].x, &p[1].x, &p[2].x};
+// The pieces of N weights x (FP16, two a word) as bytes of E5M2, the upper byte of an FP16 value: x1 + x2 / 8 + x3 / 64.
+template <int N>
+__device__ __forceinline__ void pieces_of(const float (&x)[N], uint32_t (&p)[3][N / 4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < N / 4; ++i) {
     uint32_t w[3][2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -243,7 +299,7 @@ __device__ __forceinline__ void pieces_of(const float (&x)[16], uint4 (&p)[3]) {
       }
     }
 #pragma unroll
-    for (int n = 0; n < 3; ++n) out[n][i] = __byte_perm(w[n][0], w[n][1], 0x7531);
+    for (int n = 0; n < 3; ++n) p[n][i] = __byte_perm(w[n][0], w[n][1], 0x7531);
   }
 }
 
@@ -253,69 +309,79 @@ template <typename T, int R>
 __device__ __forceinline__ void ask(const Args& a, const Segment& s, uint8_t* smem, Shared<R>& sh) {
   using C = Config<T, R>;
   using E = typename T::half_type;
-  constexpr int PER = SOFTMAX / R, CHUNKS = MAX_DC / 8 / PER;     // threads of a row, eights of values that each holds
+  constexpr int PER = SOFTMAX / R;                // threads of a row
   const int row = threadIdx.x / PER, sub = threadIdx.x % PER, f = s.r0 + row, tok = f / a.heads;
   const bool live = row < s.rows;
   const E* q = static_cast<const E*>(a.q) + (s.q.row + tok) * a.qt + (f - tok * a.heads) * a.qh;
+  const int c_chunks = a.subs * 16;
+  constexpr int N = (MAX_DC + LD_R) / 8 / PER + (R == 16);        // 72 eights at most: 16 threads take 5 of them, 8 take 9
+  union { uint4 u; E e[8]; } v[N];
+  // (what is not there is loaded from the row's start and not used: branches would keep the loads apart)
+  const auto there = [&](int c) { return live && (c < c_chunks ? c * 8 < a.k.d_c : (c - c_chunks) * 8 < a.k.d_r); };
+  const auto from = [&](int c) { return !live ? static_cast<const E*>(a.q) : !there(c) ? q : c < c_chunks ? q + c * 8 : q + a.k.d_c + (c - c_chunks) * 8; };
+  if (a.wide) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i].u = *reinterpret_cast<const uint4*>(from(sub + i * PER));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const E* p = from(sub + i * PER);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i].e[e] = p[e];
+    }
+  }
+  float most[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = sub + i * PER;
+    if (!there(c)) v[i].u = make_uint4(0, 0, 0, 0);
+    float m = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = fabsf(to_f32(v[i].e[e]));
+      m = x < INFINITY ? fmaxf(m, x) : m;
+    }
+    if (c < c_chunks) most[0] = fmaxf(most[0], m);
+    else most[1] = fmaxf(most[1], m);
+  }
+  float inv[2];
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
-    const int d = part ? a.k.d_r : a.k.d_c, from = part ? a.k.d_c : 0, chunks = part ? LD_R / 8 : a.subs * 16;
-    constexpr int N = CHUNKS;
-    union { uint4 u; E e[8]; } v[N];
-    float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = sub + i * PER;
-      v[i].u = make_uint4(0, 0, 0, 0);
-      if (live && c * 8 < d) {
-        const E* p = q + from + c * 8;
-        if (a.wide) {
-          v[i].u = *reinterpret_cast<const uint4*>(p);
-        } else {
+    for (int o = PER / 2; o > 0; o >>= 1) most[part] = fmaxf(most[part], __shfl_xor_sync(~0u, most[part], o));
+    // the smallest power of two with the largest <= 448 of it
+    const uint32_t u = __float_as_uint(most[part]);
+    const int e2 = max((int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0), -120);
+    inv[part] = __uint_as_float((uint32_t)(127 - e2) << 23);
+    if (sub == 0) (part ? sh.qr : sh.qc)[row] = __uint_as_float((uint32_t)(e2 + 127) << 23) * (a.scale * 1.44269504f);
+  }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[i].e[e] = p[e];
-        }
-      }
+  for (int i = 0; i < N; ++i) {
+    const int c = sub + i * PER;
+    if (c >= c_chunks + LD_R / 8) break;
+    const float by = c < c_chunks ? inv[0] : inv[1];
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = to_f32(v[i].e[e]);
+      x[e] = fabsf(x[e]) < INFINITY ? x[e] * by : __int_as_float(0x7FC00000);
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int n = 0; n < C::PIECES; ++n) {
+      uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = fabsf(to_f32(v[i].e[e]));
-        amax = x < INFINITY ? fmaxf(amax, x) : amax;
-      }
-#pragma unroll
-    for (int o = PER / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
-    // the smallest power of two with amax <= 448 of it
-    const uint32_t u = __float_as_uint(amax);
-    const int e2 = max((int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0), -120);
-    const float up = __uint_as_float((uint32_t)(e2 + 127) << 23), inv = __uint_as_float((uint32_t)(127 - e2) << 23);
-    if (sub == 0) (part ? sh.qr : sh.qc)[row] = up * (a.scale * 1.44269504f);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = sub + i * PER;
-      if (c >= chunks) continue;
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = to_f32(v[i].e[e]);
-        x[e] = fabsf(x[e]) < INFINITY ? x[e] * inv : __int_as_float(0x7FC00000);
-      }
-#pragma unroll
-      for (int n = 0; n < C::PIECES; ++n) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = encode2(x[2 * e], x[2 * e + 1]);
+      for (int e = 0; e < 4; ++e) {
+        w[e] = encode2(x[2 * e], x[2 * e + 1]);
+        if (n + 1 < C::PIECES) {
           const float2 back = decode2((uint16_t)w[e]);
           x[2 * e] = (x[2 * e] - back.x) * 16.0f;
           x[2 * e + 1] = (x[2 * e + 1] - back.y) * 16.0f;
         }
-        const int at = n * R + row;     // the piece's row of the operand
-        uint8_t* to = part ? smem + C::QR + at * 64 + (((c >> 1) ^ (at >> 1 & 3)) << 4)
-                           : smem + C::QC + (c >> 4) * (C::NS * 128) + at * 128 + (((c >> 1 & 7) ^ (at & 7)) << 4);
-        *reinterpret_cast<uint2*>(to + (c & 1) * 8) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
       }
+      const int at = n * R + row, g = c < c_chunks ? c : c - c_chunks;     // the piece's row of the operand, its eight
+      uint8_t* to = c < c_chunks ? smem + C::QC + (g >> 4) * (C::NS * 128) + at * 128 + (((g >> 1 & 7) ^ (at & 7)) << 4)
+                                 : smem + C::QR + at * 64 + (((g >> 1) ^ (at >> 1 & 3)) << 4);
+      *reinterpret_cast<uint2*>(to + (g & 1) * 8) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
     }
   }
 }
@@ -338,16 +404,16 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.empty[i], 1);
       mbar_init(&sh.scored[i], 1);
-      mbar_init(&sh.taken[i], 4);
-      mbar_init(&sh.weighed[i], 4);
+      mbar_init(&sh.taken[i], SOFTMAX / 32);
+      mbar_init(&sh.weighed[i], SOFTMAX / 32);
       mbar_init(&sh.summed[i], 1);
     }
-    mbar_init(&sh.asked, 4);
+    mbar_init(&sh.asked, SOFTMAX / 32);
     mbar_init(&sh.drained, 1);
     sh.lost = 0;
     mk::fence_barrier_init();
   }
-  if (warp == 5) {
+  if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     fence_before();
@@ -357,25 +423,29 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   {
     const auto count = [&](int i) {
       const Seq q = sequence(a.b, i);
-      return groups_of<R>(a, q) * units_of(a, q);
+      return groups_of<R>(a, q) * (units_of(a, q) + FIXED);
     };
-    int64_t place;
-    const int64_t total = locate<THREADS>(a.b.n, 0, count, work.b, place);
-    const int64_t lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
-    __syncthreads();
-    locate<THREADS>(a.b.n, lo, count, work.b, place);
-    work.left = hi - lo;
+    int64_t place, total = 0;
+    locate<THREADS>(
+        a.b.n, count,
+        [&](int64_t all) {
+          total = all;
+          return begin_of(all, blockIdx.x, gridDim.x);
+        },
+        work.b, place);
+    const int64_t lo = begin_of(total, blockIdx.x, gridDim.x);
+    work.left = begin_of(total, blockIdx.x + 1, gridDim.x) - lo;
     const bool any = work.b < a.b.n;
     const Seq q = any ? sequence(a.b, work.b) : Seq{0, 0, 0};
     const int units = units_of(a, q);
-    work.g = any ? place / units : 0;
-    work.u = any ? (int)(place - work.g * units) : 0;
+    work.g = any ? quotient(place, units + FIXED) : 0;
+    work.at = any ? (int)(place - work.g * (units + FIXED)) : 0;
     if (threadIdx.x == 0) {
       Meta m{};
-      m.split = any && work.u > 0;
+      m.split = any && work.at > FIXED;
       m.row = q.row * a.heads + (int)(work.g * R);
       m.rows = any ? min(R, q.n * a.heads - (int)(work.g * R)) : 0;
-      m.lo = lo - work.u;
+      m.lo = lo - work.at + FIXED;
       m.hi = m.lo + units;
       m.total = total;
       a.meta[blockIdx.x] = m;
@@ -389,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   Segment s;
   int it = 0;                   // tiles so far
 
-  if (warp == 4) {
+  if (warp == 8) {
     // ---- loads: a tile's pages, and the scales of their tokens
     bool ok = true;
     while (ok && next<R>(a, work, s)) {
@@ -426,63 +496,86 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       }
     }
     for (int i = max(it - 2, 0); i < it; ++i) wait(&sh.full[i & 1], i >> 1);   // no copy outlives the block
-  } else if (warp == 5) {
-    // ---- products, issued by one thread
-    if (lane == 0) {
-      constexpr uint32_t ASK = instruction(0, false, C::NS), SUM = instruction(1, true, C::NO);
-      bool ok = true;
-      const auto sum = [&](int i, int n, bool first) {          // O of tile i, n of whose tokens count
-        const int st = i & 1;
-        ok = ok && wait(&sh.weighed[st], i >> 1);
-        if (!ok) return;
-        fence_after();
-        for (int j = 0; j < a.subs; ++j)
-          for (int kk = 0; kk < (n + 31) / 32; ++kk)
-            mma(tmem + C::O_COL + j * C::NO, descriptor(base + st * STAGE + j * SUB + kk * 4096, SUB, 1024, SWIZZLE_128),
-                descriptor(base + C::PB + st * C::NO * 128 + kk * 512, 128, 2048, SWIZZLE_NONE), SUM, !first || kk > 0);
-        commit(&sh.empty[st]);
-        commit(&sh.summed[st]);
-      };
-      int segments = 0;
-      while (ok && next<R>(a, work, s)) {
-        if (s.tiles == 0) continue;
-        ok = wait(&sh.asked, segments++);
-        int n = 0;
-        for (int t = 0; t < s.tiles && ok; ++t, ++it) {
-          const int st = it & 1, buf = it % C::BUFS;
-          ok = wait(&sh.full[st], it >> 1) && (it < C::BUFS || wait(&sh.taken[buf], it / C::BUFS - 1));
-          if (!ok) break;
-          fence_after();
-          const uint32_t d = tmem + buf * 2 * C::NS;
-          for (int j = 0; j < a.subs; ++j)
-            for (int kk = 0; kk < 4; ++kk)
-              mma(d, descriptor(base + st * STAGE + j * SUB + kk * 32, 16, 1024, SWIZZLE_128),
-                  descriptor(base + C::QC + j * C::NS * 128 + kk * 32, 16, 1024, SWIZZLE_128), ASK, j > 0 || kk > 0);
-          for (int kk = 0; kk < 2; ++kk)
-            mma(d + C::NS, descriptor(base + st * STAGE + 4 * SUB + kk * 32, 16, 512, SWIZZLE_64),
-                descriptor(base + C::QR + kk * 32, 16, 512, SWIZZLE_64), ASK, kk > 0);
-          commit(&sh.scored[buf]);
-          if (t > 0) sum(it - 1, n, t == 1);
-          n = min(TILE, s.end - (s.u0 * UNIT + t * TILE));
-        }
-        sum(it - 1, n, s.tiles == 1);
+  } else if (warp == 9) {
+    // ---- products
+    constexpr uint32_t ASK = instruction(0, false, C::NS), SUM = instruction(1, true, C::NO);
+    const uint32_t elected = elect_one();
+    const uint64_t latents = descriptor(base, SUB, 1024, SWIZZLE_128), rotary = descriptor(base + 4 * SUB, 16, 512, SWIZZLE_64);
+    const uint64_t q_c = descriptor(base + C::QC, 16, 1024, SWIZZLE_128), q_r = descriptor(base + C::QR, 16, 512, SWIZZLE_64);
+    const uint64_t weights = descriptor(base + C::PB, 128, 2048, SWIZZLE_NONE);
+    bool ok = true;
+    const auto reached = [](bool v) { return __all_sync(~0u, v) != 0; };
+    const auto sum = [&](int i, int n, bool first) {            // O of tile i, n of whose tokens count
+      const int st = i & 1;
+      ok = ok && reached(wait(&sh.weighed[st], i >> 1));
+      if (!ok) return;
+      fence_after();
+      const uint64_t v = latents + (st * STAGE >> 4), w = weights + (st * C::NO * 128 >> 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j >= a.subs) break;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          if (kk * 32 < n)
+            mma(tmem + C::O_COL + j * C::NO, v + ((j * SUB + kk * 4096) >> 4), w + (kk * 512 >> 4), SUM, kk > 0 || !first, elected);
       }
-      commit(&sh.drained);
-      wait(&sh.drained, 0);
+      commit(&sh.empty[st], elected);
+      commit(&sh.summed[st], elected);
+    };
+    int segments = 0;
+    while (ok && next<R>(a, work, s)) {
+      if (s.tiles == 0) continue;
+      ok = reached(wait(&sh.asked, segments++));
+      int n = 0;
+      bool owed = false;        // the last tile's sum is still to come
+      for (int t = 0; t < s.tiles && ok; ++t, ++it) {
+        const int st = it & 1, buf = it % C::BUFS;
+        // whichever comes first: this tile, or the last one's weights (whose sum makes room for the next tile)
+        const uint64_t begin = mk::globaltimer();
+        while (owed && ok && !reached(reached_yet(&sh.full[st], it >> 1))) {
+          if (reached(reached_yet(&sh.weighed[st ^ 1], (it - 1) >> 1))) {
+            sum(it - 1, n, t == 1);
+            owed = false;
+          } else {
+            ok = reached(mk::globaltimer() - begin <= TIMEOUT_NS);
+          }
+        }
+        ok = ok && reached(wait(&sh.full[st], it >> 1) && (it < C::BUFS || wait(&sh.taken[buf], it / C::BUFS - 1)));
+        if (!ok) break;
+        fence_after();
+        const uint32_t d = tmem + buf * 2 * C::NS;
+        const uint64_t c = latents + (st * STAGE >> 4), r = rotary + (st * STAGE >> 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j >= a.subs) break;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma(d, c + ((j * SUB + kk * 32) >> 4), q_c + ((j * C::NS * 128 + kk * 32) >> 4), ASK, j > 0 || kk > 0, elected);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) mma(d + C::NS, r + (kk * 32 >> 4), q_r + (kk * 32 >> 4), ASK, kk > 0, elected);
+        commit(&sh.scored[buf], elected);
+        if (owed) sum(it - 1, n, t == 1);
+        n = min(TILE, s.end - (s.u0 * UNIT + t * TILE));
+        owed = true;
+      }
+      if (owed) sum(it - 1, n, s.tiles == 1);
     }
+    commit(&sh.drained, elected);
+    wait(&sh.drained, 0);
   } else {
-    // ---- softmax: this thread's token of each tile, and its latent value of each 128
-    const int tid = threadIdx.x;
-    const uint32_t lanes = tmem + ((uint32_t)warp * 32 << 16);
+    // ---- softmax: this thread's token of each tile for half of the rows, and its latent value of each 128
+    constexpr int H = C::H;
+    const int tid = threadIdx.x, tok = tid % TILE, half = warp / 4;
+    const uint32_t lanes = tmem + ((uint32_t)(warp % 4) * 32 << 16) + half * H;
     bool dead = false;
     while (next<R>(a, work, s)) {
       softmax_sync();           // the last segment's factors are read
-      const int last_row = s.q.len - s.q.n + 1;
-      const int first_sees = min(max(last_row + s.r0 / a.heads, 0), a.b.capacity);
+      const int first_row = s.q.len - s.q.n + 1, first_sees = min(max(first_row + s.r0 / a.heads, 0), a.b.capacity);
       if (tid < R) {
-        const int f = s.r0 + tid, tok = f / a.heads;
-        sh.sees[tid] = tid < s.rows ? min(max(last_row + tok, 0), a.b.capacity) : INT32_MAX;
-        sh.at[tid] = (s.q.row + tok) * a.ot + (f - tok * a.heads) * a.oh;
+        const int f = s.r0 + tid, row = f / a.heads;
+        sh.sees[tid] = tid < s.rows ? min(max(first_row + row, 0), a.b.capacity) : INT32_MAX;
+        sh.at[tid] = (s.q.row + row) * a.ot + (f - row * a.heads) * a.oh;
       }
       if (s.tiles > 0 && !dead) {
         ask<T, R>(a, s, smem, sh);
@@ -490,28 +583,26 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       }
       softmax_sync();
       if (s.tiles > 0 && !dead && lane == 0) mbar_arrive(&sh.asked);
-      float ref[R], l[R];
+      float ref[H], l[H];
 #pragma unroll
-      for (int h = 0; h < R; ++h) {
+      for (int h = 0; h < H; ++h) {
         ref[h] = -FLT_MAX;
         l[h] = 0.0f;
       }
       for (int t = 0; t < s.tiles && !dead; ++t, ++it) {
-        const int st = it & 1, buf = it % C::BUFS, pos0 = s.u0 * UNIT + t * TILE, pos = pos0 + tid;
+        const int st = it & 1, buf = it % C::BUFS, pos0 = s.u0 * UNIT + t * TILE, pos = pos0 + tok;
         bool ok = wait(&sh.full[st], it >> 1) && wait(&sh.scored[buf], it / C::BUFS);
         fence_after();
-        const float4 g = sh.gran[st][tid >> 4];
+        const float4 g = sh.gran[st][tok >> 4];
         const bool none = pos >= s.end || g.w == 0.0f;
-        float v[R];
-        bool rises = false;
+        float v[H];
+        {
+          float sc[2 * C::PIECES][H];
 #pragma unroll
-        for (int c = 0; c < R / 16; ++c) {
-          float sc[2 * C::PIECES][16];
-#pragma unroll
-          for (int p = 0; p < 2 * C::PIECES; ++p) tmem_load(lanes + buf * 2 * C::NS + p * R + c * 16, sc[p]);
+          for (int p = 0; p < 2 * C::PIECES; ++p) tmem_load(lanes + buf * 2 * C::NS + p * R, sc[p]);
           tmem_wait_load(sc);
 #pragma unroll
-          for (int h = 0; h < 16; ++h) {
+          for (int h = 0; h < H; ++h) {
             float x = sc[1][h], y = sc[C::PIECES + 1][h];
             if (C::PIECES == 3) {
               x = fmaf(sc[2][h], 0.0625f, x);
@@ -519,7 +610,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
             }
             x = fmaf(x, 0.0625f, sc[0][h]) * g.x;
             y = fmaf(y, 0.0625f, sc[C::PIECES][h]) * g.y;
-            v[c * 16 + h] = fmaf(x, sh.qc[c * 16 + h], fmaf(y, sh.qr[c * 16 + h], g.z));
+            v[h] = fmaf(x, sh.qc[half * H + h], fmaf(y, sh.qr[half * H + h], g.z));
           }
         }
         fence_before();
@@ -527,14 +618,15 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         if (lane == 0) mbar_arrive(&sh.taken[buf]);
         if (none) {
 #pragma unroll
-          for (int h = 0; h < R; ++h) v[h] = -INFINITY;
+          for (int h = 0; h < H; ++h) v[h] = -INFINITY;
         } else if (pos >= first_sees) {
 #pragma unroll
-          for (int h = 0; h < R; ++h)
-            if (pos >= sh.sees[h]) v[h] = -INFINITY;
+          for (int h = 0; h < H; ++h)
+            if (pos >= sh.sees[half * H + h]) v[h] = -INFINITY;
         }
+        bool rises = false;
 #pragma unroll
-        for (int h = 0; h < R; ++h) rises |= v[h] > ref[h] + RAISE;
+        for (int h = 0; h < H; ++h) rises |= v[h] > ref[h] + RAISE;
         if (!ok) sh.lost = 1;
         rises = softmax_any(rises);
         if (sh.lost) {
@@ -542,62 +634,63 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
           break;
         }
         if (rises) {
+          float m[H], f[H];
 #pragma unroll
-          for (int h = 0; h < R; ++h) {
-            const uint32_t m = __reduce_max_sync(~0u, key_of(fmaxf(v[h], -INFINITY)));     // (a NaN is no largest value)
-            if (lane == h) sh.red[warp][h] = of_key(m);
-          }
+          for (int h = 0; h < H; ++h) m[h] = v[h];
+          // (a NaN is no largest value)
+          sh.red[warp % 4][half * H + lane % H] = across<H>(m, [](float x, float y) { return fmaxf(x, y); });
           softmax_sync();
-          float f[R];
 #pragma unroll
-          for (int h = 0; h < R; ++h) {
-            const float m = fmaxf(ref[h], fmaxf(fmaxf(sh.red[0][h], sh.red[1][h]), fmaxf(sh.red[2][h], sh.red[3][h])));
-            f[h] = exp2_fast(ref[h] - m);
+          for (int h = 0; h < H; ++h) {
+            const int row = half * H + h;
+            const float top = fmaxf(ref[h], fmaxf(fmaxf(sh.red[0][row], sh.red[1][row]), fmaxf(sh.red[2][row], sh.red[3][row])));
+            f[h] = exp2_fast(ref[h] - top);
             l[h] *= f[h];
-            ref[h] = m;
+            ref[h] = top;
           }
           if (t > 0) {
             ok = wait(&sh.summed[st ^ 1], (it - 1) >> 1);
             fence_after();
-            for (int j = 0; j < a.subs; ++j)
+            for (int j = 0; j < a.subs; ++j) {
+              float o[3][H];
 #pragma unroll
-              for (int c = 0; c < R / 16; ++c) {
-                float o[3][16];
+              for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R, o[p]);
+              tmem_wait_load(o);
 #pragma unroll
-                for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R + c * 16, o[p]);
-                tmem_wait_load(o);
+              for (int p = 0; p < 3; ++p) {
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {
-#pragma unroll
-                  for (int h = 0; h < 16; ++h) o[p][h] *= f[c * 16 + h];
-                  tmem_store(lanes + C::O_COL + j * C::NO + p * R + c * 16, o[p]);
-                }
+                for (int h = 0; h < H; ++h) o[p][h] *= f[h];
+                tmem_store(lanes + C::O_COL + j * C::NO + p * R, o[p]);
               }
+            }
             tmem_wait_store();
           }
         }
         if (it >= 2) ok = wait(&sh.summed[st], (it - 2) >> 1) && ok;    // its weights have been used
         if (!ok) sh.lost = 1;
-        uint8_t* w = smem + C::PB + st * C::NO * 128 + tid * 16;
+        {
+          float x[H];
+          uint32_t p[3][H / 4];
 #pragma unroll
-        for (int c = 0; c < R / 16; ++c) {
-          float x[16];
-          uint4 p[3];
-#pragma unroll
-          for (int h = 0; h < 16; ++h) {
-            x[h] = exp2_fast(v[c * 16 + h] - (ref[c * 16 + h] - X_SCALE));
-            l[c * 16 + h] = fmaf(x[h], g.w, l[c * 16 + h]);
+          for (int h = 0; h < H; ++h) {
+            x[h] = exp2_fast(v[h] - (ref[h] - X_SCALE));
+            l[h] = fmaf(x[h], g.w, l[h]);
           }
           pieces_of(x, p);
+          // rows of the operand in 16s: [3 R / 16][128 tokens][16]
+          uint8_t* w = smem + C::PB + st * C::NO * 128 + tok * 16;
 #pragma unroll
-          for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4*>(w + (i * (R / 16) + c) * 2048) = p[i];
+          for (int i = 0; i < 3; ++i) {
+            if constexpr (H == 8) *reinterpret_cast<uint2*>(w + i * 2048 + half * 8) = make_uint2(p[i][0], p[i][1]);
+            else *reinterpret_cast<uint4*>(w + (i * 2 + half) * 2048) = make_uint4(p[i][0], p[i][1], p[i][2], p[i][3]);
+          }
         }
         // 0 x NaN is NaN: what no row sees becomes zero, a NaN that only later rows see (their scores are NaN) too
-        if (none || pos >= first_sees) {
-          for (int j = 0; j < a.subs; ++j)
-#pragma unroll
+        if ((none && tok < ((s.end - pos0 + 31) & ~31)) || (!none && pos >= first_sees)) {
+          for (int j = half; j < a.subs; j += 2)
+#pragma unroll 1
             for (int i = 0; i < 8; ++i) {
-              uint4* at = reinterpret_cast<uint4*>(smem + st * STAGE + j * SUB + tid * 128 + i * 16);
+              uint4* at = reinterpret_cast<uint4*>(smem + st * STAGE + j * SUB + tok * 128 + i * 16);
               uint4 u = make_uint4(0, 0, 0, 0);
               if (!none) {
                 u = *at;
@@ -615,49 +708,54 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       // ---- the segment's end: whole groups are finished, others leave their sums
       if (s.tiles > 0 && !dead && !wait(&sh.summed[(it - 1) & 1], (it - 1) >> 1)) sh.lost = 1;
       fence_after();
+      sh.red[warp % 4][half * H + lane % H] = across<H>(l, [](float x, float y) { return x + y; });
+      if (tok == 0) {
 #pragma unroll
-      for (int h = 0; h < R; ++h) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l[h] += __shfl_xor_sync(~0u, l[h], o);
-        if (lane == h % 32) sh.red[warp][h] = l[h];
+        for (int h = 0; h < H; ++h) sh.ref[half * H + h] = ref[h];
       }
       softmax_sync();
       if (sh.lost) dead = true;
       const bool whole = s.u0 == 0 && s.u1 == s.units;
       const int64_t slot = (2 * (int64_t)blockIdx.x + (s.u0 == 0)) * R;
-      const float nan = __int_as_float(0x7FC00000);
-#pragma unroll
-      for (int h = 0; h < R; ++h) {
-        l[h] = dead ? nan : sh.red[0][h] + sh.red[1][h] + sh.red[2][h] + sh.red[3][h];
-        if (tid == h && h < s.rows) {
-          if (!whole) {
-            a.stat[(slot + h) * 2] = ref[h];
-            a.stat[(slot + h) * 2 + 1] = l[h];
-          } else if (a.lse) {
-            a.lse[(int64_t)s.q.row * a.heads + s.r0 + h] = l[h] == 0.0f ? -INFINITY : (ref[h] - X_SCALE + log2f(l[h])) * 0.693147181f;
-          }
+      if (tid < s.rows) {
+        const float sum = dead ? __int_as_float(0x7FC00000) : sh.red[0][tid] + sh.red[1][tid] + sh.red[2][tid] + sh.red[3][tid];
+        if (!whole) {
+          a.stat[(slot + tid) * 2] = sh.ref[tid];
+          a.stat[(slot + tid) * 2 + 1] = sum;
+        } else if (a.lse) {
+          a.lse[(int64_t)s.q.row * a.heads + s.r0 + tid] = lse_of(sh.ref[tid], sum);
         }
-        if (whole) l[h] = l[h] == 0.0f ? 0.0f : 1.0f / l[h];
+        sh.inv[tid] = sum == 0.0f ? 0.0f : 1.0f / sum;
       }
+      softmax_sync();
+      const int rows = s.rows - half * H;
+      E* out[H];
+      float inv[H];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        out[h] = static_cast<E*>(a.out) + sh.at[half * H + h] + tok;
+        inv[h] = sh.inv[half * H + h];
+      }
+      float* part = a.part + (slot + half * H) * (a.subs * 128) + tok;
       for (int j = 0; j < a.subs; ++j) {
-        const int dim = j * 128 + tid;
+        float o[3][H];
 #pragma unroll
-        for (int c = 0; c < R / 16; ++c) {
-          float o[3][16] = {};
-          if (s.tiles > 0) {
+        for (int h = 0; h < H; ++h) o[0][h] = o[1][h] = o[2][h] = 0.0f;
+        if (s.tiles > 0) {
 #pragma unroll
-            for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R + c * 16, o[p]);
-            tmem_wait_load(o);
-          }
+          for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R, o[p]);
+          tmem_wait_load(o);
+        }
 #pragma unroll
-          for (int h = 0; h < 16; ++h) {
-            const int row = c * 16 + h;
-            const float x = fmaf(fmaf(o[2][h], 0.125f, o[1][h]), 0.125f, o[0][h]);
-            if (row < s.rows) {
-              if (!whole) a.part[(slot + row) * (a.subs * 128) + dim] = x;
-              else if (dim < k.d_c) static_cast<E*>(a.out)[sh.at[row] + dim] = from_f32<E>(l[row] == 0.0f ? 0.0f : x * l[row]);
-            }
-          }
+        for (int h = 0; h < H; ++h) o[0][h] = fmaf(fmaf(o[2][h], 0.125f, o[1][h]), 0.125f, o[0][h]);
+        if (!whole) {
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+            if (h < rows) part[h * (a.subs * 128) + j * 128] = o[0][h];
+        } else if (j * 128 + tok < k.d_c) {
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+            if (h < rows) out[h][j * 128] = from_f32<E>(inv[h] == 0.0f ? 0.0f : o[0][h] * inv[h]);
         }
       }
       fence_before();
@@ -665,7 +763,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   }
   __syncwarp();
   __syncthreads();
-  if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 // One row of each group that several blocks' runs share, by the block whose run is the second of them: the partial sums
@@ -674,23 +772,16 @@ template <typename T, int R>
 __global__ void __launch_bounds__(128) merge_kernel(const Args a, int blocks) {
   using E = typename T::half_type;
   __shared__ float weight[MAX_CTAS];
-  __shared__ int slots[MAX_CTAS];
   __shared__ float top[4], all[4];
   const int i = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Meta m = a.meta[i];
   if (!m.split || row >= m.rows) return;
-  if (i == 0 || m.total * (i - 1) / blocks > m.lo) return;             // an earlier block's run splits it too
-  // the runs that hold some of it: with fewer units than blocks one for each unit, otherwise i - 1, i, ...
-  const auto holds = [&](int64_t unit) { return (int)(((unit + 1) * blocks - 1) / m.total); };
-  const int n = m.total < blocks ? (int)(m.hi - m.lo) : holds(m.hi - 1) - i + 2;
-  for (int p = tid; p < n; p += 128) {
-    const int b = m.total < blocks ? holds(m.lo + p) : i - 1 + p;
-    slots[p] = 2 * b + (p == 0);        // the first part begins it, the others continue it
-  }
-  __syncthreads();
+  if (i == 0 || begin_of(m.total, i - 1, blocks) > m.lo) return;        // an earlier block's run splits it too
+  const int n = holder_of(m.total, m.hi - 1, blocks) - i + 2;           // the runs i - 1, i, ... hold some of it
+  const auto slot = [&](int p) { return ((int64_t)2 * (i - 1 + p) + (p == 0)) * R + row; };      // (the first part begins it)
   float ref = -FLT_MAX;
-  for (int p = tid; p < n; p += 128) ref = fmaxf(ref, a.stat[((int64_t)slots[p] * R + row) * 2]);
+  for (int p = tid; p < n; p += 128) ref = fmaxf(ref, a.stat[slot(p) * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(~0u, ref, o));
   if (tid % 32 == 0) top[tid / 32] = ref;
@@ -698,7 +789,7 @@ __global__ void __launch_bounds__(128) merge_kernel(const Args a, int blocks) {
   ref = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   float l = 0.0f;
   for (int p = tid; p < n; p += 128) {
-    const float* st = a.stat + ((int64_t)slots[p] * R + row) * 2;
+    const float* st = a.stat + slot(p) * 2;
     weight[p] = exp2_fast(st[0] - ref);
     l += weight[p] * st[1];
   }
@@ -708,14 +799,14 @@ __global__ void __launch_bounds__(128) merge_kernel(const Args a, int blocks) {
   __syncthreads();
   l = all[0] + all[1] + all[2] + all[3];
   const int f = m.row + row, tok = f / a.heads;
-  if (a.lse && tid == 0) a.lse[f] = l == 0.0f ? -INFINITY : (ref - X_SCALE + log2f(l)) * 0.693147181f;
+  if (a.lse && tid == 0) a.lse[f] = lse_of(ref, l);
   E* out = static_cast<E*>(a.out) + tok * a.ot + (f - tok * a.heads) * a.oh;
   const int ld = a.subs * 128, dim = tid * 4;
   if (dim >= ld) return;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
   for (int p = 0; p < n; ++p) {
-    const float4 v = *reinterpret_cast<const float4*>(a.part + ((int64_t)slots[p] * R + row) * ld + dim);
+    const float4 v = *reinterpret_cast<const float4*>(a.part + slot(p) * ld + dim);
     const float w = weight[p];
     o.x = fmaf(w, v.x, o.x);
     o.y = fmaf(w, v.y, o.y);
