@@ -22,7 +22,8 @@
 // The work is units of 64 tokens of a group of R rows (a row is a token's head) of a sequence; each block (one per SM)
 // takes an equal run of all units, whatever the lengths, as tiles of two. A group within one run is finished there, one
 // that several runs share leaves partial sums, which merge_kernel joins. Warps 0 to 7 are the softmax: a warp holds 32 of a
-// tile's 128 tokens (the lanes of tensor memory that it may read) for half of the rows. Warp 8 loads, warp 9 issues the products.
+// tile's 128 tokens (the lanes of tensor memory that it may read) for half of the rows. Warp 8 loads, warp 9 issues the scores' products and
+// warp 10 the sums': each only ever waits for what comes next.
 #include <cuda.h>
 
 #include <atomic>
@@ -40,7 +41,7 @@ using mk::mbar_init;
 using mk::mbar_try_wait;
 using mk::smem_u32;
 
-constexpr int MAX_CTAS = 148, TILE = 128, UNIT = 64, THREADS = 320, SOFTMAX = 256;
+constexpr int MAX_CTAS = 148, TILE = 128, UNIT = 64, THREADS = 352, SOFTMAX = 256;
 constexpr int SUB = TILE * 128, STAGE = 4 * SUB + TILE * LD_R;      // a tile: up to 4 x [128 tokens][128 B], then [128][64 B]
 constexpr uint64_t TIMEOUT_NS = 2000000000ull;
 constexpr float X_SCALE = 7.0f, RAISE = 8.0f;                       // x = 2^7 at ref, 2^15 at most
@@ -207,7 +208,7 @@ __device__ __forceinline__ void tmem_wait_load(float (&v)[N][M]) {
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ bool reached_yet(uint64_t* bar, uint32_t parity) {      // (mbarrier.try_wait may wait a while itself)
+__device__ __forceinline__ bool come(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -216,14 +217,16 @@ __device__ __forceinline__ bool reached_yet(uint64_t* bar, uint32_t parity) {   
       : "memory");
   return ok != 0;
 }
-// A wait with a limit: false where it ran out.
+// A warp's wait with a limit: false where it ran out.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-  for (int i = 0; i < 64; ++i)
-    if (mbar_try_wait(bar, parity & 1)) return true;
-  const uint64_t begin = mk::globaltimer();
-  while (!mbar_try_wait(bar, parity & 1))
-    if (mk::globaltimer() - begin > TIMEOUT_NS) return false;
-  return true;
+  bool ok = come(bar, parity);
+  if (!ok) {
+    const uint64_t begin = mk::globaltimer();
+#pragma unroll 1
+    do ok = come(bar, parity);
+    while (!ok && mk::globaltimer() - begin <= TIMEOUT_NS);
+  }
+  return __all_sync(~0u, ok);
 }
 
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -264,13 +267,14 @@ __device__ __forceinline__ float lse_of(float ref, float sum) {
 
 template <int R>
 struct Shared {
-  uint64_t full[2], empty[2], scored[2], taken[2], weighed[2], summed[2], asked, drained;
+  uint64_t full[2], empty[2], scored[2], taken[2], weighed[2], summed[2], asked, drained[2];
   uint32_t tmem;
   volatile int lost;            // a softmax thread's wait ran out
   float4 gran[2][TILE / 16];    // of each 16 tokens: sc, sr, log2 sc, 1 / sc (0: no such page)
-  float qc[R], qr[R];           // the rows' factors of the two accumulators, log2 e included
-  int sees[R];
-  int64_t at[R];                // the rows' outputs
+  // of this segment and the next:
+  float qc[2][R], qr[2][R];     // the rows' factors of the two accumulators, log2 e included
+  int sees[2][R];               // the tokens that they see
+  int64_t at[2][R];             // their outputs
   float red[4][R];              // of each 32 tokens
   float ref[R], inv[R];
 };
@@ -306,7 +310,7 @@ __device__ __forceinline__ void pieces_of(const float (&x)[N], uint32_t (&p)[3][
 // A segment's queries: each row's scales, and its values' pieces in the order that the products read (K-major, swizzled as
 // TMA does it), zeros behind its values and in absent rows. What is not finite becomes NaN.
 template <typename T, int R>
-__device__ __forceinline__ void ask(const Args& a, const Segment& s, uint8_t* smem, Shared<R>& sh) {
+__device__ __forceinline__ void ask(const Args& a, const Segment& s, uint8_t* smem, Shared<R>& sh, int set) {
   using C = Config<T, R>;
   using E = typename T::half_type;
   constexpr int PER = SOFTMAX / R;                // threads of a row
@@ -353,7 +357,7 @@ __device__ __forceinline__ void ask(const Args& a, const Segment& s, uint8_t* sm
     const uint32_t u = __float_as_uint(most[part]);
     const int e2 = max((int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0), -120);
     inv[part] = __uint_as_float((uint32_t)(127 - e2) << 23);
-    if (sub == 0) (part ? sh.qr : sh.qc)[row] = __uint_as_float((uint32_t)(e2 + 127) << 23) * (a.scale * 1.44269504f);
+    if (sub == 0) (part ? sh.qr : sh.qc)[set][row] = __uint_as_float((uint32_t)(e2 + 127) << 23) * (a.scale * 1.44269504f);
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -403,13 +407,13 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.empty[i], 1);
+      mbar_init(&sh.drained[i], 1);
       mbar_init(&sh.scored[i], 1);
       mbar_init(&sh.taken[i], SOFTMAX / 32);
       mbar_init(&sh.weighed[i], SOFTMAX / 32);
       mbar_init(&sh.summed[i], 1);
     }
     mbar_init(&sh.asked, SOFTMAX / 32);
-    mbar_init(&sh.drained, 1);
     sh.lost = 0;
     mk::fence_barrier_init();
   }
@@ -462,6 +466,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   if (warp == 8) {
     // ---- loads: a tile's pages, and the scales of their tokens
     bool ok = true;
+    const int cols = a.subs + 1, each = a.box / 16;             // a box's first 16 tokens name its page
     while (ok && next<R>(a, work, s)) {
       for (int t = 0; t < s.tiles; ++t, ++it) {
         const int st = it & 1, pos0 = s.u0 * UNIT + t * TILE, pos = pos0 + 16 * lane;
@@ -479,72 +484,44 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
             page = -1;
           }
         }
-        if (it >= 2) ok = __all_sync(~0u, wait(&sh.empty[st], (it - 2) >> 1));
-        if (!ok) break;
+        const int rows = __popc(__ballot_sync(~0u, page >= 0 && lane % each == 0)) * a.box;
+        const int y = (page << k.shift) + (pos & (k.page - 1));
+        if (it >= 2 && !(ok = wait(&sh.empty[st], (it - 2) >> 1))) break;
         if (lane < TILE / 16) sh.gran[st][lane] = g;
-        const int each = a.box / 16;                            // a box's first 16 tokens name its page
-        const bool loads = page >= 0 && lane % each == 0;
-        const int boxes = __popc(__ballot_sync(~0u, loads));
-        if (lane == 0) mbar_arrive_expect_tx(&sh.full[st], boxes * a.box * (a.subs * 128 + LD_R));
         __syncwarp();
-        if (loads) {
-          const int y = (page << k.shift) + (pos & (k.page - 1));
-          uint8_t* to = smem + st * STAGE + lane * 16 * 128;
-          for (int j = 0; j < a.subs; ++j) mk::tma_load_2d(to + j * SUB, &map_c, j * 128, y, &sh.full[st]);
-          mk::tma_load_2d(smem + st * STAGE + 4 * SUB + lane * 16 * LD_R, &map_r, 0, y, &sh.full[st]);
+        if (lane == 0) mbar_arrive_expect_tx(&sh.full[st], rows * (a.subs * 128 + LD_R));
+        // a lane's box and column (the last one: the rotary keys)
+        for (int i = lane; i < (TILE / a.box * cols + 31) / 32 * 32; i += 32) {
+          const int box = i / cols, col = i - box * cols, from = box * each;
+          const int at = __shfl_sync(~0u, y, from & 31), named = __shfl_sync(~0u, page, from & 31);
+          if (box < TILE / a.box && named >= 0) {
+            if (col == a.subs) mk::tma_load_2d(smem + st * STAGE + 4 * SUB + from * 16 * LD_R, &map_r, 0, at, &sh.full[st]);
+            else mk::tma_load_2d(smem + st * STAGE + col * SUB + from * 16 * 128, &map_c, col * 128, at, &sh.full[st]);
+          }
         }
       }
     }
-    for (int i = max(it - 2, 0); i < it; ++i) wait(&sh.full[i & 1], i >> 1);   // no copy outlives the block
+    for (int i = max(it - 2, 0); i < it; ++i) wait(&sh.full[i & 1], i >> 1);       // no copy outlives the block
   } else if (warp == 9) {
-    // ---- products
-    constexpr uint32_t ASK = instruction(0, false, C::NS), SUM = instruction(1, true, C::NO);
+    // ---- scores
+    constexpr uint32_t ASK = instruction(0, false, C::NS);
     const uint32_t elected = elect_one();
-    const uint64_t latents = descriptor(base, SUB, 1024, SWIZZLE_128), rotary = descriptor(base + 4 * SUB, 16, 512, SWIZZLE_64);
+    const uint64_t latents = descriptor(base, 16, 1024, SWIZZLE_128), rotary = descriptor(base + 4 * SUB, 16, 512, SWIZZLE_64);
     const uint64_t q_c = descriptor(base + C::QC, 16, 1024, SWIZZLE_128), q_r = descriptor(base + C::QR, 16, 512, SWIZZLE_64);
-    const uint64_t weights = descriptor(base + C::PB, 128, 2048, SWIZZLE_NONE);
     bool ok = true;
-    const auto reached = [](bool v) { return __all_sync(~0u, v) != 0; };
-    const auto sum = [&](int i, int n, bool first) {            // O of tile i, n of whose tokens count
-      const int st = i & 1;
-      ok = ok && reached(wait(&sh.weighed[st], i >> 1));
-      if (!ok) return;
-      fence_after();
-      const uint64_t v = latents + (st * STAGE >> 4), w = weights + (st * C::NO * 128 >> 4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j >= a.subs) break;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          if (kk * 32 < n)
-            mma(tmem + C::O_COL + j * C::NO, v + ((j * SUB + kk * 4096) >> 4), w + (kk * 512 >> 4), SUM, kk > 0 || !first, elected);
-      }
-      commit(&sh.empty[st], elected);
-      commit(&sh.summed[st], elected);
-    };
     int segments = 0;
     while (ok && next<R>(a, work, s)) {
       if (s.tiles == 0) continue;
-      ok = reached(wait(&sh.asked, segments++));
-      int n = 0;
-      bool owed = false;        // the last tile's sum is still to come
+      ok = wait(&sh.asked, segments++);
       for (int t = 0; t < s.tiles && ok; ++t, ++it) {
         const int st = it & 1, buf = it % C::BUFS;
-        // whichever comes first: this tile, or the last one's weights (whose sum makes room for the next tile)
-        const uint64_t begin = mk::globaltimer();
-        while (owed && ok && !reached(reached_yet(&sh.full[st], it >> 1))) {
-          if (reached(reached_yet(&sh.weighed[st ^ 1], (it - 1) >> 1))) {
-            sum(it - 1, n, t == 1);
-            owed = false;
-          } else {
-            ok = reached(mk::globaltimer() - begin <= TIMEOUT_NS);
-          }
-        }
-        ok = ok && reached(wait(&sh.full[st], it >> 1) && (it < C::BUFS || wait(&sh.taken[buf], it / C::BUFS - 1)));
+        ok = (it < C::BUFS || wait(&sh.taken[buf], it / C::BUFS - 1)) && wait(&sh.full[st], it >> 1);
         if (!ok) break;
         fence_after();
         const uint32_t d = tmem + buf * 2 * C::NS;
         const uint64_t c = latents + (st * STAGE >> 4), r = rotary + (st * STAGE >> 4);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) mma(d + C::NS, r + (kk * 32 >> 4), q_r + (kk * 32 >> 4), ASK, kk > 0, elected);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (j >= a.subs) break;
@@ -552,48 +529,138 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
           for (int kk = 0; kk < 4; ++kk)
             mma(d, c + ((j * SUB + kk * 32) >> 4), q_c + ((j * C::NS * 128 + kk * 32) >> 4), ASK, j > 0 || kk > 0, elected);
         }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) mma(d + C::NS, r + (kk * 32 >> 4), q_r + (kk * 32 >> 4), ASK, kk > 0, elected);
         commit(&sh.scored[buf], elected);
-        if (owed) sum(it - 1, n, t == 1);
-        n = min(TILE, s.end - (s.u0 * UNIT + t * TILE));
-        owed = true;
       }
-      if (owed) sum(it - 1, n, s.tiles == 1);
     }
-    commit(&sh.drained, elected);
-    wait(&sh.drained, 0);
+    commit(&sh.drained[0], elected);
+    wait(&sh.drained[0], 0);
+  } else if (warp == 10) {
+    // ---- sums (a tile's weights come after its scores, so its stage is free once they are used)
+    constexpr uint32_t SUM = instruction(1, true, C::NO);
+    const uint32_t elected = elect_one();
+    const uint64_t latents = descriptor(base, SUB, 1024, SWIZZLE_128), weights = descriptor(base + C::PB, 128, 2048, SWIZZLE_NONE);
+    bool ok = true;
+    while (ok && next<R>(a, work, s)) {
+      for (int t = 0; t < s.tiles; ++t, ++it) {
+        const int st = it & 1, n = s.end - (s.u0 * UNIT + t * TILE);       // tokens that count
+        if (!(ok = wait(&sh.weighed[st], it >> 1))) break;
+        fence_after();
+        const uint64_t v = latents + (st * STAGE >> 4), w = weights + (st * C::NO * 128 >> 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j >= a.subs) break;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            if (kk * 32 < n)
+              mma(tmem + C::O_COL + j * C::NO, v + ((j * SUB + kk * 4096) >> 4), w + (kk * 512 >> 4), SUM, kk > 0 || t > 0, elected);
+        }
+        commit(&sh.empty[st], elected);
+        commit(&sh.summed[st], elected);
+      }
+    }
+    commit(&sh.drained[1], elected);
+    wait(&sh.drained[1], 0);
   } else {
     // ---- softmax: this thread's token of each tile for half of the rows, and its latent value of each 128
     constexpr int H = C::H;
     const int tid = threadIdx.x, tok = tid % TILE, half = warp / 4;
     const uint32_t lanes = tmem + ((uint32_t)(warp % 4) * 32 << 16) + half * H;
     bool dead = false;
-    while (next<R>(a, work, s)) {
-      softmax_sync();           // the last segment's factors are read
-      const int first_row = s.q.len - s.q.n + 1, first_sees = min(max(first_row + s.r0 / a.heads, 0), a.b.capacity);
+    const auto prepare = [&](const Segment& s, int set) {
+      softmax_sync();           // what was in this set has been read
       if (tid < R) {
         const int f = s.r0 + tid, row = f / a.heads;
-        sh.sees[tid] = tid < s.rows ? min(max(first_row + row, 0), a.b.capacity) : INT32_MAX;
-        sh.at[tid] = (s.q.row + row) * a.ot + (f - row * a.heads) * a.oh;
+        sh.sees[set][tid] = tid < s.rows ? min(max(s.q.len - s.q.n + 1 + row, 0), a.b.capacity) : INT32_MAX;
+        sh.at[set][tid] = (s.q.row + row) * a.ot + (f - row * a.heads) * a.oh;
       }
       if (s.tiles > 0 && !dead) {
-        ask<T, R>(a, s, smem, sh);
+        ask<T, R>(a, s, smem, sh, set);
         mk::fence_proxy_async_smem();
       }
       softmax_sync();
       if (s.tiles > 0 && !dead && lane == 0) mbar_arrive(&sh.asked);
-      float ref[H], l[H];
+    };
+    float ref[H], l[H];
+    Segment ahead;
+    bool begun = false;
+    for (int set = 0;; set ^= 1) {
+      // a segment's queries are prepared while its predecessor's last sum runs
+      const bool more = next<R>(a, work, ahead);
+      if (more) prepare(ahead, set);
+      if (begun) {
+        // ---- the segment's end: whole groups are finished, others leave their sums
+        if (s.tiles > 0 && !dead && !wait(&sh.summed[(it - 1) & 1], (it - 1) >> 1)) sh.lost = 1;
+        fence_after();
+        sh.red[warp % 4][half * H + lane % H] = across<H>(l, [](float x, float y) { return x + y; });
+        if (tok == 0) {
+#pragma unroll
+          for (int h = 0; h < H; ++h) sh.ref[half * H + h] = ref[h];
+        }
+        softmax_sync();
+        if (sh.lost) dead = true;
+        const bool whole = s.u0 == 0 && s.u1 == s.units;
+        const int64_t slot = (2 * (int64_t)blockIdx.x + (s.u0 == 0)) * R;
+        if (tid < s.rows) {
+          const float sum = dead ? __int_as_float(0x7FC00000) : sh.red[0][tid] + sh.red[1][tid] + sh.red[2][tid] + sh.red[3][tid];
+          if (!whole) {
+            a.stat[(slot + tid) * 2] = sh.ref[tid];
+            a.stat[(slot + tid) * 2 + 1] = sum;
+          } else if (a.lse) {
+            a.lse[(int64_t)s.q.row * a.heads + s.r0 + tid] = lse_of(sh.ref[tid], sum);
+          }
+          sh.inv[tid] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        }
+        softmax_sync();
+        const int rows = s.rows - half * H;
+        E* out[H];
+        float inv[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          out[h] = static_cast<E*>(a.out) + sh.at[set ^ 1][half * H + h] + tok;
+          inv[h] = sh.inv[half * H + h];
+        }
+        float* part = a.part + (slot + half * H) * (a.subs * 128) + tok;
+        for (int j = 0; j < a.subs; ++j) {
+          float o[3][H];
+#pragma unroll
+          for (int h = 0; h < H; ++h) o[0][h] = o[1][h] = o[2][h] = 0.0f;
+          if (s.tiles > 0) {
+#pragma unroll
+            for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R, o[p]);
+            tmem_wait_load(o);
+          }
+#pragma unroll
+          for (int h = 0; h < H; ++h) o[0][h] = fmaf(fmaf(o[2][h], 0.125f, o[1][h]), 0.125f, o[0][h]);
+          if (!whole) {
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+              if (h < rows) part[h * (a.subs * 128) + j * 128] = o[0][h];
+          } else if (j * 128 + tok < k.d_c) {
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+              if (h < rows) out[h][j * 128] = from_f32<E>(inv[h] == 0.0f ? 0.0f : o[0][h] * inv[h]);
+          }
+        }
+        fence_before();
+      }
+      if (!more) break;
+      s = ahead;
+      begun = true;
+      const int first_sees = min(max(s.q.len - s.q.n + 1 + s.r0 / a.heads, 0), a.b.capacity);
+      float qc[H], qr[H];
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         ref[h] = -FLT_MAX;
         l[h] = 0.0f;
+        qc[h] = sh.qc[set][half * H + h];
+        qr[h] = sh.qr[set][half * H + h];
       }
       for (int t = 0; t < s.tiles && !dead; ++t, ++it) {
         const int st = it & 1, buf = it % C::BUFS, pos0 = s.u0 * UNIT + t * TILE, pos = pos0 + tok;
-        bool ok = wait(&sh.full[st], it >> 1) && wait(&sh.scored[buf], it / C::BUFS);
-        fence_after();
+        bool ok = wait(&sh.full[st], it >> 1);
         const float4 g = sh.gran[st][tok >> 4];
+        ok = wait(&sh.scored[buf], it / C::BUFS) && ok;
+        fence_after();
         const bool none = pos >= s.end || g.w == 0.0f;
         float v[H];
         {
@@ -610,7 +677,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
             }
             x = fmaf(x, 0.0625f, sc[0][h]) * g.x;
             y = fmaf(y, 0.0625f, sc[C::PIECES][h]) * g.y;
-            v[h] = fmaf(x, sh.qc[half * H + h], fmaf(y, sh.qr[half * H + h], g.z));
+            v[h] = fmaf(x, qc[h], fmaf(y, qr[h], g.z));
           }
         }
         fence_before();
@@ -622,18 +689,17 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         } else if (pos >= first_sees) {
 #pragma unroll
           for (int h = 0; h < H; ++h)
-            if (pos >= sh.sees[half * H + h]) v[h] = -INFINITY;
+            if (pos >= sh.sees[set][half * H + h]) v[h] = -INFINITY;
         }
         bool rises = false;
 #pragma unroll
         for (int h = 0; h < H; ++h) rises |= v[h] > ref[h] + RAISE;
         if (!ok) sh.lost = 1;
-        rises = softmax_any(rises);
-        if (sh.lost) {
-          dead = true;
-          break;
-        }
-        if (rises) {
+        if (softmax_any(rises || !ok)) {
+          if (sh.lost) {
+            dead = true;
+            break;
+          }
           float m[H], f[H];
 #pragma unroll
           for (int h = 0; h < H; ++h) m[h] = v[h];
@@ -649,7 +715,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
             ref[h] = top;
           }
           if (t > 0) {
-            ok = wait(&sh.summed[st ^ 1], (it - 1) >> 1);
+            if (!wait(&sh.summed[st ^ 1], (it - 1) >> 1)) sh.lost = 1;
             fence_after();
             for (int j = 0; j < a.subs; ++j) {
               float o[3][H];
@@ -666,9 +732,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
             tmem_wait_store();
           }
         }
-        if (it >= 2) ok = wait(&sh.summed[st], (it - 2) >> 1) && ok;    // its weights have been used
-        if (!ok) sh.lost = 1;
         {
+          // (this stage's tile before has been summed, so its weights' place is free too)
           float x[H];
           uint32_t p[3][H / 4];
 #pragma unroll
@@ -705,60 +770,6 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.weighed[st]);
       }
-      // ---- the segment's end: whole groups are finished, others leave their sums
-      if (s.tiles > 0 && !dead && !wait(&sh.summed[(it - 1) & 1], (it - 1) >> 1)) sh.lost = 1;
-      fence_after();
-      sh.red[warp % 4][half * H + lane % H] = across<H>(l, [](float x, float y) { return x + y; });
-      if (tok == 0) {
-#pragma unroll
-        for (int h = 0; h < H; ++h) sh.ref[half * H + h] = ref[h];
-      }
-      softmax_sync();
-      if (sh.lost) dead = true;
-      const bool whole = s.u0 == 0 && s.u1 == s.units;
-      const int64_t slot = (2 * (int64_t)blockIdx.x + (s.u0 == 0)) * R;
-      if (tid < s.rows) {
-        const float sum = dead ? __int_as_float(0x7FC00000) : sh.red[0][tid] + sh.red[1][tid] + sh.red[2][tid] + sh.red[3][tid];
-        if (!whole) {
-          a.stat[(slot + tid) * 2] = sh.ref[tid];
-          a.stat[(slot + tid) * 2 + 1] = sum;
-        } else if (a.lse) {
-          a.lse[(int64_t)s.q.row * a.heads + s.r0 + tid] = lse_of(sh.ref[tid], sum);
-        }
-        sh.inv[tid] = sum == 0.0f ? 0.0f : 1.0f / sum;
-      }
-      softmax_sync();
-      const int rows = s.rows - half * H;
-      E* out[H];
-      float inv[H];
-#pragma unroll
-      for (int h = 0; h < H; ++h) {
-        out[h] = static_cast<E*>(a.out) + sh.at[half * H + h] + tok;
-        inv[h] = sh.inv[half * H + h];
-      }
-      float* part = a.part + (slot + half * H) * (a.subs * 128) + tok;
-      for (int j = 0; j < a.subs; ++j) {
-        float o[3][H];
-#pragma unroll
-        for (int h = 0; h < H; ++h) o[0][h] = o[1][h] = o[2][h] = 0.0f;
-        if (s.tiles > 0) {
-#pragma unroll
-          for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R, o[p]);
-          tmem_wait_load(o);
-        }
-#pragma unroll
-        for (int h = 0; h < H; ++h) o[0][h] = fmaf(fmaf(o[2][h], 0.125f, o[1][h]), 0.125f, o[0][h]);
-        if (!whole) {
-#pragma unroll
-          for (int h = 0; h < H; ++h)
-            if (h < rows) part[h * (a.subs * 128) + j * 128] = o[0][h];
-        } else if (j * 128 + tok < k.d_c) {
-#pragma unroll
-          for (int h = 0; h < H; ++h)
-            if (h < rows) out[h][j * 128] = from_f32<E>(inv[h] == 0.0f ? 0.0f : o[0][h] * inv[h]);
-        }
-      }
-      fence_before();
     }
   }
   __syncwarp();
