@@ -170,6 +170,14 @@ __device__ __forceinline__ void commit(uint64_t* bar, uint32_t elected) {
       "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(elected)
       : "memory");
 }
+// a box of a tensor map, brought by the elected lane (`issues`)
+__device__ __forceinline__ void copy(uint32_t to, const CUtensorMap* map, int x, int y, uint32_t bar, uint32_t issues) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(to), "l"(map),
+      "r"(x), "r"(y), "r"(bar), "r"(issues)
+      : "memory");
+}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // 8 or 16 columns of this warp's 32 lanes
@@ -466,7 +474,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   if (warp == 8) {
     // ---- loads: a tile's pages, and the scales of their tokens
     bool ok = true;
-    const int cols = a.subs + 1, each = a.box / 16;             // a box's first 16 tokens name its page
+    const int each = a.box / 16;                                // a box's first 16 tokens name its page
+    const uint32_t elected = elect_one();
     while (ok && next<R>(a, work, s)) {
       for (int t = 0; t < s.tiles; ++t, ++it) {
         const int st = it & 1, pos0 = s.u0 * UNIT + t * TILE, pos = pos0 + 16 * lane;
@@ -490,14 +499,15 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         if (lane < TILE / 16) sh.gran[st][lane] = g;
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(&sh.full[st], rows * (a.subs * 128 + LD_R));
-        // a lane's box and column (the last one: the rotary keys)
-        for (int i = lane; i < (TILE / a.box * cols + 31) / 32 * 32; i += 32) {
-          const int box = i / cols, col = i - box * cols, from = box * each;
-          const int at = __shfl_sync(~0u, y, from & 31), named = __shfl_sync(~0u, page, from & 31);
-          if (box < TILE / a.box && named >= 0) {
-            if (col == a.subs) mk::tma_load_2d(smem + st * STAGE + 4 * SUB + from * 16 * LD_R, &map_r, 0, at, &sh.full[st]);
-            else mk::tma_load_2d(smem + st * STAGE + col * SUB + from * 16 * 128, &map_c, col * 128, at, &sh.full[st]);
-          }
+        const uint32_t to = base + st * STAGE, full = smem_u32(&sh.full[st]);
+#pragma unroll 1
+        for (int from = 0; from < TILE / 16; from += each) {
+          const int at = __shfl_sync(~0u, y, from), named = __shfl_sync(~0u, page, from);
+          const uint32_t issues = elected != 0 && named >= 0;
+          copy(to + 4 * SUB + from * 16 * LD_R, &map_r, 0, at, full, issues);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            copy(to + j * SUB + from * 16 * 128, &map_c, j * 128, at, full, issues && j < a.subs);
         }
       }
     }
@@ -551,8 +561,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
           if (j >= a.subs) break;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            if (kk * 32 < n)
-              mma(tmem + C::O_COL + j * C::NO, v + ((j * SUB + kk * 4096) >> 4), w + (kk * 512 >> 4), SUM, kk > 0 || t > 0, elected);
+            mma(tmem + C::O_COL + j * C::NO, v + ((j * SUB + kk * 4096) >> 4), w + (kk * 512 >> 4), SUM, kk > 0 || t > 0, elected && kk * 32 < n);
         }
         commit(&sh.empty[st], elected);
         commit(&sh.summed[st], elected);
