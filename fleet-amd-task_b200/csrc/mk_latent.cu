@@ -75,14 +75,14 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Write a) {
   __shared__ float most[2][THREADS / 32];
   const Cache& k = a.k;
   int s = blockIdx.x, first;
-  int64_t nth = 0;
+  int nth = 0;
   if (a.b.starts)
     locate<THREADS>(a.b.n, [&](int i) { int f; return pages_of(k, a.b, sequence(a.b, i), f); },
-                    [](int64_t) { return (int64_t)blockIdx.x; }, s, nth);
+                    [](int) { return (int)blockIdx.x; }, s, nth);
   if (s >= a.b.n) return;
   const Seq q = sequence(a.b, s);
   if (nth >= pages_of(k, a.b, q, first)) return;
-  const int j = first + (int)nth;
+  const int j = first + nth;
   const int p = a.b.table[s * a.b.ldt + j];
   if (p < 0 || p >= k.pages) return;
   // the page's new tokens [lo, hi), offsets in the page; its first new token is row `row`

@@ -77,43 +77,40 @@ __device__ __forceinline__ uint16_t encode2(float a, float b) {      // NaN stay
   return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 
-// The item (of n with count(i) >= 0 parts each) that holds part which(all parts) of them, and the part's place in it; every
-// thread of the block calls it, once. item is n if there is no such part.
+// The item (of n with count(i) parts each, fewer than 2^31 in all) that holds part which(all parts) of them, and the
+// part's place in it; every thread of the block calls it, once. item is n if there is no such part.
 template <int THREADS, typename Count, typename Which>
-__device__ __forceinline__ void locate(int n, Count count, Which which, int& item, int64_t& place) {
-  __shared__ int64_t warps[THREADS / 32];
-  __shared__ int64_t found_place;
-  __shared__ int found_item;
+__device__ __forceinline__ void locate(int n, Count count, Which which, int& item, int& place) {
+  __shared__ int warps[THREADS / 32], found[2];
   const int per = (n + THREADS - 1) / THREADS, lo = min((int)threadIdx.x * per, n), hi = min(lo + per, n);
-  int64_t mine = 0;
+  int mine = 0;
   for (int i = lo; i < hi; ++i) mine += count(i);
-  int64_t upto = mine;
+  int upto = mine;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+    const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
     if (lane >= o) upto += v;
   }
-  if (threadIdx.x == 0) found_item = n;
+  if (threadIdx.x == 0) found[0] = n;
   if (lane == 31) warps[warp] = upto;
   __syncthreads();
-  int64_t total = 0;
+  int total = 0;
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) {
     if (w < warp) upto += warps[w];
     total += warps[w];
   }
-  const int64_t at = which(total);
+  const int at = which(total);
   if (at >= upto - mine && at < upto) {
-    int64_t left = at - (upto - mine);
-    int i = lo;
-    for (int64_t c; left >= (c = count(i)); ++i) left -= c;
-    found_item = i;
-    found_place = left;
+    int left = at - (upto - mine), i = lo;
+    for (int c; i < hi - 1 && left >= (c = count(i)); ++i) left -= c;
+    found[0] = i;
+    found[1] = left;
   }
   __syncthreads();
-  item = found_item;
-  place = found_place;
+  item = found[0];
+  place = found[1];
 }
 
 inline int fail(int code, const char* msg) { return mk::set_last_error(code, msg); }

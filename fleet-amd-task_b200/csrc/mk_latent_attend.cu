@@ -46,22 +46,33 @@ constexpr int SUB = TILE * 128, STAGE = 4 * SUB + TILE * LD_R;      // a tile: u
 constexpr uint64_t TIMEOUT_NS = 2000000000ull;
 constexpr float X_SCALE = 7.0f, RAISE = 8.0f;                       // x = 2^7 at ref, 2^15 at most
 
+struct Bf16 {
+  using half_type = __nv_bfloat16;
+  using pair_type = __nv_bfloat162;
+  static constexpr int pieces = 2;
+};
+struct Fp16 {
+  using half_type = __half;
+  using pair_type = __half2;
+  static constexpr int pieces = 3;
+};
+
 template <typename T, int R_>
 struct Config {
-  static constexpr int R = R_, H = R_ / 2, PIECES = sizeof(typename T::half_type) == 2 && T::exact3 ? 3 : 2;
+  static constexpr int R = R_, H = R_ / 2, PIECES = T::pieces;
   static constexpr int NS = R * PIECES, NO = R * 3;
   static constexpr int BUFS = 4 * NS + 4 * NO <= 512 ? 2 : 1;       // buffers of scores in tensor memory
   static constexpr int O_COL = BUFS * 2 * NS;
   static constexpr int QC = 2 * STAGE, QR = QC + 4 * NS * 128, PB = QR + NS * 64, SMEM = PB + 2 * NO * 128;
   static_assert(O_COL + 4 * NO <= 512 && SMEM + 1024 + 2048 <= 232448, "tensor memory, shared memory");
 };
-struct Bf16 { using half_type = __nv_bfloat16; static constexpr bool exact3 = false; };
-struct Fp16 { using half_type = __half; static constexpr bool exact3 = true; };
 
-struct Meta {                   // where a block's run begins
-  int split, row, rows, pad;    // within a group: whose flat rows [row, row + rows)
-  int64_t lo, hi, total;        // the places of the group's units, of all
+// Division by a number that the host knows: x / d = (mulhi(x, mul) + x) >> shift for x < 2^31.
+struct Div {
+  uint32_t mul;
+  int shift;
 };
+__device__ __forceinline__ int operator/(int x, const Div& d) { return (int)((__umulhi((uint32_t)x, d.mul) + (uint32_t)x) >> d.shift); }
 
 struct Args {
   Cache k;
@@ -71,42 +82,41 @@ struct Args {
   float* lse;
   int64_t qt, qh, ot, oh;
   int heads, subs, box, wide;   // subs: 128-byte columns of a latent; box: rows of a TMA box; wide: 16-byte loads of q
+  int coarse;                   // a place is 1 << coarse units (more than one only where places would pass 2^31)
+  Div by_heads, by_subs;
   float scale;
-  Meta* meta;                   // [blocks]
+  int4* meta;                   // [blocks]: of a group that begins in the run before and goes on in this one, the runs that
+                                // hold some of it (or 0), its first row, its rows
   float* stat;                  // [2 blocks][R][2]: ref, sum
   float* part;                  // [2 blocks][R][128 subs]
 };
 
 // ---- a block's share of the units ----------------------------------------------------------
+// Runs are cut by cost, in places: a group costs its units and FIXED more (its queries, its first tile's maximum, its
+// outputs; fitted: a unit 0.8 us, a group 4.7 us).
+constexpr int FIXED = 6;
 template <int R>
-__device__ __forceinline__ int64_t groups_of(const Args& a, const Seq& q) { return ((int64_t)q.n * a.heads + R - 1) / R; }
+__device__ __forceinline__ int groups_of(const Args& a, const Seq& q) { return (q.n * a.heads + R - 1) / R; }
 __device__ __forceinline__ int units_of(const Args& a, const Seq& q) { return max(1, (min(q.len, a.b.capacity) + UNIT - 1) / UNIT); }
-
-// Runs are cut by cost: a group costs its units and FIXED more (its queries, its first tile's maximum, its outputs).
-constexpr int FIXED = 3;
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {      // of values above -1
-  return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
-}
-__device__ __forceinline__ int64_t begin_of(int64_t total, int block, int blocks) {
-  const int64_t each = quotient(total, blocks), more = total - each * blocks;
-  return each * block + (block < more ? block : more);
+__device__ __forceinline__ int places_of(const Args& a, int units) { return ((units - 1) >> a.coarse) + 1 + FIXED; }
+__device__ __forceinline__ int begin_of(int total, int block, int blocks) {
+  const int each = (uint32_t)total / (uint32_t)blocks, more = total - each * blocks;
+  return each * block + min(block, more);
 }
 // the block whose run holds place `at` < total
-__device__ __forceinline__ int holder_of(int64_t total, int64_t at, int blocks) {
-  const int64_t each = quotient(total, blocks), more = total - each * blocks;
-  return (int)(at < more * (each + 1) ? quotient(at, each + 1) : more + quotient(at - more * (each + 1), each));
+__device__ __forceinline__ int holder_of(int total, int at, int blocks) {
+  const int each = (uint32_t)total / (uint32_t)blocks, more = total - each * blocks, wide = more * (each + 1);
+  return at < wide ? (uint32_t)at / (uint32_t)(each + 1) : more + (uint32_t)(at - wide) / (uint32_t)max(each, 1);
 }
 
 struct Work {
-  int b, at;                    // the sequence, the place in its group's cost
-  int64_t g, left;              // the group, what is left of the run
+  int b, g, at, left;           // the sequence, its group, the place in the group's cost, what is left of the run
 };
 struct Segment {
   Seq q;
   int s;                        // the sequence
   int r0, rows;                 // rows [r0, r0 + rows) of the sequence's n x heads
   int u0, u1, units;            // units [u0, u1) of the group's
-  int lim;                      // tokens that its last row sees
   int end;                      // past the last token of this segment
   int tiles;
 };
@@ -122,20 +132,20 @@ __device__ __forceinline__ bool next(const Args& a, Work& w, Segment& s) {
     }
     s.s = w.b;
     s.units = units_of(a, s.q);
-    const int to = (int)min((int64_t)s.units + FIXED, w.at + w.left);
-    s.u0 = max(w.at - FIXED, 0);
-    s.u1 = max(to - FIXED, 0);
-    w.left -= to - w.at;
-    s.r0 = (int)(w.g * R);
+    const int places = places_of(a, s.units), to = min(places, w.at + w.left);
+    s.u0 = max(w.at - FIXED, 0) << a.coarse;
+    s.u1 = min(max(to - FIXED, 0) << a.coarse, s.units);
+    s.r0 = w.g * R;
     s.rows = min(R, s.q.n * a.heads - s.r0);
+    w.left -= to - w.at;
     w.at = to;
-    if (s.u1 == s.units) {
+    if (to == places) {
       ++w.g;
       w.at = 0;
     }
-    if (s.u1 == s.u0) continue;
-    s.lim = min(max(s.q.len - s.q.n + (s.r0 + s.rows - 1) / a.heads + 1, 0), a.b.capacity);
-    s.end = min(s.u1 * UNIT, s.lim);
+    if (s.u1 <= s.u0) continue;
+    // past the tokens that its last row sees
+    s.end = min(min(s.u1 * UNIT, a.b.capacity), s.q.len - s.q.n + (s.r0 + s.rows - 1) / a.by_heads + 1);
     s.tiles = max(0, (s.end - s.u0 * UNIT + TILE - 1) / TILE);
     return true;
   }
@@ -315,85 +325,86 @@ __device__ __forceinline__ void pieces_of(const float (&x)[N], uint32_t (&p)[3][
   }
 }
 
+// Eight values from any address.
+__device__ __noinline__ uint4 load_apart(const uint16_t* p) {
+  return make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+}
+__device__ __forceinline__ float2 unpack(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+__device__ __forceinline__ float2 unpack(__half2 v) { return __half22float2(v); }
+
 // A segment's queries: each row's scales, and its values' pieces in the order that the products read (K-major, swizzled as
-// TMA does it), zeros behind its values and in absent rows. What is not finite becomes NaN.
+// TMA does it), zeros behind its values and in absent rows. x = q / scale_q has at most 448 and is exact in FP16 down to
+// 2^-24. A row with an infinity or a NaN gets a NaN for its factor, which makes all its scores and outputs NaN.
 template <typename T, int R>
 __device__ __forceinline__ void ask(const Args& a, const Segment& s, uint8_t* smem, Shared<R>& sh, int set) {
   using C = Config<T, R>;
-  using E = typename T::half_type;
-  constexpr int PER = SOFTMAX / R;                // threads of a row
-  const int row = threadIdx.x / PER, sub = threadIdx.x % PER, f = s.r0 + row, tok = f / a.heads;
-  const bool live = row < s.rows;
-  const E* q = static_cast<const E*>(a.q) + (s.q.row + tok) * a.qt + (f - tok * a.heads) * a.qh;
-  const int c_chunks = a.subs * 16;
+  using E2 = typename T::pair_type;
+  constexpr int PER = SOFTMAX / R;                      // threads of a row
   constexpr int N = (MAX_DC + LD_R) / 8 / PER + (R == 16);        // 72 eights at most: 16 threads take 5 of them, 8 take 9
-  union { uint4 u; E e[8]; } v[N];
-  // (what is not there is loaded from the row's start and not used: branches would keep the loads apart)
-  const auto there = [&](int c) { return live && (c < c_chunks ? c * 8 < a.k.d_c : (c - c_chunks) * 8 < a.k.d_r); };
-  const auto from = [&](int c) { return !live ? static_cast<const E*>(a.q) : !there(c) ? q : c < c_chunks ? q + c * 8 : q + a.k.d_c + (c - c_chunks) * 8; };
-  if (a.wide) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i].u = *reinterpret_cast<const uint4*>(from(sub + i * PER));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const E* p = from(sub + i * PER);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i].e[e] = p[e];
-    }
-  }
-  float most[2] = {0.0f, 0.0f};
+  const int row = threadIdx.x / PER, sub = threadIdx.x % PER, c_chunks = a.subs * 16;
+  const bool live = row < s.rows;
+  const int f = s.r0 + (live ? row : 0), tok = f / a.by_heads;
+  const uint16_t* q = static_cast<const uint16_t*>(a.q) + (s.q.row + tok) * a.qt + (f - tok * a.heads) * a.qh;
+  union Eight { uint4 u; E2 e[4]; } v[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int c = sub + i * PER;
-    if (!there(c)) v[i].u = make_uint4(0, 0, 0, 0);
-    float m = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = fabsf(to_f32(v[i].e[e]));
-      m = x < INFINITY ? fmaxf(m, x) : m;
+    const bool there = live && (c < c_chunks ? c * 8 < a.k.d_c : (c - c_chunks) * 8 < a.k.d_r);
+    const uint16_t* p = q + (c < c_chunks ? c * 8 : a.k.d_c + (c - c_chunks) * 8);
+    v[i].u = make_uint4(0, 0, 0, 0);
+    if (a.wide) {
+      if (there) v[i].u = *reinterpret_cast<const uint4*>(p);
+    } else {
+      if (there) v[i].u = load_apart(p);
     }
-    if (c < c_chunks) most[0] = fmaxf(most[0], m);
-    else most[1] = fmaxf(most[1], m);
+  }
+  E2 most[2];
+  memset(most, 0, sizeof(most));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const E2 m = __hmax2_nan(__hmax2_nan(__habs2(v[i].e[0]), __habs2(v[i].e[1])), __hmax2_nan(__habs2(v[i].e[2]), __habs2(v[i].e[3])));
+    const int part = sub + i * PER >= c_chunks;
+    most[0] = part ? most[0] : __hmax2_nan(most[0], m);
+    most[1] = part ? __hmax2_nan(most[1], m) : most[1];
   }
   float inv[2];
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
+    // (bits of values that are not negative have their order, a NaN's are above an infinity's)
+    uint32_t u = __float_as_uint(unpack(most[part]).x);
+    u = max(u, __float_as_uint(unpack(most[part]).y));
 #pragma unroll
-    for (int o = PER / 2; o > 0; o >>= 1) most[part] = fmaxf(most[part], __shfl_xor_sync(~0u, most[part], o));
+    for (int o = PER / 2; o > 0; o >>= 1) u = max(u, __shfl_xor_sync(~0u, u, o));
     // the smallest power of two with the largest <= 448 of it
-    const uint32_t u = __float_as_uint(most[part]);
     const int e2 = max((int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0), -120);
     inv[part] = __uint_as_float((uint32_t)(127 - e2) << 23);
-    if (sub == 0) (part ? sh.qr : sh.qc)[set][row] = __uint_as_float((uint32_t)(e2 + 127) << 23) * (a.scale * 1.44269504f);
+    if (sub == 0)
+      (part ? sh.qr : sh.qc)[set][row] = u < 0x7F800000u ? __uint_as_float((uint32_t)(e2 + 127) << 23) * (a.scale * 1.44269504f) : __int_as_float(0x7FC00000);
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int c = sub + i * PER;
     if (c >= c_chunks + LD_R / 8) break;
     const float by = c < c_chunks ? inv[0] : inv[1];
-    float x[8];
+    __half2 x[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = to_f32(v[i].e[e]);
-      x[e] = fabsf(x[e]) < INFINITY ? x[e] * by : __int_as_float(0x7FC00000);
+    for (int e = 0; e < 4; ++e) {
+      const float2 y = unpack(v[i].e[e]);
+      x[e] = __floats2half2_rn(y.x * by, y.y * by);
     }
+    // the eight's place in the piece's row: 16-byte cells, swizzled by the row
+    const int g = c < c_chunks ? c : c - c_chunks, width = c < c_chunks ? 128 : 64;
+    uint8_t* to = smem + (c < c_chunks ? C::QC + (g >> 4) * (C::NS * 128) : C::QR) + row * width + (g & 1) * 8 +
+                  (((g >> 1 & 7) ^ (c < c_chunks ? row & 7 : row >> 1 & 3)) << 4);
 #pragma unroll
     for (int n = 0; n < C::PIECES; ++n) {
       uint32_t w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        w[e] = encode2(x[2 * e], x[2 * e + 1]);
-        if (n + 1 < C::PIECES) {
-          const float2 back = decode2((uint16_t)w[e]);
-          x[2 * e] = (x[2 * e] - back.x) * 16.0f;
-          x[2 * e + 1] = (x[2 * e + 1] - back.y) * 16.0f;
-        }
+        w[e] = __nv_cvt_halfraw2_to_fp8x2(x[e], __NV_SATFINITE, __NV_E4M3);
+        if (n + 1 < C::PIECES) x[e] = __hmul2(__hsub2(x[e], __half2(__nv_cvt_fp8x2_to_halfraw2((uint16_t)w[e], __NV_E4M3))), __float2half2_rn(16.0f));
       }
-      const int at = n * R + row, g = c < c_chunks ? c : c - c_chunks;     // the piece's row of the operand, its eight
-      uint8_t* to = c < c_chunks ? smem + C::QC + (g >> 4) * (C::NS * 128) + at * 128 + (((g >> 1 & 7) ^ (at & 7)) << 4)
-                                 : smem + C::QR + at * 64 + (((g >> 1) ^ (at >> 1 & 3)) << 4);
-      *reinterpret_cast<uint2*>(to + (g & 1) * 8) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+      *reinterpret_cast<uint2*>(to + n * R * width) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);      // (R is a multiple of 16)
     }
   }
 }
@@ -433,34 +444,32 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   // this block's run of the units
   Work work{};
   {
+    int place, total = 0, lo = 0;
     const auto count = [&](int i) {
       const Seq q = sequence(a.b, i);
-      return groups_of<R>(a, q) * (units_of(a, q) + FIXED);
+      return groups_of<R>(a, q) * places_of(a, units_of(a, q));
     };
-    int64_t place, total = 0;
-    locate<THREADS>(
-        a.b.n, count,
-        [&](int64_t all) {
-          total = all;
-          return begin_of(all, blockIdx.x, gridDim.x);
-        },
-        work.b, place);
-    const int64_t lo = begin_of(total, blockIdx.x, gridDim.x);
+    const auto which = [&](int all) {
+      total = all;
+      return lo = begin_of(all, blockIdx.x, gridDim.x);
+    };
+    locate<THREADS>(a.b.n, count, which, work.b, place);
     work.left = begin_of(total, blockIdx.x + 1, gridDim.x) - lo;
-    const bool any = work.b < a.b.n;
-    const Seq q = any ? sequence(a.b, work.b) : Seq{0, 0, 0};
-    const int units = units_of(a, q);
-    work.g = any ? quotient(place, units + FIXED) : 0;
-    work.at = any ? (int)(place - work.g * (units + FIXED)) : 0;
-    if (threadIdx.x == 0) {
-      Meta m{};
-      m.split = any && work.at > FIXED;
-      m.row = q.row * a.heads + (int)(work.g * R);
-      m.rows = any ? min(R, q.n * a.heads - (int)(work.g * R)) : 0;
-      m.lo = lo - work.at + FIXED;
-      m.hi = m.lo + units;
-      m.total = total;
-      a.meta[blockIdx.x] = m;
+    if (work.b < a.b.n) {
+      const Seq q = sequence(a.b, work.b);
+      const int places = places_of(a, units_of(a, q));
+      work.g = (uint32_t)place / (uint32_t)places;
+      work.at = place - work.g * places;
+      if (threadIdx.x == THREADS - 1) {
+        // the group's first unit is at place `first`: this run is the second that holds some of it, or not
+        const int first = lo - work.at + FIXED, last = lo - work.at + places - 1;
+        int4 m = make_int4(0, q.row * a.heads + work.g * R, min(R, q.n * a.heads - work.g * R), 0);
+        if (work.at > FIXED && blockIdx.x > 0 && begin_of(total, blockIdx.x - 1, gridDim.x) <= first)
+          m.x = min(holder_of(total, last, gridDim.x), (int)gridDim.x - 1) - (int)blockIdx.x + 2;
+        a.meta[blockIdx.x] = m;
+      }
+    } else if (threadIdx.x == THREADS - 1) {
+      a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
     }
   }
   fence_before();
@@ -578,7 +587,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
     const auto prepare = [&](const Segment& s, int set) {
       softmax_sync();           // what was in this set has been read
       if (tid < R) {
-        const int f = s.r0 + tid, row = f / a.heads;
+        const int f = s.r0 + tid, row = f / a.by_heads;
         sh.sees[set][tid] = tid < s.rows ? min(max(s.q.len - s.q.n + 1 + row, 0), a.b.capacity) : INT32_MAX;
         sh.at[set][tid] = (s.q.row + row) * a.ot + (f - row * a.heads) * a.oh;
       }
@@ -647,7 +656,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
           } else if (j * 128 + tok < k.d_c) {
 #pragma unroll
             for (int h = 0; h < H; ++h)
-              if (h < rows) out[h][j * 128] = from_f32<E>(inv[h] == 0.0f ? 0.0f : o[0][h] * inv[h]);
+              if (h < rows) out[h][j * 128] = from_f32<E>(o[0][h] * inv[h]);      // (what no token adds to is 0 x 0)
           }
         }
         fence_before();
@@ -655,7 +664,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       if (!more) break;
       s = ahead;
       begun = true;
-      const int first_sees = min(max(s.q.len - s.q.n + 1 + s.r0 / a.heads, 0), a.b.capacity);
+      const int first_sees = min(max(s.q.len - s.q.n + 1 + s.r0 / a.by_heads, 0), a.b.capacity);
       float qc[H], qr[H];
 #pragma unroll
       for (int h = 0; h < H; ++h) {
@@ -786,57 +795,100 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-// One row of each group that several blocks' runs share, by the block whose run is the second of them: the partial sums
-// of all, in their order.
+// The groups that several blocks' runs share: a job is 128 latent values of one row of one, the partial sums of all its runs
+// in their order, by a warp; where there are few jobs (one sequence over all blocks) by a block's 8 warps, an eighth of the
+// runs each.
+constexpr int MERGE_WARPS = 8;
 template <typename T, int R>
-__global__ void __launch_bounds__(128) merge_kernel(const Args a, int blocks) {
+__global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const Args a, int blocks) {
   using E = typename T::half_type;
-  __shared__ float weight[MAX_CTAS];
-  __shared__ float top[4], all[4];
-  const int i = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+  static_assert(MAX_CTAS <= MERGE_WARPS * 32, "a thread for each block's run");
+  __shared__ int4 groups[MAX_CTAS];                     // of each: the runs, the first row, the rows, the second run
+  __shared__ int counts[MERGE_WARPS];
+  __shared__ float weights[MERGE_WARPS][MAX_CTAS];
+  __shared__ float4 sums[MERGE_WARPS][32];
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Meta m = a.meta[i];
-  if (!m.split || row >= m.rows) return;
-  if (i == 0 || begin_of(m.total, i - 1, blocks) > m.lo) return;        // an earlier block's run splits it too
-  const int n = holder_of(m.total, m.hi - 1, blocks) - i + 2;           // the runs i - 1, i, ... hold some of it
-  const auto slot = [&](int p) { return ((int64_t)2 * (i - 1 + p) + (p == 0)) * R + row; };      // (the first part begins it)
-  float ref = -FLT_MAX;
-  for (int p = tid; p < n; p += 128) ref = fmaxf(ref, a.stat[slot(p) * 2]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(~0u, ref, o));
-  if (tid % 32 == 0) top[tid / 32] = ref;
+  int4 g = make_int4(0, 0, 0, 0);
+  if (tid < blocks) g = a.meta[tid];
+  g.w = tid;
+  const uint32_t ballot = __ballot_sync(~0u, g.x > 0);
+  if (lane == 0) counts[warp] = __popc(ballot);
   __syncthreads();
-  ref = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  float l = 0.0f;
-  for (int p = tid; p < n; p += 128) {
-    const float* st = a.stat + slot(p) * 2;
-    weight[p] = exp2_fast(st[0] - ref);
-    l += weight[p] * st[1];
+  int n_groups = 0, at = 0;
+#pragma unroll
+  for (int w = 0; w < MERGE_WARPS; ++w) {
+    if (w == warp) at = n_groups;
+    n_groups += counts[w];
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-  if (tid % 32 == 0) all[tid / 32] = l;
+  if (g.x > 0) groups[at + __popc(ballot & ((1u << lane) - 1))] = g;
   __syncthreads();
-  l = all[0] + all[1] + all[2] + all[3];
-  const int f = m.row + row, tok = f / a.heads;
-  if (a.lse && tid == 0) a.lse[f] = lse_of(ref, l);
-  E* out = static_cast<E*>(a.out) + tok * a.ot + (f - tok * a.heads) * a.oh;
-  const int ld = a.subs * 128, dim = tid * 4;
-  if (dim >= ld) return;
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const int jobs = n_groups * R * a.subs, ld = a.subs * 128;
+  const bool alone = jobs >= (int)gridDim.x * MERGE_WARPS;
+  const int share = alone ? 1 : MERGE_WARPS, part = alone ? 0 : warp;
+#pragma unroll 1
+  for (int job = alone ? blockIdx.x * MERGE_WARPS + warp : blockIdx.x; job < jobs; job += gridDim.x * (MERGE_WARPS / share)) {
+    const int row = job % R, rest = job / R, group = rest / a.by_subs, col = rest - group * a.subs;
+    g = groups[group];
+    if (row >= g.z) continue;
+    const int n = g.x, dim = col * 128 + lane * 4;
+    // the first part begins the group (its block's second place), the others continue it
+    const float2* stat = reinterpret_cast<const float2*>(a.stat) + (int64_t)2 * (g.w - 1) * R + row;
+    const float* parts = a.part + ((int64_t)2 * (g.w - 1) * R + row) * ld + dim;
+    const auto place = [&](int p) { return (2 * p + (p == 0)) * R; };
+    const auto load = [&](int p) { return *reinterpret_cast<const float4*>(parts + place(p) * ld); };
+    float4 ahead = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (part < n) ahead = load(part);
+    constexpr int CHUNKS = (MAX_CTAS + 31) / 32;
+    float2 st[CHUNKS];
+    float ref = -FLT_MAX, l = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      st[c] = make_float2(-FLT_MAX, 0.0f);
+      if (c * 32 + lane < n) st[c] = stat[place(c * 32 + lane)];
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) ref = fmaxf(ref, st[c].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(~0u, ref, o));
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+      if (c * 32 + lane < n) {
+        const float w = exp2_fast(st[c].x - ref);
+        weights[warp][c * 32 + lane] = w;
+        l = fmaf(w, st[c].y, l);
+      }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+    __syncwarp();
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const auto add = [&](float w, const float4& x) {
+      o.x = fmaf(w, x.x, o.x);
+      o.y = fmaf(w, x.y, o.y);
+      o.z = fmaf(w, x.z, o.z);
+      o.w = fmaf(w, x.w, o.w);
+    };
+    if (part < n) add(weights[warp][part], ahead);
 #pragma unroll 8
-  for (int p = 0; p < n; ++p) {
-    const float4 v = *reinterpret_cast<const float4*>(a.part + slot(p) * ld + dim);
-    const float w = weight[p];
-    o.x = fmaf(w, v.x, o.x);
-    o.y = fmaf(w, v.y, o.y);
-    o.z = fmaf(w, v.z, o.z);
-    o.w = fmaf(w, v.w, o.w);
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l, v[4] = {o.x, o.y, o.z, o.w};
+    for (int p = part + share; p < n; p += share) add(weights[warp][p], load(p));
+    __syncwarp();
+    if (!alone) {
+      sums[warp][lane] = o;
+      __syncthreads();
+      o = sums[0][lane];
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (dim + e < a.k.d_c) out[dim + e] = from_f32<E>(l == 0.0f ? 0.0f : v[e] * inv);
+      for (int w = 1; w < MERGE_WARPS; ++w) add(1.0f, sums[w][lane]);
+      __syncthreads();
+      if (warp > 0) continue;
+    }
+    const int f = g.y + row, tok = f / a.by_heads;
+    if (a.lse && col == 0 && lane == 0) a.lse[f] = lse_of(ref, l);
+    E* out = static_cast<E*>(a.out) + tok * a.ot + (f - tok * a.heads) * a.oh + dim;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l, x[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (dim + e < a.k.d_c) out[e] = from_f32<E>(x[e] * inv);
+  }
 }
 
 // ---- the host's side -----------------------------------------------------------------------
@@ -881,8 +933,8 @@ int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device
     cudaLaunchAttribute overlap[1];
     overlap[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     overlap[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)blocks, R);
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(2 * (unsigned)blocks);
+    cfg.blockDim = dim3(MERGE_WARPS * 32);
     cfg.dynamicSmemBytes = 0;
     cfg.attrs = overlap;
     cfg.numAttrs = 1;
@@ -891,7 +943,14 @@ int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
 }
 
-constexpr int64_t META_BYTES = (MAX_CTAS * sizeof(Meta) + 255) / 256 * 256;
+Div div_by(int d) {
+  Div v{0, 0};
+  while ((1 << v.shift) < d) ++v.shift;
+  v.mul = (uint32_t)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
+  return v;
+}
+
+constexpr int64_t META_BYTES = (MAX_CTAS * sizeof(int4) + 255) / 256 * 256;
 int64_t workspace(int rows, int subs) { return META_BYTES + (int64_t)2 * MAX_CTAS * rows * (2 + subs * 128) * 4; }
 
 }  // namespace
@@ -932,7 +991,12 @@ extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const
   a.scale = scale;
   a.box = a.k.page < UNIT ? a.k.page : UNIT;
   a.wide = (uintptr_t)q % 16 == 0 && qt % 8 == 0 && qh % 8 == 0;
-  a.meta = static_cast<Meta*>(workspace);
+  a.by_heads = div_by(heads);
+  a.by_subs = div_by(a.subs);
+  // groups and their places at most; no more than 2^31 in all
+  const int64_t groups = (int64_t)rows * heads / 16 + b->n, units = a.b.capacity / UNIT + 1;
+  while (groups * ((units >> a.coarse) + 1 + FIXED) > INT32_MAX && a.coarse < 31) ++a.coarse;
+  a.meta = static_cast<int4*>(workspace);
   a.stat = reinterpret_cast<float*>(static_cast<char*>(workspace) + META_BYTES);
   a.part = a.stat + (int64_t)2 * MAX_CTAS * 16 * 2;
   CUtensorMap c, r;
