@@ -74,6 +74,8 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS) append_kernel(const Write a) {
   __shared__ float most[2][THREADS / 32];
   const Cache& k = a.k;
+  start_dependents();
+  wait_predecessor();
   int s = blockIdx.x, first;
   int nth = 0;
   if (a.b.starts)
@@ -154,6 +156,8 @@ struct Read {
 template <typename T>
 __global__ void __launch_bounds__(THREADS) read_kernel(const Read a) {
   const Cache& k = a.k;
+  start_dependents();
+  wait_predecessor();
   const int row = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= a.b.rows) return;
   int s = row;
@@ -224,12 +228,9 @@ extern "C" int mk_latent_append(const MkLatent* l, const MkLatentBatch* b, const
   a.wide[1] = wide(r, ldr);
   // a sequence's rows are in at most rows / page + 2 pages, and in no more pages than rows
   const int64_t most = b->starts ? rows / l->page + 2 * (int64_t)b->n : rows;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(most < rows ? most : rows));
-  cfg.blockDim = dim3(THREADS);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == MK_BF16 ? cudaLaunchKernelEx(&cfg, append_kernel<__nv_bfloat16>, a)
-                                          : cudaLaunchKernelEx(&cfg, append_kernel<__half>, a);
+  const unsigned grid = (unsigned)(most < rows ? most : rows);
+  const cudaError_t e = launch_early(dtype == MK_BF16 ? append_kernel<__nv_bfloat16> : append_kernel<__half>, grid, THREADS, 0,
+                                     static_cast<cudaStream_t>(stream), a);
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
 }
 
@@ -247,11 +248,8 @@ extern "C" int mk_latent_read(const MkLatent* l, const MkLatentBatch* b, void* c
   a.wide[0] = wide(c, ldc);
   a.wide[1] = wide(r, ldr);
   a.fill = fill != 0;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(((unsigned)rows + THREADS / 32 - 1) / (THREADS / 32));
-  cfg.blockDim = dim3(THREADS);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == MK_BF16 ? cudaLaunchKernelEx(&cfg, read_kernel<__nv_bfloat16>, a)
-                                          : cudaLaunchKernelEx(&cfg, read_kernel<__half>, a);
+  const unsigned grid = ((unsigned)rows + THREADS / 32 - 1) / (THREADS / 32);
+  const cudaError_t e = launch_early(dtype == MK_BF16 ? read_kernel<__nv_bfloat16> : read_kernel<__half>, grid, THREADS, 0,
+                                     static_cast<cudaStream_t>(stream), a);
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
 }

@@ -113,6 +113,25 @@ __device__ __forceinline__ void locate(int n, Count count, Which which, int& ite
   place = found[1];
 }
 
+// Every kernel here is launched so that it may start before its predecessor on the stream has ended, and reads and writes
+// nothing before wait_predecessor(); start_dependents() lets its successor do the same.
+__device__ __forceinline__ void wait_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void start_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = s;
+  c.attrs = early;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
 inline int fail(int code, const char* msg) { return mk::set_last_error(code, msg); }
 
 // The host's checks of what every call is handed; MK_OK and the kernels' structs, or the error.

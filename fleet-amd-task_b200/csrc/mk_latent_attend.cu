@@ -36,9 +36,7 @@ namespace latent {
 namespace {
 
 using mk::mbar_arrive;
-using mk::mbar_arrive_expect_tx;
 using mk::mbar_init;
-using mk::mbar_try_wait;
 using mk::smem_u32;
 
 constexpr int MAX_CTAS = 148, TILE = 128, UNIT = 64, THREADS = 352, SOFTMAX = 256;
@@ -179,6 +177,9 @@ __device__ __forceinline__ void commit(uint64_t* bar, uint32_t elected) {
       "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
       "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(elected)
       : "memory");
+}
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // a box of a tensor map, brought by the elected lane (`issues`)
 __device__ __forceinline__ void copy(uint32_t to, const CUtensorMap* map, int x, int y, uint32_t bar, uint32_t issues) {
@@ -422,18 +423,22 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Cache& k = a.k;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], 1);
-      mbar_init(&sh.drained[i], 1);
-      mbar_init(&sh.scored[i], 1);
-      mbar_init(&sh.taken[i], SOFTMAX / 32);
-      mbar_init(&sh.weighed[i], SOFTMAX / 32);
-      mbar_init(&sh.summed[i], 1);
+  if (warp == 8) {
+    if (lane < 2) {
+      mbar_init(&sh.full[lane], 1);
+      mbar_init(&sh.empty[lane], 1);
+      mbar_init(&sh.drained[lane], 1);
+      mbar_init(&sh.scored[lane], 1);
+      mbar_init(&sh.taken[lane], SOFTMAX / 32);
+      mbar_init(&sh.weighed[lane], SOFTMAX / 32);
+      mbar_init(&sh.summed[lane], 1);
     }
-    mbar_init(&sh.asked, SOFTMAX / 32);
-    sh.lost = 0;
+    if (lane == 0) {
+      mbar_init(&sh.asked, SOFTMAX / 32);
+      sh.lost = 0;
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_c) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_r) : "memory");
+    }
     mk::fence_barrier_init();
   }
   if (warp == 9) {
@@ -441,6 +446,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     fence_before();
   }
+  start_dependents();
+  wait_predecessor();
   // this block's run of the units
   Work work{};
   {
@@ -475,7 +482,6 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   fence_before();
   __syncthreads();
   fence_after();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = sh.tmem;
   Segment s;
   int it = 0;                   // tiles so far
@@ -489,26 +495,16 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       for (int t = 0; t < s.tiles; ++t, ++it) {
         const int st = it & 1, pos0 = s.u0 * UNIT + t * TILE, pos = pos0 + 16 * lane;
         int page = -1;
-        float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (lane < TILE / 16 && pos < s.end) {
           page = a.b.table[s.s * a.b.ldt + (pos >> k.shift)];
-          if (page >= 0 && page < k.pages) {
-            g.x = k.scales[2 * (int64_t)page];
-            g.y = k.scales[2 * (int64_t)page + 1];
-            const float v = fmaxf(g.x, 5.42101086e-20f);        // 2^-64: a page that was never written has scale 0
-            g.z = log2f(v);
-            g.w = 1.0f / v;
-          } else {
-            page = -1;
-          }
+          if (page >= k.pages) page = -1;
         }
         const int rows = __popc(__ballot_sync(~0u, page >= 0 && lane % each == 0)) * a.box;
         const int y = (page << k.shift) + (pos & (k.page - 1));
         if (it >= 2 && !(ok = wait(&sh.empty[st], (it - 2) >> 1))) break;
-        if (lane < TILE / 16) sh.gran[st][lane] = g;
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&sh.full[st], rows * (a.subs * 128 + LD_R));
         const uint32_t to = base + st * STAGE, full = smem_u32(&sh.full[st]);
+        if (lane == 0) expect_bytes(full, rows * (a.subs * 128 + LD_R));
+        __syncwarp();
 #pragma unroll 1
         for (int from = 0; from < TILE / 16; from += each) {
           const int at = __shfl_sync(~0u, y, from), named = __shfl_sync(~0u, page, from);
@@ -518,6 +514,17 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
           for (int j = 0; j < 4; ++j)
             copy(to + j * SUB + from * 16 * 128, &map_c, j * 128, at, full, issues && j < a.subs);
         }
+        if (lane < TILE / 16) {
+          float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (page >= 0) {
+            const float2 scale = *reinterpret_cast<const float2*>(k.scales + 2 * (int64_t)page);
+            const float v = fmaxf(scale.x, 5.42101086e-20f);    // 2^-64: a page that was never written has scale 0
+            g = make_float4(scale.x, scale.y, log2f(v), 1.0f / v);
+          }
+          sh.gran[st][lane] = g;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.full[st]);
       }
     }
     for (int i = max(it - 2, 0); i < it; ++i) wait(&sh.full[i & 1], i >> 1);       // no copy outlives the block
@@ -796,8 +803,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
 }
 
 // The groups that several blocks' runs share: a job is 128 latent values of one row of one, the partial sums of all its runs
-// in their order, by a warp; where there are few jobs (one sequence over all blocks) by a block's 8 warps, an eighth of the
-// runs each.
+// in their order, by one warp or, where there are fewer jobs than warps, by up to 8 of a block with a share of the runs each.
 constexpr int MERGE_WARPS = 8;
 template <typename T, int R>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const Args a, int blocks) {
@@ -808,7 +814,8 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const Args a, i
   __shared__ float weights[MERGE_WARPS][MAX_CTAS];
   __shared__ float4 sums[MERGE_WARPS][32];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  start_dependents();
+  wait_predecessor();
   int4 g = make_int4(0, 0, 0, 0);
   if (tid < blocks) g = a.meta[tid];
   g.w = tid;
@@ -824,21 +831,30 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const Args a, i
   if (g.x > 0) groups[at + __popc(ballot & ((1u << lane) - 1))] = g;
   __syncthreads();
   const int jobs = n_groups * R * a.subs, ld = a.subs * 128;
-  const bool alone = jobs >= (int)gridDim.x * MERGE_WARPS;
-  const int share = alone ? 1 : MERGE_WARPS, part = alone ? 0 : warp;
+  int share = 1;
+  while (share < MERGE_WARPS && 2 * share * jobs <= (int)gridDim.x * MERGE_WARPS) share *= 2;
+  const int teams = MERGE_WARPS / share, team = warp / share, part = warp % share;
 #pragma unroll 1
-  for (int job = alone ? blockIdx.x * MERGE_WARPS + warp : blockIdx.x; job < jobs; job += gridDim.x * (MERGE_WARPS / share)) {
-    const int row = job % R, rest = job / R, group = rest / a.by_subs, col = rest - group * a.subs;
+  for (int first = blockIdx.x * teams; first < jobs; first += gridDim.x * teams) {
+    const int job = min(first + team, jobs - 1), row = job % R, rest = job / R, group = rest / a.by_subs, col = rest - group * a.subs;
     g = groups[group];
-    if (row >= g.z) continue;
-    const int n = g.x, dim = col * 128 + lane * 4;
+    const int n = first + team < jobs && row < g.z ? g.x : 0, dim = col * 128 + lane * 4;
     // the first part begins the group (its block's second place), the others continue it
     const float2* stat = reinterpret_cast<const float2*>(a.stat) + (int64_t)2 * (g.w - 1) * R + row;
     const float* parts = a.part + ((int64_t)2 * (g.w - 1) * R + row) * ld + dim;
     const auto place = [&](int p) { return (2 * p + (p == 0)) * R; };
     const auto load = [&](int p) { return *reinterpret_cast<const float4*>(parts + place(p) * ld); };
-    float4 ahead = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (part < n) ahead = load(part);
+    // four parts at a time, the first on their way before their weights are known (a loop's rest would wait for each)
+    constexpr int AT_ONCE = 4;
+    float4 v[AT_ONCE];
+    const auto fetch = [&](int from) {
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (from + k * share < n) v[k] = load(from + k * share);
+      }
+    };
+    fetch(part);
     constexpr int CHUNKS = (MAX_CTAS + 31) / 32;
     float2 st[CHUNKS];
     float ref = -FLT_MAX, l = 0.0f;
@@ -868,19 +884,24 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const Args a, i
       o.z = fmaf(w, x.z, o.z);
       o.w = fmaf(w, x.w, o.w);
     };
-    if (part < n) add(weights[warp][part], ahead);
-#pragma unroll 8
-    for (int p = part + share; p < n; p += share) add(weights[warp][p], load(p));
+    for (int from = part; from < n; from += AT_ONCE * share) {
+      float4 now[AT_ONCE];
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) now[k] = v[k];
+      fetch(from + AT_ONCE * share);
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k)
+        if (from + k * share < n) add(weights[warp][from + k * share], now[k]);
+    }
     __syncwarp();
-    if (!alone) {
+    if (share > 1) {
       sums[warp][lane] = o;
       __syncthreads();
-      o = sums[0][lane];
-#pragma unroll
-      for (int w = 1; w < MERGE_WARPS; ++w) add(1.0f, sums[w][lane]);
+      o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int w = 0; w < share; ++w) add(1.0f, sums[team * share + w][lane]);
       __syncthreads();
-      if (warp > 0) continue;
     }
+    if (n == 0 || part > 0) continue;
     const int f = g.y + row, tok = f / a.by_heads;
     if (a.lse && col == 0 && lane == 0) a.lse[f] = lse_of(ref, l);
     E* out = static_cast<E*>(a.out) + tok * a.ot + (f - tok * a.heads) * a.oh + dim;
@@ -923,23 +944,8 @@ int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device
     e = cudaFuncSetAttribute(attend_kernel<T, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, Config<T, R>::SMEM + 1024);
     if (e == cudaSuccess) ready[device].store(true, std::memory_order_release);
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = Config<T, R>::SMEM + 1024;
-  cfg.stream = s;
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, attend_kernel<T, R>, a, c, r);
-  if (e == cudaSuccess) {
-    cudaLaunchAttribute overlap[1];
-    overlap[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    overlap[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(2 * (unsigned)blocks);
-    cfg.blockDim = dim3(MERGE_WARPS * 32);
-    cfg.dynamicSmemBytes = 0;
-    cfg.attrs = overlap;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, merge_kernel<T, R>, a, blocks);
-  }
+  if (e == cudaSuccess) e = launch_early(attend_kernel<T, R>, blocks, THREADS, Config<T, R>::SMEM + 1024, s, a, c, r);
+  if (e == cudaSuccess) e = launch_early(merge_kernel<T, R>, 2 * blocks, MERGE_WARPS * 32, 0, s, a, blocks);
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
 }
 

@@ -14,17 +14,7 @@
 // each thread takes VEC pairs of a head at a time: 16-byte loads and stores where all rows allow them,
 // single values otherwise. A head's pairs are in one warp, loaded before any is stored, so the output may
 // be the input even where the layout changes.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
-#include <cstdint>
-
-#include "../../include/fleet_mk.h"
-
-namespace mk {
-int set_last_error(int code, const char* msg);   // mk_runtime.cu: the message mk_last_error() returns
-}
+#include "mk_latent.cuh"
 
 namespace {
 
@@ -39,8 +29,7 @@ struct Args {
   float scale;
 };
 
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+using latent::to_f32;
 __device__ __forceinline__ void from_f32(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void from_f32(__half& d, float v) { d = __float2half_rn(v); }
 
@@ -51,6 +40,8 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
   __shared__ float2 turn[TABLE];        // (cos, sin) times the scale
   using V = Vec<T, VEC>;
+  latent::start_dependents();
+  latent::wait_predecessor();
   const int pairs = a.dim / 2, units = pairs / VEC;
   const int64_t first = (int64_t)blockIdx.x * a.tokens;
   const int count = (int)min((int64_t)a.tokens, a.t - first);
@@ -125,18 +116,15 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
   }
 }
 
-int fail(int code, const char* msg) { return mk::set_last_error(code, msg); }
+using latent::fail;
 
 template <typename T>
 cudaError_t launch(Args a, cudaStream_t s) {
   const bool wide = ((uintptr_t)a.x | (uintptr_t)a.out) % 16 == 0 && (a.xt | a.xh | a.ot | a.oh) % 8 == 0 &&
                     a.dim % 16 == 0 && a.start % 8 == 0 && a.width % 8 == 0;
   a.tokens = 1;
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3((unsigned)((a.t + (int64_t)a.tokens - 1) / a.tokens));
-  c.blockDim = dim3(THREADS);
-  c.stream = s;
-  return wide ? cudaLaunchKernelEx(&c, rope_kernel<T, 8>, a) : cudaLaunchKernelEx(&c, rope_kernel<T, 1>, a);
+  const unsigned grid = (unsigned)((a.t + (int64_t)a.tokens - 1) / a.tokens);
+  return latent::launch_early(wide ? rope_kernel<T, 8> : rope_kernel<T, 1>, grid, THREADS, 0, s, a);
 }
 
 }  // namespace
