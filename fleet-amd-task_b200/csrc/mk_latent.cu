@@ -7,28 +7,19 @@
 // writes the new codes: one rounding to E4M3, x / scale being exact. What is not finite becomes NaN and
 // does not count for the scale; |x| beyond 448 2^32 saturates.
 //
-// read: code x scale of each row, rounded once (exact in BF16).
+// All of a page's new values are loaded at once and kept in registers (16 bytes a load, 18 loads a thread at most), so they
+// are read once, and their loads do not wait for one another.
+//
+// read: code x scale of each row, rounded once (exact in BF16): a block takes 32 rows, resolves their places, then each
+// thread widens 16 codes at a time.
 #include "mk_latent.cuh"
 
 namespace latent {
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 512, READERS = 256, READ_ROWS = 32;
 
-// 8 values of a row, from 16-byte aligned memory or one by one
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool wide, float (&v)[8]) {
-  union { uint4 u; T t[8]; } r;
-  if (wide) {
-    r.u = *reinterpret_cast<const uint4*>(p);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.t[i] = p[i];
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = to_f32(r.t[i]);
-}
-
+// 8 values of a row, to 16-byte aligned memory or one by one
 template <typename T>
 __device__ __forceinline__ void store8(T* p, bool wide, const float (&v)[8]) {
   union { uint4 u; T t[8]; } r;
@@ -70,7 +61,8 @@ __device__ __forceinline__ int pages_of(const Cache& k, const Batch& b, const Se
   return hi > lo ? ((hi - 1) >> k.shift) - first + 1 : 0;
 }
 
-template <typename T>
+// LOADS: eights of values that a thread holds, enough for a page's
+template <typename T, int LOADS>
 __global__ void __launch_bounds__(THREADS) append_kernel(const Write a) {
   __shared__ float most[2][THREADS / 32];
   const Cache& k = a.k;
@@ -84,64 +76,102 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Write a) {
   if (s >= a.b.n) return;
   const Seq q = sequence(a.b, s);
   if (nth >= pages_of(k, a.b, q, first)) return;
-  const int j = first + nth;
-  const int p = a.b.table[s * a.b.ldt + j];
-  if (p < 0 || p >= k.pages) return;
+  const int j = first + nth, p = a.b.table[s * a.b.ldt + j];
   // the page's new tokens [lo, hi), offsets in the page; its first new token is row `row`
   const int begin = max(q.len - q.n, 0), lo = max(begin - (j << k.shift), 0);
   const int hi = min(min(q.len, a.b.capacity) - (j << k.shift), k.page), m = hi - lo;
   const int row = q.row + ((j << k.shift) + lo) - (q.len - q.n);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // an item is 8 values: all tokens' latents, then their rotary keys
+  const int c_eights = k.d_c / 8, r_eights = k.d_r / 8, latents = m * c_eights, items = latents + m * r_eights;
+  const auto part_of = [&](int i) { return i >= latents; };
+  const auto place_of = [&](int i, int& token, int& at) {
+    const int part = part_of(i), eights = part ? r_eights : c_eights, e = part ? i - latents : i;
+    token = e / eights;
+    at = (e - token * eights) * 8;
+  };
+  union Eight { uint4 u; T t[8]; } v[LOADS];
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    const int chunks = (part ? k.d_r : k.d_c) / 8;
-    const T* x = static_cast<const T*>(a.x[part]) + row * a.ld[part];
-    float amax = 0.0f;
-    for (int i = threadIdx.x; i < m * chunks; i += THREADS) {
-      float v[8];
-      load8(x + (i / chunks) * a.ld[part] + i % chunks * 8, a.wide[part], v);
+  for (int l = 0; l < LOADS; ++l) {
+    const int i = threadIdx.x + l * THREADS;
+    v[l].u = make_uint4(0, 0, 0, 0);
+    if (i < items) {
+      int token, at;
+      place_of(i, token, at);
+      const int part = part_of(i);
+      const T* x = static_cast<const T*>(a.x[part]) + (row + token) * a.ld[part] + at;
+      if (a.wide[part]) {
+        v[l].u = *reinterpret_cast<const uint4*>(x);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(v[e]));
+        for (int e = 0; e < 8; ++e) v[l].t[e] = x[e];
+      }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-    if (lane == 0) most[part][warp] = amax;
   }
-  const float old[2] = {k.scales[2 * (int64_t)p], k.scales[2 * (int64_t)p + 1]};
-  __syncthreads();
+  if (p < 0 || p >= k.pages) return;
+  const float2 old = *reinterpret_cast<const float2*>(k.scales + 2 * (int64_t)p);
+  float amax[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int l = 0; l < LOADS; ++l) {
+    if (threadIdx.x + l * THREADS >= items) break;
+    float big = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) big = fmaxf(big, finite_abs(to_f32(v[l].t[e])));
+    const int part = part_of(threadIdx.x + l * THREADS);
+    amax[0] = part ? amax[0] : fmaxf(amax[0], big);
+    amax[1] = part ? fmaxf(amax[1], big) : amax[1];
+  }
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
-    float amax = 0.0f;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) amax = fmaxf(amax, most[part][w]);
-    float scale = scale_of(amax);
-    if (lo > 0) scale = fmaxf(scale, old[part]);
-    const int d = part ? k.d_r : k.d_c, ld = part ? LD_R : k.ld_c, chunks = d / 8;
+    for (int o = 16; o > 0; o >>= 1) amax[part] = fmaxf(amax[part], __shfl_xor_sync(0xFFFFFFFFu, amax[part], o));
+    if (lane == 0) most[part][warp] = amax[part];
+  }
+  __syncthreads();              // (and every thread has the old scales)
+  float scale[2], inv[2];
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    float big = 0.0f;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) big = fmaxf(big, most[part][w]);
+    const float was = part ? old.y : old.x;
+    scale[part] = scale_of(big);
+    if (lo > 0) scale[part] = fmaxf(scale[part], was);
+    inv[part] = 1.0f / scale[part];
+    const int ld = part ? LD_R : k.ld_c, eights = part ? r_eights : c_eights;
     uint8_t* codes = (part ? k.r : k.c) + ((int64_t)p << k.shift) * ld;
-    if (lo > 0 && scale != old[part]) {
-      const float ratio = old[part] / scale;
-      for (int i = threadIdx.x; i < lo * chunks; i += THREADS) {
-        uint16_t* at = reinterpret_cast<uint16_t*>(codes + (i / chunks) * ld + i % chunks * 8);
+    if (lo > 0 && scale[part] != was) {
+      const float ratio = was / scale[part];
+      for (int i = threadIdx.x; i < lo * eights; i += THREADS) {
+        const int token = i / eights;
+        uint16_t* at = reinterpret_cast<uint16_t*>(codes + token * ld + (i - token * eights) * 8);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 v = decode2(at[e]);
-          at[e] = encode2(v.x * ratio, v.y * ratio);
+          const float2 f = decode2(at[e]);
+          at[e] = encode2(f.x * ratio, f.y * ratio);
         }
       }
     }
-    const T* x = static_cast<const T*>(a.x[part]) + row * a.ld[part];
-    const float inv = 1.0f / scale, nan = __int_as_float(0x7FC00000);
-    for (int i = threadIdx.x; i < m * chunks; i += THREADS) {
-      float v[8];
-      load8(x + (i / chunks) * a.ld[part] + i % chunks * 8, a.wide[part], v);
+  }
+  if (threadIdx.x == 0) *reinterpret_cast<float2*>(k.scales + 2 * (int64_t)p) = make_float2(scale[0], scale[1]);
+  const float nan = __int_as_float(0x7FC00000);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = isfinite(v[e]) ? v[e] * inv : nan;
-      uint2 w;
-      w.x = encode2(v[0], v[1]) | (uint32_t)encode2(v[2], v[3]) << 16;
-      w.y = encode2(v[4], v[5]) | (uint32_t)encode2(v[6], v[7]) << 16;
-      *reinterpret_cast<uint2*>(codes + (lo + i / chunks) * ld + i % chunks * 8) = w;
+  for (int l = 0; l < LOADS; ++l) {
+    const int i = threadIdx.x + l * THREADS;
+    if (i >= items) break;
+    int token, at;
+    place_of(i, token, at);
+    const int part = part_of(i);
+    const float by = part ? inv[1] : inv[0];
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = to_f32(v[l].t[e]);
+      x[e] = isfinite(x[e]) ? x[e] * by : nan;
     }
-    if (threadIdx.x == 0) k.scales[2 * (int64_t)p + part] = scale;
+    uint8_t* codes = part ? k.r + (((int64_t)p << k.shift) + lo + token) * LD_R : k.c + (((int64_t)p << k.shift) + lo + token) * k.ld_c;
+    *reinterpret_cast<uint2*>(codes + at) = make_uint2(encode2(x[0], x[1]) | (uint32_t)encode2(x[2], x[3]) << 16,
+                                                       encode2(x[4], x[5]) | (uint32_t)encode2(x[6], x[7]) << 16);
   }
 }
 
@@ -154,54 +184,67 @@ struct Read {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) read_kernel(const Read a) {
+__global__ void __launch_bounds__(READERS) read_kernel(const Read a) {
+  __shared__ int64_t token_of[READ_ROWS];               // a row's token in the cache, -1: in none, -2: the row is left alone
+  __shared__ float2 scale_of_row[READ_ROWS];
   const Cache& k = a.k;
   start_dependents();
   wait_predecessor();
-  const int row = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= a.b.rows) return;
-  int s = row;
-  if (a.b.starts) {             // the last sequence that starts at or before the row
-    int lo = 0, hi = a.b.n;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (a.b.starts[mid] <= row) lo = mid + 1;
-      else hi = mid;
+  const int first = blockIdx.x * READ_ROWS, rows = min(READ_ROWS, a.b.rows - first);
+  if ((int)threadIdx.x < rows) {
+    const int row = first + threadIdx.x;
+    int s = row;
+    if (a.b.starts) {           // the last sequence that starts at or before the row
+      int lo = 0, hi = a.b.n;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (a.b.starts[mid] <= row) lo = mid + 1;
+        else hi = mid;
+      }
+      s = lo - 1;
     }
-    s = lo - 1;
-  }
-  int p = -1, off = 0;
-  bool mine = false;
-  if (s >= 0 && s < a.b.n) {
-    const Seq q = sequence(a.b, s);
-    mine = row >= q.row && row < q.row + q.n;
-    const int pos = q.len - q.n + (row - q.row);
-    if (mine && pos >= 0 && pos < a.b.capacity) {
-      p = a.b.table[s * a.b.ldt + (pos >> k.shift)];
-      off = pos & (k.page - 1);
-    }
-  }
-  if (!mine && !a.fill) return;
-  const bool live = p >= 0 && p < k.pages;
-#pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    const int d = part ? k.d_r : k.d_c, ld = part ? LD_R : k.ld_c;
-    const uint8_t* codes = (part ? k.r : k.c) + (((int64_t)p << k.shift) + off) * ld;
-    const float scale = live ? k.scales[2 * (int64_t)p + part] : 0.0f;
-    T* out = static_cast<T*>(a.out[part]) + row * a.ld[part];
-    for (int i = lane * 8; i < d; i += 256) {
-      float v[8] = {};
-      if (live) {
-        const uint2 w = *reinterpret_cast<const uint2*>(codes + i);
-        const uint32_t u[2] = {w.x, w.y};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = decode2((uint16_t)(u[e / 2] >> (e % 2 * 16)));
-          v[2 * e] = f.x * scale;
-          v[2 * e + 1] = f.y * scale;
+    int64_t token = a.fill ? -1 : -2;
+    float2 scale = make_float2(0.0f, 0.0f);
+    if (s >= 0 && s < a.b.n) {
+      const Seq q = sequence(a.b, s);
+      if (row >= q.row && row < q.row + q.n) {
+        const int pos = q.len - q.n + (row - q.row);
+        token = -1;
+        if (pos >= 0 && pos < a.b.capacity) {
+          const int p = a.b.table[s * a.b.ldt + (pos >> k.shift)];
+          if (p >= 0 && p < k.pages) {
+            token = ((int64_t)p << k.shift) + (pos & (k.page - 1));
+            scale = *reinterpret_cast<const float2*>(k.scales + 2 * (int64_t)p);
+          }
         }
       }
-      store8(out + i, a.wide[part], v);
+    }
+    token_of[threadIdx.x] = token;
+    scale_of_row[threadIdx.x] = scale;
+  }
+  __syncthreads();
+  // an item is 16 codes (8 at a row's end)
+  const int c_items = (k.d_c + 15) / 16, each = c_items + (k.d_r + 15) / 16;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < rows * each; i += READERS) {
+    const int r = i / each, item = i - r * each, part = item >= c_items, at = (part ? item - c_items : item) * 16;
+    const int64_t token = token_of[r];
+    if (token == -2) continue;
+    const float scale = part ? scale_of_row[r].y : scale_of_row[r].x;
+    uint4 codes = make_uint4(0, 0, 0, 0);
+    if (token >= 0) codes = *reinterpret_cast<const uint4*>(part ? k.r + token * LD_R + at : k.c + token * k.ld_c + at);
+    const uint32_t u[4] = {codes.x, codes.y, codes.z, codes.w};
+    T* out = static_cast<T*>(a.out[part]) + (first + r) * a.ld[part] + at;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = decode2((uint16_t)(u[2 * half + e / 2] >> (e % 2 * 16)));
+        v[2 * e] = f.x * scale;
+        v[2 * e + 1] = f.y * scale;
+      }
+      if (at + 8 * half < (part ? k.d_r : k.d_c)) store8(out + 8 * half, a.wide[part], v);
     }
   }
 }
@@ -229,8 +272,14 @@ extern "C" int mk_latent_append(const MkLatent* l, const MkLatentBatch* b, const
   // a sequence's rows are in at most rows / page + 2 pages, and in no more pages than rows
   const int64_t most = b->starts ? rows / l->page + 2 * (int64_t)b->n : rows;
   const unsigned grid = (unsigned)(most < rows ? most : rows);
-  const cudaError_t e = launch_early(dtype == MK_BF16 ? append_kernel<__nv_bfloat16> : append_kernel<__half>, grid, THREADS, 0,
-                                     static_cast<cudaStream_t>(stream), a);
+  // a page's eights of values over the threads: of few rows (a token of each sequence) no page holds many
+  const int64_t held = l->page < rows ? l->page : rows, eights = held * ((l->d_c + l->d_r) / 8);
+  const auto s = static_cast<cudaStream_t>(stream);
+  const auto launch = [&](auto kernel) { return launch_early(kernel, dim3(grid), THREADS, 0, s, a); };
+  cudaError_t e;
+  if (eights <= THREADS) e = dtype == MK_BF16 ? launch(append_kernel<__nv_bfloat16, 1>) : launch(append_kernel<__half, 1>);
+  else if (eights <= 9 * THREADS) e = dtype == MK_BF16 ? launch(append_kernel<__nv_bfloat16, 9>) : launch(append_kernel<__half, 9>);
+  else e = dtype == MK_BF16 ? launch(append_kernel<__nv_bfloat16, 18>) : launch(append_kernel<__half, 18>);
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
 }
 
@@ -248,8 +297,8 @@ extern "C" int mk_latent_read(const MkLatent* l, const MkLatentBatch* b, void* c
   a.wide[0] = wide(c, ldc);
   a.wide[1] = wide(r, ldr);
   a.fill = fill != 0;
-  const unsigned grid = ((unsigned)rows + THREADS / 32 - 1) / (THREADS / 32);
-  const cudaError_t e = launch_early(dtype == MK_BF16 ? read_kernel<__nv_bfloat16> : read_kernel<__half>, grid, THREADS, 0,
+  const unsigned grid = ((unsigned)rows + READ_ROWS - 1) / READ_ROWS;
+  const cudaError_t e = launch_early(dtype == MK_BF16 ? read_kernel<__nv_bfloat16> : read_kernel<__half>, dim3(grid), READERS, 0,
                                      static_cast<cudaStream_t>(stream), a);
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
 }

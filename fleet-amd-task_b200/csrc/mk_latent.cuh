@@ -118,18 +118,31 @@ __device__ __forceinline__ void locate(int n, Count count, Which which, int& ite
 __device__ __forceinline__ void wait_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void start_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 template <typename... P, typename... A>
-cudaError_t launch_early(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t s, A... args) {
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A... args) {
   cudaLaunchAttribute early[1];
   early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t c{};
-  c.gridDim = dim3(grid);
+  c.gridDim = grid;
   c.blockDim = dim3(threads);
   c.dynamicSmemBytes = smem;
   c.stream = s;
   c.attrs = early;
   c.numAttrs = 1;
   return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
+// Division by a number that the host knows: x / d = (mulhi(x, mul) + x) >> shift for 0 <= x < 2^31.
+struct Div {
+  uint32_t mul;
+  int shift, d;
+};
+__device__ __forceinline__ int operator/(int x, const Div& d) { return (int)((__umulhi((uint32_t)x, d.mul) + (uint32_t)x) >> d.shift); }
+inline Div div_by(int d) {
+  Div v{0, 0, d};
+  while ((1ll << v.shift) < d) ++v.shift;
+  v.mul = (uint32_t)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
+  return v;
 }
 
 inline int fail(int code, const char* msg) { return mk::set_last_error(code, msg); }

@@ -65,13 +65,6 @@ struct Config {
   static_assert(O_COL + 4 * NO <= 512 && SMEM + 1024 + 2048 <= 232448, "tensor memory, shared memory");
 };
 
-// Division by a number that the host knows: x / d = (mulhi(x, mul) + x) >> shift for x < 2^31.
-struct Div {
-  uint32_t mul;
-  int shift;
-};
-__device__ __forceinline__ int operator/(int x, const Div& d) { return (int)((__umulhi((uint32_t)x, d.mul) + (uint32_t)x) >> d.shift); }
-
 struct Args {
   Cache k;
   Batch b;
@@ -944,16 +937,9 @@ int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device
     e = cudaFuncSetAttribute(attend_kernel<T, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, Config<T, R>::SMEM + 1024);
     if (e == cudaSuccess) ready[device].store(true, std::memory_order_release);
   }
-  if (e == cudaSuccess) e = launch_early(attend_kernel<T, R>, blocks, THREADS, Config<T, R>::SMEM + 1024, s, a, c, r);
-  if (e == cudaSuccess) e = launch_early(merge_kernel<T, R>, 2 * blocks, MERGE_WARPS * 32, 0, s, a, blocks);
+  if (e == cudaSuccess) e = launch_early(attend_kernel<T, R>, dim3(blocks), THREADS, Config<T, R>::SMEM + 1024, s, a, c, r);
+  if (e == cudaSuccess) e = launch_early(merge_kernel<T, R>, dim3(2 * blocks), MERGE_WARPS * 32, 0, s, a, blocks);
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
-}
-
-Div div_by(int d) {
-  Div v{0, 0};
-  while ((1 << v.shift) < d) ++v.shift;
-  v.mul = (uint32_t)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
-  return v;
 }
 
 constexpr int64_t META_BYTES = (MAX_CTAS * sizeof(int4) + 255) / 256 * 256;
