@@ -52,6 +52,7 @@ struct Write {
   const void *x[2];       // latents, rotary keys
   int64_t ld[2];
   int wide[2];
+  Div by_c, by_r;         // eights of a token's latents, of its rotary keys
 };
 
 // the pages that a sequence's new tokens are in: [first, first + count)
@@ -86,9 +87,9 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Write a) {
   const int c_eights = k.d_c / 8, r_eights = k.d_r / 8, latents = m * c_eights, items = latents + m * r_eights;
   const auto part_of = [&](int i) { return i >= latents; };
   const auto place_of = [&](int i, int& token, int& at) {
-    const int part = part_of(i), eights = part ? r_eights : c_eights, e = part ? i - latents : i;
-    token = e / eights;
-    at = (e - token * eights) * 8;
+    const int part = part_of(i), e = part ? i - latents : i;
+    token = part ? e / a.by_r : e / a.by_c;
+    at = (e - token * (part ? r_eights : c_eights)) * 8;
   };
   union Eight { uint4 u; T t[8]; } v[LOADS];
 #pragma unroll
@@ -109,7 +110,8 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Write a) {
     }
   }
   if (p < 0 || p >= k.pages) return;
-  const float2 old = *reinterpret_cast<const float2*>(k.scales + 2 * (int64_t)p);
+  float2 old = make_float2(0.0f, 0.0f);
+  if (lo > 0) old = *reinterpret_cast<const float2*>(k.scales + 2 * (int64_t)p);
   float amax[2] = {0.0f, 0.0f};
 #pragma unroll
   for (int l = 0; l < LOADS; ++l) {
@@ -181,6 +183,7 @@ struct Read {
   void* out[2];
   int64_t ld[2];
   int wide[2], fill;      // fill: rows of no sequence become zeros
+  Div by_each;            // the items of a row
 };
 
 template <typename T>
@@ -191,18 +194,22 @@ __global__ void __launch_bounds__(READERS) read_kernel(const Read a) {
   start_dependents();
   wait_predecessor();
   const int first = blockIdx.x * READ_ROWS, rows = min(READ_ROWS, a.b.rows - first);
+  // the sequences that start at or before the block's first row: all threads count, a search would wait for each of its steps
+  __shared__ int begun;
+  if (a.b.starts) {
+    if (threadIdx.x == 0) begun = 0;
+    __syncthreads();
+    int mine = 0;
+    for (int i = threadIdx.x; i < a.b.n; i += READERS) mine += a.b.starts[i] <= first;
+    mine = __reduce_add_sync(0xFFFFFFFFu, mine);
+    if (threadIdx.x % 32 == 0 && mine > 0) atomicAdd(&begun, mine);
+    __syncthreads();
+  }
   if ((int)threadIdx.x < rows) {
     const int row = first + threadIdx.x;
     int s = row;
-    if (a.b.starts) {           // the last sequence that starts at or before the row
-      int lo = 0, hi = a.b.n;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (a.b.starts[mid] <= row) lo = mid + 1;
-        else hi = mid;
-      }
-      s = lo - 1;
-    }
+    if (a.b.starts)             // the last one that starts at or before the row
+      for (s = begun - 1; s + 1 < a.b.n && a.b.starts[s + 1] <= row;) ++s;
     int64_t token = a.fill ? -1 : -2;
     float2 scale = make_float2(0.0f, 0.0f);
     if (s >= 0 && s < a.b.n) {
@@ -223,17 +230,23 @@ __global__ void __launch_bounds__(READERS) read_kernel(const Read a) {
     scale_of_row[threadIdx.x] = scale;
   }
   __syncthreads();
-  // an item is 16 codes (8 at a row's end)
-  const int c_items = (k.d_c + 15) / 16, each = c_items + (k.d_r + 15) / 16;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < rows * each; i += READERS) {
-    const int r = i / each, item = i - r * each, part = item >= c_items, at = (part ? item - c_items : item) * 16;
-    const int64_t token = token_of[r];
-    if (token == -2) continue;
+  // an item is 16 codes (8 at a row's end); all of a thread's are loaded before the first is stored
+  constexpr int ITEMS = (READ_ROWS * (MAX_DC + LD_R) / 16 + READERS - 1) / READERS;
+  const int each = a.by_each.d, c_items = (k.d_c + 15) / 16;
+  uint4 codes[ITEMS];
+#pragma unroll
+  for (int l = 0; l < ITEMS; ++l) {
+    const int i = threadIdx.x + l * READERS, r = i / a.by_each, item = i - r * each, part = item >= c_items, at = (part ? item - c_items : item) * 16;
+    codes[l] = make_uint4(0, 0, 0, 0);
+    if (r < rows && token_of[r] >= 0)
+      codes[l] = *reinterpret_cast<const uint4*>(part ? k.r + token_of[r] * LD_R + at : k.c + token_of[r] * k.ld_c + at);
+  }
+#pragma unroll
+  for (int l = 0; l < ITEMS; ++l) {
+    const int i = threadIdx.x + l * READERS, r = i / a.by_each, item = i - r * each, part = item >= c_items, at = (part ? item - c_items : item) * 16;
+    if (r >= rows || token_of[r] == -2) continue;
     const float scale = part ? scale_of_row[r].y : scale_of_row[r].x;
-    uint4 codes = make_uint4(0, 0, 0, 0);
-    if (token >= 0) codes = *reinterpret_cast<const uint4*>(part ? k.r + token * LD_R + at : k.c + token * k.ld_c + at);
-    const uint32_t u[4] = {codes.x, codes.y, codes.z, codes.w};
+    const uint32_t u[4] = {codes[l].x, codes[l].y, codes[l].z, codes[l].w};
     T* out = static_cast<T*>(a.out[part]) + (first + r) * a.ld[part] + at;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -269,6 +282,8 @@ extern "C" int mk_latent_append(const MkLatent* l, const MkLatentBatch* b, const
   a.ld[1] = ldr;
   a.wide[0] = wide(c, ldc);
   a.wide[1] = wide(r, ldr);
+  a.by_c = div_by(l->d_c / 8);
+  a.by_r = div_by(l->d_r / 8);
   // a sequence's rows are in at most rows / page + 2 pages, and in no more pages than rows
   const int64_t most = b->starts ? rows / l->page + 2 * (int64_t)b->n : rows;
   const unsigned grid = (unsigned)(most < rows ? most : rows);
@@ -297,6 +312,7 @@ extern "C" int mk_latent_read(const MkLatent* l, const MkLatentBatch* b, void* c
   a.wide[0] = wide(c, ldc);
   a.wide[1] = wide(r, ldr);
   a.fill = fill != 0;
+  a.by_each = div_by((l->d_c + 15) / 16 + (l->d_r + 15) / 16);
   const unsigned grid = ((unsigned)rows + READ_ROWS - 1) / READ_ROWS;
   const cudaError_t e = launch_early(dtype == MK_BF16 ? read_kernel<__nv_bfloat16> : read_kernel<__half>, dim3(grid), READERS, 0,
                                      static_cast<cudaStream_t>(stream), a);
