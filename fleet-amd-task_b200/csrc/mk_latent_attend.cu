@@ -85,7 +85,7 @@ struct Args {
 // ---- a block's share of the units ----------------------------------------------------------
 // Runs are cut by cost, in places: a group costs its units and FIXED more (its queries, its first tile's maximum, its
 // outputs; fitted: a unit 0.8 us, a group 4.7 us).
-constexpr int FIXED = 6;
+constexpr int FIXED = 5;
 template <int R>
 __device__ __forceinline__ int groups_of(const Args& a, const Seq& q) { return (q.n * a.heads + R - 1) / R; }
 __device__ __forceinline__ int units_of(const Args& a, const Seq& q) { return max(1, (min(q.len, a.b.capacity) + UNIT - 1) / UNIT); }
@@ -929,6 +929,15 @@ int tensor_map(CUtensorMap* map, void* base, uint64_t cols, uint64_t rows, uint3
 
 constexpr int MAX_DEVICES = 64;
 
+cudaError_t multiprocessors(int device, int* n) {
+  static std::atomic<int> known[MAX_DEVICES];
+  *n = known[device].load(std::memory_order_relaxed);
+  if (*n) return cudaSuccess;
+  const cudaError_t e = cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, device);
+  if (e == cudaSuccess) known[device].store(*n, std::memory_order_relaxed);
+  return e;
+}
+
 template <typename T, int R>
 int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device, int blocks, cudaStream_t s) {
   static std::atomic<bool> ready[MAX_DEVICES];   // the kernel may use that much shared memory on the device
@@ -943,6 +952,10 @@ int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device
 }
 
 constexpr int64_t META_BYTES = (MAX_CTAS * sizeof(int4) + 255) / 256 * 256;
+// Rows of a group: 32 where that makes a group for every block (512 tokens of a prompt behind 3584: 169 us, with 16 rows
+// 196), so that a sequence's tokens are brought half as often; 16 otherwise, whose scores have two buffers in tensor
+// memory and whose tiles pass faster (8 sequences of up to 4 drafts: 17.8 us, with 32 rows 21.9).
+int rows_of_group(int64_t rows, int64_t heads) { return rows * heads >= 32 * MAX_CTAS ? 32 : 16; }
 int64_t workspace(int rows, int subs) { return META_BYTES + (int64_t)2 * MAX_CTAS * rows * (2 + subs * 128) * 4; }
 
 }  // namespace
@@ -952,7 +965,7 @@ using namespace latent;
 
 extern "C" int mk_latent_attend_workspace(const MkLatent* l, int32_t n, int32_t rows, int32_t heads, int64_t* bytes) {
   if (!l || !bytes || n < 0 || rows < 0 || heads < 1) return fail(MK_EINVAL, "null pointer or a negative size");
-  *bytes = workspace(16, (l->d_c + 127) / 128);
+  *bytes = workspace(rows_of_group(rows, heads), (l->d_c + 127) / 128);
   return MK_OK;
 }
 
@@ -967,10 +980,11 @@ extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const
   if (((uintptr_t)q | (uintptr_t)out) & 1 || (uintptr_t)lse & 3 || (uintptr_t)workspace & 255)
     return fail(MK_EINVAL, "misaligned q, out, lse or workspace (256 bytes)");
   a.subs = a.k.ld_c / 128;
-  if (workspace_bytes < latent::workspace(16, a.subs)) return fail(MK_EINVAL, "the workspace is too small");
+  const int group = rows_of_group(rows, heads);
+  if (workspace_bytes < latent::workspace(group, a.subs)) return fail(MK_EINVAL, "the workspace is too small");
   int device = 0, sms = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= MAX_DEVICES ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+      multiprocessors(device, &sms) != cudaSuccess)
     return fail(MK_ECUDA, "cudaGetDevice failed or device ordinal out of range");
   a.q = q;
   a.out = out;
@@ -990,12 +1004,14 @@ extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const
   while (groups * ((units >> a.coarse) + 1 + FIXED) > INT32_MAX && a.coarse < 31) ++a.coarse;
   a.meta = static_cast<int4*>(workspace);
   a.stat = reinterpret_cast<float*>(static_cast<char*>(workspace) + META_BYTES);
-  a.part = a.stat + (int64_t)2 * MAX_CTAS * 16 * 2;
+  a.part = a.stat + (int64_t)2 * MAX_CTAS * group * 2;
   CUtensorMap c, r;
   const uint64_t tokens = (uint64_t)a.k.pages * a.k.page;
   if (const int e = tensor_map(&c, a.k.c, a.k.ld_c, tokens, a.box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
   if (const int e = tensor_map(&r, a.k.r, LD_R, tokens, a.box, CU_TENSOR_MAP_SWIZZLE_64B)) return e;
   const int blocks = sms < MAX_CTAS ? sms : MAX_CTAS;
-  return dtype == MK_BF16 ? launch<Bf16, 16>(a, c, r, device, blocks, static_cast<cudaStream_t>(stream))
-                          : launch<Fp16, 16>(a, c, r, device, blocks, static_cast<cudaStream_t>(stream));
+  const auto s = static_cast<cudaStream_t>(stream);
+  // (FP16's three pieces of a query leave no room for 32 rows in tensor memory)
+  if (dtype == MK_FP16) return launch<Fp16, 16>(a, c, r, device, blocks, s);
+  return group == 32 ? launch<Bf16, 32>(a, c, r, device, blocks, s) : launch<Bf16, 16>(a, c, r, device, blocks, s);
 }
