@@ -9,7 +9,7 @@
 // of shared memory written and read back). So the codes go to tcgen05.mma (kind::f8f6f4) as they arrive by TMA, twice:
 // as the keys of S = K q^T (128 tokens x N, K-major) and, the same bytes, as the values of O = C^T P (128 latent
 // values x N, MN-major). What is not in 8 bits is split into pieces that are, each a column of its own, for the tensor core's
-// time goes by the 128 rows of the tile, not by N, up to 64 columns:
+// time goes by the 128 rows of the tile (32 + N / 4 clocks a product of 128 x N x 32, measured, in any layout):
 //   q    = scale_q (q1 + q2 / 16 (+ q3 / 256)) in E4M3: each piece takes 4 bits and the remainder's sign one more, so
 //          two hold a BF16 value and three an FP16 value exactly, down to 2^-23 of the row's largest;
 //   p    = x 2^-7, x rounded to FP16 = x1 + x2 / 8 + x3 / 64 in E5M2: within 2^-11 (3, 4 and 4 bits are all of FP16's
@@ -18,6 +18,11 @@
 // goes into the exponent: t = s + log2 sc, p = 2^(t - ref), so the pieces are relative to the largest p |c|, and the sum
 // of the weights takes p / sc. ref is a tile's maximum of t, taken anew (with O rescaled in tensor memory) only where some t
 // is more than 8 above it.
+//
+// What bounds it, on B200: a tile of 16 rows takes 1420 clocks of products and about 3300 in the middle of a run, which is
+// HBM's rate (6.2 of the measured 6.5 TB/s); 64 sequences of up to 8192 tokens (153 MB, 23.5 us at that rate) take 43 us, of which
+// 6 are the start (the batch's lengths, a table's page, the first tile and the queries, one after the other), 2 a
+// run's end, 5 merge_kernel. A single sequence of 32768 tokens takes 17 us, most of it those.
 //
 // The work is units of 64 tokens of a group of R rows (a row is a token's head) of a sequence; each block (one per SM)
 // takes an equal run of all units, whatever the lengths, as tiles of two. A group within one run is finished there, one
@@ -220,6 +225,8 @@ __device__ __forceinline__ void tmem_wait_load(float (&v)[N][M]) {
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Whether a barrier's phase is over. (mbarrier.try_wait may sleep, and woke up 700 to 2000 clocks late: 66 us for the 64
+// sequences of up to 8192 tokens that took 55 without it.)
 __device__ __forceinline__ bool come(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -434,13 +441,14 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
     }
     mk::fence_barrier_init();
   }
+  start_dependents();
+  wait_predecessor();
+  // (not before: a predecessor on this SM may still have to allocate tensor memory of its own)
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     fence_before();
   }
-  start_dependents();
-  wait_predecessor();
   // this block's run of the units
   Work work{};
   {
@@ -974,7 +982,7 @@ extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const
                                 void* workspace, int64_t workspace_bytes, void* stream) {
   Args a{};
   if (const int e = check(l, b, rows, dtype, a.k, a.b)) return e;
-  if (heads < 1 || heads > 1024 || (int64_t)rows * heads > INT32_MAX) return fail(MK_EINVAL, "heads are from 1 to 1024, rows x heads below 2^31");
+  if (heads < 1 || heads > 1024 || (int64_t)rows * heads > 1 << 30) return fail(MK_EINVAL, "heads are from 1 to 1024, rows x heads at most 2^30");
   if (rows == 0 || b->n == 0) return MK_OK;
   if (!q || !out || !workspace) return fail(MK_EINVAL, "null pointer");
   if (((uintptr_t)q | (uintptr_t)out) & 1 || (uintptr_t)lse & 3 || (uintptr_t)workspace & 255)

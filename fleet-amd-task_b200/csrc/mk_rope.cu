@@ -144,7 +144,7 @@ cudaError_t launch(Args a, int width, cudaStream_t s) {
   a.rest = rest - copied;
   a.group = most < a.heads ? most : a.heads;
   // whole tokens where they fit, but a block for each of the SMs first
-  const int fit = most / a.heads, held = TABLE / (a.dim / 2), spread = (a.t + 2 * SMS - 1) / (2 * SMS);
+  const int fit = most / a.heads, held = TABLE / (a.dim / 2), spread = (a.t - 1) / (2 * SMS) + 1;
   a.tokens = fit < 1 ? 1 : fit < held ? fit : held;
   a.tokens = a.tokens < spread ? a.tokens : spread;
   a.by_turned = latent::div_by(turned);

@@ -1,0 +1,136 @@
+"""The launches of the latent attention's host code without a GPU, over a CUDA runtime that records them and fails the one
+it is told to; and rules that the kernels' sources keep."""
+import ctypes
+import re
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+from fleet import mk
+
+CSRC = Path(__file__).resolve().parent.parent / "fleet-amd-task_b200" / "csrc"
+OBJ = CSRC.parent / "lib" / "obj"
+CUDA = Path(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc").resolve().parent.parent / "include"
+P = 1 << 20
+
+
+def test_every_kernel_waits_before_it_reads():
+    """Launched early, a kernel may run beside its predecessor: it waits before its first access, and nothing it is given is
+    __restrict__ (whose loads could move before the wait)."""
+    found = 0
+    for name in ("mk_rope.cu", "mk_latent.cu", "mk_latent_attend.cu"):
+        text = (CSRC / name).read_text()
+        assert "__restrict__" not in text and "__ldg" not in text
+        for m in re.finditer(r"__global__ void (?:__launch_bounds__\(.*?\) )?(\w+)\((.*?)\) \{\n(.*?)\n\}\n", text, re.S):
+            before, wait, _ = m[3].partition("wait_predecessor();")
+            assert wait, m[1]
+            assert not re.search(r"\ba\.b\.(lens|table|starts)|k\.scales|a\.(x|q|out|meta|stat|part|positions|inv_freq)\b", before), m[1]
+            found += 1
+    assert found == 5
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    objects = [OBJ / f"{n}.o" for n in ("mk_rope", "mk_latent", "mk_latent_attend")]
+    if not all(o.exists() for o in objects) or not (CUDA / "cuda_runtime.h").exists() or not shutil.which("g++"):
+        pytest.skip("needs the built objects, the CUDA headers and g++")
+    so = tmp_path_factory.mktemp("fake") / "host.so"
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-Wl,-Bsymbolic", f"-I{CUDA}", "-o", str(so),
+                    str(Path(__file__).with_name("fake_latent_cudart.cpp")), *map(str, objects)], check=True)
+    L, real = ctypes.CDLL(str(so)), mk.lib()
+    for name in ("mk_rope", "mk_latent_append", "mk_latent_read", "mk_latent_attend", "mk_latent_attend_workspace"):
+        getattr(L, name).argtypes = getattr(real, name).argtypes
+    L.fake_launches.restype = L.fake_message.restype = ctypes.c_char_p
+    return L
+
+
+def launched(host):
+    """[(kernel, grid, rows of the grid, threads, dynamic shared memory, launched early)] of the last call."""
+    rows = []
+    for line in host.fake_launches().decode().splitlines():
+        name, x, y, threads, smem, *early = line.split()
+        rows.append((re.search(r"(rope|append|read|attend|merge)_kernel", name)[1], int(x), int(y), int(threads), int(smem), bool(early)))
+    return rows
+
+
+def rope(host, t=1, heads=16, width=192, dim=64, start=128, out=2 * P, x=P, fail=-1, dtype=0):
+    r = mk.MkRope(P, dim, 0, dtype, 1, 1.0, 0)
+    host.fake_begin(fail)
+    return host.mk_rope(ctypes.addressof(r), P, t, x, heads * width, width, heads, width, start, out, heads * width, width, None)
+
+
+def latent(host, call, rows=3, n=3, starts=None, page=64, d_c=512, d_r=64, pages=100, width=40, heads=16, dtype=0, lse=None, fail=-1, nbytes=None, ws=P):
+    l = mk.MkLatent(P, P, P, pages, page, d_c, d_r)
+    b = mk.MkLatentBatch(P, P, starts, width, n, width)
+    pl, pb = ctypes.addressof(l), ctypes.addressof(b)
+    host.fake_begin(fail)
+    if call == "append":
+        return host.mk_latent_append(pl, pb, P, d_c, P, d_r, rows, dtype, None)
+    if call == "read":
+        return host.mk_latent_read(pl, pb, P, d_c, P, d_r, rows, dtype, 1, None)
+    need = ctypes.c_int64()
+    assert host.mk_latent_attend_workspace(pl, n, rows, heads, ctypes.byref(need)) == mk.MK_OK
+    return host.mk_latent_attend(pl, pb, P, heads * (d_c + d_r), d_c + d_r, rows, heads, dtype, 1.0, P, heads * d_c, d_c, lse, ws,
+                                 need.value if nbytes is None else nbytes + need.value, None)
+
+
+def test_one_launch_or_two(host):
+    assert rope(host) == mk.MK_OK and [v[0] for v in launched(host)] == ["rope"]
+    for call, kernels in (("append", ["append"]), ("read", ["read"]), ("attend", ["attend", "merge"])):
+        assert latent(host, call) == mk.MK_OK
+        assert [v[0] for v in launched(host)] == kernels
+        assert all(v[5] for v in launched(host))
+
+
+def test_a_launch_that_fails_ends_the_call(host):
+    assert rope(host, fail=0) == mk.MK_ECUDA and host.fake_message() == b"a launch that was told to fail"
+    for call in ("append", "read", "attend"):
+        assert latent(host, call, fail=0) == mk.MK_ECUDA and len(launched(host)) == 1
+    assert latent(host, "attend", fail=1) == mk.MK_ECUDA and len(launched(host)) == 2
+
+
+@pytest.mark.parametrize("t,heads,width,dim,start", [(1, 1, 2, 2, 0), (2 ** 31 - 1, 1, 16, 16, 0), (2 ** 31 - 1, 1, 2, 2, 0), (1, 65535, 512, 512, 0),
+                                                     (7, 65535, 32000, 2, 31998), (100000, 128, 192, 64, 128), (3, 5, 33, 30, 1)])
+def test_rope_grids(host, t, heads, width, dim, start):
+    """Every head of every token is some block's, whatever the sizes, within a grid's limits."""
+    for x in (P, P + 2):
+        assert rope(host, t, heads, width, dim, start, x=x) == mk.MK_OK
+        (_, gx, gy, threads, smem, _), = launched(host)
+        assert 1 <= gx < 2 ** 31 and 1 <= gy <= 65535 and threads == 256 and smem == 0
+
+
+def test_pages_at_most(host):
+    """append has a block for each page that rows can be in: rows / page + 2 a sequence, and no more than rows."""
+    for rows, n, page in ((1, 1, 16), (10, 3, 16), (10, 10, 128), (8192, 1, 64), (1000, 7, 16), (2 ** 31 - 1, 1, 128)):
+        assert latent(host, "append", rows, n, starts=P, page=page) == mk.MK_OK
+        assert launched(host)[0][1] == min(rows, rows // page + 2 * n)
+    assert latent(host, "append", 50, 50) == mk.MK_OK and launched(host)[0][1] == 50
+    for page, d_c, d_r in ((128, 512, 64), (64, 512, 64), (16, 8, 8)):      # a page's values fit the threads' registers
+        held = {1: 1, 9: 9, 18: 18}
+        assert latent(host, "append", 4096, 1, starts=P, page=page, d_c=d_c, d_r=d_r) == mk.MK_OK
+        name = host.fake_launches().decode().split()[0]
+        loads = int(re.search(r"Li(\d+)E", name)[1])
+        assert loads in held and loads * 512 * 8 >= page * (d_c + d_r)
+        assert latent(host, "append", 3, 3, page=page, d_c=d_c, d_r=d_r) == mk.MK_OK
+
+
+def test_attend_forms(host):
+    form = lambda: re.search(r"(Bf16|Fp16)ELi(\d+)E", host.fake_launches().decode()).groups()  # noqa: E731
+    for rows, heads, dtype, want in ((1, 16, 0, ("Bf16", "16")), (295, 16, 0, ("Bf16", "16")), (296, 16, 0, ("Bf16", "32")), (296, 16, 1, ("Fp16", "16")),
+                                     (37, 128, 0, ("Bf16", "32"))):
+        assert latent(host, "attend", rows, 1, starts=P, heads=heads, dtype=dtype) == mk.MK_OK
+        assert form() == want
+        assert all(v[1] in (148, 296) and v[4] <= 232448 for v in launched(host))
+
+
+def test_attend_refusals(host):
+    assert latent(host, "attend", nbytes=-1) == mk.MK_EINVAL and b"workspace" in host.fake_message()
+    assert latent(host, "attend", ws=P + 128) == mk.MK_EINVAL
+    assert latent(host, "attend", ws=None) == mk.MK_EINVAL
+    assert latent(host, "attend", rows=2 ** 21, n=1, starts=P, heads=1024) == mk.MK_EINVAL
+    assert latent(host, "attend", rows=2 ** 20, n=1, starts=P, heads=1024) == mk.MK_OK
+    # places near 2^31: counted in coarser ones
+    assert latent(host, "attend", rows=2 ** 20, n=1, starts=P, heads=1024, width=2 ** 24, pages=2 ** 24) == mk.MK_OK
+    assert not launched(host)[0][0] == "merge"
