@@ -82,6 +82,21 @@ __device__ __forceinline__ uint16_t encode2(float a, float b) {      // NaN stay
 template <int THREADS, typename Count, typename Which>
 __device__ __forceinline__ void locate(int n, Count count, Which which, int& item, int& place) {
   __shared__ int warps[THREADS / 32], found[2];
+  if (n <= 32) {                // every warp by itself, an item a lane
+    const int i = threadIdx.x & 31, mine = i < n ? count(i) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (i >= o) upto += v;
+    }
+    const int at = which(__shfl_sync(0xFFFFFFFFu, upto, 31));
+    const uint32_t holds = __ballot_sync(0xFFFFFFFFu, at >= upto - mine && at < upto);
+    const int lane = holds ? __ffs(holds) - 1 : 0;
+    item = holds ? lane : n;
+    place = at - __shfl_sync(0xFFFFFFFFu, upto - mine, lane);
+    return;
+  }
   const int per = (n + THREADS - 1) / THREADS, lo = min((int)threadIdx.x * per, n), hi = min(lo + per, n);
   int mine = 0;
   for (int i = lo; i < hi; ++i) mine += count(i);

@@ -27,8 +27,9 @@
 // The work is units of 64 tokens of a group of R rows (a row is a token's head) of a sequence; each block (one per SM)
 // takes an equal run of all units, whatever the lengths, as tiles of two. A group within one run is finished there, one
 // that several runs share leaves partial sums, which merge_kernel joins. Warps 0 to 7 are the softmax: a warp holds 32 of a
-// tile's 128 tokens (the lanes of tensor memory that it may read) for half of the rows. Warp 8 loads, warp 9 issues the scores' products and
-// warp 10 the sums': each only ever waits for what comes next.
+// tile's 128 tokens (the lanes of tensor memory that it may read) for half of the rows. Warp 9 issues the scores' products and
+// warp 10 the sums', warps 8 and 11 the loads (every other page each: a copy takes 80 clocks to issue); each only ever waits
+// for what comes next.
 #include <cuda.h>
 
 #include <atomic>
@@ -44,7 +45,7 @@ using mk::mbar_arrive;
 using mk::mbar_init;
 using mk::smem_u32;
 
-constexpr int MAX_CTAS = 148, TILE = 128, UNIT = 64, THREADS = 352, SOFTMAX = 256;
+constexpr int MAX_CTAS = 148, TILE = 128, UNIT = 64, THREADS = 384, SOFTMAX = 256, LOADERS = 2;
 constexpr int SUB = TILE * 128, STAGE = 4 * SUB + TILE * LD_R;      // a tile: up to 4 x [128 tokens][128 B], then [128][64 B]
 constexpr uint64_t TIMEOUT_NS = 2000000000ull;
 constexpr float X_SCALE = 7.0f, RAISE = 8.0f;                       // x = 2^7 at ref, 2^15 at most
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
 
   if (warp == 8) {
     if (lane < 2) {
-      mbar_init(&sh.full[lane], 1);
+      mbar_init(&sh.full[lane], LOADERS);
       mbar_init(&sh.empty[lane], 1);
       mbar_init(&sh.drained[lane], 1);
       mbar_init(&sh.scored[lane], 1);
@@ -487,16 +488,18 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   Segment s;
   int it = 0;                   // tiles so far
 
-  if (warp == 8) {
+  if (warp == 8 || warp == 11) {
     // ---- loads: a tile's pages, and the scales of their tokens
     bool ok = true;
-    const int each = a.box / 16;                                // a box's first 16 tokens name its page
+    // this loader's boxes: every other one (a box's first 16 tokens name its page)
+    const int each = a.box / 16, loader = warp == 11;
     const uint32_t elected = elect_one();
     while (ok && next<R>(a, work, s)) {
       for (int t = 0; t < s.tiles; ++t, ++it) {
         const int st = it & 1, pos0 = s.u0 * UNIT + t * TILE, pos = pos0 + 16 * lane;
         int page = -1;
-        if (lane < TILE / 16 && pos < s.end) {
+        const bool mine = lane < TILE / 16 && lane / each % LOADERS == loader;
+        if (mine && pos < s.end) {
           page = a.b.table[s.s * a.b.ldt + (pos >> k.shift)];
           if (page >= k.pages) page = -1;
         }
@@ -507,15 +510,17 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         if (lane == 0) expect_bytes(full, rows * (a.subs * 128 + LD_R));
         __syncwarp();
 #pragma unroll 1
-        for (int from = 0; from < TILE / 16; from += each) {
+        for (int from = loader * each; from < TILE / 16; from += LOADERS * each) {
           const int at = __shfl_sync(~0u, y, from), named = __shfl_sync(~0u, page, from);
           const uint32_t issues = elected != 0 && named >= 0;
           copy(to + 4 * SUB + from * 16 * LD_R, &map_r, 0, at, full, issues);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            copy(to + j * SUB + from * 16 * 128, &map_c, j * 128, at, full, issues && j < a.subs);
+          for (int j = 0; j < 4; ++j) {
+            if (j >= a.subs) break;
+            copy(to + j * SUB + from * 16 * 128, &map_c, j * 128, at, full, issues);
+          }
         }
-        if (lane < TILE / 16) {
+        if (mine) {
           float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           if (page >= 0) {
             const float2 scale = *reinterpret_cast<const float2*>(k.scales + 2 * (int64_t)page);
