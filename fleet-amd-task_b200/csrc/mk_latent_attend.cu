@@ -786,7 +786,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
           for (int j = half; j < a.subs; j += 2)
 #pragma unroll 1
             for (int i = 0; i < 8; ++i) {
-              uint4* at = reinterpret_cast<uint4*>(smem + st * STAGE + j * SUB + tok * 128 + i * 16);
+              // (the lanes' rows begin in one bank: each begins at a cell of its own)
+              uint4* at = reinterpret_cast<uint4*>(smem + st * STAGE + j * SUB + tok * 128 + (i ^ (tok & 7)) * 16);
               uint4 u = make_uint4(0, 0, 0, 0);
               if (!none) {
                 u = *at;
