@@ -78,17 +78,14 @@ class LatentCache:
         self.tensors = self._c, self._r, self.scales
         self._need = {}            # (sequences, rows, heads) -> workspace bytes
 
-    def _batch(self, batch, rows):
+    def _refuse_batch(self, batch, rows):
         if batch.index != self.index:
             raise ValueError(f"the batch is on {batch.lens.device}, the cache on {self.device}")
-        if batch.starts is None and rows != batch.n:
-            raise ValueError(f"without starts a batch has one row for each of its {batch.n} sequences, got {rows} rows")
+        raise ValueError(f"without starts a batch has one row for each of its {batch.n} sequences, got {rows} rows")
 
-    def _rows(self, t, d, name, dtype=None, T=None):
-        if t.dim() != 2 or t.shape[1] != d or t.stride(1) != 1 or t.get_device() != self.index or \
-                (t.dtype not in DTYPES if dtype is None else t.dtype is not dtype) or (T is not None and t.shape[0] != T):
-            raise ValueError(f"{name}: {dtype or 'bfloat16 or float16'} [{'rows' if T is None else T}, {d}] with unit stride along its rows on "
-                             f"{self.device} expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()} on {t.device}")
+    def _refuse(self, t, d, name, dtype=None, T=None):
+        raise ValueError(f"{name}: {dtype or 'bfloat16 or float16'} [{'rows' if T is None else T}, {d}] with unit stride along its rows on "
+                         f"{self.device} expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()} on {t.device}")
 
     def append(self, c_kv, k_pe, batch, stream=None):
         """Write the rows' latents c_kv [rows, d_c] (after their norm) and rotary keys k_pe [rows, d_r] (after
@@ -104,11 +101,16 @@ class LatentCache:
         index = self.index
         if index < 0 or device() != index:
             return mk.off_device("mk_latent_append", index, context, lambda: self.append(c_kv, k_pe, batch))
-        self._rows(c_kv, self.d_c, "c_kv")
+        dtype = c_kv.dtype
+        if c_kv.dim() != 2 or c_kv.shape[1] != self.d_c or c_kv.stride(1) != 1 or c_kv.get_device() != index or dtype not in DTYPES:
+            self._refuse(c_kv, self.d_c, "c_kv")
         rows = c_kv.shape[0]
-        self._rows(k_pe, self.d_r, "k_pe", c_kv.dtype, rows)
-        self._batch(batch, rows)
-        rc = call(self.ptr, batch.ptr, c_kv.data_ptr(), c_kv.stride(0), k_pe.data_ptr(), k_pe.stride(0), rows, DTYPES[c_kv.dtype],
+        if k_pe.dim() != 2 or k_pe.shape[1] != self.d_r or k_pe.shape[0] != rows or k_pe.stride(1) != 1 or k_pe.get_device() != index or \
+                k_pe.dtype is not dtype:
+            self._refuse(k_pe, self.d_r, "k_pe", dtype, rows)
+        if batch.index != index or (batch.starts is None and rows != batch.n):
+            self._refuse_batch(batch, rows)
+        rc = call(self.ptr, batch.ptr, c_kv.data_ptr(), c_kv.stride(0), k_pe.data_ptr(), k_pe.stride(0), rows, DTYPES[dtype],
                   current_stream(index))
         if rc:
             mk._check(rc, "mk_latent_append")
@@ -126,20 +128,24 @@ class LatentCache:
             return mk.off_device("mk_latent_read", index, context, lambda: self.read(batch, rows, dtype, out))
         if dtype not in DTYPES:
             raise TypeError(f"dtype is bfloat16 or float16, not {dtype}")
-        self._batch(batch, rows)
-        fill = out is None
+        if batch.index != index or (batch.starts is None and rows != batch.n):
+            self._refuse_batch(batch, rows)
+        d_c, d_r, fill = self.d_c, self.d_r, out is None
         if fill:
-            out = (torch.empty_strided((rows, self.d_c), (self.d_c, 1), dtype=dtype, device=self.device),
-                   torch.empty_strided((rows, self.d_r), (self.d_r, 1), dtype=dtype, device=self.device))
-        c, r = out
-        if not fill:
-            self._rows(c, self.d_c, "out[0]", dtype, rows)
-            self._rows(r, self.d_r, "out[1]", dtype, rows)
+            c = torch.empty_strided((rows, d_c), (d_c, 1), dtype=dtype, device=self.device)
+            r = torch.empty_strided((rows, d_r), (d_r, 1), dtype=dtype, device=self.device)
+            ldc, ldr = d_c, d_r
+        else:
+            c, r = out
+            for t, d, name in ((c, d_c, "out[0]"), (r, d_r, "out[1]")):
+                if t.dim() != 2 or t.shape[1] != d or t.shape[0] != rows or t.stride(1) != 1 or t.get_device() != index or t.dtype is not dtype:
+                    self._refuse(t, d, name, dtype, rows)
+            ldc, ldr = c.stride(0), r.stride(0)
             if rows > 1 and (c.stride(0) < self.d_c or r.stride(0) < self.d_r):
                 raise ValueError(f"out: rows overlap (strides {c.stride(0)} and {r.stride(0)})")
             if (overlap(c, r) and not _beside(c, r)) or any(t is not None and overlap(o, t) for o in out for t in (*self.tensors, *batch.tensors)):
                 raise ValueError("out: its tensors are apart from one another, the cache and the batch")
-        rc = call(self.ptr, batch.ptr, c.data_ptr(), c.stride(0), r.data_ptr(), r.stride(0), rows, DTYPES[dtype], fill,
+        rc = call(self.ptr, batch.ptr, c.data_ptr(), ldc, r.data_ptr(), ldr, rows, DTYPES[dtype], fill,
                   current_stream(index))
         if rc:
             mk._check(rc, "mk_latent_read")
@@ -170,31 +176,31 @@ class LatentCache:
         index = self.index
         if index < 0 or device() != index:
             return mk.off_device("mk_latent_attend", index, context, lambda: self.attend(q, batch, scale, out, return_lse))
-        d = self.d_c + self.d_r
-        if q.dim() != 3 or q.shape[2] != d or q.stride(2) != 1 or q.get_device() != index or q.dtype not in DTYPES:
-            raise ValueError(f"q: bfloat16 or float16 [rows, heads, {d}] with unit stride along its values on {self.device} expected, got "
+        d_c, dtype = self.d_c, q.dtype
+        if q.dim() != 3 or q.shape[2] != d_c + self.d_r or q.stride(2) != 1 or q.get_device() != index or dtype not in DTYPES:
+            raise ValueError(f"q: bfloat16 or float16 [rows, heads, {d_c + self.d_r}] with unit stride along its values on {self.device} expected, got "
                              f"{q.dtype} {tuple(q.shape)}, strides {q.stride()} on {q.device}")
         rows, heads, _ = q.shape
-        self._batch(batch, rows)
-        shape = (rows, heads, self.d_c)
+        if batch.index != index or (batch.starts is None and rows != batch.n):
+            self._refuse_batch(batch, rows)
         if out is None:
-            out = torch.empty_strided(shape, (heads * self.d_c, self.d_c, 1), dtype=q.dtype, device=self.device)
+            ot, oh = heads * d_c, d_c
+            out = torch.empty_strided((rows, heads, d_c), (ot, oh, 1), dtype=dtype, device=self.device)
         else:
-            if out.shape != shape or out.dtype != q.dtype or out.get_device() != index or out.stride(2) != 1:
-                raise ValueError(f"out: {q.dtype} {shape} with unit stride along its values on {self.device} expected, got "
+            shape = (rows, heads, d_c)
+            if out.shape != shape or out.dtype != dtype or out.get_device() != index or out.stride(2) != 1:
+                raise ValueError(f"out: {dtype} {shape} with unit stride along its values on {self.device} expected, got "
                                  f"{out.dtype} {tuple(out.shape)}, strides {out.stride()} on {out.device}")
             if not _apart(shape, out.stride()):
-                raise ValueError(f"out: heads overlap (strides {out.stride()}, {self.d_c} values)")
+                raise ValueError(f"out: heads overlap (strides {out.stride()}, {d_c} values)")
             if any(t is not None and overlap(out, t) for t in (q, *self.tensors, *batch.tensors)):
                 raise ValueError("out is apart from q, the cache and the batch")
+            ot, oh, _ = out.stride()
         lse = torch.empty_strided((rows, heads), (heads, 1), dtype=torch.float32, device=self.device) if return_lse else None
-        nbytes = self._need.get((batch.n, rows, heads))
-        if nbytes is None:
-            nbytes = self.workspace_bytes(batch.n, rows, heads)
+        nbytes = self._need.get((batch.n, rows, heads)) or self.workspace_bytes(batch.n, rows, heads)
         ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=self.device)
         qt, qh, _ = q.stride()
-        ot, oh, _ = out.stride()
-        rc = call(self.ptr, batch.ptr, q.data_ptr(), qt, qh, rows, heads, DTYPES[q.dtype], scale, out.data_ptr(), ot, oh,
+        rc = call(self.ptr, batch.ptr, q.data_ptr(), qt, qh, rows, heads, DTYPES[dtype], scale, out.data_ptr(), ot, oh,
                   lse.data_ptr() if return_lse else None, ws.data_ptr(), nbytes, current_stream(index))
         if rc:
             mk._check(rc, "mk_latent_attend")

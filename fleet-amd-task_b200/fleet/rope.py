@@ -64,7 +64,7 @@ class Rope:
         self.dim, self.layout, self.scale = 2 * inv_freq.shape[0], layout, float(scale)
         self.device = inv_freq.device
         self.index = -1 if inv_freq.device.index is None else inv_freq.device.index
-        self._c = {}           # (dtype, dtype of the positions) -> struct and its address
+        self._c, self._structs = {}, []        # (dtype, dtype of the positions) -> a struct's address
 
     @classmethod
     def yarn(cls, dim, layout="pairs_to_half", device="cuda", **parameters):
@@ -76,13 +76,12 @@ class Rope:
         return cls(inv.to(device), scale, layout)
 
     def _params(self, dtype, positions):
-        p = self._c.get((dtype, positions))
-        if p is None:
-            if dtype not in DTYPES or positions not in POSITIONS:
-                raise TypeError(f"x is bfloat16 or float16 and positions are int32 or int64, not {dtype} and {positions}")
-            c = mk.MkRope(self.inv_freq.data_ptr(), self.dim, LAYOUTS[self.layout], DTYPES[dtype], POSITIONS[positions], self.scale, 0)
-            p = self._c[(dtype, positions)] = c, ctypes.addressof(c)
-        return p[1]
+        if dtype not in DTYPES or positions not in POSITIONS:
+            raise TypeError(f"x is bfloat16 or float16 and positions are int32 or int64, not {dtype} and {positions}")
+        c = mk.MkRope(self.inv_freq.data_ptr(), self.dim, LAYOUTS[self.layout], DTYPES[dtype], POSITIONS[positions], self.scale, 0)
+        self._structs.append(c)
+        p = self._c[(dtype, positions)] = ctypes.addressof(c)
+        return p
 
     def __call__(self, x, positions, start=0, out=None, stream=None):
         if stream is not None:
@@ -97,16 +96,16 @@ class Rope:
                 raise ValueError(f"out: {x.dtype} {tuple(x.shape)} expected, got {out.dtype} {tuple(out.shape)}")
             y = self(x[:, None], positions, start, None if out is None else out[:, None])
             return y[:, 0] if out is None else out
-        if x.dim() != 3 or x.get_device() != index or (x.shape[2] > 1 and x.stride(2) != 1):
+        if x.dim() != 3 or x.get_device() != index or (x.stride(2) != 1 and x.shape[2] > 1):
             raise ValueError(f"x [T, heads, width] with unit stride along width on {self.device} expected, got "
                              f"{tuple(x.shape)}, strides {x.stride()} on {x.device}")
         T, H, W = x.shape
-        if positions.shape != (T,) or positions.get_device() != index or (T > 1 and positions.stride(0) != 1):
+        xt, xh, _ = x.stride()
+        if positions.dim() != 1 or positions.shape[0] != T or positions.get_device() != index or (T > 1 and positions.stride(0) != 1):
             raise ValueError(f"positions: contiguous [{T}] on {self.device} expected, got {tuple(positions.shape)} on {positions.device}")
         if not 0 <= start <= W - self.dim:
             raise ValueError(f"the {self.dim} rotary values from {start} on do not lie within a head of {W}")
-        params = self._params(x.dtype, positions.dtype)
-        xt, xh, _ = x.stride()
+        params = self._c.get((x.dtype, positions.dtype)) or self._params(x.dtype, positions.dtype)
         if out is None:
             out = torch.empty_strided((T, H, W), (H * W, W, 1), dtype=x.dtype, device=x.device)
             ot, oh = H * W, W
