@@ -15,12 +15,14 @@
 // loads are on their way, then all is turned and stored. Nothing of the block is stored before all of it is loaded,
 // so the output may be the input even where the layout changes.
 //
-// 8192 tokens of 16 heads of 192 values, the last 64 turned: 101 MB, a floor of 15.4 us.
+// 8192 tokens of 16 heads of 192 values, the last 64 turned: 101 MB, a floor of 15.4 us; 17.5 us on the device.
 #include "mk_latent.cuh"
 
 namespace {
 
-constexpr int THREADS = 256, MAX_DIM = 512, TABLE = 1024, COPIES = 4, SMS = 148;     // TABLE: pairs whose turns a block holds
+constexpr int MAX_DIM = 512, TABLE = 1024, COPIES = 4, SMS = 148;     // TABLE: pairs whose turns a block holds
+// threads of a block: a head's pairs at least; for the wide form 128 (8192 tokens: 17.5 us, 256 threads 19.0, 512 20.7)
+__host__ __device__ constexpr int threads_of(int vec) { return vec == 8 ? 128 : MAX_DIM / 2; }
 
 using latent::Div;
 using latent::fail;
@@ -38,11 +40,15 @@ struct Args {
   float scale;
 };
 
+__device__ __forceinline__ void two(__nv_bfloat16* d, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(d) = __floats2bfloat162_rn(a, b); }
+__device__ __forceinline__ void two(__half* d, float a, float b) { *reinterpret_cast<__half2*>(d) = __floats2half2_rn(a, b); }
+
 template <typename T, int VEC>
 struct Vec { alignas(VEC * sizeof(T)) T v[VEC]; };
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
+__global__ void __launch_bounds__(threads_of(VEC)) rope_kernel(const Args a) {
+  constexpr int THREADS = threads_of(VEC);
   __shared__ float2 turn[TABLE];        // (cos, sin) times the scale
   __shared__ bool live[TABLE];
   using V = Vec<T, VEC>;
@@ -96,18 +102,23 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const Args a) {
   if (turns && live[tok]) {
     const float2* cs = turn + tok * pairs + i * VEC;
     V lo, hi;
+    float ra[VEC], rb[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       // split: pair j of the 2 VEC neighbours u, w
       const float va = to_f32(split ? (2 * j < VEC ? u.v[2 * j % VEC] : w.v[2 * j % VEC]) : u.v[j]);
       const float vb = to_f32(split ? (2 * j + 1 < VEC ? u.v[(2 * j + 1) % VEC] : w.v[(2 * j + 1) % VEC]) : w.v[j]);
-      const T ra = latent::from_f32<T>(va * cs[j].x - vb * cs[j].y), rb = latent::from_f32<T>(vb * cs[j].x + va * cs[j].y);
-      if (join) {
-        (2 * j < VEC ? lo.v[2 * j % VEC] : hi.v[2 * j % VEC]) = ra;
-        (2 * j + 1 < VEC ? lo.v[(2 * j + 1) % VEC] : hi.v[(2 * j + 1) % VEC]) = rb;
-      } else {
-        lo.v[j] = ra;
-        hi.v[j] = rb;
+      ra[j] = va * cs[j].x - vb * cs[j].y;
+      rb[j] = vb * cs[j].x + va * cs[j].y;
+    }
+    if constexpr (VEC == 1) {
+      lo.v[0] = latent::from_f32<T>(ra[0]);
+      hi.v[0] = latent::from_f32<T>(rb[0]);
+    } else {                    // two values a conversion
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) {
+        two(lo.v + 2 * j, join ? ra[j] : ra[2 * j], join ? rb[j] : ra[2 * j + 1]);
+        two(hi.v + 2 * j, join ? ra[j + VEC / 2] : rb[2 * j], join ? rb[j + VEC / 2] : rb[2 * j + 1]);
       }
     }
     T* p = out + tok * a.ot + h * a.oh + a.start;
@@ -137,7 +148,7 @@ template <typename T>
 cudaError_t launch(Args a, int width, cudaStream_t s) {
   const bool wide = ((uintptr_t)a.x | (uintptr_t)a.out) % 16 == 0 && (a.xt | a.xh | a.ot | a.oh) % 8 == 0 &&
                     a.dim % 16 == 0 && a.start % 8 == 0 && width % 8 == 0;
-  const int vec = wide ? 8 : 1, turned = a.dim / 2 / vec, rest = a.x != a.out ? (width - a.dim) / vec : 0;
+  const int vec = wide ? 8 : 1, THREADS = threads_of(vec), turned = a.dim / 2 / vec, rest = a.x != a.out ? (width - a.dim) / vec : 0;
   const int copied = rest <= THREADS * COPIES ? rest : 0;
   int most = THREADS / turned;                  // heads that a block's threads hold
   if (copied > 0 && THREADS * COPIES / copied < most) most = THREADS * COPIES / copied;

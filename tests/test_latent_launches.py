@@ -98,7 +98,7 @@ def test_rope_grids(host, t, heads, width, dim, start):
     for x in (P, P + 2):
         assert rope(host, t, heads, width, dim, start, x=x) == mk.MK_OK
         (_, gx, gy, threads, smem, _), = launched(host)
-        assert 1 <= gx < 2 ** 31 and 1 <= gy <= 65535 and threads == 256 and smem == 0
+        assert 1 <= gx < 2 ** 31 and 1 <= gy <= 65535 and threads in (128, 256) and smem == 0
 
 
 def test_pages_at_most(host):
