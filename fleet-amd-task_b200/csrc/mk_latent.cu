@@ -10,14 +10,15 @@
 // All of a page's new values are loaded at once and kept in registers (16 bytes a load, 18 loads a thread at most), so they
 // are read once, and their loads do not wait for one another.
 //
-// read: code x scale of each row, rounded once (exact in BF16): a block takes 32 rows, resolves their places, then each
-// thread widens 16 codes at a time.
+// read: code x scale of each row, rounded once (exact in BF16): a warp resolves the places of the block's 16 rows (32 rows:
+// 12.5 us for 16384 tokens, with 16 10.3), then each thread widens 8 codes at a
+// time.
 #include "mk_latent.cuh"
 
 namespace latent {
 namespace {
 
-constexpr int THREADS = 512, READERS = 256, READ_ROWS = 32;
+constexpr int THREADS = 512, READERS = 256, READ_ROWS = 16;
 
 // 8 values of a row, to 16-byte aligned memory or one by one
 template <typename T>
@@ -62,10 +63,14 @@ __device__ __forceinline__ int pages_of(const Cache& k, const Batch& b, const Se
   return hi > lo ? ((hi - 1) >> k.shift) - first + 1 : 0;
 }
 
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <> struct Pair<__half> { using type = __half2; };
+
 // LOADS: eights of values that a thread holds, enough for a page's
 template <typename T, int LOADS>
 __global__ void __launch_bounds__(THREADS) append_kernel(const Write a) {
-  __shared__ float most[2][THREADS / 32];
+  __shared__ uint32_t most[2][THREADS / 32];
   const Cache& k = a.k;
   start_dependents();
   wait_predecessor();
@@ -91,7 +96,8 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Write a) {
     token = part ? e / a.by_r : e / a.by_c;
     at = (e - token * (part ? r_eights : c_eights)) * 8;
   };
-  union Eight { uint4 u; T t[8]; } v[LOADS];
+  using T2 = typename Pair<T>::type;
+  union Eight { uint4 u; T t[8]; T2 pair[4]; } v[LOADS];
 #pragma unroll
   for (int l = 0; l < LOADS; ++l) {
     const int i = threadIdx.x + l * THREADS;
@@ -112,32 +118,53 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Write a) {
   if (p < 0 || p >= k.pages) return;
   float2 old = make_float2(0.0f, 0.0f);
   if (lo > 0) old = *reinterpret_cast<const float2*>(k.scales + 2 * (int64_t)p);
-  float amax[2] = {0.0f, 0.0f};
+  // the largest |x| as bits, whose order that of numbers above 0 is, NaN's above infinity's; only where something is not finite
+  // the finite values' apart
+  const auto largest = [&](bool finite, uint32_t (&out)[2]) {
+    uint32_t top[2] = {0, 0};
 #pragma unroll
-  for (int l = 0; l < LOADS; ++l) {
-    if (threadIdx.x + l * THREADS >= items) break;
-    float big = 0.0f;
+    for (int l = 0; l < LOADS; ++l) {
+      if (threadIdx.x + l * THREADS >= items) break;
+      uint32_t big;
+      if (finite) {
+        float m = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) big = fmaxf(big, finite_abs(to_f32(v[l].t[e])));
-    const int part = part_of(threadIdx.x + l * THREADS);
-    amax[0] = part ? amax[0] : fmaxf(amax[0], big);
-    amax[1] = part ? fmaxf(amax[1], big) : amax[1];
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(to_f32(v[l].t[e])));
+        big = __float_as_uint(m);
+      } else {
+        const auto m = __hmax2_nan(__hmax2_nan(__habs2(v[l].pair[0]), __habs2(v[l].pair[1])), __hmax2_nan(__habs2(v[l].pair[2]), __habs2(v[l].pair[3])));
+        big = __float_as_uint(to_f32(__hmax_nan(m.x, m.y)));
+      }
+      const int part = part_of(threadIdx.x + l * THREADS);
+      top[0] = part ? top[0] : max(top[0], big);
+      top[1] = part ? max(top[1], big) : top[1];
+    }
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      top[part] = __reduce_max_sync(0xFFFFFFFFu, top[part]);
+      if (lane == 0) most[part][warp] = top[part];
+    }
+    __syncthreads();            // (and every thread has the old scales)
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      out[part] = 0;
+#pragma unroll
+      for (int w = 0; w < THREADS / 32; ++w) out[part] = max(out[part], most[part][w]);
+    }
+  };
+  constexpr uint32_t INF = 0x7F800000u;
+  uint32_t top[2];
+  largest(false, top);
+  const bool odd = top[0] >= INF || top[1] >= INF;
+  if (odd) {
+    __syncthreads();
+    largest(true, top);
   }
-#pragma unroll
-  for (int part = 0; part < 2; ++part) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax[part] = fmaxf(amax[part], __shfl_xor_sync(0xFFFFFFFFu, amax[part], o));
-    if (lane == 0) most[part][warp] = amax[part];
-  }
-  __syncthreads();              // (and every thread has the old scales)
   float scale[2], inv[2];
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
-    float big = 0.0f;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) big = fmaxf(big, most[part][w]);
     const float was = part ? old.y : old.x;
-    scale[part] = scale_of(big);
+    scale[part] = scale_of(__uint_as_float(top[part]));
     if (lo > 0) scale[part] = fmaxf(scale[part], was);
     inv[part] = 1.0f / scale[part];
     const int ld = part ? LD_R : k.ld_c, eights = part ? r_eights : c_eights;
@@ -169,7 +196,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Write a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       x[e] = to_f32(v[l].t[e]);
-      x[e] = isfinite(x[e]) ? x[e] * by : nan;
+      x[e] = odd && !isfinite(x[e]) ? nan : x[e] * by;
     }
     uint8_t* codes = part ? k.r + (((int64_t)p << k.shift) + lo + token) * LD_R : k.c + (((int64_t)p << k.shift) + lo + token) * k.ld_c;
     *reinterpret_cast<uint2*>(codes + at) = make_uint2(encode2(x[0], x[1]) | (uint32_t)encode2(x[2], x[3]) << 16,
@@ -189,14 +216,14 @@ struct Read {
 template <typename T>
 __global__ void __launch_bounds__(READERS) read_kernel(const Read a) {
   __shared__ int64_t token_of[READ_ROWS];               // a row's token in the cache, -1: in none, -2: the row is left alone
-  __shared__ float2 scale_of_row[READ_ROWS];
+  __shared__ int page_of[READ_ROWS];
+  __shared__ int begun;
   const Cache& k = a.k;
   start_dependents();
   wait_predecessor();
   const int first = blockIdx.x * READ_ROWS, rows = min(READ_ROWS, a.b.rows - first);
-  // the sequences that start at or before the block's first row: all threads count, a search would wait for each of its steps
-  __shared__ int begun;
-  if (a.b.starts) {
+  const bool few = a.b.n <= 32;
+  if (a.b.starts && !few) {     // the sequences that start at or before the block's first row: all threads count them
     if (threadIdx.x == 0) begun = 0;
     __syncthreads();
     int mine = 0;
@@ -205,60 +232,71 @@ __global__ void __launch_bounds__(READERS) read_kernel(const Read a) {
     if (threadIdx.x % 32 == 0 && mine > 0) atomicAdd(&begun, mine);
     __syncthreads();
   }
-  if ((int)threadIdx.x < rows) {
-    const int row = first + threadIdx.x;
+  if (threadIdx.x < 32) {       // a lane for each row
+    const int lane = threadIdx.x, row = first + lane;
     int s = row;
-    if (a.b.starts)             // the last one that starts at or before the row
-      for (s = begun - 1; s + 1 < a.b.n && a.b.starts[s + 1] <= row;) ++s;
+    Seq q{0, 0, 0};
+    if (a.b.starts && few) {    // a lane for each sequence too: the last that starts at or before the row, by halves
+      const int start = lane < a.b.n ? a.b.starts[lane] : INT32_MAX;
+      const Seq held = lane < a.b.n ? sequence(a.b, lane) : q;
+      s = -1;
+#pragma unroll
+      for (int step = 32; step >= 1; step /= 2) {
+        const int next = s + step, there = __shfl_sync(0xFFFFFFFFu, start, min(next, 31));
+        if (next < a.b.n && there <= row) s = next;
+      }
+      q.row = __shfl_sync(0xFFFFFFFFu, held.row, max(s, 0));
+      q.n = __shfl_sync(0xFFFFFFFFu, held.n, max(s, 0));
+      q.len = __shfl_sync(0xFFFFFFFFu, held.len, max(s, 0));
+    } else {
+      if (a.b.starts)
+        for (s = begun - 1; s + 1 < a.b.n && a.b.starts[s + 1] <= row;) ++s;
+      if (lane < rows && s >= 0 && s < a.b.n) q = sequence(a.b, s);
+    }
     int64_t token = a.fill ? -1 : -2;
-    float2 scale = make_float2(0.0f, 0.0f);
-    if (s >= 0 && s < a.b.n) {
-      const Seq q = sequence(a.b, s);
-      if (row >= q.row && row < q.row + q.n) {
-        const int pos = q.len - q.n + (row - q.row);
-        token = -1;
-        if (pos >= 0 && pos < a.b.capacity) {
-          const int p = a.b.table[s * a.b.ldt + (pos >> k.shift)];
-          if (p >= 0 && p < k.pages) {
-            token = ((int64_t)p << k.shift) + (pos & (k.page - 1));
-            scale = *reinterpret_cast<const float2*>(k.scales + 2 * (int64_t)p);
-          }
-        }
+    int p = -1;
+    if (lane < rows && s >= 0 && s < a.b.n && row >= q.row && row < q.row + q.n) {
+      const int pos = q.len - q.n + (row - q.row);
+      token = -1;
+      if (pos >= 0 && pos < a.b.capacity) {
+        p = a.b.table[s * a.b.ldt + (pos >> k.shift)];
+        if (p >= 0 && p < k.pages) token = ((int64_t)p << k.shift) + (pos & (k.page - 1));
       }
     }
-    token_of[threadIdx.x] = token;
-    scale_of_row[threadIdx.x] = scale;
+    if (lane < rows) {
+      token_of[lane] = token;
+      page_of[lane] = p;
+    }
   }
   __syncthreads();
-  // an item is 16 codes (8 at a row's end); all of a thread's are loaded before the first is stored
-  constexpr int ITEMS = (READ_ROWS * (MAX_DC + LD_R) / 16 + READERS - 1) / READERS;
-  const int each = a.by_each.d, c_items = (k.d_c + 15) / 16;
-  uint4 codes[ITEMS];
+  // an item is 8 codes, so that a warp's stores lie side by side; all of a thread's are loaded before the first is stored
+  constexpr int ITEMS = (READ_ROWS * (MAX_DC + LD_R) / 8 + READERS - 1) / READERS;
+  const int each = a.by_each.d, c_items = k.d_c / 8;
+  uint2 codes[ITEMS];
+  float scales[ITEMS];
 #pragma unroll
   for (int l = 0; l < ITEMS; ++l) {
-    const int i = threadIdx.x + l * READERS, r = i / a.by_each, item = i - r * each, part = item >= c_items, at = (part ? item - c_items : item) * 16;
-    codes[l] = make_uint4(0, 0, 0, 0);
-    if (r < rows && token_of[r] >= 0)
-      codes[l] = *reinterpret_cast<const uint4*>(part ? k.r + token_of[r] * LD_R + at : k.c + token_of[r] * k.ld_c + at);
+    const int i = threadIdx.x + l * READERS, r = i / a.by_each, item = i - r * each, part = item >= c_items, at = (part ? item - c_items : item) * 8;
+    codes[l] = make_uint2(0, 0);
+    scales[l] = 0.0f;
+    if (r < rows && token_of[r] >= 0) {
+      codes[l] = *reinterpret_cast<const uint2*>(part ? k.r + token_of[r] * LD_R + at : k.c + token_of[r] * k.ld_c + at);
+      scales[l] = k.scales[2 * (int64_t)page_of[r] + part];
+    }
   }
 #pragma unroll
   for (int l = 0; l < ITEMS; ++l) {
-    const int i = threadIdx.x + l * READERS, r = i / a.by_each, item = i - r * each, part = item >= c_items, at = (part ? item - c_items : item) * 16;
+    const int i = threadIdx.x + l * READERS, r = i / a.by_each, item = i - r * each, part = item >= c_items, at = (part ? item - c_items : item) * 8;
     if (r >= rows || token_of[r] == -2) continue;
-    const float scale = part ? scale_of_row[r].y : scale_of_row[r].x;
-    const uint32_t u[4] = {codes[l].x, codes[l].y, codes[l].z, codes[l].w};
-    T* out = static_cast<T*>(a.out[part]) + (first + r) * a.ld[part] + at;
+    const uint32_t u[2] = {codes[l].x, codes[l].y};
+    float v[8];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = decode2((uint16_t)(u[2 * half + e / 2] >> (e % 2 * 16)));
-        v[2 * e] = f.x * scale;
-        v[2 * e + 1] = f.y * scale;
-      }
-      if (at + 8 * half < (part ? k.d_r : k.d_c)) store8(out + 8 * half, a.wide[part], v);
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = decode2((uint16_t)(u[e / 2] >> (e % 2 * 16)));
+      v[2 * e] = f.x * scales[l];
+      v[2 * e + 1] = f.y * scales[l];
     }
+    store8(static_cast<T*>(a.out[part]) + (first + r) * a.ld[part] + at, a.wide[part], v);
   }
 }
 
@@ -312,7 +350,7 @@ extern "C" int mk_latent_read(const MkLatent* l, const MkLatentBatch* b, void* c
   a.wide[0] = wide(c, ldc);
   a.wide[1] = wide(r, ldr);
   a.fill = fill != 0;
-  a.by_each = div_by((l->d_c + 15) / 16 + (l->d_r + 15) / 16);
+  a.by_each = div_by((l->d_c + l->d_r) / 8);
   const unsigned grid = ((unsigned)rows + READ_ROWS - 1) / READ_ROWS;
   const cudaError_t e = launch_early(dtype == MK_BF16 ? read_kernel<__nv_bfloat16> : read_kernel<__half>, dim3(grid), READERS, 0,
                                      static_cast<cudaStream_t>(stream), a);
