@@ -325,8 +325,8 @@ extern "C" int mk_latent_append(const MkLatent* l, const MkLatentBatch* b, const
   // a sequence's rows are in at most rows / page + 2 pages, and in no more pages than rows
   const int64_t most = b->starts ? rows / l->page + 2 * (int64_t)b->n : rows;
   const unsigned grid = (unsigned)(most < rows ? most : rows);
-  // a page's eights of values over the threads: of few rows (a token of each sequence) no page holds many
-  const int64_t held = l->page < rows ? l->page : rows, eights = held * ((l->d_c + l->d_r) / 8);
+  // a page's eights of values over the threads (without starts a page gets one token)
+  const int64_t held = !b->starts ? 1 : l->page < rows ? l->page : rows, eights = held * ((l->d_c + l->d_r) / 8);
   const auto s = static_cast<cudaStream_t>(stream);
   const auto launch = [&](auto kernel) { return launch_early(kernel, dim3(grid), THREADS, 0, s, a); };
   cudaError_t e;
