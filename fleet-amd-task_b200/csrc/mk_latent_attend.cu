@@ -971,10 +971,14 @@ int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device
 }
 
 constexpr int64_t META_BYTES = (MAX_CTAS * sizeof(int4) + 255) / 256 * 256;
-// Rows of a group: 32 where that makes a group for every block (512 tokens of a prompt behind 3584: 169 us, with 16 rows
-// 196), so that a sequence's tokens are brought half as often; 16 otherwise, whose scores have two buffers in tensor
-// memory and whose tiles pass faster (8 sequences of up to 4 drafts: 17.8 us, with 32 rows 21.9).
-int rows_of_group(int64_t rows, int64_t heads) { return rows * heads >= 32 * MAX_CTAS ? 32 : 16; }
+// Rows of a group: 32 where sequences have 64 rows or more each and 16 would make 24 tiles a block or more, by the table's width:
+// their tokens are brought and multiplied half as often (37 sequences at 4096, 128 heads: 93 us, with 16 rows 126; 512
+// tokens of a prompt behind 3584: 160, with 16 199). 16 otherwise, whose scores have two buffers in tensor memory and whose
+// runs start sooner (1 sequence at 8192, 128 heads: 23.5 us, with 32 rows 27.5), and with fewer rows a group of 32 is half
+// empty (300 sequences of up to 4096, 16 heads: 93 us, with 32 rows 128).
+int rows_of_group(int64_t n, int64_t rows, int64_t heads, int64_t capacity) {
+  return rows * heads >= 64 * n && rows * heads / 16 * (capacity / TILE) >= 24 * MAX_CTAS ? 32 : 16;
+}
 int64_t workspace(int rows, int subs) { return META_BYTES + (int64_t)2 * MAX_CTAS * rows * (2 + subs * 128) * 4; }
 
 }  // namespace
@@ -984,7 +988,7 @@ using namespace latent;
 
 extern "C" int mk_latent_attend_workspace(const MkLatent* l, int32_t n, int32_t rows, int32_t heads, int64_t* bytes) {
   if (!l || !bytes || n < 0 || rows < 0 || heads < 1) return fail(MK_EINVAL, "null pointer or a negative size");
-  *bytes = workspace(rows_of_group(rows, heads), (l->d_c + 127) / 128);
+  *bytes = workspace(rows_of_group(n, rows, heads, 1 << 30), (l->d_c + 127) / 128);      // the most, whatever the table
   return MK_OK;
 }
 
@@ -999,7 +1003,7 @@ extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const
   if (((uintptr_t)q | (uintptr_t)out) & 1 || (uintptr_t)lse & 3 || (uintptr_t)workspace & 255)
     return fail(MK_EINVAL, "misaligned q, out, lse or workspace (256 bytes)");
   a.subs = a.k.ld_c / 128;
-  const int group = rows_of_group(rows, heads);
+  const int group = rows_of_group(b->n, rows, heads, a.b.capacity);
   if (workspace_bytes < latent::workspace(group, a.subs)) return fail(MK_EINVAL, "the workspace is too small");
   int device = 0, sms = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= MAX_DEVICES ||

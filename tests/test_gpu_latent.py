@@ -190,7 +190,7 @@ def test_strides():
         assert not out[:, :off].any() and not out[:, off + 576:].any()
 
 
-def check_attend(cache, q, table, lens, counts, scale, batch=None, ref=None):
+def check_attend(cache, q, table, lens, counts, scale, batch=None, ref=None, floor=0.0):
     ks = counts or [1] * len(lens)
     batch = batch or batch_of(table, lens, counts)
     out, lse = cache.attend(q, batch, scale, return_lse=True)
@@ -203,7 +203,7 @@ def check_attend(cache, q, table, lens, counts, scale, batch=None, ref=None):
     eps = torch.finfo(q.dtype).eps
     bound = eps / 2 * np.abs(want) + (1 + eps) * (2 * e[..., None] + 2.0 ** -11 + 2.0 ** -20 + 2 * L * U) * size
     tiny = float(torch.finfo(q.dtype).smallest_normal) * eps / 2
-    assert (np.abs(got - want) <= bound + tiny).all(), (np.abs(got - want) - bound).max()
+    assert (np.abs(got - want) <= bound + floor + tiny).all(), (np.abs(got - want) - bound - floor).max()
     empty = np.isneginf(want_lse)
     assert np.array_equal(np.isneginf(got_lse), empty)
     d = np.abs(got_lse[~empty] - want_lse[~empty])

@@ -118,9 +118,10 @@ def test_pages_at_most(host):
 
 def test_attend_forms(host):
     form = lambda: re.search(r"(Bf16|Fp16)ELi(\d+)E", host.fake_launches().decode()).groups()  # noqa: E731
-    for rows, heads, dtype, want in ((1, 16, 0, ("Bf16", "16")), (295, 16, 0, ("Bf16", "16")), (296, 16, 0, ("Bf16", "32")), (296, 16, 1, ("Fp16", "16")),
-                                     (37, 128, 0, ("Bf16", "32"))):
-        assert latent(host, "attend", rows, 1, starts=P, heads=heads, dtype=dtype) == mk.MK_OK
+    # (40 pages of 64 are 20 tiles: 178 groups of 16 rows make 24 of them a block)
+    for rows, n, heads, dtype, want in ((1, 1, 16, 0, ("Bf16", "16")), (177, 1, 16, 0, ("Bf16", "16")), (178, 1, 16, 0, ("Bf16", "32")), (178, 1, 16, 1, ("Fp16", "16")),
+                                        (23, 23, 128, 0, ("Bf16", "32")), (300, 300, 16, 0, ("Bf16", "16")), (300, 75, 16, 0, ("Bf16", "32"))):
+        assert latent(host, "attend", rows, n, starts=P, heads=heads, dtype=dtype) == mk.MK_OK
         assert form() == want
         assert all(v[1] in (148, 296) and v[4] <= 232448 for v in launched(host))
 
