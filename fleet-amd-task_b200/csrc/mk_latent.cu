@@ -8,11 +8,12 @@
 // does not count for the scale; |x| beyond 448 2^32 saturates.
 //
 // All of a page's new values are loaded at once and kept in registers (16 bytes a load, 18 loads a thread at most), so they
-// are read once, and their loads do not wait for one another.
+// are read once, and their loads do not wait for one another. 8192 tokens of 576 values (14 MB): 7.2 us on B200, 64 of as many
+// sequences 2.3, most of it the chain lengths, table, scales, codes.
 //
-// read: code x scale of each row, rounded once (exact in BF16): a warp resolves the places of the block's 16 rows (32 rows:
-// 12.5 us for 16384 tokens, with 16 10.3), then each thread widens 8 codes at a
-// time.
+// read: code x scale of each row, rounded once (exact in BF16): a warp resolves the places of the block's 16 rows (of 32 rows:
+// 12.5 us for 16384 tokens where 16 took 10.3), then each thread widens 8 codes at a time, so that a warp's stores lie side by
+// side: 9.2 us for 16384 tokens (28 MB).
 #include "mk_latent.cuh"
 
 namespace latent {
