@@ -341,18 +341,18 @@ template <typename T, int R>
 __device__ __forceinline__ void ask(const Args& a, const Segment& s, uint8_t* smem, Shared<R>& sh, int set) {
   using C = Config<T, R>;
   using E2 = typename T::pair_type;
-  constexpr int PER = SOFTMAX / R;                      // threads of a row
-  constexpr int N = (MAX_DC + LD_R) / 8 / PER + (R == 16);        // 72 eights at most: 16 threads take 5 of them, 8 take 9
-  const int row = threadIdx.x / PER, sub = threadIdx.x % PER, c_chunks = a.subs * 16;
+  constexpr int PER = SOFTMAX / R, EACH = 16 / PER;     // threads of a row, their eights of 128 latent values
+  constexpr int N = 4 * EACH + 1;                       // a thread's eights: latents, and one of the rotary part
+  const int row = threadIdx.x / PER, sub = threadIdx.x % PER, n = a.subs * EACH;
   const bool live = row < s.rows;
   const int f = s.r0 + (live ? row : 0), tok = f / a.by_heads;
   const uint16_t* q = static_cast<const uint16_t*>(a.q) + (s.q.row + tok) * a.qt + (f - tok * a.heads) * a.qh;
   union Eight { uint4 u; E2 e[4]; } v[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int c = sub + i * PER;
-    const bool there = live && (c < c_chunks ? c * 8 < a.k.d_c : (c - c_chunks) * 8 < a.k.d_r);
-    const uint16_t* p = q + (c < c_chunks ? c * 8 : a.k.d_c + (c - c_chunks) * 8);
+    const int at = i + 1 < N ? (sub + i * PER) * 8 : sub * 8;
+    const bool there = live && (i + 1 < N ? at < a.k.d_c : sub < LD_R / 8 && at < a.k.d_r);
+    const uint16_t* p = q + (i + 1 < N ? at : a.k.d_c + at);
     v[i].u = make_uint4(0, 0, 0, 0);
     if (a.wide) {
       if (there) v[i].u = *reinterpret_cast<const uint4*>(p);
@@ -365,9 +365,7 @@ __device__ __forceinline__ void ask(const Args& a, const Segment& s, uint8_t* sm
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const E2 m = __hmax2_nan(__hmax2_nan(__habs2(v[i].e[0]), __habs2(v[i].e[1])), __hmax2_nan(__habs2(v[i].e[2]), __habs2(v[i].e[3])));
-    const int part = sub + i * PER >= c_chunks;
-    most[0] = part ? most[0] : __hmax2_nan(most[0], m);
-    most[1] = part ? __hmax2_nan(most[1], m) : most[1];
+    most[i + 1 == N] = __hmax2_nan(most[i + 1 == N], m);
   }
   float inv[2];
 #pragma unroll
@@ -383,21 +381,14 @@ __device__ __forceinline__ void ask(const Args& a, const Segment& s, uint8_t* sm
     if (sub == 0)
       (part ? sh.qr : sh.qc)[set][row] = u < 0x7F800000u ? __uint_as_float((uint32_t)(e2 + 127) << 23) * (a.scale * 1.44269504f) : __int_as_float(0x7FC00000);
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int c = sub + i * PER;
-    if (c >= c_chunks + LD_R / 8) break;
-    const float by = c < c_chunks ? inv[0] : inv[1];
+  // an eight's pieces to `to` and on, R rows of `width` bytes apart (R is a multiple of 16, so the swizzle is the same)
+  const auto split = [](const Eight& v, float by, uint8_t* to, int width) {
     __half2 x[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 y = unpack(v[i].e[e]);
+      const float2 y = unpack(v.e[e]);
       x[e] = __floats2half2_rn(y.x * by, y.y * by);
     }
-    // the eight's place in the piece's row: 16-byte cells, swizzled by the row
-    const int g = c < c_chunks ? c : c - c_chunks, width = c < c_chunks ? 128 : 64;
-    uint8_t* to = smem + (c < c_chunks ? C::QC + (g >> 4) * (C::NS * 128) : C::QR) + row * width + (g & 1) * 8 +
-                  (((g >> 1 & 7) ^ (c < c_chunks ? row & 7 : row >> 1 & 3)) << 4);
 #pragma unroll
     for (int n = 0; n < C::PIECES; ++n) {
       uint32_t w[4];
@@ -406,9 +397,17 @@ __device__ __forceinline__ void ask(const Args& a, const Segment& s, uint8_t* sm
         w[e] = __nv_cvt_halfraw2_to_fp8x2(x[e], __NV_SATFINITE, __NV_E4M3);
         if (n + 1 < C::PIECES) x[e] = __hmul2(__hsub2(x[e], __half2(__nv_cvt_fp8x2_to_halfraw2((uint16_t)w[e], __NV_E4M3))), __float2half2_rn(16.0f));
       }
-      *reinterpret_cast<uint2*>(to + n * R * width) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);      // (R is a multiple of 16)
+      *reinterpret_cast<uint2*>(to + n * R * width) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
     }
+  };
+  // (16-byte cells, swizzled by the row)
+  const auto cell = [](int eight, int by) { return (eight & 1) * 8 + ((eight >> 1 ^ by) << 4); };
+#pragma unroll
+  for (int i = 0; i + 1 < N; ++i) {
+    if (i >= n) break;
+    split(v[i], inv[0], smem + C::QC + i / EACH * (C::NS * 128) + row * 128 + cell(sub + i % EACH * PER, row & 7), 128);
   }
+  if (sub < LD_R / 8) split(v[N - 1], inv[1], smem + C::QR + row * 64 + cell(sub, row >> 1 & 3), 64);
 }
 
 // ---- the attention -------------------------------------------------------------------------
@@ -598,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
     wait(&sh.drained[1], 0);
   } else {
     // ---- softmax: this thread's token of each tile for half of the rows, and its latent value of each 128
-    constexpr int H = C::H;
+    constexpr int H = C::H, AHEAD = R == 16 ? 4 : 1;      // (32 rows' registers allow one column of the outputs at a time)
     const int tid = threadIdx.x, tok = tid % TILE, half = warp / 4;
     const uint32_t lanes = tmem + ((uint32_t)(warp % 4) * 32 << 16) + half * H;
     bool dead = false;
@@ -646,7 +645,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
           }
           sh.inv[tid] = sum == 0.0f ? 0.0f : 1.0f / sum;
         }
-        softmax_sync();
+        if (whole) softmax_sync();
         const int rows = s.rows - half * H;
         E* out[H];
         float inv[H];
@@ -656,7 +655,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
           inv[h] = sh.inv[half * H + h];
         }
         float* part = a.part + (slot + half * H) * (a.subs * 128) + tok;
-        for (int j = 0; j < a.subs; ++j) {
+#pragma unroll AHEAD
+        for (int j = 0; j < 4; ++j) {
+          if (j >= a.subs) break;
           float o[3][H];
 #pragma unroll
           for (int h = 0; h < H; ++h) o[0][h] = o[1][h] = o[2][h] = 0.0f;
