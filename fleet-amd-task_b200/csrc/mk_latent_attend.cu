@@ -789,19 +789,22 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         }
         // 0 x NaN is NaN: what no row sees becomes zero, a NaN that only later rows see (their scores are NaN) too
         if ((none && tok < ((s.end - pos0 + 31) & ~31)) || (!none && pos >= first_sees)) {
-          for (int j = half; j < a.subs; j += 2)
+          for (int j = half; j < a.subs; j += 2) {
+            // (the lanes' rows begin in one bank: each begins at a cell of its own)
+            uint8_t* const from = smem + st * STAGE + j * SUB + tok * 128;
+            const auto cell = [&](int i) { return reinterpret_cast<uint4*>(from + (i ^ (tok & 7)) * 16); };
+            if (none) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) *cell(i) = make_uint4(0, 0, 0, 0);
+            } else {
+              const auto clean = [](uint32_t x) { return x & ~((((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) / 128 * 255); };
 #pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
-              // (the lanes' rows begin in one bank: each begins at a cell of its own)
-              uint4* at = reinterpret_cast<uint4*>(smem + st * STAGE + j * SUB + tok * 128 + (i ^ (tok & 7)) * 16);
-              uint4 u = make_uint4(0, 0, 0, 0);
-              if (!none) {
-                u = *at;
-                const auto clean = [](uint32_t x) { return x & ~((((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) / 128 * 255); };
-                u = make_uint4(clean(u.x), clean(u.y), clean(u.z), clean(u.w));
+              for (int i = 0; i < 8; ++i) {
+                const uint4 u = *cell(i);
+                *cell(i) = make_uint4(clean(u.x), clean(u.y), clean(u.z), clean(u.w));
               }
-              *at = u;
             }
+          }
         }
         mk::fence_proxy_async_smem();
         fence_before();
