@@ -80,7 +80,7 @@ struct Args {
   int64_t qt, qh, ot, oh;
   int heads, subs, box, wide;   // subs: 128-byte columns of a latent; box: rows of a TMA box; wide: 16-byte loads of q
   int coarse;                   // a place is 1 << coarse units (more than one only where places would pass 2^31)
-  Div by_heads, by_subs;
+  Div by_heads, by_subs, by_blocks;
   float scale;
   int4* meta;                   // [blocks]: of a group that begins in the run before and goes on in this one, the runs that
                                 // hold some of it (or 0), its first row, its rows
@@ -96,8 +96,8 @@ template <int R>
 __device__ __forceinline__ int groups_of(const Args& a, const Seq& q) { return (q.n * a.heads + R - 1) / R; }
 __device__ __forceinline__ int units_of(const Args& a, const Seq& q) { return max(1, (min(q.len, a.b.capacity) + UNIT - 1) / UNIT); }
 __device__ __forceinline__ int places_of(const Args& a, int units) { return ((units - 1) >> a.coarse) + 1 + FIXED; }
-__device__ __forceinline__ int begin_of(int total, int block, int blocks) {
-  const int each = (uint32_t)total / (uint32_t)blocks, more = total - each * blocks;
+__device__ __forceinline__ int begin_of(int total, int block, const Div& blocks) {
+  const int each = total / blocks, more = total - each * blocks.d;
   return each * block + min(block, more);
 }
 // the block whose run holds place `at` < total
@@ -461,14 +461,17 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
     };
     const auto which = [&](int all) {
       total = all;
-      return lo = begin_of(all, blockIdx.x, gridDim.x);
+      return lo = begin_of(all, blockIdx.x, a.by_blocks);
     };
     locate<THREADS>(a.b.n, count, which, work.b, place);
-    work.left = begin_of(total, blockIdx.x + 1, gridDim.x) - lo;
+    work.left = begin_of(total, blockIdx.x + 1, a.by_blocks) - lo;
     if (work.b < a.b.n) {
       const int places = places_of(a, units_of(a, sequence(a.b, work.b)));
-      work.g = (uint32_t)place / (uint32_t)places;
-      work.at = place - work.g * places;
+      work.at = place;
+      if (place >= places) {
+        work.g = (uint32_t)place / (uint32_t)places;
+        work.at = place - work.g * places;
+      }
     }
   }
   const Work start = work;
@@ -570,7 +573,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         // the group's first unit is at place `first`: this run is the second that holds some of it, or not
         const int first = lo - start.at + FIXED, last = lo - start.at + places_of(a, units_of(a, q)) - 1;
         m = make_int4(0, q.row * a.heads + start.g * R, min(R, q.n * a.heads - start.g * R), 0);
-        if (start.at > FIXED && blockIdx.x > 0 && begin_of(total, blockIdx.x - 1, gridDim.x) <= first)
+        if (start.at > FIXED && blockIdx.x > 0 && begin_of(total, blockIdx.x - 1, a.by_blocks) <= first)
           m.x = min(holder_of(total, last, gridDim.x), (int)gridDim.x - 1) - (int)blockIdx.x + 2;
       }
       a.meta[blockIdx.x] = m;
@@ -1037,6 +1040,7 @@ extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const
   if (const int e = tensor_map(&c, a.k.c, a.k.ld_c, tokens, a.box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
   if (const int e = tensor_map(&r, a.k.r, LD_R, tokens, a.box, CU_TENSOR_MAP_SWIZZLE_64B)) return e;
   const int blocks = sms < MAX_CTAS ? sms : MAX_CTAS;
+  a.by_blocks = div_by(blocks);
   const auto s = static_cast<cudaStream_t>(stream);
   // (FP16's three pieces of a query leave no room for 32 rows in tensor memory)
   if (dtype == MK_FP16) return launch<Fp16, 16>(a, c, r, device, blocks, s);
