@@ -619,73 +619,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       if (s.tiles > 0 && !dead && lane == 0) mbar_arrive(&sh.asked);
     };
     float ref[H], l[H];
-    Segment ahead = s;
-    bool begun = false;
-    for (int set = 0;; set ^= 1) {
-      // a segment's queries are prepared while its predecessor's last sum runs
-      if (begun) more = next<R>(a, work, ahead);
-      if (more) prepare(ahead, set);
-      if (begun) {
-        // ---- the segment's end: whole groups are finished, others leave their sums
-        if (s.tiles > 0 && !dead && !wait(&sh.summed[(it - 1) & 1], (it - 1) >> 1)) sh.lost = 1;
-        fence_after();
-        sh.red[warp % 4][half * H + lane % H] = across<H>(l, [](float x, float y) { return x + y; });
-        if (tok == 0) {
-#pragma unroll
-          for (int h = 0; h < H; ++h) sh.ref[half * H + h] = ref[h];
-        }
-        softmax_sync();
-        if (sh.lost) dead = true;
-        const bool whole = s.u0 == 0 && s.u1 == s.units;
-        const int64_t slot = (2 * (int64_t)blockIdx.x + (s.u0 == 0)) * R;
-        if (tid < s.rows) {
-          const float sum = dead ? __int_as_float(0x7FC00000) : sh.red[0][tid] + sh.red[1][tid] + sh.red[2][tid] + sh.red[3][tid];
-          if (!whole) {
-            a.stat[(slot + tid) * 2] = sh.ref[tid];
-            a.stat[(slot + tid) * 2 + 1] = sum;
-          } else if (a.lse) {
-            a.lse[(int64_t)s.q.row * a.heads + s.r0 + tid] = lse_of(sh.ref[tid], sum);
-          }
-          sh.inv[tid] = sum == 0.0f ? 0.0f : 1.0f / sum;
-        }
-        if (whole) softmax_sync();
-        const int rows = s.rows - half * H;
-        E* out[H];
-        float inv[H];
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-          out[h] = static_cast<E*>(a.out) + sh.at[set ^ 1][half * H + h] + tok;
-          inv[h] = sh.inv[half * H + h];
-        }
-        float* part = a.part + (slot + half * H) * (a.subs * 128) + tok;
-#pragma unroll AHEAD
-        for (int j = 0; j < 4; ++j) {
-          if (j >= a.subs) break;
-          float o[3][H];
-#pragma unroll
-          for (int h = 0; h < H; ++h) o[0][h] = o[1][h] = o[2][h] = 0.0f;
-          if (s.tiles > 0) {
-#pragma unroll
-            for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R, o[p]);
-            tmem_wait_load(o);
-          }
-#pragma unroll
-          for (int h = 0; h < H; ++h) o[0][h] = fmaf(fmaf(o[2][h], 0.125f, o[1][h]), 0.125f, o[0][h]);
-          if (!whole) {
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-              if (h < rows) part[h * (a.subs * 128) + j * 128] = o[0][h];
-          } else if (j * 128 + tok < k.d_c) {
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-              if (h < rows) out[h][j * 128] = from_f32<E>(o[0][h] * inv[h]);      // (what no token adds to is 0 x 0)
-          }
-        }
-        fence_before();
-      }
-      if (!more) break;
-      s = ahead;
-      begun = true;
+    Segment ahead;
+    if (more) prepare(s, 0);
+    for (int set = 0; more; set ^= 1) {
       const int first_sees = min(max(s.q.len - s.q.n + 1 + s.r0 / a.by_heads, 0), a.b.capacity);
       float qc[H], qr[H];
 #pragma unroll
@@ -814,6 +750,66 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.weighed[st]);
       }
+      // the next segment's queries are prepared while this one's last sum runs
+      more = next<R>(a, work, ahead);
+      if (more) prepare(ahead, set ^ 1);
+      // ---- the segment's end: whole groups are finished, others leave their sums
+      if (s.tiles > 0 && !dead && !wait(&sh.summed[(it - 1) & 1], (it - 1) >> 1)) sh.lost = 1;
+      fence_after();
+      sh.red[warp % 4][half * H + lane % H] = across<H>(l, [](float x, float y) { return x + y; });
+      if (tok == 0) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) sh.ref[half * H + h] = ref[h];
+      }
+      softmax_sync();
+      if (sh.lost) dead = true;
+      const bool whole = s.u0 == 0 && s.u1 == s.units;
+      const int64_t slot = (2 * (int64_t)blockIdx.x + (s.u0 == 0)) * R;
+      if (tid < s.rows) {
+        const float sum = dead ? __int_as_float(0x7FC00000) : sh.red[0][tid] + sh.red[1][tid] + sh.red[2][tid] + sh.red[3][tid];
+        if (!whole) {
+          a.stat[(slot + tid) * 2] = sh.ref[tid];
+          a.stat[(slot + tid) * 2 + 1] = sum;
+        } else if (a.lse) {
+          a.lse[(int64_t)s.q.row * a.heads + s.r0 + tid] = lse_of(sh.ref[tid], sum);
+        }
+        sh.inv[tid] = sum == 0.0f ? 0.0f : 1.0f / sum;
+      }
+      if (whole) softmax_sync();
+      const int rows = s.rows - half * H;
+      E* out[H];
+      float inv[H];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        out[h] = static_cast<E*>(a.out) + sh.at[set][half * H + h] + tok;
+        inv[h] = sh.inv[half * H + h];
+      }
+      float* part = a.part + (slot + half * H) * (a.subs * 128) + tok;
+#pragma unroll AHEAD
+      for (int j = 0; j < 4; ++j) {
+        if (j >= a.subs) break;
+        float o[3][H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) o[0][h] = o[1][h] = o[2][h] = 0.0f;
+        if (s.tiles > 0) {
+#pragma unroll
+          for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R, o[p]);
+          tmem_wait_load(o);
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h) o[0][h] = fmaf(fmaf(o[2][h], 0.125f, o[1][h]), 0.125f, o[0][h]);
+        if (!whole) {
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+            if (h < rows) part[h * (a.subs * 128) + j * 128] = o[0][h];
+        } else if (j * 128 + tok < k.d_c) {
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+            if (h < rows) out[h][j * 128] = from_f32<E>(o[0][h] * inv[h]);      // (what no token adds to is 0 x 0)
+        }
+      }
+      fence_before();
+      s = ahead;
     }
   }
   __syncwarp();
