@@ -84,7 +84,7 @@ struct Args {
   float scale;
   int4* meta;                   // [blocks]: of a group that begins in the run before and goes on in this one, the runs that
                                 // hold some of it (or 0), its first row, its rows
-  float* stat;                  // [2 blocks][R][2]: ref, sum
+  float2* stat;                 // [R][2][MAX_CTAS]: ref, sum of the group's middle or end, of its beginning (side by side for the join)
   float* part;                  // [2 blocks][R][128 subs]
 };
 
@@ -768,8 +768,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       if (tid < s.rows) {
         const float sum = dead ? __int_as_float(0x7FC00000) : sh.red[0][tid] + sh.red[1][tid] + sh.red[2][tid] + sh.red[3][tid];
         if (!whole) {
-          a.stat[(slot + tid) * 2] = sh.ref[tid];
-          a.stat[(slot + tid) * 2 + 1] = sum;
+          a.stat[(tid * 2 + (s.u0 == 0)) * MAX_CTAS + blockIdx.x] = make_float2(sh.ref[tid], sum);
         } else if (a.lse) {
           a.lse[(int64_t)s.q.row * a.heads + s.r0 + tid] = lse_of(sh.ref[tid], sum);
         }
@@ -855,7 +854,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const Args a, i
     g = groups[group];
     const int n = first + team < jobs && row < g.z ? g.x : 0, dim = col * 128 + lane * 4;
     // the first part begins the group (its block's second place), the others continue it
-    const float2* stat = reinterpret_cast<const float2*>(a.stat) + (int64_t)2 * (g.w - 1) * R + row;
+    const float2* stat = a.stat + row * 2 * MAX_CTAS + g.w - 1;
     const float* parts = a.part + ((int64_t)2 * (g.w - 1) * R + row) * ld + dim;
     const auto place = [&](int p) { return (2 * p + (p == 0)) * R; };
     const auto load = [&](int p) { return *reinterpret_cast<const float4*>(parts + place(p) * ld); };
@@ -876,7 +875,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const Args a, i
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       st[c] = make_float2(-FLT_MAX, 0.0f);
-      if (c * 32 + lane < n) st[c] = stat[place(c * 32 + lane)];
+      if (c * 32 + lane < n) st[c] = stat[c * 32 + lane + (c * 32 + lane == 0 ? MAX_CTAS : 0)];
     }
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) ref = fmaxf(ref, st[c].x);
@@ -1029,8 +1028,8 @@ extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const
   const int64_t groups = (int64_t)rows * heads / 16 + b->n, units = a.b.capacity / UNIT + 1;
   while (groups * ((units >> a.coarse) + 1 + FIXED) > INT32_MAX && a.coarse < 31) ++a.coarse;
   a.meta = static_cast<int4*>(workspace);
-  a.stat = reinterpret_cast<float*>(static_cast<char*>(workspace) + META_BYTES);
-  a.part = a.stat + (int64_t)2 * MAX_CTAS * group * 2;
+  a.stat = reinterpret_cast<float2*>(static_cast<char*>(workspace) + META_BYTES);
+  a.part = reinterpret_cast<float*>(a.stat + (int64_t)2 * MAX_CTAS * group);
   CUtensorMap c, r;
   const uint64_t tokens = (uint64_t)a.k.pages * a.k.page;
   if (const int e = tensor_map(&c, a.k.c, a.k.ld_c, tokens, a.box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
