@@ -819,47 +819,26 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
 // The groups that several blocks' runs share: a job is 128 latent values of one row of one, the partial sums of all its runs
 // in their order, by one warp or, where there are fewer jobs than warps, by up to 8 of a block with a share of the runs each.
 constexpr int MERGE_WARPS = 8;
-template <typename T, int R>
-__global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const Args a, int blocks) {
+template <typename T, int R, int SIDE>          // SIDE: the parts that a warp reads side by side, of 128 / SIDE values each
+__device__ __forceinline__ void join(const Args& a, const int4* groups, int n_groups, float (*weights)[MAX_CTAS], float4 (*sums)[32]) {
   using E = typename T::half_type;
-  static_assert(MAX_CTAS <= MERGE_WARPS * 32, "a thread for each block's run");
-  __shared__ int4 groups[MAX_CTAS];                     // of each: the runs, the first row, the rows, the second run
-  __shared__ int counts[MERGE_WARPS];
-  __shared__ float weights[MERGE_WARPS][MAX_CTAS];
-  __shared__ float4 sums[MERGE_WARPS][32];
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  start_dependents();
-  wait_predecessor();
-  int4 g = make_int4(0, 0, 0, 0);
-  if (tid < blocks) g = a.meta[tid];
-  g.w = tid;
-  const uint32_t ballot = __ballot_sync(~0u, g.x > 0);
-  if (lane == 0) counts[warp] = __popc(ballot);
-  __syncthreads();
-  int n_groups = 0, at = 0;
-#pragma unroll
-  for (int w = 0; w < MERGE_WARPS; ++w) {
-    if (w == warp) at = n_groups;
-    n_groups += counts[w];
-  }
-  if (g.x > 0) groups[at + __popc(ballot & ((1u << lane) - 1))] = g;
-  __syncthreads();
-  const int jobs = n_groups * R * a.subs, ld = a.subs * 128;
-  int share = 1;
-  while (share < MERGE_WARPS && 2 * share * jobs <= (int)gridDim.x * MERGE_WARPS) share *= 2;
-  const int teams = MERGE_WARPS / share, team = warp / share, part = warp % share;
+  constexpr int LANES = 32 / SIDE;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, ld = a.subs * 128, jobs = n_groups * R * a.subs * SIDE;
+  int warps = 1;
+  while (warps < MERGE_WARPS && 2 * warps * jobs <= (int)gridDim.x * MERGE_WARPS) warps *= 2;
+  const int teams = MERGE_WARPS / warps, team = warp / warps, share = warps * SIDE, part = warp % warps * SIDE + lane / LANES;
 #pragma unroll 1
   for (int first = blockIdx.x * teams; first < jobs; first += gridDim.x * teams) {
-    const int job = min(first + team, jobs - 1), row = job % R, rest = job / R, group = rest / a.by_subs, col = rest - group * a.subs;
-    g = groups[group];
-    const int n = first + team < jobs && row < g.z ? g.x : 0, dim = col * 128 + lane * 4;
+    const int job = min(first + team, jobs - 1), row = job % R, rest = job / R, group = rest / SIDE / a.by_subs;
+    const int4 g = groups[group];
+    const int n = first + team < jobs && row < g.z ? g.x : 0, dim = (rest - group * a.subs * SIDE) * (128 / SIDE) + lane % LANES * 4;
     // the first part begins the group (its block's second place), the others continue it
     const float2* stat = a.stat + row * 2 * MAX_CTAS + g.w - 1;
     const float* parts = a.part + ((int64_t)2 * (g.w - 1) * R + row) * ld + dim;
     const auto place = [&](int p) { return (2 * p + (p == 0)) * R; };
     const auto load = [&](int p) { return *reinterpret_cast<const float4*>(parts + place(p) * ld); };
-    // four parts at a time, the first on their way before their weights are known (a loop's rest would wait for each)
-    constexpr int AT_ONCE = 4;
+    // several parts at a time, the first on their way before their weights are known (a loop's rest would wait for each)
+    constexpr int AT_ONCE = SIDE == 1 ? 4 : 5;
     float4 v[AT_ONCE];
     const auto fetch = [&](int from) {
 #pragma unroll
@@ -908,22 +887,56 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const Args a, i
         if (from + k * share < n) add(weights[warp][from + k * share], now[k]);
     }
     __syncwarp();
-    if (share > 1) {
+#pragma unroll
+    for (int x = LANES; x < 32; x *= 2) {
+      o.x += __shfl_xor_sync(~0u, o.x, x);
+      o.y += __shfl_xor_sync(~0u, o.y, x);
+      o.z += __shfl_xor_sync(~0u, o.z, x);
+      o.w += __shfl_xor_sync(~0u, o.w, x);
+    }
+    if (warps > 1) {
       sums[warp][lane] = o;
       __syncthreads();
       o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int w = 0; w < share; ++w) add(1.0f, sums[team * share + w][lane]);
+      for (int w = 0; w < warps; ++w) add(1.0f, sums[team * warps + w][lane]);
       __syncthreads();
     }
     if (n == 0 || part > 0) continue;
     const int f = g.y + row, tok = f / a.by_heads;
-    if (a.lse && col == 0 && lane == 0) a.lse[f] = lse_of(ref, l);
+    if (a.lse && dim == 0) a.lse[f] = lse_of(ref, l);
     E* out = static_cast<E*>(a.out) + tok * a.ot + (f - tok * a.heads) * a.oh + dim;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l, x[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (dim + e < a.k.d_c) out[e] = from_f32<E>(x[e] * inv);
   }
+}
+
+template <typename T, int R, int SIDE>
+__global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const Args a, int blocks) {
+  static_assert(MAX_CTAS <= MERGE_WARPS * 32, "a thread for each block's run");
+  __shared__ int4 groups[MAX_CTAS];                     // of each: the runs, the first row, the rows, the second run
+  __shared__ int counts[MERGE_WARPS];
+  __shared__ float weights[MERGE_WARPS][MAX_CTAS];
+  __shared__ float4 sums[MERGE_WARPS][32];
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  start_dependents();
+  wait_predecessor();
+  int4 g = make_int4(0, 0, 0, 0);
+  if (tid < blocks) g = a.meta[tid];
+  g.w = tid;
+  const uint32_t ballot = __ballot_sync(~0u, g.x > 0);
+  if (lane == 0) counts[warp] = __popc(ballot);
+  __syncthreads();
+  int n_groups = 0, at = 0;
+#pragma unroll
+  for (int w = 0; w < MERGE_WARPS; ++w) {
+    if (w == warp) at = n_groups;
+    n_groups += counts[w];
+  }
+  if (g.x > 0) groups[at + __popc(ballot & ((1u << lane) - 1))] = g;
+  __syncthreads();
+  join<T, R, SIDE>(a, groups, n_groups, weights, sums);
 }
 
 // ---- the host's side -----------------------------------------------------------------------
@@ -960,7 +973,7 @@ cudaError_t multiprocessors(int device, int* n) {
 }
 
 template <typename T, int R>
-int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device, int blocks, cudaStream_t s) {
+int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device, int blocks, bool side, cudaStream_t s) {
   static std::atomic<bool> ready[MAX_DEVICES];   // the kernel may use that much shared memory on the device
   cudaError_t e = cudaSuccess;
   if (!ready[device].load(std::memory_order_acquire)) {
@@ -968,7 +981,7 @@ int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device
     if (e == cudaSuccess) ready[device].store(true, std::memory_order_release);
   }
   if (e == cudaSuccess) e = launch_early(attend_kernel<T, R>, dim3(blocks), THREADS, Config<T, R>::SMEM + 1024, s, a, c, r);
-  if (e == cudaSuccess) e = launch_early(merge_kernel<T, R>, dim3(2 * blocks), MERGE_WARPS * 32, 0, s, a, blocks);
+  if (e == cudaSuccess) e = launch_early(side ? merge_kernel<T, R, 4> : merge_kernel<T, R, 1>, dim3(2 * blocks), MERGE_WARPS * 32, 0, s, a, blocks);
   return e == cudaSuccess ? MK_OK : fail(MK_ECUDA, cudaGetErrorString(e));
 }
 
@@ -1036,8 +1049,13 @@ extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const
   if (const int e = tensor_map(&r, a.k.r, LD_R, tokens, a.box, CU_TENSOR_MAP_SWIZZLE_64B)) return e;
   const int blocks = sms < MAX_CTAS ? sms : MAX_CTAS;
   a.by_blocks = div_by(blocks);
+  // Few groups that may be shared by all runs, by the table's width: the join takes quarters of the columns, a warp reading 4
+  // parts side by side, so that all of a row's are on their way at once (1 sequence at 32768: 14.5 us, without 15.7). Otherwise
+  // not: few parts do not pay for it (1 sequence at 1027: 9.9 us, with it 10.4).
+  const int64_t shared = (rows * (int64_t)heads + b->n * (int64_t)(group - 1)) / group;
+  const bool side = 4 * shared * group * a.subs <= 2 * blocks && units > MAX_CTAS;
   const auto s = static_cast<cudaStream_t>(stream);
   // (FP16's three pieces of a query leave no room for 32 rows in tensor memory)
-  if (dtype == MK_FP16) return launch<Fp16, 16>(a, c, r, device, blocks, s);
-  return group == 32 ? launch<Bf16, 32>(a, c, r, device, blocks, s) : launch<Bf16, 16>(a, c, r, device, blocks, s);
+  if (dtype == MK_FP16) return launch<Fp16, 16>(a, c, r, device, blocks, side, s);
+  return group == 32 ? launch<Bf16, 32>(a, c, r, device, blocks, side, s) : launch<Bf16, 16>(a, c, r, device, blocks, side, s);
 }

@@ -104,3 +104,11 @@ def test_a_workspace_is_enough_for_any_table():
     for t in (table, widened(table, 32), table):
         check_attend(cache, q, t, [777], None, 0.1)
     assert np.isfinite(cache.attend(q, batch_of(table, [777]), 0.1).float().cpu().numpy()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,heads,d_c", [([20000], 16, 512), ([12345], 3, 200), ([15000, 9000], 16, 136), ([20000, 0, 70], 5, 64), ([9600], 40, 128)])
+def test_few_rows_of_long_sequences(lens, heads, d_c, dtype):
+    """Partial sums of all blocks for few groups: the join that reads several of a row's side by side."""
+    cache, table = filled(lens, 64, d_c, 32, seed=heads)
+    check_attend(cache, queries(len(lens), heads, d_c + 32, heads, dtype), widened(table, 64), lens, None, 2.75 / (d_c + 32) ** 0.5)

@@ -126,6 +126,17 @@ def test_attend_forms(host):
         assert all(v[1] in (148, 296) and v[4] <= 232448 for v in launched(host))
 
 
+def test_join_forms(host):
+    """The join reads parts side by side where few groups (of few columns) may be shared by all blocks: by their most, the rows
+    and 15 (31) more of each sequence over 16 (32)."""
+    form = lambda: re.search(r"merge_kernel\S*ELi(\d+)ELi(\d+)E", host.fake_launches().decode()).groups()  # noqa: E731
+    for rows, n, heads, width, d_c, dtype, want in ((1, 1, 16, 149, 512, 0, ("16", "4")), (1, 1, 16, 147, 512, 0, ("16", "1")), (1, 1, 17, 149, 512, 0, ("16", "1")),
+                                                    (1, 1, 17, 149, 256, 0, ("16", "4")), (2, 2, 16, 149, 128, 1, ("16", "4")), (4, 4, 16, 149, 128, 1, ("16", "1")),
+                                                    (1, 1, 64, 2 ** 15, 128, 0, ("32", "4")), (1, 1, 64, 2 ** 15, 136, 0, ("32", "1"))):
+        assert latent(host, "attend", rows, n, heads=heads, width=width, d_c=d_c, dtype=dtype) == mk.MK_OK
+        assert form() == want
+
+
 def test_attend_refusals(host):
     assert latent(host, "attend", nbytes=-1) == mk.MK_EINVAL and b"workspace" in host.fake_message()
     assert latent(host, "attend", ws=P + 128) == mk.MK_EINVAL
