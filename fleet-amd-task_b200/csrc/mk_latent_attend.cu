@@ -20,9 +20,9 @@
 // is more than 8 above it.
 //
 // What bounds it, on B200: a tile of 16 rows takes 1420 clocks of products and about 3300 in the middle of a run, which is
-// HBM's rate (6.2 of the measured 6.5 TB/s); 64 sequences of up to 8192 tokens (153 MB, 23.5 us at that rate) take 43 us, of which
-// 6 are the start (the batch's lengths, a table's page, the first tile and the queries, one after the other), 2 a
-// run's end, 5 merge_kernel. A single sequence of 32768 tokens takes 17 us, most of it those.
+// HBM's rate (6.2 of the measured 6.5 TB/s); 64 sequences of up to 8192 tokens (153 MB, 23.5 us at that rate) take 42 us, of which
+// 5.5 are the start (the batch's lengths, a table's page, the first tile and the queries, one after the other), 1.2 a
+// run's end, 5 merge_kernel. A single sequence of 32768 tokens takes 14 us, most of it those.
 //
 // The work is units of 64 tokens of a group of R rows (a row is a token's head) of a sequence; each block (one per SM)
 // takes an equal run of all units, whatever the lengths, as tiles of two. A group within one run is finished there, one
@@ -90,8 +90,8 @@ struct Args {
 
 // ---- a block's share of the units ----------------------------------------------------------
 // Runs are cut by cost, in places: a group costs its units and FIXED more (its queries, its first tile's maximum, its
-// outputs; fitted: a unit 0.8 us, a group 4.7 us).
-constexpr int FIXED = 5;
+// outputs; fitted: a unit 0.8 us, a group 4; 5 units cost 300 sequences of up to 4096 tokens 1 us of 89).
+constexpr int FIXED = 4;
 template <int R>
 __device__ __forceinline__ int groups_of(const Args& a, const Seq& q) { return (q.n * a.heads + R - 1) / R; }
 __device__ __forceinline__ int units_of(const Args& a, const Seq& q) { return max(1, (min(q.len, a.b.capacity) + UNIT - 1) / UNIT); }
@@ -987,10 +987,10 @@ int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device
 
 constexpr int64_t META_BYTES = (MAX_CTAS * sizeof(int4) + 255) / 256 * 256;
 // Rows of a group: 32 where sequences have 64 rows or more each and 16 would make 24 tiles a block or more, by the table's width:
-// their tokens are brought and multiplied half as often (37 sequences at 4096, 128 heads: 93 us, with 16 rows 126; 512
-// tokens of a prompt behind 3584: 160, with 16 199). 16 otherwise, whose scores have two buffers in tensor memory and whose
-// runs start sooner (1 sequence at 8192, 128 heads: 23.5 us, with 32 rows 27.5), and with fewer rows a group of 32 is half
-// empty (300 sequences of up to 4096, 16 heads: 93 us, with 32 rows 128).
+// their tokens are brought and multiplied half as often (37 sequences at 4096, 128 heads: 94 us, with 16 rows 121; 512
+// tokens of a prompt behind 3584: 164, with 16 190). 16 otherwise, whose scores have two buffers in tensor memory and whose
+// runs start sooner (1 sequence at 8192, 128 heads: 22.5 us, with 32 rows 26.6), and with fewer rows a group of 32 is half
+// empty (300 sequences of up to 4096, 16 heads: 90 us, with 32 rows 132).
 int rows_of_group(int64_t n, int64_t rows, int64_t heads, int64_t capacity) {
   return rows * heads >= 64 * n && rows * heads / 16 * (capacity / TILE) >= 24 * MAX_CTAS ? 32 : 16;
 }
