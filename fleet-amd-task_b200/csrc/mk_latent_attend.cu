@@ -774,7 +774,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         }
         sh.inv[tid] = sum == 0.0f ? 0.0f : 1.0f / sum;
       }
-      if (whole) softmax_sync();
+      softmax_sync();           // (what was read here may be written again from now on: the next segment may have no tile)
       const int rows = s.rows - half * H;
       E* out[H];
       float inv[H];

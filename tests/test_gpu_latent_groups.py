@@ -112,3 +112,17 @@ def test_few_rows_of_long_sequences(lens, heads, d_c, dtype):
     """Partial sums of all blocks for few groups: the join that reads several of a row's side by side."""
     cache, table = filled(lens, 64, d_c, 32, seed=heads)
     check_attend(cache, queries(len(lens), heads, d_c + 32, heads, dtype), widened(table, 64), lens, None, 2.75 / (d_c + 32) ** 0.5)
+
+
+@pytest.mark.parametrize("heads", [16, 20])
+def test_empty_sequences_behind_shared_groups(heads):
+    """A run that ends a group of several and goes on with sequences that hold nothing, again and again."""
+    lens = [2000, 0, 0, 1500, 0, 900, 0, 0, 0] * 3
+    cache, table = filled(lens, 64, 256, 32, seed=heads)
+    q = queries(len(lens), heads, 288, heads)
+    first = None
+    for _ in range(20):
+        out, lse = cache.attend(q, batch_of(table, lens), 0.1, return_lse=True)
+        first = first or (out, lse)
+        assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+    check_attend(cache, q, table, lens, None, 0.1)
