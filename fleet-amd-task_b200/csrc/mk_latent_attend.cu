@@ -12,8 +12,11 @@
 // time goes by the 128 rows of the tile (32 + N / 4 clocks a product of 128 x N x 32, measured, in any layout):
 //   q    = scale_q (q1 + q2 / 16 (+ q3 / 256)) in E4M3: each piece takes 4 bits and the remainder's sign one more, so
 //          two hold a BF16 value and three an FP16 value exactly, down to 2^-23 of the row's largest;
-//   p    = x 2^-7, x rounded to FP16 = x1 + x2 / 8 + x3 / 64 in E5M2: within 2^-11 (3, 4 and 4 bits are all of FP16's
-//          11), or 2^-30 of the row's largest where that is more.
+//   p    = x 2^-7, for BF16 x rounded to FP16 = x1 + x2 / 8 + x3 / 64 in E5M2: within 2^-11 (3, 4 and 4 bits are all of
+//          FP16's 11), or 2^-30 of the row's largest where that is more: a quarter of half a step of a BF16 output. An FP16
+//          output's half step is 2^-11 itself, so there x = ... + x4 / 512 has what the rounding to FP16 took away: within
+//          2^-15 + 2^-18, or 2^-33 of the row's largest (64 sequences of up to 8192 tokens
+//          41.9 us, with three pieces 41.0; 512 tokens behind 3584 189 and 182). The sum of the weights takes x unrounded.
 // A page's scales (keys: sc latent, sr rotary) multiply the scores' two accumulators in FP32. As the values' scale, sc
 // goes into the exponent: t = s + log2 sc, p = 2^(t - ref), so the pieces are relative to the largest p |c|, and the sum
 // of the weights takes p / sc. ref is a tile's maximum of t, taken anew (with O rescaled in tensor memory) only where some t
@@ -53,18 +56,18 @@ constexpr float X_SCALE = 7.0f, RAISE = 8.0f;                       // x = 2^7 a
 struct Bf16 {
   using half_type = __nv_bfloat16;
   using pair_type = __nv_bfloat162;
-  static constexpr int pieces = 2;
+  static constexpr int pieces = 2, weights = 3;
 };
 struct Fp16 {
   using half_type = __half;
   using pair_type = __half2;
-  static constexpr int pieces = 3;
+  static constexpr int pieces = 3, weights = 4;
 };
 
 template <typename T, int R_>
 struct Config {
-  static constexpr int R = R_, H = R_ / 2, PIECES = T::pieces;
-  static constexpr int NS = R * PIECES, NO = R * 3;
+  static constexpr int R = R_, H = R_ / 2, PIECES = T::pieces, W = T::weights;
+  static constexpr int NS = R * PIECES, NO = R * W;
   static constexpr int BUFS = 4 * NS + 4 * NO <= 512 ? 2 : 1;       // buffers of scores in tensor memory
   static constexpr int O_COL = BUFS * 2 * NS;
   static constexpr int QC = 2 * STAGE, QR = QC + 4 * NS * 128, PB = QR + NS * 64, SMEM = PB + 2 * NO * 128;
@@ -299,31 +302,39 @@ struct Shared {
   float ref[R], inv[R];
 };
 
-// The pieces of N weights x (FP16, two a word) as bytes of E5M2, the upper byte of an FP16 value: x1 + x2 / 8 + x3 / 64.
-template <int N>
-__device__ __forceinline__ void pieces_of(const float (&x)[N], uint32_t (&p)[3][N / 4]) {
+// The W pieces of N weights x as bytes of E5M2, the upper byte of an FP16 value: x1 + x2 / 8 + x3 / 64 of x rounded to FP16
+// or, with what that rounding took away, ... + x4 / 512 of x.
+template <int W, int N>
+__device__ __forceinline__ void pieces_of(const float (&x)[N], uint32_t (&p)[W][N / 4]) {
 #pragma unroll
   for (int i = 0; i < N / 4; ++i) {
-    uint32_t w[3][2];
+    uint32_t w[W][2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      __half2 v = __floats2half2_rn(x[4 * i + 2 * k], x[4 * i + 2 * k + 1]);
+      const float x0 = x[4 * i + 2 * k], x1 = x[4 * i + 2 * k + 1];
+      __half2 v = __floats2half2_rn(x0, x1), rest;
+      if constexpr (W == 4) {
+        const float2 f = __half22float2(v);
+        rest = __floats2half2_rn((x0 - f.x) * 64.0f, (x1 - f.y) * 64.0f);
+      }
 #pragma unroll
-      for (int n = 0; n < 3; ++n) {
+      for (int n = 0; n < W; ++n) {
         uint32_t u;
         memcpy(&u, &v, 4);
         u += 0x00800080u;       // to nearest: magnitudes stay below 2^15.8, so nothing carries over
         w[n][k] = u;
-        if (n < 2) {
+        if (n + 1 < W) {
           u &= 0xFF00FF00u;
           __half2 h;
           memcpy(&h, &u, 4);
           v = __hmul2(__hsub2(v, h), __float2half2_rn(8.0f));
+          if constexpr (W == 4)
+            if (n == 1) v = __hadd2(v, rest);
         }
       }
     }
 #pragma unroll
-    for (int n = 0; n < 3; ++n) p[n][i] = __byte_perm(w[n][0], w[n][1], 0x7531);
+    for (int n = 0; n < W; ++n) p[n][i] = __byte_perm(w[n][0], w[n][1], 0x7531);
   }
 }
 
@@ -694,12 +705,12 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
             if (!wait(&sh.summed[st ^ 1], (it - 1) >> 1)) sh.lost = 1;
             fence_after();
             for (int j = 0; j < a.subs; ++j) {
-              float o[3][H];
+              float o[C::W][H];
 #pragma unroll
-              for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R, o[p]);
+              for (int p = 0; p < C::W; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R, o[p]);
               tmem_wait_load(o);
 #pragma unroll
-              for (int p = 0; p < 3; ++p) {
+              for (int p = 0; p < C::W; ++p) {
 #pragma unroll
                 for (int h = 0; h < H; ++h) o[p][h] *= f[h];
                 tmem_store(lanes + C::O_COL + j * C::NO + p * R, o[p]);
@@ -711,17 +722,17 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         {
           // (this stage's tile before has been summed, so its weights' place is free too)
           float x[H];
-          uint32_t p[3][H / 4];
+          uint32_t p[C::W][H / 4];
 #pragma unroll
           for (int h = 0; h < H; ++h) {
             x[h] = exp2_fast(v[h] - (ref[h] - X_SCALE));
             l[h] = fmaf(x[h], g.w, l[h]);
           }
           pieces_of(x, p);
-          // rows of the operand in 16s: [3 R / 16][128 tokens][16]
+          // rows of the operand in 16s: [W R / 16][128 tokens][16]
           uint8_t* w = smem + C::PB + st * C::NO * 128 + tok * 16;
 #pragma unroll
-          for (int i = 0; i < 3; ++i) {
+          for (int i = 0; i < C::W; ++i) {
             if constexpr (H == 8) *reinterpret_cast<uint2*>(w + i * 2048 + half * 8) = make_uint2(p[i][0], p[i][1]);
             else *reinterpret_cast<uint4*>(w + (i * 2 + half) * 2048) = make_uint4(p[i][0], p[i][1], p[i][2], p[i][3]);
           }
@@ -787,16 +798,20 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
 #pragma unroll AHEAD
       for (int j = 0; j < 4; ++j) {
         if (j >= a.subs) break;
-        float o[3][H];
+        float o[C::W][H];
 #pragma unroll
-        for (int h = 0; h < H; ++h) o[0][h] = o[1][h] = o[2][h] = 0.0f;
+        for (int p = 0; p < C::W; ++p)
+#pragma unroll
+          for (int h = 0; h < H; ++h) o[p][h] = 0.0f;
         if (s.tiles > 0) {
 #pragma unroll
-          for (int p = 0; p < 3; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R, o[p]);
+          for (int p = 0; p < C::W; ++p) tmem_load(lanes + C::O_COL + j * C::NO + p * R, o[p]);
           tmem_wait_load(o);
         }
 #pragma unroll
-        for (int h = 0; h < H; ++h) o[0][h] = fmaf(fmaf(o[2][h], 0.125f, o[1][h]), 0.125f, o[0][h]);
+        for (int p = C::W - 1; p > 0; --p)
+#pragma unroll
+          for (int h = 0; h < H; ++h) o[p - 1][h] = fmaf(o[p][h], 0.125f, o[p - 1][h]);
         if (!whole) {
 #pragma unroll
           for (int h = 0; h < H; ++h)
