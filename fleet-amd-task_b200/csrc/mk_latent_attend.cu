@@ -50,6 +50,7 @@ using mk::smem_u32;
 
 constexpr int MAX_CTAS = 148, TILE = 128, UNIT = 64, THREADS = 384, SOFTMAX = 256, LOADERS = 2;
 constexpr int SUB = TILE * 128, STAGE = 4 * SUB + TILE * LD_R;      // a tile: up to 4 x [128 tokens][128 B], then [128][64 B]
+// A wait's default limit, and that of a block's end for its own copies and products in flight, which no caller shortens.
 constexpr uint64_t TIMEOUT_NS = 2000000000ull;
 constexpr float X_SCALE = 7.0f, RAISE = 8.0f;                       // x = 2^7 at ref, 2^15 at most
 
@@ -89,6 +90,8 @@ struct Args {
                                 // hold some of it (or 0), its first row, its rows
   float2* stat;                 // [R][2][MAX_CTAS]: ref, sum of the group's middle or end, of its beginning (side by side for the join)
   float* part;                  // [2 blocks][R][128 subs]
+  int32_t* error;               // (or null) where a block whose wait ran out leaves its code
+  uint64_t limit;               // of a wait, in ns
 };
 
 // ---- a block's share of the units ----------------------------------------------------------
@@ -240,14 +243,14 @@ __device__ __forceinline__ bool come(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// A warp's wait with a limit: false where it ran out.
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+// A warp's wait of at most `limit` ns: false where it ran out.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint64_t limit) {
   bool ok = come(bar, parity);
   if (!ok) {
     const uint64_t begin = mk::globaltimer();
 #pragma unroll 1
     do ok = come(bar, parity);
-    while (!ok && mk::globaltimer() - begin <= TIMEOUT_NS);
+    while (!ok && mk::globaltimer() - begin <= limit);
   }
   return __all_sync(~0u, ok);
 }
@@ -292,7 +295,7 @@ template <int R>
 struct Shared {
   uint64_t full[2], empty[2], scored[2], taken[2], weighed[2], summed[2], asked, drained[2];
   uint32_t tmem;
-  volatile int lost;            // a softmax thread's wait ran out
+  volatile int lost;            // a wait ran out: what the block has left to write becomes NaN, and it reports it
   float4 gran[2][TILE / 16];    // of each 16 tokens: sc, sr, log2 sc, 1 / sc (0: no such page)
   // of this segment and the next:
   float qc[2][R], qr[2][R];     // the rows' factors of the two accumulators, log2 e included
@@ -510,7 +513,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         }
         const int rows = __popc(__ballot_sync(~0u, page >= 0 && lane % each == 0)) * a.box;
         const int y = (page << k.shift) + (pos & (k.page - 1));
-        if (it >= 2 && !(ok = wait(&sh.empty[st], (it - 2) >> 1))) break;
+        if (it >= 2 && !(ok = wait(&sh.empty[st], (it - 2) >> 1, a.limit))) break;
         const uint32_t to = base + st * STAGE, full = smem_u32(&sh.full[st]);
         if (lane == 0) expect_bytes(full, rows * (a.subs * 128 + LD_R));
         __syncwarp();
@@ -538,7 +541,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
         if (lane == 0) mbar_arrive(&sh.full[st]);
       }
     }
-    for (int i = max(it - 2, 0); i < it; ++i) wait(&sh.full[i & 1], i >> 1);       // no copy outlives the block
+    for (int i = max(it - 2, 0); i < it; ++i)                                      // no copy outlives the block
+      if (!wait(&sh.full[i & 1], i >> 1, TIMEOUT_NS)) sh.lost = 1;
   } else if (warp == 9) {
     // ---- scores
     constexpr uint32_t ASK = instruction(0, false, C::NS);
@@ -549,10 +553,10 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
     int segments = 0;
     for (; ok && more; more = next<R>(a, work, s)) {
       if (s.tiles == 0) continue;
-      ok = wait(&sh.asked, segments++);
+      ok = wait(&sh.asked, segments++, a.limit);
       for (int t = 0; t < s.tiles && ok; ++t, ++it) {
         const int st = it & 1, buf = it % C::BUFS;
-        ok = (it < C::BUFS || wait(&sh.taken[buf], it / C::BUFS - 1)) && wait(&sh.full[st], it >> 1);
+        ok = (it < C::BUFS || wait(&sh.taken[buf], it / C::BUFS - 1, a.limit)) && wait(&sh.full[st], it >> 1, a.limit);
         if (!ok) break;
         fence_after();
         const uint32_t d = tmem + buf * 2 * C::NS;
@@ -570,7 +574,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       }
     }
     commit(&sh.drained[0], elected);
-    wait(&sh.drained[0], 0);
+    if (!wait(&sh.drained[0], 0, TIMEOUT_NS)) sh.lost = 1;
   } else if (warp == 10) {
     // ---- sums (a tile's weights come after its scores, so its stage is free once they are used)
     constexpr uint32_t SUM = instruction(1, true, C::NO);
@@ -593,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
     for (; ok && more; more = next<R>(a, work, s)) {
       for (int t = 0; t < s.tiles; ++t, ++it) {
         const int st = it & 1, n = s.end - (s.u0 * UNIT + t * TILE);       // tokens that count
-        if (!(ok = wait(&sh.weighed[st], it >> 1))) break;
+        if (!(ok = wait(&sh.weighed[st], it >> 1, a.limit))) break;
         fence_after();
         const uint64_t v = latents + (st * STAGE >> 4), w = weights + (st * C::NO * 128 >> 4);
 #pragma unroll
@@ -608,7 +612,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       }
     }
     commit(&sh.drained[1], elected);
-    wait(&sh.drained[1], 0);
+    if (!wait(&sh.drained[1], 0, TIMEOUT_NS)) sh.lost = 1;
   } else {
     // ---- softmax: this thread's token of each tile for half of the rows, and its latent value of each 128
     constexpr int H = C::H, AHEAD = R == 16 ? 4 : 1;      // (32 rows' registers allow one column of the outputs at a time)
@@ -644,9 +648,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       }
       for (int t = 0; t < s.tiles && !dead; ++t, ++it) {
         const int st = it & 1, buf = it % C::BUFS, pos0 = s.u0 * UNIT + t * TILE, pos = pos0 + tok;
-        bool ok = wait(&sh.full[st], it >> 1);
+        bool ok = wait(&sh.full[st], it >> 1, a.limit);
         const float4 g = sh.gran[st][tok >> 4];
-        ok = wait(&sh.scored[buf], it / C::BUFS) && ok;
+        ok = wait(&sh.scored[buf], it / C::BUFS, a.limit) && ok;
         fence_after();
         const bool none = pos >= s.end || g.w == 0.0f;
         float v[H];
@@ -702,7 +706,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
             ref[h] = top;
           }
           if (t > 0) {
-            if (!wait(&sh.summed[st ^ 1], (it - 1) >> 1)) sh.lost = 1;
+            if (!wait(&sh.summed[st ^ 1], (it - 1) >> 1, a.limit)) sh.lost = 1;
             fence_after();
             for (int j = 0; j < a.subs; ++j) {
               float o[C::W][H];
@@ -765,7 +769,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       more = next<R>(a, work, ahead);
       if (more) prepare(ahead, set ^ 1);
       // ---- the segment's end: whole groups are finished, others leave their sums
-      if (s.tiles > 0 && !dead && !wait(&sh.summed[(it - 1) & 1], (it - 1) >> 1)) sh.lost = 1;
+      if (s.tiles > 0 && !dead && !wait(&sh.summed[(it - 1) & 1], (it - 1) >> 1, a.limit)) sh.lost = 1;
       fence_after();
       sh.red[warp % 4][half * H + lane % H] = across<H>(l, [](float x, float y) { return x + y; });
       if (tok == 0) {
@@ -828,6 +832,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   }
   __syncwarp();
   __syncthreads();
+  if (threadIdx.x == 0 && sh.lost && a.error) *a.error = MK_DERR_WAIT_TIMEOUT;
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
@@ -1025,9 +1030,16 @@ extern "C" int mk_latent_attend_workspace(const MkLatent* l, int32_t n, int32_t 
 extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const void* q, int64_t qt, int64_t qh, int32_t rows,
                                 int32_t heads, int32_t dtype, float scale, void* out, int64_t ot, int64_t oh, float* lse,
                                 void* workspace, int64_t workspace_bytes, void* stream) {
+  return mk_latent_attend_status(l, b, q, qt, qh, rows, heads, dtype, scale, out, ot, oh, lse, workspace, workspace_bytes, nullptr, 0, stream);
+}
+
+extern "C" int mk_latent_attend_status(const MkLatent* l, const MkLatentBatch* b, const void* q, int64_t qt, int64_t qh, int32_t rows,
+                                       int32_t heads, int32_t dtype, float scale, void* out, int64_t ot, int64_t oh, float* lse,
+                                       void* workspace, int64_t workspace_bytes, int32_t* error, int64_t wait_ns, void* stream) {
   Args a{};
   if (const int e = check(l, b, rows, dtype, a.k, a.b)) return e;
   if (heads < 1 || heads > 1024 || (int64_t)rows * heads > 1 << 30) return fail(MK_EINVAL, "heads are from 1 to 1024, rows x heads at most 2^30");
+  if (wait_ns < 0 || (uintptr_t)error & 3) return fail(MK_EINVAL, "a negative limit or a misaligned error word");
   if (rows == 0 || b->n == 0) return MK_OK;
   if (!q || !out || !workspace) return fail(MK_EINVAL, "null pointer");
   if (((uintptr_t)q | (uintptr_t)out) & 1 || (uintptr_t)lse & 3 || (uintptr_t)workspace & 255)
@@ -1048,6 +1060,8 @@ extern "C" int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const
   a.oh = oh;
   a.heads = heads;
   a.scale = scale;
+  a.error = error;
+  a.limit = wait_ns ? (uint64_t)wait_ns : TIMEOUT_NS;
   a.box = a.k.page < UNIT ? a.k.page : UNIT;
   a.wide = (uintptr_t)q % 16 == 0 && qt % 8 == 0 && qh % 8 == 0;
   a.by_heads = div_by(heads);

@@ -58,25 +58,40 @@ class LatentCache:
     """A cache of `pages` pages of `page` tokens (16, 32, 64 or 128), d_c and d_r multiples of 8 up to 512 and 64.
 
     `c_codes` [pages, page, d_c] and `r_codes` [pages, page, d_r] uint8 and `scales` [pages, 2] float32
-    are the cache's own memory, zero at first; a program may copy, save and fill them."""
+    are the cache's own memory, zero at first; a program may copy, save and fill them. attend's waits end after
+    `wait_timeout_s` each; what a block that gave up had still to write is NaN then, and status() says so."""
 
-    def __init__(self, pages, page, d_c, d_r, device="cuda"):
+    def __init__(self, pages, page, d_c, d_r, device="cuda", wait_timeout_s=2.0):
         if page not in PAGES:
             raise ValueError(f"page {page} is one of {PAGES}")
         if not 8 <= d_c <= 512 or d_c % 8 or not 8 <= d_r <= 64 or d_r % 8:
             raise ValueError(f"d_c from 8 to 512 and d_r from 8 to 64, multiples of 8, expected, got {d_c} and {d_r}")
         if pages < 1 or pages * page >= 2 ** 31:
             raise ValueError(f"from 1 page to 2^31 - 1 tokens expected, got {pages} pages of {page}")
+        self.wait_ns = int(wait_timeout_s * 1e9)
+        if not 0 < self.wait_ns < 2 ** 63:
+            raise ValueError(f"wait_timeout_s {wait_timeout_s} is from 1e-9 on")
         self.pages, self.page, self.d_c, self.d_r = pages, page, d_c, d_r
         self._c = torch.zeros(pages, page, -(-d_c // 128) * 128, dtype=torch.uint8, device=device)
         self._r = torch.zeros(pages, page, 64, dtype=torch.uint8, device=device)
         self.scales = torch.zeros(pages, 2, dtype=torch.float32, device=device)
+        self.error = torch.zeros(1, dtype=torch.int32, device=device)
         self.c_codes, self.r_codes = self._c[..., :d_c], self._r[..., :d_r]
         self.device, self.index = self._c.device, self._c.get_device()
         self.c = mk.MkLatent(self._c.data_ptr(), self._r.data_ptr(), self.scales.data_ptr(), pages, page, d_c, d_r)
-        self.ptr = ctypes.addressof(self.c)
-        self.tensors = self._c, self._r, self.scales
+        self.ptr, self._error = ctypes.addressof(self.c), self.error.data_ptr()
+        self.tensors = self._c, self._r, self.scales, self.error
         self._need = {}            # (sequences, rows, heads) -> workspace bytes
+
+    def status(self, raise_on_error=True):
+        """{"error": 0, or 1 if a wait of attend ran out since the last reset()} (waits for the current stream)."""
+        st = {"error": int(self.error.item())}
+        if st["error"] and raise_on_error:
+            raise mk.MkError(mk.MK_EDEVICE, "LatentCache.attend: a wait ran out, its outputs hold NaN", st)
+        return st
+
+    def reset(self):
+        self.error.zero_()
 
     def _refuse_batch(self, batch, rows):
         if batch.index != self.index:
@@ -172,7 +187,7 @@ class LatentCache:
         if stream is not None:
             with mk.on_stream(q, stream, out, *batch.tensors, *self.tensors):
                 return self.attend(q, batch, scale, out, return_lse)
-        call, device, current_stream, context = mk.entry("mk_latent_attend")
+        call, device, current_stream, context = mk.entry("mk_latent_attend_status")
         index = self.index
         if index < 0 or device() != index:
             return mk.off_device("mk_latent_attend", index, context, lambda: self.attend(q, batch, scale, out, return_lse))
@@ -201,7 +216,7 @@ class LatentCache:
         ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=self.device)
         qt, qh, _ = q.stride()
         rc = call(self.ptr, batch.ptr, q.data_ptr(), qt, qh, rows, heads, DTYPES[dtype], scale, out.data_ptr(), ot, oh,
-                  lse.data_ptr() if return_lse else None, ws.data_ptr(), nbytes, current_stream(index))
+                  lse.data_ptr() if return_lse else None, ws.data_ptr(), nbytes, self._error, self.wait_ns, current_stream(index))
         if rc:
-            mk._check(rc, "mk_latent_attend")
+            mk._check(rc, "mk_latent_attend_status")
         return (out, lse) if return_lse else out

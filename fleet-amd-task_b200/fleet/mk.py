@@ -116,7 +116,7 @@ EXPORTS = ["mk_version", "mk_last_error", "mk_create", "mk_add_op", "mk_finalize
            "mk_mla_decode_noalloc", "mk_set_op_deps", "mk_ep_alloc", "mk_ep_free", "mk_ep_ipc_handle",
            "mk_ep_ipc_open", "mk_ep_ipc_close", "mk_route", "mk_w4_linear", "mk_w4_experts_workspace",
            "mk_w4_experts", "mk_rope", "mk_latent_append", "mk_latent_read", "mk_latent_attend_workspace",
-           "mk_latent_attend"]
+           "mk_latent_attend", "mk_latent_attend_status"]
 
 _lib = None
 
@@ -168,6 +168,7 @@ def lib():
         L.mk_latent_read.argtypes = [vp, vp, vp, i64, vp, i64, i32, i32, i32, vp]
         L.mk_latent_attend_workspace.argtypes = [vp, i32, i32, i32, ctypes.POINTER(i64)]
         L.mk_latent_attend.argtypes = [vp, vp, vp, i64, i64, i32, i32, i32, ctypes.c_float, vp, i64, i64, vp, vp, i64, vp]
+        L.mk_latent_attend_status.argtypes = [*L.mk_latent_attend.argtypes[:-1], vp, i64, vp]
         for name in EXPORTS:
             getattr(L, name).restype = ctypes.c_int if name != "mk_last_error" else ctypes.c_char_p
         _lib = L

@@ -442,6 +442,12 @@ int mk_latent_attend_workspace(const MkLatent* l, int32_t n, int32_t rows, int32
 int mk_latent_attend(const MkLatent* l, const MkLatentBatch* b, const void* q, int64_t qt, int64_t qh, int32_t rows,
                      int32_t heads, int32_t dtype, float scale, void* out, int64_t ot, int64_t oh, float* lse, void* workspace,
                      int64_t workspace_bytes, void* stream);
+/* mk_latent_attend with its waits' limit (0: 2 s, as in mk_latent_attend) and a word for what became of them: a block whose
+   wait ran out leaves NaN in what it had still to write and MK_DERR_WAIT_TIMEOUT in *error (device memory, or NULL), which
+   otherwise stays as it was. A block ends only when its own copies and products have, whatever the limit. */
+int mk_latent_attend_status(const MkLatent* l, const MkLatentBatch* b, const void* q, int64_t qt, int64_t qh, int32_t rows,
+                            int32_t heads, int32_t dtype, float scale, void* out, int64_t ot, int64_t oh, float* lse, void* workspace,
+                            int64_t workspace_bytes, int32_t* error, int64_t wait_ns, void* stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop
