@@ -18,6 +18,7 @@ from fleet.rope import _apart, overlap
 
 DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 PAGES = (16, 32, 64, 128)
+MOST = 2 ** 31 - 1       # what the library counts sequences, pages, rows and heads with has 32 bits
 
 
 def _beside(a, b):
@@ -45,6 +46,8 @@ class LatentBatch:
             raise ValueError(f"table: int32 [{B}, P] with unit stride along P expected, got {table.dtype} {tuple(table.shape)}, strides {table.stride()}")
         if starts is not None and (starts.dtype != torch.int32 or tuple(starts.shape) != (B + 1,) or not starts.is_contiguous()):
             raise ValueError(f"starts: contiguous int32 [{B + 1}] expected, got {starts.dtype} {tuple(starts.shape)}")
+        if B > MOST or table.shape[1] > MOST:
+            raise ValueError(f"a batch has fewer than 2^31 sequences of fewer than 2^31 pages each, got table {tuple(table.shape)}")
         if any(v is not None and v.device != lens.device for v in (table, starts)):
             raise ValueError("table, lens and starts are on one device")
         self.table, self.lens, self.starts = table, lens, starts
@@ -96,6 +99,8 @@ class LatentCache:
     def _refuse_batch(self, batch, rows):
         if batch.index != self.index:
             raise ValueError(f"the batch is on {batch.lens.device}, the cache on {self.device}")
+        if rows > MOST:
+            raise ValueError(f"a call has fewer than 2^31 rows, got {rows}")
         raise ValueError(f"without starts a batch has one row for each of its {batch.n} sequences, got {rows} rows")
 
     def _refuse(self, t, d, name, dtype=None, T=None):
@@ -123,7 +128,7 @@ class LatentCache:
         if k_pe.dim() != 2 or k_pe.shape[1] != self.d_r or k_pe.shape[0] != rows or k_pe.stride(1) != 1 or k_pe.get_device() != index or \
                 k_pe.dtype is not dtype:
             self._refuse(k_pe, self.d_r, "k_pe", dtype, rows)
-        if batch.index != index or (batch.starts is None and rows != batch.n):
+        if batch.index != index or rows > MOST or (batch.starts is None and rows != batch.n):
             self._refuse_batch(batch, rows)
         rc = call(self.ptr, batch.ptr, c_kv.data_ptr(), c_kv.stride(0), k_pe.data_ptr(), k_pe.stride(0), rows, DTYPES[dtype],
                   current_stream(index))
@@ -143,7 +148,7 @@ class LatentCache:
             return mk.off_device("mk_latent_read", index, context, lambda: self.read(batch, rows, dtype, out))
         if dtype not in DTYPES:
             raise TypeError(f"dtype is bfloat16 or float16, not {dtype}")
-        if batch.index != index or (batch.starts is None and rows != batch.n):
+        if batch.index != index or rows > MOST or (batch.starts is None and rows != batch.n):
             self._refuse_batch(batch, rows)
         d_c, d_r, fill = self.d_c, self.d_r, out is None
         if fill:
@@ -169,6 +174,8 @@ class LatentCache:
     def workspace_bytes(self, n, rows, heads):
         got = self._need.get((n, rows, heads))
         if got is None:
+            if max(n, rows, heads) > MOST:
+                raise ValueError(f"sequences, rows and heads are below 2^31, got {n}, {rows} and {heads}")
             need = ctypes.c_int64()
             mk._check(mk.lib().mk_latent_attend_workspace(self.ptr, n, rows, heads, ctypes.byref(need)), "mk_latent_attend_workspace")
             if len(self._need) > 4096:
@@ -196,8 +203,10 @@ class LatentCache:
             raise ValueError(f"q: bfloat16 or float16 [rows, heads, {d_c + self.d_r}] with unit stride along its values on {self.device} expected, got "
                              f"{q.dtype} {tuple(q.shape)}, strides {q.stride()} on {q.device}")
         rows, heads, _ = q.shape
-        if batch.index != index or (batch.starts is None and rows != batch.n):
+        if batch.index != index or rows > MOST or (batch.starts is None and rows != batch.n):
             self._refuse_batch(batch, rows)
+        if heads > MOST:
+            raise ValueError(f"q: fewer than 2^31 heads expected, got {heads}")
         if out is None:
             ot, oh = heads * d_c, d_c
             out = torch.empty_strided((rows, heads, d_c), (ot, oh, 1), dtype=dtype, device=self.device)

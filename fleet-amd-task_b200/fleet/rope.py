@@ -14,6 +14,7 @@ from fleet import capture, mk
 LAYOUTS = {"half": 0, "interleaved": 1, "pairs_to_half": 2}
 DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 POSITIONS = {torch.int32: 0, torch.int64: 1}
+MOST = 2 ** 31 - 1       # what the library counts tokens, heads and their values with has 32 bits
 
 
 def _apart(shape, strides):
@@ -101,6 +102,8 @@ class Rope:
                              f"{tuple(x.shape)}, strides {x.stride()} on {x.device}")
         T, H, W = x.shape
         xt, xh, _ = x.stride()
+        if T > MOST or H > MOST or W > MOST:
+            raise ValueError(f"x: fewer than 2^31 tokens, heads and values of a head expected, got {tuple(x.shape)}")
         if positions.dim() != 1 or positions.shape[0] != T or positions.get_device() != index or (T > 1 and positions.stride(0) != 1):
             raise ValueError(f"positions: contiguous [{T}] on {self.device} expected, got {tuple(positions.shape)} on {positions.device}")
         if not 0 <= start <= W - self.dim:
