@@ -51,7 +51,7 @@ struct Seq {
   int row, n, len;
 };
 
-__device__ __forceinline__ Seq sequence(const Batch& b, int s) {
+__host__ __device__ __forceinline__ Seq sequence(const Batch& b, int s) {
   Seq q;
   q.len = max(b.lens[s], 0);
   if (!b.starts) {
@@ -59,7 +59,7 @@ __device__ __forceinline__ Seq sequence(const Batch& b, int s) {
     q.n = s < b.rows ? 1 : 0;
   } else {
     q.row = min(max(b.starts[s], 0), b.rows);
-    q.n = max(min(b.starts[s + 1], b.rows) - q.row, 0);
+    q.n = max(min(max(b.starts[s + 1], 0), b.rows) - q.row, 0);        // (both in [0, rows]: their difference has 32 bits)
   }
   return q;
 }
