@@ -12,7 +12,9 @@
 // A batch is a table of pages, the sequences' lengths (this step's tokens included) and, if not one row each,
 // the starts of their rows. What these arrays hold is not known on the host, so kernels take nothing of it on trust: a
 // length is cut to the table's width and not below 0, rows to the call's tokens, and a page outside the cache holds
-// no token.
+// no token. starts ascend; where they do not, sequences share rows and pages, so that results are undefined, but no address
+// leaves the call's tensors, and sums over the sequences saturate (plus), so that a call does no more than one of its
+// sizes may.
 #ifndef MK_LATENT_CUH
 #define MK_LATENT_CUH
 
@@ -77,7 +79,14 @@ __device__ __forceinline__ uint16_t encode2(float a, float b) {      // NaN stay
   return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 
-// The item (of n with count(i) parts each, fewer than 2^31 in all) that holds part which(all parts) of them, and the
+// The sum of two numbers that are not negative, 2^31 - 1 at most: rows of starts that go down count again and again, and
+// their parts may pass that.
+__host__ __device__ __forceinline__ int plus(int a, int b) {
+  const uint32_t sum = (uint32_t)a + (uint32_t)b;
+  return sum < 0x7FFFFFFFu ? (int)sum : 0x7FFFFFFF;
+}
+
+// The item (of n with count(i) parts each, at most 2^31 - 1 in all) that holds part which(all parts) of them, and the
 // part's place in it; every thread of the block calls it, once. item is n if there is no such part.
 template <int THREADS, typename Count, typename Which>
 __device__ __forceinline__ void locate(int n, Count count, Which which, int& item, int& place) {
@@ -88,7 +97,7 @@ __device__ __forceinline__ void locate(int n, Count count, Which which, int& ite
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-      if (i >= o) upto += v;
+      if (i >= o) upto = plus(upto, v);
     }
     const int at = which(__shfl_sync(0xFFFFFFFFu, upto, 31));
     const uint32_t holds = __ballot_sync(0xFFFFFFFFu, at >= upto - mine && at < upto);
@@ -99,13 +108,13 @@ __device__ __forceinline__ void locate(int n, Count count, Which which, int& ite
   }
   const int per = (n + THREADS - 1) / THREADS, lo = min((int)threadIdx.x * per, n), hi = min(lo + per, n);
   int mine = 0;
-  for (int i = lo; i < hi; ++i) mine += count(i);
+  for (int i = lo; i < hi; ++i) mine = plus(mine, count(i));
   int upto = mine;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-    if (lane >= o) upto += v;
+    if (lane >= o) upto = plus(upto, v);
   }
   if (threadIdx.x == 0) found[0] = n;
   if (lane == 31) warps[warp] = upto;
@@ -113,8 +122,8 @@ __device__ __forceinline__ void locate(int n, Count count, Which which, int& ite
   int total = 0;
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) upto += warps[w];
-    total += warps[w];
+    if (w < warp) upto = plus(upto, warps[w]);
+    total = plus(total, warps[w]);
   }
   const int at = which(total);
   if (at >= upto - mine && at < upto) {

@@ -30,7 +30,7 @@ def _beside(a, b):
 class LatentBatch:
     """The sequences of a call: `table` [B, P] int32, the pages of each; `lens` [B] int32, the tokens of
     each, the ones of this step included; `starts` [B + 1] int32, where the rows of each begin in the
-    call's tensors (ascending; rows from starts[B] on belong to nobody), or None for one row each, row b
+    call's tensors (ascending, or results are undefined; rows from starts[B] on belong to nobody), or None for one row each, row b
     being sequence b's. Row i of the n of a sequence is its token lens - n + i.
 
     The tensors are held and may change between calls (a captured graph reads what they hold then).

@@ -418,7 +418,7 @@ typedef struct MkLatent {
   int32_t d_c, d_r;      /* multiples of 8: 8 to 512, 8 to 64 */
 } MkLatent;
 /* n sequences: table [n, pages] with row stride ldt, lens [n] (this step's tokens included) and starts [n + 1] of
-   their rows in a call, or NULL for one row each. Row i of a sequence's m is its token len - m + i. A length
+   their rows in a call (ascending; results are undefined otherwise), or NULL for one row each. Row i of a sequence's m is its token len - m + i. A length
    past the table counts as the table's end, below 0 as 0; a page outside the cache holds no token. */
 typedef struct MkLatentBatch {
   const int32_t* table;

@@ -1,4 +1,5 @@
-"""The rows that a batch's starts give its sequences (csrc/mk_latent.cuh), on the host: within the call's whatever the starts are."""
+"""The rows that a batch's starts give its sequences (csrc/mk_latent.cuh), on the host: within the call's whatever the starts are; and
+the sums that they go into, which stay at 2^31 - 1 where starts that go down count rows again and again."""
 import shutil
 import subprocess
 from pathlib import Path
@@ -35,3 +36,27 @@ def test_rows_stay_within_the_calls(tmp_path):
         }
   return 0;
 """) == 0
+
+
+def test_sums_saturate(tmp_path):
+    assert run(tmp_path, r"""
+  const int64_t top = INT32_MAX, v[] = {0, 1, 2, 1 << 20, 1 << 30, top - 1, top};
+  for (int64_t a : v)
+    for (int64_t b : v)
+      if (latent::plus((int)a, (int)b) != (a + b < top ? a + b : top)) return 1;
+  // 1000 sequences that have all of 2^20 rows each, 512 places of units a row: never below what came before
+  int upto = 0;
+  for (int i = 0; i < 1000; ++i) {
+    const int next = latent::plus(upto, 1 << 29);
+    if (next < upto) return 2;
+    upto = next;
+  }
+  return upto == top ? 0 : 3;
+""") == 0
+
+
+def test_every_sum_over_the_sequences_saturates():
+    text = (CSRC / "mk_latent.cuh").read_text()
+    body = text[text.index("void locate("):text.index("// Every kernel here")]
+    for name in ("mine", "upto", "total"):
+        assert f"{name} +=" not in body and f"{name} = plus({name}, " in body
