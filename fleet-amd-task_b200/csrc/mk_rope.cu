@@ -8,7 +8,8 @@
 //
 // An angle of a far position needs more than 32 bits (position 2^20 times an inv_freq of 1 leaves 4 bits
 // of an FP32 angle's fraction), so turns are counted in 64: p (inv_freq / 2 pi) less its nearest whole
-// number, then sincospif in FP32: within 2^-25 of a turn for positions up to 2^31.
+// number, then sincospif in FP32: within 2^-23 of a turn for positions up to 2^31 and frequencies up to 1 (the product's two
+// roundings and that of 1 / 2 pi, each 2^-53 of up to 2^28.4 turns), within 2^-25 for positions up to 2^28.
 //
 // A block takes some tokens, or some heads of one. Each thread loads VEC pairs of a head and COPIES times VEC values that are
 // copied, 16 bytes at a time where all rows allow it; then the block computes its tokens' sines and cosines while the
