@@ -11,8 +11,9 @@
 //
 // A batch is a table of pages, the sequences' lengths (this step's tokens included) and, if not one row each,
 // the starts of their rows. What these arrays hold is not known on the host, so kernels take nothing of it on trust: a
-// length is cut to the table's width and not below 0, rows to the call's tokens, and a page outside the cache holds
-// no token. starts ascend; where they do not, sequences share rows and pages, so that results are undefined, but no address
+// length below 0 counts as 0, rows are cut to the call's, and a token past the table's width or in a page outside the cache
+// is none: it is not written, reads as zeros and is seen by nobody. (The rows' tokens go by the length as given, so of a length
+// past the table the last rows have none.) starts ascend; where they do not, sequences share rows and pages, so that results are undefined, but no address
 // leaves the call's tensors, and sums over the sequences saturate (plus), so that a call does no more than one of its
 // sizes may.
 #ifndef MK_LATENT_CUH

@@ -34,8 +34,9 @@ class LatentBatch:
     being sequence b's. Row i of the n of a sequence is its token lens - n + i.
 
     The tensors are held and may change between calls (a captured graph reads what they hold then).
-    What they say is the device's: a length counts as at most the P pages and at least 0, and a page
-    outside the cache holds no token."""
+    What they say is the device's: a length below 0 counts as 0, and a token past the P pages or in a page
+    outside the cache is none: it is not written, reads as zeros and is seen by nobody. (Where a length is past the
+    pages, the rows' tokens still go by it, so that the last rows have none.)"""
 
     def __init__(self, table, lens, starts=None):
         B = lens.shape[0] if lens.dim() == 1 else -1

@@ -419,7 +419,8 @@ typedef struct MkLatent {
 } MkLatent;
 /* n sequences: table [n, pages] with row stride ldt, lens [n] (this step's tokens included) and starts [n + 1] of
    their rows in a call (ascending; results are undefined otherwise), or NULL for one row each. Row i of a sequence's m is its token len - m + i. A length
-   past the table counts as the table's end, below 0 as 0; a page outside the cache holds no token. */
+   below 0 counts as 0; a token past the table or in a page outside the cache is none: not written, read as zeros, seen
+   by nobody. */
 typedef struct MkLatentBatch {
   const int32_t* table;
   const int32_t* lens;
