@@ -170,6 +170,16 @@ inline Div div_by(int d) {
   return v;
 }
 
+// Places of the attention's work are 1 << coarse units, so many that all groups' together pass 2^31 - 1 for no lengths: a call has at
+// most rows x heads / 16 groups and one more for each sequence, of `capacity` tokens in units of 64 and `fixed` places more. -1: too many
+// groups for any.
+inline int coarse_of(int64_t rows, int64_t heads, int64_t n, int64_t capacity, int fixed) {
+  const int64_t groups = rows * heads / 16 + n, units = capacity / 64 + 1;
+  for (int coarse = 0; coarse < 31; ++coarse)
+    if (groups * ((units >> coarse) + 1 + fixed) <= INT32_MAX) return coarse;
+  return -1;
+}
+
 inline int fail(int code, const char* msg) { return mk::set_last_error(code, msg); }
 
 // The host's checks of what every call is handed; MK_OK and the kernels' structs, or the error.

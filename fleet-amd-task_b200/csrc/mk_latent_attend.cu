@@ -1044,6 +1044,8 @@ extern "C" int mk_latent_attend_status(const MkLatent* l, const MkLatentBatch* b
   if (!q || !out || !workspace) return fail(MK_EINVAL, "null pointer");
   if (((uintptr_t)q | (uintptr_t)out) & 1 || (uintptr_t)lse & 3 || (uintptr_t)workspace & 255)
     return fail(MK_EINVAL, "misaligned q, out, lse or workspace (256 bytes)");
+  a.coarse = coarse_of(rows, heads, b->n, a.b.capacity, FIXED);
+  if (a.coarse < 0) return fail(MK_EINVAL, "a call has at most 2^31 / 5 groups of 16 rows of a sequence");
   a.subs = a.k.ld_c / 128;
   const int group = rows_of_group(b->n, rows, heads, a.b.capacity);
   if (workspace_bytes < latent::workspace(group, a.subs)) return fail(MK_EINVAL, "the workspace is too small");
@@ -1066,9 +1068,6 @@ extern "C" int mk_latent_attend_status(const MkLatent* l, const MkLatentBatch* b
   a.wide = (uintptr_t)q % 16 == 0 && qt % 8 == 0 && qh % 8 == 0;
   a.by_heads = div_by(heads);
   a.by_subs = div_by(a.subs);
-  // groups and their places at most; no more than 2^31 in all
-  const int64_t groups = (int64_t)rows * heads / 16 + b->n, units = a.b.capacity / UNIT + 1;
-  while (groups * ((units >> a.coarse) + 1 + FIXED) > INT32_MAX && a.coarse < 31) ++a.coarse;
   a.meta = static_cast<int4*>(workspace);
   a.stat = reinterpret_cast<float2*>(static_cast<char*>(workspace) + META_BYTES);
   a.part = reinterpret_cast<float*>(a.stat + (int64_t)2 * MAX_CTAS * group);
@@ -1082,7 +1081,7 @@ extern "C" int mk_latent_attend_status(const MkLatent* l, const MkLatentBatch* b
   // parts side by side, so that all of a row's are on their way at once (1 sequence at 32768: 14.5 us, without 15.7). Otherwise
   // not: few parts do not pay for it (1 sequence at 1027: 9.9 us, with it 10.4).
   const int64_t shared = (rows * (int64_t)heads + b->n * (int64_t)(group - 1)) / group;
-  const bool side = 4 * shared * group * a.subs <= 2 * blocks && units > MAX_CTAS;
+  const bool side = 4 * shared * group * a.subs <= 2 * blocks && a.b.capacity / UNIT + 1 > MAX_CTAS;
   const auto s = static_cast<cudaStream_t>(stream);
   // (FP16's three pieces of a query leave no room for 32 rows in tensor memory)
   if (dtype == MK_FP16) return launch<Fp16, 16>(a, c, r, device, blocks, side, s);

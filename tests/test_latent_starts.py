@@ -1,5 +1,6 @@
 """The rows that a batch's starts give its sequences (csrc/mk_latent.cuh), on the host: within the call's whatever the starts are; and
-the sums that they go into, which stay at 2^31 - 1 where starts that go down count rows again and again."""
+the sums that they go into, which stay at 2^31 - 1 where starts that go down count rows again and again;
+and the size of the attention's places, whose count has 31 bits too."""
 import shutil
 import subprocess
 from pathlib import Path
@@ -60,3 +61,26 @@ def test_every_sum_over_the_sequences_saturates():
     body = text[text.index("void locate("):text.index("// Every kernel here")]
     for name in ("mine", "upto", "total"):
         assert f"{name} +=" not in body and f"{name} = plus({name}, " in body
+
+
+def test_places_have_31_bits(tmp_path):
+    """Whatever the lengths: each sequence's rows x heads are whole groups of 16 and one more, each of all units and 4 more. And they
+    are no coarser than that takes: at twice the count there is one unit a place fewer."""
+    assert run(tmp_path, r"""
+  int most = 0;
+  for (int64_t rows : {1ll, 4ll, 300ll, 16384ll, 1ll << 20, 1ll << 27})
+    for (int64_t heads : {1ll, 16ll, 128ll, 1000ll, 1024ll})
+      for (int64_t n : {1ll, 4ll, 300ll, 1ll << 20})
+        for (int64_t capacity : {16ll, 64ll, 4096ll, 1ll << 20, (1ll << 30) - 128, 1ll << 30}) {
+          if (rows * heads > 1 << 30 || n > rows) continue;
+          const int c = latent::coarse_of(rows, heads, n, capacity, 4);
+          const int64_t units = (capacity + 63) / 64, groups = rows * heads / 16 + n, places = ((units - 1) >> c) + 1 + 4;
+          if (c < 0 || groups * places > INT32_MAX) return 1;
+          if (c > 0 && groups * (((units >> (c - 1)) + 2) + 4) <= INT32_MAX) return 2;
+          most = c > most ? c : most;
+        }
+  if (latent::coarse_of(4, 1024, 4, 1 << 30, 4) != 2 || latent::coarse_of(16, 1024, 16, 1 << 30, 4) != 4 || latent::coarse_of(64, 16, 64, 8192, 4)) return 3;
+  // 5 places a group at least, a group for each sequence: 2^29 of them are too many
+  if (latent::coarse_of(1 << 28, 1, 1 << 28, 64, 4) < 0 || latent::coarse_of(1 << 29, 1, 1 << 29, 64, 4) >= 0) return 5;
+  return most > 10 ? 0 : 4;
+""") == 0
