@@ -126,8 +126,11 @@ class W4Layers:
         return logits.argmax(-1), logits, residuals, routes
 
     def plain(self, x, routes):
-        """The residuals and logits of step(x) in FP32 over the dequantised weights, with step's routing (and cached latents),
-        and the largest sum of a score's terms."""
+        """The residuals and logits of step(x) in FP32 over the dequantised weights, with step's routing (and cached latents)."""
+        return self.plain_and_terms(x, routes)[:2]
+
+    def plain_and_terms(self, x, routes):
+        """plain(x, routes), and the largest sum of a score's terms in the attention (0 without it)."""
         d, residuals, spread = self.dims, [], 0.0
         for attention, norm, (w13, w2), (ids, weights) in zip(self.attention, self.norms, self.codes, routes):
             if attention is not None:
@@ -179,7 +182,7 @@ def main(argv=None):
     torch.cuda.synchronize()
     out = {"tokens": a.tokens, "layers": a.layers, "ms_per_step": begin.elapsed_time(end) / a.steps, "ids": ids.tolist()}
     if a.check:
-        want, want_logits, spread = model.plain(x, routes)
+        want, want_logits, spread = model.plain_and_terms(x, routes)
         out["residual_distance"] = [distance(r, p) for r, p in zip(residuals, want)]
         out["logits_distance"] = distance(logits, want_logits)
         if lens is not None:
