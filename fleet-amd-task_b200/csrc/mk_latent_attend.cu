@@ -295,7 +295,10 @@ template <int R>
 struct Shared {
   uint64_t full[2], empty[2], scored[2], taken[2], weighed[2], summed[2], asked, drained[2];
   uint32_t tmem;
-  volatile int lost;            // a wait ran out: what the block has left to write becomes NaN, and it reports it
+  // A softmax thread's wait ran out: what the block has left to write becomes NaN, and it reports it. (Written by those threads alone,
+  // with a barrier before each reading: they all leave a segment, or none does.)
+  volatile int lost;
+  volatile int late;            // a wait for the block's own copies or products ran out: reported
   float4 gran[2][TILE / 16];    // of each 16 tokens: sc, sr, log2 sc, 1 / sc (0: no such page)
   // of this segment and the next:
   float qc[2][R], qr[2][R];     // the rows' factors of the two accumulators, log2 e included
@@ -449,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
     }
     if (lane == 0) {
       mbar_init(&sh.asked, SOFTMAX / 32);
-      sh.lost = 0;
+      sh.lost = sh.late = 0;
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_c) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_r) : "memory");
     }
@@ -542,7 +545,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       }
     }
     for (int i = max(it - 2, 0); i < it; ++i)                                      // no copy outlives the block
-      if (!wait(&sh.full[i & 1], i >> 1, TIMEOUT_NS)) sh.lost = 1;
+      if (!wait(&sh.full[i & 1], i >> 1, TIMEOUT_NS)) sh.late = 1;
   } else if (warp == 9) {
     // ---- scores
     constexpr uint32_t ASK = instruction(0, false, C::NS);
@@ -574,7 +577,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       }
     }
     commit(&sh.drained[0], elected);
-    if (!wait(&sh.drained[0], 0, TIMEOUT_NS)) sh.lost = 1;
+    if (!wait(&sh.drained[0], 0, TIMEOUT_NS)) sh.late = 1;
   } else if (warp == 10) {
     // ---- sums (a tile's weights come after its scores, so its stage is free once they are used)
     constexpr uint32_t SUM = instruction(1, true, C::NO);
@@ -612,7 +615,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
       }
     }
     commit(&sh.drained[1], elected);
-    if (!wait(&sh.drained[1], 0, TIMEOUT_NS)) sh.lost = 1;
+    if (!wait(&sh.drained[1], 0, TIMEOUT_NS)) sh.late = 1;
   } else {
     // ---- softmax: this thread's token of each tile for half of the rows, and its latent value of each 128
     constexpr int H = C::H, AHEAD = R == 16 ? 4 : 1;      // (32 rows' registers allow one column of the outputs at a time)
@@ -832,7 +835,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const __grid_constan
   }
   __syncwarp();
   __syncthreads();
-  if (threadIdx.x == 0 && sh.lost && a.error) *a.error = MK_DERR_WAIT_TIMEOUT;
+  if (threadIdx.x == 0 && (sh.lost || sh.late) && a.error) *a.error = MK_DERR_WAIT_TIMEOUT;
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 

@@ -43,3 +43,12 @@ def test_abi():
     for bad in (dict(wait_ns=-1), dict(error=P + 2)):
         assert call(**bad) == mk.MK_EINVAL, bad
     assert call(error=P, wait_ns=1, rows=0, n=0) == mk.MK_OK
+
+
+def test_only_the_softmax_says_that_its_segment_is_lost():
+    """All softmax threads leave a segment or none does, by a word that each reads behind a barrier: no other warp may write it, which
+    could come between two readings."""
+    text = (mk.PKG / "csrc" / "mk_latent_attend.cu").read_text()
+    kernel = text[text.index("void __launch_bounds__(THREADS, 1) attend_kernel"):text.index("// The groups that several blocks' runs share")]
+    others, softmax = kernel.split("    // ---- softmax:")
+    assert "sh.lost = 1" not in others and softmax.count("sh.lost = 1") == 3 and others.count("sh.late = 1") == 3
