@@ -5,15 +5,16 @@
 // A row that sees no token (an empty sequence, P < 0, pages outside the cache) gives zeros and lse -inf.
 //
 // Why E4M3 operands, and how nothing is lost by them. A token is 576 bytes and 16 heads do 35 thousand operations on
-// it: HBM brings an SM a tile of 128 tokens in 3200 clocks, which leaves no time to widen its codes to 16 bits (147 KB
+// it: HBM brings an SM a tile of 128 tokens in 1.7 us, which leaves no time to widen its codes to 16 bits (147 KB
 // of shared memory written and read back). So the codes go to tcgen05.mma (kind::f8f6f4) as they arrive by TMA, twice:
 // as the keys of S = K q^T (128 tokens x N, K-major) and, the same bytes, as the values of O = C^T P (128 latent
 // values x N, MN-major). What is not in 8 bits is split into pieces that are, each a column of its own, for the tensor core's
-// time goes by the 128 rows of the tile (32 + N / 4 clocks a product of 128 x N x 32, measured, in any layout):
+// time goes by the 128 rows of the tile (32 + N / 4 clocks a product of 128 x N x 32, measured alone, in any layout):
 //   q    = scale_q (q1 + q2 / 16 (+ q3 / 256)) in E4M3: each piece takes 4 bits and the remainder's sign one more, so
-//          two hold a BF16 value and three an FP16 value exactly, down to 2^-23 of the row's largest;
+//          two hold a BF16 value but for what is below 2^-14 of an x of up to 448 (the row's largest has 224 or more: 2^-21.8 of
+//          it), three an FP16 value but for what is below 2^-18 (2^-25.8);
 //   p    = x 2^-7, for BF16 x rounded to FP16 = x1 + x2 / 8 + x3 / 64 in E5M2: within 2^-11 (3, 4 and 4 bits are all of
-//          FP16's 11), or 2^-30 of the row's largest where that is more: a quarter of half a step of a BF16 output. An FP16
+//          FP16's 11), or 2^-30 of the row's largest where that is more: an eighth to a quarter of half a step of a BF16 output. An FP16
 //          output's half step is 2^-11 itself, so there x = ... + x4 / 512 has what the rounding to FP16 took away: within
 //          2^-15 + 2^-18, or 2^-33 of the row's largest (64 sequences of up to 8192 tokens
 //          41.9 us, with three pieces 41.0; 512 tokens behind 3584 189 and 182). The sum of the weights takes x unrounded.
@@ -22,10 +23,13 @@
 // of the weights takes p / sc. ref is a tile's maximum of t, taken anew (with O rescaled in tensor memory) only where some t
 // is more than 8 above it.
 //
-// What bounds it, on B200: a tile of 16 rows takes 1420 clocks of products and about 3300 in the middle of a run, which is
-// HBM's rate (6.2 of the measured 6.5 TB/s); 64 sequences of up to 8192 tokens (153 MB, 23.5 us at that rate) take 42 us, of which
-// 5.5 are the start (the batch's lengths, a table's page, the first tile and the queries, one after the other), 1.2 a
-// run's end, 5 merge_kernel. A single sequence of 32768 tokens takes 14 us, most of it those.
+// What bounds it, on B200 (64 sequences of 8192 and of 16384 tokens, their difference): in the middle of a run a tile of 16
+// rows takes 1.73 us from HBM, 6.3 of the measured 6.5 TB/s, and 1.29 where all sequences name the same 64 pages, which L2
+// holds: the chain of load, scores, softmax and sums over two stages. FP16, whose products have a third to
+// a half more columns: 1.83 and 1.61. With 256 latent values the chain counts from HBM too: 1.32 (4.6 TB/s) and 1.13. 64 sequences of up
+// to 8192 tokens (153 MB, 23.5 us at HBM's rate) take 42 us, of which 5.5 are the start (the batch's lengths, a table's
+// page, the first tile and the queries, one after the other), 1.2 a run's end, 5 merge_kernel. A single sequence of 32768
+// tokens takes 14 us, most of it those.
 //
 // The work is units of 64 tokens of a group of R rows (a row is a token's head) of a sequence; each block (one per SM)
 // takes an equal run of all units, whatever the lengths, as tiles of two. A group within one run is finished there, one
@@ -1010,10 +1014,12 @@ int launch(const Args& a, const CUtensorMap& c, const CUtensorMap& r, int device
 
 constexpr int64_t META_BYTES = (MAX_CTAS * sizeof(int4) + 255) / 256 * 256;
 // Rows of a group: 32 where sequences have 64 rows or more each and 16 would make 24 tiles a block or more, by the table's width:
-// their tokens are brought and multiplied half as often (37 sequences at 4096, 128 heads: 94 us, with 16 rows 121; 512
-// tokens of a prompt behind 3584: 164, with 16 190). 16 otherwise, whose scores have two buffers in tensor memory and whose
-// runs start sooner (1 sequence at 8192, 128 heads: 22.5 us, with 32 rows 26.6), and with fewer rows a group of 32 is half
-// empty (300 sequences of up to 4096, 16 heads: 90 us, with 32 rows 132).
+// their tokens are brought and multiplied half as often (37 sequences at 4096, 128 heads: 79 us, with 16 rows 110; 512
+// tokens of a prompt behind 3584: 137, with 16 178). 16 otherwise, whose scores have two buffers in tensor memory and whose
+// runs start sooner (1 sequence at 8192, 128 heads: 16.4 us, with 32 rows 18.5), and with fewer rows a group of 32 is half
+// empty (300 sequences of up to 4096, 16 heads: 82 us, with 32 rows 121). The lengths are the device's, so a table that is much wider
+// than its sequences takes 32 rows sooner than they would: 8 sequences of up to 8192, 4 drafts each, behind 65536: 28 us, with 16 23.
+// (Calls in a row in a captured graph, on the device.)
 int rows_of_group(int64_t n, int64_t rows, int64_t heads, int64_t capacity) {
   return rows * heads >= 64 * n && rows * heads / 16 * (capacity / TILE) >= 24 * MAX_CTAS ? 32 : 16;
 }
@@ -1081,8 +1087,8 @@ extern "C" int mk_latent_attend_status(const MkLatent* l, const MkLatentBatch* b
   const int blocks = sms < MAX_CTAS ? sms : MAX_CTAS;
   a.by_blocks = div_by(blocks);
   // Few groups that may be shared by all runs, by the table's width: the join takes quarters of the columns, a warp reading 4
-  // parts side by side, so that all of a row's are on their way at once (1 sequence at 32768: 14.5 us, without 15.7). Otherwise
-  // not: few parts do not pay for it (1 sequence at 1027: 9.9 us, with it 10.4).
+  // parts side by side, so that all of a row's are on their way at once (1 sequence at 32768: 13.1 us, without 14.4). Otherwise
+  // not: few parts do not pay for it (1 sequence at 1027: 10.4 us, with it 11.0; 8 sequences of 4 drafts 22.9 and 26.3).
   const int64_t shared = (rows * (int64_t)heads + b->n * (int64_t)(group - 1)) / group;
   const bool side = 4 * shared * group * a.subs <= 2 * blocks && a.b.capacity / UNIT + 1 > MAX_CTAS;
   const auto s = static_cast<cudaStream_t>(stream);
