@@ -72,9 +72,9 @@ class LatentCache:
             raise ValueError(f"d_c from 8 to 512 and d_r from 8 to 64, multiples of 8, expected, got {d_c} and {d_r}")
         if pages < 1 or pages * page >= 2 ** 31:
             raise ValueError(f"from 1 page to 2^31 - 1 tokens expected, got {pages} pages of {page}")
+        if not 1e-9 <= wait_timeout_s <= 1e9:
+            raise ValueError(f"wait_timeout_s {wait_timeout_s} is from 1e-9 to 1e9")
         self.wait_ns = int(wait_timeout_s * 1e9)
-        if not 0 < self.wait_ns < 2 ** 63:
-            raise ValueError(f"wait_timeout_s {wait_timeout_s} is from 1e-9 on")
         self.pages, self.page, self.d_c, self.d_r = pages, page, d_c, d_r
         self._c = torch.zeros(pages, page, -(-d_c // 128) * 128, dtype=torch.uint8, device=device)
         self._r = torch.zeros(pages, page, 64, dtype=torch.uint8, device=device)

@@ -51,3 +51,26 @@ def test_weights_of_fp16(n, d_c, heads):
     bound = half_step(np.abs(want) + b) + b
     assert (off <= bound).all(), ((off > bound).mean(), (off / bound).max())
     assert (np.abs(f64(lse) - want_lse) <= 2 * 2.0 ** -16 + 2 * n * u).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_what_is_not_finite_keeps_to_its_row(dtype):
+    """Weights of neighbouring heads are packed side by side: a NaN or an infinity in one head's query, in every place of a group, and a
+    NaN in a token that only the later rows see leave the others' bits as they were."""
+    lens, counts, heads = [300, 70], [1, 3], 20
+    cache, table = filled(lens, 64, 64, 16, seed=5)
+    q = torch.randn(4, heads, 80, generator=torch.Generator(device=DEV).manual_seed(5), device=DEV).to(dtype)
+    batch = batch_of(table, lens, counts)
+    clean, clean_lse = cache.attend(q, batch, 0.1, return_lse=True)
+    assert torch.isfinite(clean).all()
+    for h in range(heads):
+        bad = q.clone()
+        bad[0, h, 3], bad[2, h, 70] = float("nan"), float("inf") if h % 2 else -float("inf")
+        got, lse = cache.attend(bad, batch, 0.1, return_lse=True)
+        hit = torch.zeros(4, heads, dtype=torch.bool, device=DEV)
+        hit[0, h] = hit[2, h] = True
+        assert got[hit].isnan().all() and lse[hit].isnan().all()
+        assert torch.equal(got[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
+    cache.c_codes[table[1][1], 5, 9] = 127                  # token 69 of the second: its last row alone sees it
+    got, lse = cache.attend(q, batch, 0.1, return_lse=True)
+    assert got[3].isnan().all() and torch.equal(got[:3], clean[:3]) and torch.equal(lse[:3], clean_lse[:3])

@@ -26,7 +26,7 @@ def test_status_and_reset():
 def test_limits():
     assert LatentCache(2, 16, 64, 16, device="cpu").wait_ns == 2 * 10 ** 9
     assert LatentCache(2, 16, 64, 16, device="cpu", wait_timeout_s=1e-9).wait_ns == 1
-    for s in (0, -1, 1e-12, 1e30):
+    for s in (0, -1, 1e-12, 1e30, float("inf"), float("nan")):
         with pytest.raises(ValueError):
             LatentCache(2, 16, 64, 16, device="cpu", wait_timeout_s=s)
 
