@@ -13,9 +13,9 @@
 // the starts of their rows. What these arrays hold is not known on the host, so kernels take nothing of it on trust: a
 // length below 0 counts as 0, rows are cut to the call's, and a token past the table's width or in a page outside the cache
 // is none: it is not written, reads as zeros and is seen by nobody. (The rows' tokens go by the length as given, so of a length
-// past the table the last rows have none.) starts ascend; where they do not, sequences share rows and pages, so that results are undefined, but no address
-// leaves the call's tensors, and sums over the sequences saturate (plus), so that a call does no more than one of its
-// sizes may.
+// past the table the last rows have none.) starts ascend; where they do not, sequences share rows and pages, so that results
+// are undefined, but no address leaves the call's tensors, and sums over the sequences saturate (plus), so that a call
+// does no more than one of its sizes may.
 #ifndef MK_LATENT_CUH
 #define MK_LATENT_CUH
 
@@ -170,9 +170,9 @@ inline Div div_by(int d) {
   return v;
 }
 
-// Places of the attention's work are 1 << coarse units, so many that all groups' together pass 2^31 - 1 for no lengths: a call has at
-// most rows x heads / 16 groups and one more for each sequence, of `capacity` tokens in units of 64 and `fixed` places more. -1: too many
-// groups for any.
+// Places of the attention's work are 1 << coarse units, so many that all groups' together pass 2^31 - 1 for no lengths: a
+// call has at most rows x heads / 16 groups and one more for each sequence, of `capacity` tokens in units of 64 and `fixed`
+// places more. -1: too many groups for any.
 inline int coarse_of(int64_t rows, int64_t heads, int64_t n, int64_t capacity, int fixed) {
   const int64_t groups = rows * heads / 16 + n, units = capacity / 64 + 1;
   for (int coarse = 0; coarse < 31; ++coarse)

@@ -418,8 +418,8 @@ typedef struct MkLatent {
   int32_t d_c, d_r;      /* multiples of 8: 8 to 512, 8 to 64 */
 } MkLatent;
 /* n sequences: table [n, pages] with row stride ldt, lens [n] (this step's tokens included) and starts [n + 1] of
-   their rows in a call (ascending; results are undefined otherwise), or NULL for one row each. Row i of a sequence's m is its token len - m + i. A length
-   below 0 counts as 0; a token past the table or in a page outside the cache is none: not written, read as zeros, seen
+   their rows in a call (ascending; results are undefined otherwise), or NULL for one row each. Row i of a sequence's m
+   is its token len - m + i. A length below 0 counts as 0; a token past the table or in a page outside the cache is none: not written, read as zeros, seen
    by nobody. */
 typedef struct MkLatentBatch {
   const int32_t* table;
